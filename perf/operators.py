@@ -245,14 +245,14 @@ def _place(case, d):
         return s
     c = _Arena(ql, ctx, cache=d["cache"])
     T, row = d["cache"].shape[1], KV * D * size
-    offs = [c.off["cache"] + i * T * row for i in range(2 * layers)]
+    offs = ql.offsets([c.off["cache"] + i * T * row for i in range(2 * layers)])
     if "path" in d:
         a = _Arena(ql, ctx, path=d["path"])
         args = (c.arena, offs, T, c.arena, offs, T, row, case["past"], case["past"], case["n"], a.arena, a.off["path"])
         s.keep, s.outputs = (a, c), [c.view("cache", d["cache"].shape, t)[:, case["past"]:]]
     else:
         to = _Arena(ql, ctx, to=d["to"])
-        args = (to.arena, [to.off["to"] + i * T * row for i in range(2 * layers)], T, c.arena, offs, T, row, 0, 0, case["n"])
+        args = (to.arena, ql.offsets([to.off["to"] + i * T * row for i in range(2 * layers)]), T, c.arena, offs, T, row, 0, 0, case["n"])
         s.keep, s.outputs = (c, to), [to.view("to", d["to"].shape, t)]
     s.call = lambda: ctx.kv_move(*args)
     return s
