@@ -268,6 +268,72 @@ int ql_add_rmsnorm(ql_ctx* ctx, ql_arena* act, uint64_t x_off, uint64_t d_off, c
  *   siluMulRef, qwen-ref.ts:114-121); offsets 16-byte aligned. */
 int ql_silu_mul(ql_ctx* ctx, ql_arena* act, uint64_t gate_off, uint64_t up_off, int64_t n, uint64_t y_off);
 
+/* ---- speculative decoding: a pass over M drafted tokens (a tree) after past_len cached positions.
+ * Row m of a pass lies in the cache at slot past_len + m, whatever its depth in the tree; its position, which turns it, is
+ * past_len + depth. The order of a step: linears, ql_qk_norm_rope, ql_attention_tree, linears, lm_head, ql_token_logprobs;
+ * then the host accepts a path and ql_kv_move brings its rows together. Caches are as ql_kv_store's, fp32 or fp16. */
+
+/* Heads, rotation and cache type of ql_qk_norm_rope (the model's, made once). */
+typedef struct ql_rope_desc {
+    uint64_t q_norm_off;   /* fp32 [D] RMSNorm weight of every query head in `weights`, or QL_NONE */
+    uint64_t k_norm_off;   /* of every key head, or QL_NONE */
+    uint64_t table_off;    /* fp32 [max_pos, rot_dim] in `weights`: a position's rot_dim/2 cosines, then its sines */
+    int32_t max_pos;
+    int32_t n_head, n_kv_head, D;   /* D: 8..256, a multiple of 8 */
+    int32_t rot_dim;       /* values of a head that turn, from its first: 8..D, a multiple of 8 */
+    int32_t interleaved;   /* 0: pairs (i, i + rot_dim/2), as ropeHalfRef; 1: pairs (2i, 2i + 1) */
+    int32_t q_stride, k_stride, v_stride;   /* values from a row to the next, a multiple of 4; 0: heads * D */
+    int32_t cache_dtype;   /* QL_DTYPE_F32 or QL_DTYPE_F16 */
+    float norm_eps;
+    int32_t reserved;      /* 0 */
+} ql_rope_desc;
+/* fills a table: cos and sin of p * theta^(-2i / rot_dim), the angle in fp64, rounded once (ropeHalfRef,
+ * reference/qwen-ref.ts). A program with other frequencies writes its own with ql_arena_write. table_off 16-byte aligned. */
+int ql_rope_table(ql_ctx* ctx, ql_arena* weights, uint64_t table_off, int32_t max_pos, int32_t rot_dim, double theta);
+/* q and k RMSNormed per head (where the descriptor has weights) and turned by pos[m], q to q_out [M, n_head, D], k and v
+ * to rows slot0 + m of the caches [max_t, n_kv_head * D] (fp16: rounded once). pos is int32 [M] in `act`. A row whose position
+ * is not in 0..max_pos-1 is padding: its q_out row and its cache rows stay as they were. q_out may be q itself (same
+ * offset, dense rows); any other overlap of what is written with what is read fails with QL_E_INVALID. M = 1..65535;
+ * slot0 + M > max_t fails with QL_E_RANGE. Offsets 16-byte aligned (pos: 4). */
+int ql_qk_norm_rope(ql_ctx* ctx, const ql_rope_desc* desc, const ql_arena* weights, ql_arena* act, uint64_t q_off, uint64_t k_off,
+                    uint64_t v_off, uint64_t pos_off, int32_t M, uint64_t q_out_off, ql_arena* cache, uint64_t k_cache_off,
+                    uint64_t v_cache_off, int32_t max_t, int32_t slot0);
+/* Host only: masks [M, ceil(M/64)] (bit j % 64 of word j / 64 of row m: token j is m or one that m continues) and depths [M]
+ * (0: continues the context) of a tree. parents[m] is -1 or an earlier row (< m); anything else fails with QL_E_INVALID.
+ * masks or depths may be null. M = 1..256. */
+int ql_tree_masks(int32_t M, const int32_t* parents, uint64_t* masks, int32_t* depths);
+/* out[m, h, :] = softmax_s(q[m, h] . K[s, h / (n_head / n_kv_head)] / sqrt(D)) V[s, ...] over s < past_len and the drafted rows
+ * s = past_len + j whose bit j is set in row m of mask (uint64 [M, ceil(M/64)] at mask_off in `act`; bits from M on are ignored;
+ * QL_NONE: j <= m, causal rows). A row that sees nothing is zero. What a row does not see adds nothing to it,
+ * infinities and NaN included. M = 1..256, D = 8..256 (a multiple of 8), past_len + M <= max_t (the cache may be longer
+ * than ql_attention_decode's 8192); fp32 q and out, sums and softmax in fp32; caches fp32 or fp16. Offsets 16-byte
+ * aligned (mask: 8). Uses the context's 64 MiB workspace, as ql_attention_decode. */
+int ql_attention_tree(ql_ctx* ctx, ql_arena* act, uint64_t q_off, const ql_arena* cache, uint64_t k_off, uint64_t v_off,
+                      int32_t cache_dtype, int32_t max_t, int32_t M, int32_t n_head, int32_t n_kv_head, int32_t D, int32_t past_len,
+                      uint64_t mask_off, uint64_t out_off);
+/* Log probabilities over M rows of V fp32 logits (stride values apart, stride >= V; ql_gemv_f16w's y has stride V), natural
+ * logarithms, no temperature:
+ *   logprob [M, n_tok] fp32    of tokens [M, n_tok] int32; 0 for an id outside 0..V-1 (a padding entry)
+ *   entropy [M] fp32           -sum p log p of the row (entropy_off QL_NONE: not wanted)
+ *   top_id, top_logprob [M, top_k] int32, fp32: the largest logits in order, equal ones by the lower id; beyond V
+ *                              entries -1 and -inf
+ * all in `act`. -inf logits are tokens of no probability; a row of nothing else has log probabilities of -inf and entropy 0. A
+ * NaN or +inf in a row makes its log probabilities and its entropy NaN; NaN comes first among the alternatives. M = 1..65535, V =
+ * 1..2^24, n_tok 0..256, top_k 0..32 (the offsets of what is not wanted are ignored). Offsets 4-byte aligned; nothing
+ * written may overlap anything else. Uses the context's 64 MiB workspace. */
+int ql_token_logprobs(ql_ctx* ctx, ql_arena* act, uint64_t logits_off, int32_t stride, int32_t M, int32_t V, uint64_t tokens_off,
+                      int32_t n_tok, int32_t top_k, uint64_t logprob_off, uint64_t entropy_off, uint64_t top_id_off, uint64_t top_logprob_off);
+/* Rows of `count` cache regions: row dst_row + i of region r of `dst` (at dst_offs[r], dst_max_t rows of row_bytes) becomes row
+ * src_row + rows[i] of region r of `src` (at src_offs[r], src_max_t rows), for i < n. rows is int32 [n] at rows_off in
+ * `act`; QL_NONE: rows src_row + i (act may be null). An entry that is negative or leads outside the source leaves its destination
+ * row as it was. A region may be moved onto itself (same arena and offset; n <= 256): every row is read before any is
+ * written, so the list may have any order and name a row twice. Any other overlap of a written row with a source region, with
+ * rows, or with another written row fails with QL_E_INVALID. count 1..256, n 0..2^24 (0: nothing is done), row_bytes a multiple of 16,
+ * offsets 16-byte aligned (rows: 4). */
+int ql_kv_move(ql_ctx* ctx, ql_arena* dst, const uint64_t* dst_offs, int32_t dst_max_t, const ql_arena* src, const uint64_t* src_offs,
+               int32_t src_max_t, int32_t count, int32_t row_bytes, int32_t dst_row, int32_t src_row, int32_t n, const ql_arena* act,
+               uint64_t rows_off);
+
 /* several independent linears in one launch (e.g. q/k/v on one input, gate/up on another);
  * linear i reads x_offs[i] and writes y_offs[i]; scratch for all of them starts at scratch_off
  * (ql_plan_batch gives the size). M and x_dtype are shared; at most 8 linears. */

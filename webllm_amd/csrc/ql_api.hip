@@ -2586,6 +2586,303 @@ int ql_silu_mul(ql_ctx* ctx, ql_arena* act, uint64_t gate_off, uint64_t up_off, 
     return QL_OK;
 }
 
+// ---- speculative decoding
+
+namespace {
+
+// bytes of an arena that a call reads or writes
+struct Span {
+    const ql_arena* arena;
+    uint64_t off, bytes;
+};
+
+bool meet(const Span& a, const Span& b)
+{
+    return a.arena == b.arena && a.bytes && b.bytes && a.off < b.off + b.bytes && b.off < a.off + a.bytes;
+}
+
+// whether a written span meets a read one or another written one
+bool any_meet(const Span* writes, int nw, const Span* reads, int nr)
+{
+    for (int i = 0; i < nw; i++) {
+        for (int k = 0; k < nr; k++)
+            if (meet(writes[i], reads[k])) return true;
+        for (int k = 0; k < i; k++)
+            if (meet(writes[i], writes[k])) return true;
+    }
+    return false;
+}
+
+int check_devices(const ql_ctx* ctx, const ql_arena* a, const ql_arena* b, const ql_arena* c)
+{
+    for (const ql_arena* x : {a, b, c})
+        if (x && x->device != ctx->device) return fail(QL_E_INVALID, "arena of device %d, context of device %d", x->device, ctx->device);
+    return QL_OK;
+}
+
+bool dtype_bytes(int32_t dtype, uint64_t* bytes)
+{
+    *bytes = dtype == QL_DTYPE_F16 ? 2 : 4;
+    return dtype == QL_DTYPE_F16 || dtype == QL_DTYPE_F32;
+}
+
+}  // namespace
+
+int ql_rope_table(ql_ctx* ctx, ql_arena* weights, uint64_t table_off, int32_t max_pos, int32_t rot_dim, double theta)
+{
+    if (!ctx || !weights) return fail(QL_E_INVALID, "null context or arena");
+    if (max_pos < 1 || max_pos > (1 << 24)) return fail(QL_E_INVALID, "max_pos must be 1..2^24 (got %d)", max_pos);
+    if (rot_dim < 8 || rot_dim > ql::kRopeMaxD || rot_dim % 8) return fail(QL_E_INVALID, "rot_dim must be 8..%d, a multiple of 8 (got %d)", ql::kRopeMaxD, rot_dim);
+    if (!(theta > 0) || !std::isfinite(theta)) return fail(QL_E_INVALID, "theta must be positive and finite");
+    int rc = check_devices(ctx, weights, nullptr, nullptr);
+    if (rc) return rc;
+    if (!in_range(table_off, (uint64_t)max_pos * rot_dim * 4, weights->size)) return fail(QL_E_RANGE, "table [max_pos, rot_dim] outside the weight arena");
+    if (table_off % 16) return fail(QL_E_ALIGN, "table offset must be 16-byte aligned");
+    if ((rc = set_device(ctx))) return rc;
+    QL_HIP(ql::launch_rope_table(reinterpret_cast<float*>(weights->base + table_off), max_pos, rot_dim, theta, ctx->stream));
+    return QL_OK;
+}
+
+int ql_qk_norm_rope(ql_ctx* ctx, const ql_rope_desc* d, const ql_arena* weights, ql_arena* act, uint64_t q_off, uint64_t k_off,
+                    uint64_t v_off, uint64_t pos_off, int32_t M, uint64_t q_out_off, ql_arena* cache, uint64_t k_cache_off,
+                    uint64_t v_cache_off, int32_t max_t, int32_t slot0)
+{
+    if (!ctx || !d || !weights || !act || !cache) return fail(QL_E_INVALID, "null context, descriptor or arena");
+    if (M < 1 || M > 65535) return fail(QL_E_INVALID, "M must be 1..65535 (got %d)", M);
+    if (d->n_head < 1 || d->n_head > 4096 || d->n_kv_head < 1 || d->n_kv_head > 4096) return fail(QL_E_INVALID, "n_head and n_kv_head must be 1..4096");
+    if (d->D < 8 || d->D > ql::kRopeMaxD || d->D % 8) return fail(QL_E_INVALID, "head dim must be 8..%d, a multiple of 8 (got %d)", ql::kRopeMaxD, d->D);
+    if (d->rot_dim < 8 || d->rot_dim > d->D || d->rot_dim % 8) return fail(QL_E_INVALID, "rot_dim must be 8..D, a multiple of 8 (got %d)", d->rot_dim);
+    if (d->max_pos < 1 || (d->interleaved & ~1) || d->reserved) return fail(QL_E_INVALID, "max_pos must be positive, interleaved 0 or 1, reserved 0");
+    uint64_t cb;
+    if (!dtype_bytes(d->cache_dtype, &cb)) return fail(QL_E_INVALID, "bad cache_dtype %d", d->cache_dtype);
+    if (!(d->norm_eps >= 0.f)) return fail(QL_E_INVALID, "norm_eps must be >= 0");
+    if (max_t < 1 || slot0 < 0) return fail(QL_E_INVALID, "max_t must be positive, slot0 >= 0");
+    if ((int64_t)slot0 + M > max_t) return fail(QL_E_RANGE, "context length %lld exceeds the cache's %d positions", (long long)slot0 + M, max_t);
+    const uint64_t D = (uint64_t)d->D, hq = d->n_head * D, hk = d->n_kv_head * D;
+    const int32_t strides[3] = {d->q_stride, d->k_stride, d->v_stride};
+    uint64_t stride[3];
+    for (int i = 0; i < 3; i++) {
+        const uint64_t dense = i ? hk : hq;
+        stride[i] = strides[i] ? (uint64_t)strides[i] : dense;
+        if (strides[i] < 0 || stride[i] < dense || stride[i] % 4) return fail(QL_E_INVALID, "row strides must be 0 or at least a row's values, a multiple of 4");
+    }
+    int rc = check_devices(ctx, weights, act, cache);
+    if (rc) return rc;
+    const uint64_t rows = (uint64_t)M - 1, offs[3] = {q_off, k_off, v_off};
+    Span reads[7];
+    for (int i = 0; i < 3; i++) {
+        reads[i] = {act, offs[i], (rows * stride[i] + (i ? hk : hq)) * 4};
+        if (!in_range(offs[i], reads[i].bytes, act->size)) return fail(QL_E_RANGE, "q, k or v rows outside the activation arena");
+        if (offs[i] % 16) return fail(QL_E_ALIGN, "q, k and v offsets must be 16-byte aligned");
+    }
+    reads[3] = {act, pos_off, (uint64_t)M * 4};
+    reads[4] = {weights, d->table_off, (uint64_t)d->max_pos * d->rot_dim * 4};
+    reads[5] = {weights, d->q_norm_off, d->q_norm_off == QL_NONE ? 0 : D * 4};
+    reads[6] = {weights, d->k_norm_off, d->k_norm_off == QL_NONE ? 0 : D * 4};
+    if (!in_range(pos_off, reads[3].bytes, act->size)) return fail(QL_E_RANGE, "positions [M] outside the activation arena");
+    for (int i = 4; i < 7; i++) {
+        if (reads[i].bytes == 0) continue;
+        if (!in_range(reads[i].off, reads[i].bytes, weights->size)) return fail(QL_E_RANGE, "table or norm weight outside the weight arena");
+        if (reads[i].off % 16) return fail(QL_E_ALIGN, "table and norm weight offsets must be 16-byte aligned");
+    }
+    const uint64_t region = (uint64_t)max_t * hk * cb, first = (uint64_t)slot0 * hk * cb, stored = (uint64_t)M * hk * cb;
+    if (!in_range(q_out_off, (uint64_t)M * hq * 4, act->size)) return fail(QL_E_RANGE, "q_out [M, n_head, D] outside the activation arena");
+    if (!in_range(k_cache_off, region, cache->size) || !in_range(v_cache_off, region, cache->size))
+        return fail(QL_E_RANGE, "K/V cache [max_t, n_kv_head * D] outside its arena");
+    if (q_out_off % 16 || k_cache_off % 16 || v_cache_off % 16 || pos_off % 4) return fail(QL_E_ALIGN, "q_out and cache offsets must be 16-byte aligned, positions 4-byte");
+    const Span writes[3] = {{act, q_out_off, (uint64_t)M * hq * 4}, {cache, k_cache_off + first, stored}, {cache, v_cache_off + first, stored}};
+    const bool in_place = q_out_off == q_off && stride[0] == hq;
+    if (in_place ? any_meet(writes, 3, reads + 1, 6) || meet(writes[1], reads[0]) || meet(writes[2], reads[0]) : any_meet(writes, 3, reads, 7))
+        return fail(QL_E_INVALID, "q_out or the cache rows overlap an input or each other");
+    if ((rc = set_device(ctx))) return rc;
+    ql::RopeArgs a;
+    a.q = reinterpret_cast<const float*>(act->base + q_off);
+    a.k = reinterpret_cast<const float*>(act->base + k_off);
+    a.v = reinterpret_cast<const float*>(act->base + v_off);
+    a.q_norm = reads[5].bytes ? reinterpret_cast<const float*>(weights->base + d->q_norm_off) : nullptr;
+    a.k_norm = reads[6].bytes ? reinterpret_cast<const float*>(weights->base + d->k_norm_off) : nullptr;
+    a.table = reinterpret_cast<const float*>(weights->base + d->table_off);
+    a.pos = reinterpret_cast<const int32_t*>(act->base + pos_off);
+    a.q_out = reinterpret_cast<float*>(act->base + q_out_off);
+    a.k_cache = cache->base + k_cache_off;
+    a.v_cache = cache->base + v_cache_off;
+    a.q_stride = stride[0];
+    a.k_stride = stride[1];
+    a.v_stride = stride[2];
+    a.M = M;
+    a.H = d->n_head;
+    a.KV = d->n_kv_head;
+    a.D = d->D;
+    a.rot = d->rot_dim;
+    a.interleaved = d->interleaved;
+    a.max_pos = d->max_pos;
+    a.half = cb == 2;
+    a.slot0 = slot0;
+    a.eps = d->norm_eps;
+    QL_HIP(ql::launch_qk_norm_rope(a, ctx->stream));
+    return QL_OK;
+}
+
+int ql_tree_masks(int32_t M, const int32_t* parents, uint64_t* masks, int32_t* depths)
+{
+    if (!parents) return fail(QL_E_INVALID, "null parents");
+    if (M < 1 || M > ql::kTreeMaxRows) return fail(QL_E_INVALID, "M must be 1..%d (got %d)", ql::kTreeMaxRows, M);
+    for (int m = 0; m < M; m++)
+        if (parents[m] < -1 || parents[m] >= m) return fail(QL_E_INVALID, "the parent of row %d must be -1 or an earlier row (got %d)", m, parents[m]);
+    const int words = (M + 63) / 64;
+    int32_t depth[ql::kTreeMaxRows];
+    for (int m = 0; m < M; m++) {
+        const int p = parents[m];
+        depth[m] = p < 0 ? 0 : depth[p] + 1;
+        if (depths) depths[m] = depth[m];
+        if (!masks) continue;
+        for (int w = 0; w < words; w++) masks[(size_t)m * words + w] = p < 0 ? 0 : masks[(size_t)p * words + w];
+        masks[(size_t)m * words + m / 64] |= 1ull << (m % 64);
+    }
+    return QL_OK;
+}
+
+int ql_attention_tree(ql_ctx* ctx, ql_arena* act, uint64_t q_off, const ql_arena* cache, uint64_t k_off, uint64_t v_off,
+                      int32_t cache_dtype, int32_t max_t, int32_t M, int32_t n_head, int32_t n_kv_head, int32_t D, int32_t past_len,
+                      uint64_t mask_off, uint64_t out_off)
+{
+    if (!ctx || !act || !cache) return fail(QL_E_INVALID, "null context or arena");
+    if (M < 1 || M > ql::kTreeMaxRows) return fail(QL_E_INVALID, "M must be 1..%d (got %d)", ql::kTreeMaxRows, M);
+    if (n_head < 1 || n_head > 4096 || n_kv_head < 1 || past_len < 0 || max_t < 1) return fail(QL_E_INVALID, "bad attention dimensions");
+    if (n_head % n_kv_head) return fail(QL_E_INVALID, "n_head (%d) must be a multiple of n_kv_head (%d)", n_head, n_kv_head);
+    if (D < 8 || D > ql::kAttnMaxD || D % 8) return fail(QL_E_INVALID, "head dim must be 8..%d, a multiple of 8 (got %d)", ql::kAttnMaxD, D);
+    uint64_t cb;
+    if (!dtype_bytes(cache_dtype, &cb)) return fail(QL_E_INVALID, "bad cache_dtype %d", cache_dtype);
+    if ((int64_t)past_len + M > max_t) return fail(QL_E_RANGE, "context length %lld exceeds the cache's %d positions", (long long)past_len + M, max_t);
+    int rc = check_devices(ctx, act, cache, nullptr);
+    if (rc) return rc;
+    const int words = (M + 63) / 64;
+    const uint64_t qo = (uint64_t)M * n_head * D * 4, row = (uint64_t)n_kv_head * D * cb, seen = (uint64_t)(past_len + M) * row;
+    const bool masked = mask_off != QL_NONE;
+    const Span out = {act, out_off, qo};
+    const Span reads[4] = {{act, q_off, qo}, {act, mask_off, masked ? (uint64_t)M * words * 8 : 0}, {cache, k_off, seen}, {cache, v_off, seen}};
+    if (!in_range(q_off, qo, act->size)) return fail(QL_E_RANGE, "q [M, n_head, D] outside the activation arena");
+    if (!in_range(out_off, qo, act->size)) return fail(QL_E_RANGE, "out [M, n_head, D] outside the activation arena");
+    if (masked && !in_range(mask_off, reads[1].bytes, act->size)) return fail(QL_E_RANGE, "mask [M, ceil(M/64)] outside the activation arena");
+    if (!in_range(k_off, max_t * row, cache->size) || !in_range(v_off, max_t * row, cache->size))
+        return fail(QL_E_RANGE, "K/V cache [max_t, n_kv_head * D] outside its arena");
+    if (q_off % 16 || out_off % 16 || k_off % 16 || v_off % 16 || (masked && mask_off % 8))
+        return fail(QL_E_ALIGN, "offsets must be 16-byte aligned (mask 8-byte)");
+    if (any_meet(&out, 1, reads, 4)) return fail(QL_E_INVALID, "out overlaps an input");
+    if ((rc = set_device(ctx))) return rc;
+    ql::TreeArgs a;
+    a.q = reinterpret_cast<const float*>(act->base + q_off);
+    a.k = cache->base + k_off;
+    a.v = cache->base + v_off;
+    a.mask = masked ? reinterpret_cast<const uint64_t*>(act->base + mask_off) : nullptr;
+    a.out = reinterpret_cast<float*>(act->base + out_off);
+    a.M = M;
+    a.H = n_head;
+    a.KV = n_kv_head;
+    a.G = n_head / n_kv_head;
+    a.D = D;
+    a.past = past_len;
+    a.words = words;
+    a.half = cb == 2;
+    a.scale = (float)(1.4426950408889634 / std::sqrt((double)D));
+    QL_HIP(ql::launch_attention_tree(a, ctx->stream));
+    return QL_OK;
+}
+
+int ql_token_logprobs(ql_ctx* ctx, ql_arena* act, uint64_t logits_off, int32_t stride, int32_t M, int32_t V, uint64_t tokens_off,
+                      int32_t n_tok, int32_t top_k, uint64_t logprob_off, uint64_t entropy_off, uint64_t top_id_off, uint64_t top_logprob_off)
+{
+    if (!ctx || !act) return fail(QL_E_INVALID, "null context or arena");
+    if (M < 1 || M > 65535) return fail(QL_E_INVALID, "M must be 1..65535 (got %d)", M);
+    if (V < 1 || V > (1 << 24) || stride < V) return fail(QL_E_DIMS, "V must be 1..2^24 and stride at least V");
+    if (n_tok < 0 || n_tok > 256 || top_k < 0 || top_k > ql::kLogprobMaxTop)
+        return fail(QL_E_INVALID, "n_tok must be 0..256 and top_k 0..%d", ql::kLogprobMaxTop);
+    int rc = check_devices(ctx, act, nullptr, nullptr);
+    if (rc) return rc;
+    const uint64_t nt = (uint64_t)M * n_tok * 4, nk = (uint64_t)M * top_k * 4, ne = entropy_off == QL_NONE ? 0 : (uint64_t)M * 4;
+    if (!nt && !nk && !ne) return fail(QL_E_INVALID, "nothing is asked for");
+    const Span reads[2] = {{act, logits_off, ((uint64_t)(M - 1) * stride + V) * 4}, {act, tokens_off, nt}};
+    const Span writes[4] = {{act, logprob_off, nt}, {act, entropy_off, ne}, {act, top_id_off, nk}, {act, top_logprob_off, nk}};
+    for (const Span& s : {reads[0], reads[1], writes[0], writes[1], writes[2], writes[3]}) {
+        if (!s.bytes) continue;
+        if (!in_range(s.off, s.bytes, act->size)) return fail(QL_E_RANGE, "logits, tokens or a result outside the activation arena");
+        if (s.off % 4) return fail(QL_E_ALIGN, "offsets must be 4-byte aligned");
+    }
+    if (any_meet(writes, 4, reads, 2)) return fail(QL_E_INVALID, "a result overlaps the logits, the tokens or another result");
+    if ((rc = set_device(ctx))) return rc;
+    ql::LogprobArgs a;
+    a.logits = reinterpret_cast<const float*>(act->base + logits_off);
+    a.tokens = reinterpret_cast<const int32_t*>(act->base + (nt ? tokens_off : 0));
+    a.logprob = reinterpret_cast<float*>(act->base + (nt ? logprob_off : 0));
+    a.entropy = ne ? reinterpret_cast<float*>(act->base + entropy_off) : nullptr;
+    a.top_id = reinterpret_cast<int32_t*>(act->base + (nk ? top_id_off : 0));
+    a.top_logprob = reinterpret_cast<float*>(act->base + (nk ? top_logprob_off : 0));
+    a.stride = stride;
+    a.M = M;
+    a.V = V;
+    a.n_tok = n_tok;
+    a.top_k = top_k;
+    QL_HIP(ql::launch_token_logprobs(a, ctx->stream));
+    return QL_OK;
+}
+
+int ql_kv_move(ql_ctx* ctx, ql_arena* dst, const uint64_t* dst_offs, int32_t dst_max_t, const ql_arena* src, const uint64_t* src_offs,
+               int32_t src_max_t, int32_t count, int32_t row_bytes, int32_t dst_row, int32_t src_row, int32_t n, const ql_arena* act,
+               uint64_t rows_off)
+{
+    if (!ctx || !dst || !src || !dst_offs || !src_offs) return fail(QL_E_INVALID, "null context, arena or offsets");
+    const bool listed = rows_off != QL_NONE;
+    if (listed && !act) return fail(QL_E_INVALID, "a row list needs its arena");
+    if (count < 1 || count > 2 * ql::kMoveMaxRegions) return fail(QL_E_INVALID, "count must be 1..%d (got %d)", 2 * ql::kMoveMaxRegions, count);
+    if (row_bytes < 16 || row_bytes % 16) return fail(QL_E_INVALID, "row_bytes must be a positive multiple of 16 (got %d)", row_bytes);
+    if (dst_max_t < 1 || src_max_t < 1 || dst_row < 0 || src_row < 0 || n < 0 || n > (1 << 24)) return fail(QL_E_INVALID, "bad row counts");
+    if ((int64_t)n * (row_bytes / 16) >= (1ll << 31)) return fail(QL_E_INVALID, "n x row_bytes too large");
+    if ((int64_t)dst_row + n > dst_max_t) return fail(QL_E_RANGE, "rows %d..%lld outside the destination's %d", dst_row, (long long)dst_row + n - 1, dst_max_t);
+    if (listed ? src_row > src_max_t : (int64_t)src_row + n > src_max_t) return fail(QL_E_RANGE, "rows from %d outside the source's %d", src_row, src_max_t);
+    int rc = check_devices(ctx, dst, src, listed ? act : nullptr);
+    if (rc) return rc;
+    const uint64_t rb = (uint64_t)row_bytes;
+    const Span rows = {act, rows_off, listed ? (uint64_t)n * 4 : 0};
+    if (listed && !in_range(rows_off, rows.bytes, act->size)) return fail(QL_E_RANGE, "rows [n] outside the activation arena");
+    if (listed && rows_off % 4) return fail(QL_E_ALIGN, "the row list must be 4-byte aligned");
+    // what region r's move writes, and what it may read
+    auto put = [&](int r) { return Span{dst, dst_offs[r] + dst_row * rb, n * rb}; };
+    auto get = [&](int r) { return Span{src, src_offs[r] + src_row * rb, (uint64_t)(listed ? src_max_t - src_row : n) * rb}; };
+    bool in_place = false, apart = true;   // apart: whole regions, in ascending order, none beginning before the last's end
+    for (int r = 0; r < count; r++) {
+        if (!in_range(dst_offs[r], dst_max_t * rb, dst->size) || !in_range(src_offs[r], src_max_t * rb, src->size))
+            return fail(QL_E_RANGE, "cache region %d outside its arena", r);
+        if (dst_offs[r] % 16 || src_offs[r] % 16) return fail(QL_E_ALIGN, "cache offsets must be 16-byte aligned");
+        if (meet(put(r), rows)) return fail(QL_E_INVALID, "the row list overlaps the rows written");
+        if (meet(put(r), get(r))) {
+            if (dst_offs[r] != src_offs[r]) return fail(QL_E_INVALID, "region %d overlaps its source", r);
+            in_place = true;
+        }
+        apart = apart && (dst != src || (dst_offs[r] == src_offs[r] && dst_max_t == src_max_t)) &&
+                (!r || dst_offs[r] >= dst_offs[r - 1] + dst_max_t * rb);
+    }
+    for (int r = 0; r < count && !apart; r++)
+        for (int k = 0; k < count; k++)
+            if (k != r && (meet(put(r), get(k)) || meet(put(r), put(k)))) return fail(QL_E_INVALID, "region %d is written over region %d", r, k);
+    if (in_place && n > ql::kMoveInPlaceRows) return fail(QL_E_INVALID, "a region is moved onto itself %d rows at most (got %d)", ql::kMoveInPlaceRows, n);
+    if (!n) return QL_OK;
+    if ((rc = set_device(ctx))) return rc;
+    ql::MoveArgs a;
+    a.rows = listed ? reinterpret_cast<const int32_t*>(act->base + rows_off) : nullptr;
+    a.src_row = src_row;
+    a.src_max_t = src_max_t;
+    a.dst_row = dst_row;
+    a.n = n;
+    a.row16 = row_bytes / 16;
+    a.in_place = in_place;
+    for (int at = 0; at < count; at += ql::kMoveMaxRegions) {
+        a.count = std::min(count - at, ql::kMoveMaxRegions);
+        for (int r = 0; r < a.count; r++) a.region[r] = {dst->base + dst_offs[at + r], src->base + src_offs[at + r]};
+        QL_HIP(ql::launch_kv_move(a, ctx->stream));
+    }
+    return QL_OK;
+}
+
 int ql_plan_batch(int32_t count, const ql_gptq_desc* descs, int32_t M, uint64_t* scratch_bytes)
 {
     if (!descs || !scratch_bytes || count <= 0 || count > ql::kMaxBatch)

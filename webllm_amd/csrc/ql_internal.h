@@ -298,6 +298,60 @@ hipError_t launch_attention(const AttnArgs& a, hipStream_t stream);
 hipError_t launch_kv_store(const float* src, float* dst, int rows, int row_len, int pos0, hipStream_t stream);
 
 // ----------------------------------------------------------------------------------------------
+// Speculative decoding: rotation and store, attention of a drafted tree, log probabilities, cache rows moved.
+
+constexpr int kRopeMaxD = 256;
+struct RopeArgs {
+    const float *q, *k, *v;    // rows of H or KV heads, strides in values
+    const float *q_norm, *k_norm;   // [D] or nullptr
+    const float* table;        // [max_pos, rot]: cosines, then sines
+    const int32_t* pos;        // [M]; outside 0..max_pos-1: the row is left out
+    float* q_out;              // [M, H, D]
+    void *k_cache, *v_cache;   // [max_t, KV * D], fp32 or fp16 (half)
+    size_t q_stride, k_stride, v_stride;
+    int M, H, KV, D, rot, interleaved, max_pos, half, slot0;
+    float eps;
+};
+hipError_t launch_qk_norm_rope(const RopeArgs& a, hipStream_t stream);
+hipError_t launch_rope_table(float* table, int max_pos, int rot, double theta, hipStream_t stream);
+
+constexpr int kTreeMaxRows = 256;
+struct TreeArgs {
+    const float* q;            // [M, H, D]
+    const void *k, *v;         // cache [max_t, KV * D], fp32 or fp16 (half)
+    const uint64_t* mask;      // [M, words], or nullptr: row m sees the drafted rows 0..m
+    float* out;                // [M, H, D]
+    int M, H, KV, G, D, past, words, half;
+    float scale;               // fp32(log2(e) / sqrt(D))
+};
+hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t stream);
+
+constexpr int kLogprobMaxTop = 32;
+struct LogprobArgs {
+    const float* logits;       // rows of V values, stride apart
+    const int32_t* tokens;     // [M, n_tok]
+    float *logprob, *entropy;  // [M, n_tok]; [M] or nullptr
+    int32_t* top_id;           // [M, top_k]
+    float* top_logprob;
+    size_t stride;
+    int M, V, n_tok, top_k;
+};
+hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream);
+
+constexpr int kMoveInPlaceRows = 256;
+constexpr int kMoveMaxRegions = 128;   // regions of a launch, in its arguments
+struct MoveArgs {
+    struct {
+        char* dst;
+        const char* src;
+    } region[kMoveMaxRegions];
+    const int32_t* rows;       // [n] or nullptr
+    long long src_row, src_max_t, dst_row;
+    int n, row16, count, in_place, strip;   // row16: 16-byte pieces of a row
+};
+hipError_t launch_kv_move(MoveArgs& a, hipStream_t stream);
+
+// ----------------------------------------------------------------------------------------------
 // Linear sequences: many decode linears (M <= 16) in one persistent launch. Linear i may read the
 // output of an earlier linear; the kernel orders them on the device.
 

@@ -97,6 +97,23 @@ class AttnInfo(ctypes.Structure):
                 ("workgroups", ctypes.c_int32), ("keys_per_split", ctypes.c_int32)]
 
 
+class RopeDesc(ctypes.Structure):
+    """Heads, rotation and cache type of Context.qk_norm_rope (ql_rope_desc)."""
+    _fields_ = [("q_norm_off", ctypes.c_uint64), ("k_norm_off", ctypes.c_uint64), ("table_off", ctypes.c_uint64),
+                ("max_pos", ctypes.c_int32), ("n_head", ctypes.c_int32), ("n_kv_head", ctypes.c_int32), ("D", ctypes.c_int32),
+                ("rot_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("q_stride", ctypes.c_int32),
+                ("k_stride", ctypes.c_int32), ("v_stride", ctypes.c_int32), ("cache_dtype", ctypes.c_int32),
+                ("norm_eps", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+def make_rope(table_off: int, max_pos: int, n_head: int, n_kv_head: int, D: int, rot_dim: int | None = None, interleaved: bool = False,
+              q_norm_off: int | None = None, k_norm_off: int | None = None, norm_eps: float = 1e-6, q_stride: int = 0, k_stride: int = 0,
+              v_stride: int = 0, cache_dtype: int = DTYPE_F32) -> RopeDesc:
+    return RopeDesc(QL_NONE if q_norm_off is None else q_norm_off, QL_NONE if k_norm_off is None else k_norm_off, table_off, max_pos,
+                    n_head, n_kv_head, D, D if rot_dim is None else rot_dim, int(interleaved), q_stride, k_stride, v_stride, cache_dtype,
+                    norm_eps, 0)
+
+
 _lib = None
 
 
@@ -145,6 +162,12 @@ def lib():
         "ql_silu_mul": (I, [P, P, U64, U64, ctypes.c_int64, U64]),
         "ql_attention_decode": (I, [P, P, U64, P, U64, U64, I, I, I, I, I, I, U64]),
         "ql_plan_attention": (I, [I, I, I, I, I, I, ctypes.POINTER(AttnInfo)]),
+        "ql_rope_table": (I, [P, P, U64, I, I, ctypes.c_double]),
+        "ql_qk_norm_rope": (I, [P, ctypes.POINTER(RopeDesc), P, P, U64, U64, U64, U64, I, U64, P, U64, U64, I, I]),
+        "ql_tree_masks": (I, [I, P, P, P]),
+        "ql_attention_tree": (I, [P, P, U64, P, U64, U64, I, I, I, I, I, I, I, U64, U64]),
+        "ql_token_logprobs": (I, [P, P, U64, I, I, I, U64, I, I, U64, U64, U64, U64]),
+        "ql_kv_move": (I, [P, P, ctypes.POINTER(U64), I, P, ctypes.POINTER(U64), I, I, I, I, I, I, P, U64]),
         "ql_linear": (I, [P, ctypes.POINTER(GptqDesc), P, P, U64, I, I, U64, U64]),
         "ql_linear_noalloc": (I, [P, ctypes.POINTER(GptqDesc), P, P, U64, I, I, U64]),
         "ql_plan_batch": (I, [I, ctypes.POINTER(GptqDesc), I, ctypes.POINTER(U64)]),
@@ -201,6 +224,21 @@ def plan_attention(max_t: int, M: int, n_head: int, n_kv_head: int, D: int, past
     info = AttnInfo()
     _check(lib().ql_plan_attention(max_t, M, n_head, n_kv_head, D, past_len, ctypes.byref(info)))
     return info
+
+
+def tree_masks(parents) -> tuple[np.ndarray, np.ndarray]:
+    """(masks uint64 [M, ceil(M/64)], depths int32 [M]) of a drafted tree: parents[m] is -1 (continues the context) or an earlier
+    row (host only)."""
+    p = np.ascontiguousarray(parents, dtype=np.int32)
+    M = p.size
+    masks, depths = np.empty((M, (M + 63) // 64), np.uint64), np.empty(M, np.int32)
+    _check(lib().ql_tree_masks(M, p.ctypes.data, masks.ctypes.data, depths.ctypes.data))
+    return masks, depths
+
+
+def offsets(offs):
+    """Offsets as the array that ql_kv_move takes; a program that moves often keeps it."""
+    return offs if isinstance(offs, ctypes.Array) else (ctypes.c_uint64 * len(offs))(*offs)
 
 
 def plan_batch(descs: list[GptqDesc], M: int) -> int:
@@ -406,6 +444,38 @@ class Context:
     def silu_mul(self, act: Arena, gate_off: int, up_off: int, n: int, y_off: int):
         """y = silu(gate) * up (activation/silu_mul.wgsl)."""
         _check(lib().ql_silu_mul(self.handle, act.handle, gate_off, up_off, n, y_off))
+
+    def rope_table(self, weights: Arena, table_off: int, max_pos: int, rot_dim: int, theta: float):
+        """Fills the fp32 [max_pos, rot_dim] table of cosines and sines (ropeHalfRef's angles, in fp64) in the weight arena."""
+        _check(lib().ql_rope_table(self.handle, weights.handle, table_off, max_pos, rot_dim, theta))
+
+    def qk_norm_rope(self, desc: RopeDesc, weights: Arena, act: Arena, q_off: int, k_off: int, v_off: int, pos_off: int, M: int,
+                     q_out_off: int, cache: Arena, k_cache_off: int, v_cache_off: int, max_t: int, slot0: int):
+        """q and k normed per head and turned by their rows' positions; q to q_out, k and v to cache rows slot0 + m."""
+        _check(lib().ql_qk_norm_rope(self.handle, ctypes.byref(desc), weights.handle, act.handle, q_off, k_off, v_off, pos_off, M,
+                                     q_out_off, cache.handle, k_cache_off, v_cache_off, max_t, slot0))
+
+    def attention_tree(self, act: Arena, q_off: int, cache: Arena, k_off: int, v_off: int, cache_dtype: int, max_t: int, M: int,
+                       n_head: int, n_kv_head: int, D: int, past_len: int, mask_off, out_off: int):
+        """GQA attention of M drafted rows over past_len cached positions and the drafted rows that the masks (tree_masks) name;
+        mask_off None: rows in order, causal."""
+        _check(lib().ql_attention_tree(self.handle, act.handle, q_off, cache.handle, k_off, v_off, cache_dtype, max_t, M, n_head,
+                                       n_kv_head, D, past_len, QL_NONE if mask_off is None else mask_off, out_off))
+
+    def token_logprobs(self, act: Arena, logits_off: int, stride: int, M: int, V: int, tokens_off: int, n_tok: int, top_k: int,
+                       logprob_off: int, entropy_off, top_id_off: int, top_logprob_off: int):
+        """Log probabilities of n_tok given tokens a row, the rows' entropies (entropy_off None: none) and top_k alternatives."""
+        _check(lib().ql_token_logprobs(self.handle, act.handle, logits_off, stride, M, V, tokens_off, n_tok, top_k, logprob_off,
+                                       QL_NONE if entropy_off is None else entropy_off, top_id_off, top_logprob_off))
+
+    def kv_move(self, dst: Arena, dst_offs, dst_max_t: int, src: Arena, src_offs, src_max_t: int, row_bytes: int, dst_row: int,
+                src_row: int, n: int, act: Arena | None = None, rows_off=None):
+        """Row dst_row + i of each region of dst = row src_row + rows[i] (without a list: src_row + i) of that of src, i < n."""
+        d, s = offsets(dst_offs), offsets(src_offs)
+        if len(d) != len(s):
+            raise ValueError(f"{len(d)} destination regions for {len(s)} source regions")
+        _check(lib().ql_kv_move(self.handle, dst.handle, d, dst_max_t, src.handle, s, src_max_t, len(d), row_bytes, dst_row, src_row, n,
+                                None if act is None else act.handle, QL_NONE if rows_off is None else rows_off))
 
     def unpack_f32(self, desc: GptqDesc, weights: Arena, out: Arena, out_off: int,
                    scales_dtype: int = DTYPE_F16):
