@@ -171,8 +171,12 @@ def _library():
 
 
 class _Bytes:
-    def __init__(self, address, shape, kind):
-        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": kind, "version": 3, "data": (address, False)}
+    """Memory of an arena, which lives as long as a tensor over it."""
+
+    def __init__(self, arena, off, shape, kind):
+        self.arena = arena
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": kind, "version": 3,
+                                         "data": (arena.device_ptr + off, False)}
 
 
 _KINDS = {torch.float32: "<f4", torch.float16: "<f2", torch.int32: "<i4", torch.int64: "<i8"}
@@ -190,7 +194,7 @@ class _Arena:
                 self.view(n, t.shape, t.dtype).copy_(t)
 
     def view(self, name, shape, dtype=torch.float32):
-        return torch.as_tensor(_Bytes(self.arena.device_ptr + self.off[name], shape, _KINDS[dtype]), device="cuda")
+        return torch.as_tensor(_Bytes(self.arena, self.off[name], shape, _KINDS[dtype]), device="cuda")
 
 
 class _Handles:
