@@ -2785,6 +2785,11 @@ int ql_attention_tree(ql_ctx* ctx, ql_arena* act, uint64_t q_off, const ql_arena
     a.words = words;
     a.half = cb == 2;
     a.scale = (float)(1.4426950408889634 / std::sqrt((double)D));
+    const uint64_t bytes = ql::plan_attention_tree(&a, ql::kAttnTileWsBytes);
+    std::lock_guard<std::mutex> guard(ctx->ws_lock);
+    void* ws;
+    QL_HIP(workspace(ctx, ctx->tile_ws, bytes, &ws));
+    a.ws = static_cast<float*>(ws);
     QL_HIP(ql::launch_attention_tree(a, ctx->stream));
     return QL_OK;
 }

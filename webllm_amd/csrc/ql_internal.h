@@ -321,9 +321,12 @@ struct TreeArgs {
     const void *k, *v;         // cache [max_t, KV * D], fp32 or fp16 (half)
     const uint64_t* mask;      // [M, words], or nullptr: row m sees the drafted rows 0..m
     float* out;                // [M, H, D]
+    float* ws;                 // key ranges' partials, as attn_kernel's
     int M, H, KV, G, D, past, words, half;
     float scale;               // fp32(log2(e) / sqrt(D))
+    int nt, groups, nsplit;    // plan_attention_tree: 16 nt pairs a workgroup, groups of them, key ranges
 };
+uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes);   // the workspace it needs
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t stream);
 
 constexpr int kLogprobMaxTop = 32;
