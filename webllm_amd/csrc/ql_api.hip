@@ -2827,7 +2827,11 @@ int ql_token_logprobs(ql_ctx* ctx, ql_arena* act, uint64_t logits_off, int32_t s
     a.V = V;
     a.n_tok = n_tok;
     a.top_k = top_k;
-    QL_HIP(ql::launch_token_logprobs(a, ctx->stream));
+    const uint64_t bytes = std::min<uint64_t>(ql::token_logprobs_bytes(M, V), ql::kAttnTileWsBytes);
+    std::lock_guard<std::mutex> guard(ctx->ws_lock);
+    void* ws;
+    QL_HIP(workspace(ctx, ctx->tile_ws, bytes, &ws));
+    QL_HIP(ql::launch_token_logprobs(a, ws, bytes, ctx->stream));
     return QL_OK;
 }
 

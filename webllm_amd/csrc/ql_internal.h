@@ -338,8 +338,13 @@ struct LogprobArgs {
     float* top_logprob;
     size_t stride;
     int M, V, n_tok, top_k;
+    // launch_token_logprobs fills these
+    int units;                 // of 1024 logits
+    float* stat;               // [M, units, 4]
+    uint64_t* best;            // [M, units, 4]
 };
-hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream);
+uint64_t token_logprobs_bytes(int M, int V);   // workspace of M rows in one go; a row needs 48 bytes per 1024 logits
+hipError_t launch_token_logprobs(LogprobArgs a, void* ws, size_t ws_bytes, hipStream_t stream);
 
 constexpr int kMoveInPlaceRows = 256;
 constexpr int kMoveMaxRegions = 128;   // regions of a launch, in its arguments

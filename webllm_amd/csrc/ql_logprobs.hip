@@ -4,6 +4,14 @@
 //   lse = m + ln sum e^(x - m),  log p(t) = x_t - lse,  H = ln S - (sum (x - m) e^(x - m)) / S,  S = sum e^(x - m)
 // with m the row's largest logit, so nothing cancels however large the logits are; -inf logits (a mask) add nothing. A
 // row without any other: log p = -inf, H = 0. Alternatives are ordered by value, equal ones by index.
+//
+// logprob_scan_kernel reads the logits, once: a wave has a unit of 1024 of a row in registers, and leaves the unit's (m, S, sum (x - m)
+// e^(x - m)) and, where alternatives are wanted, the largest (value, index) of each of its four parts of 256. No LDS, no barrier.
+// logprob_row_kernel joins a row's units, and finds the top k exactly from the parts' largest: a part whose largest is not
+// among the k largest of those has none of the top k (k others are larger), so the k parts that are hold them all; what
+// lies below the smallest of those k is left out, and the rest is sorted. Whatever the logits, that is k * 256 of them at most.
+// Bound: 4 bytes a logit from memory; with few rows the two launches and their chains of loads.
+#include <algorithm>
 #include <cmath>
 
 #include "ql_device.h"
@@ -14,102 +22,277 @@ namespace ql {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kUnit = 1024, kPart = 256, kParts = kUnit / kPart;   // logits of a wave, of its 16-lane rows
+constexpr int kWaves = 16;                                          // of a row's workgroup where alternatives are wanted
+constexpr float kLog2e = 1.4426950408889634f;
 
-// A logit's order and place as one unsigned number: larger logits first, of equal ones the lower index. NaN above all.
-__device__ __forceinline__ uint64_t order_key(float x, uint32_t index)
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // rows start at any multiple of 4 bytes
+
+// A logit's order and place as one unsigned number: larger logits first, of equal ones the lower index. NaN above all; 0: none.
+__device__ __forceinline__ uint32_t order_bits(float x)
 {
-    uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
-    b = x != x ? 0xFFFFFFFFu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
-    return (uint64_t)b << 32 | (uint32_t)~index;
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
+    return x != x ? 0xFFFFFFFFu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float value_of(uint64_t key)
+{
+    const uint32_t h = (uint32_t)(key >> 32);
+    return __builtin_bit_cast(float, h & 0x80000000u ? h ^ 0x80000000u : ~h);
+}
+__device__ __forceinline__ uint64_t key_of(uint32_t bits, uint32_t index) { return (uint64_t)bits << 32 | (uint32_t)~index; }
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) { return (uint64_t)__shfl_xor((unsigned long long)v, o); }
 
-__device__ __forceinline__ float reduce_max(float v, float* lds)
+__device__ __forceinline__ float wave_max(float v)
 {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = lds[0];
-    for (int i = 1; i < kThreads / 64; i++) v = fmaxf(v, lds[i]);
     return v;
 }
-
-__device__ __forceinline__ float reduce_sum(float v, float* lds)
+__device__ __forceinline__ float wave_sum(float v)
 {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = lds[0];
-    for (int i = 1; i < kThreads / 64; i++) v += lds[i];
     return v;
 }
 
-// one workgroup per row
-__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(const LogprobArgs a)
+// four logits from index i on; those past the row's end are -inf
+__device__ __forceinline__ f32x4 load4(const float* x, int i, int V)
 {
-    __shared__ float red[kThreads / 64];
-    __shared__ uint64_t best[kThreads / 64];
-    const int row = blockIdx.x, V = a.V, tid = threadIdx.x;
-    const float* x = a.logits + (size_t)row * a.stride;
-    float m = -INFINITY;
-    bool nan = false;
-    for (int i = tid; i < V; i += kThreads) {
-        m = fmaxf(m, x[i]);
-        nan |= x[i] != x[i];
+    if (i + 3 < V) {
+        const f32x4u v = *QL_GLOBAL(const f32x4u, x + i);
+        return f32x4{v.x, v.y, v.z, v.w};
     }
-    m = reduce_max(m, red);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f, t = 0.f;
-    for (int i = tid; i < V; i += kThreads) {
-        const float d = x[i] - ref, e = expf(d);
-        s += e;
-        t += d == -INFINITY ? 0.f : d * e;
-    }
-    s = reduce_sum(s, red);
-    t = reduce_sum(t, red);
-    if (__syncthreads_or(nan)) s = t = NAN;
-    const float ls = logf(s);
-    const bool none = s == 0.f;
-    if (tid == 0 && a.entropy) a.entropy[row] = none ? 0.f : ls - t / s;
-    for (int i = tid; i < a.n_tok; i += kThreads) {
-        const int tok = a.tokens[(size_t)row * a.n_tok + i];
-        a.logprob[(size_t)row * a.n_tok + i] = tok < 0 || tok >= V ? 0.f : none ? -INFINITY : x[tok] - ref - ls;
-    }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < a.top_k; k++) {
-        uint64_t b = 0;
-        for (int i = tid; i < V; i += kThreads) {
-            const uint64_t key = order_key(x[i], i);
-            if (key < last && key > b) b = key;
-        }
+    f32x4 v;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t other = __shfl_xor((unsigned long long)b, o);
-            b = b > other ? b : other;
+    for (int c = 0; c < 4; c++) v[c] = i + c < V ? ld_global(x + i + c) : -INFINITY;
+    return v;
+}
+
+template <bool TOP>
+__global__ __launch_bounds__(256) void logprob_scan_kernel(const LogprobArgs a)
+{
+    const int lane = threadIdx.x & 63, unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const size_t row = blockIdx.y;
+    if (unit >= a.units) return;
+    const float* x = a.logits + row * a.stride;
+    const int i0 = unit * kUnit + 4 * lane;
+    f32x4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) v[u] = load4(x, i0 + kPart * u, a.V);
+    float mx = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) mx = fmaxf(mx, v[u][c]);
+    const float m = wave_max(mx), ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f, t = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const float d = v[u][c] - ref, e = __builtin_amdgcn_exp2f(d * kLog2e);
+            s += e;
+            t += d == -INFINITY ? 0.f : d * e;
+        }
+    s = wave_sum(s);
+    t = wave_sum(t);
+    if (lane == 0) st_global(reinterpret_cast<f32x4*>(a.stat) + row * a.units + unit, f32x4{m, s, t, 0.f});
+    if (TOP) {
+        uint32_t best = 0, at = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int i = i0 + kPart * u + c;
+                const uint32_t b = i < a.V ? order_bits(v[u][c]) : 0u;
+                if (b > best) {
+                    best = b;
+                    at = i;
+                }
+            }
+        uint64_t key = best ? key_of(best, at) : 0;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) key = larger(key, shfl_xor64(key, o));
+        if ((lane & 15) == 0) st_global(a.best + (row * a.units + unit) * kParts + (lane >> 4), key);
+    }
+}
+
+// descending over the wave's lanes
+__device__ __forceinline__ uint64_t merge_step(uint64_t v, int lane, int j, bool down)
+{
+    const uint64_t o = shfl_xor64(v, j);
+    return ((lane & j) == 0) == down ? larger(v, o) : (v > o ? o : v);
+}
+__device__ __forceinline__ uint64_t sort64(uint64_t v, int lane)
+{
+#pragma unroll
+    for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+        for (int j = k >> 1; j > 0; j >>= 1) v = merge_step(v, lane, j, (lane & k) == 0);
+    return v;
+}
+// the largest 64 of two descending lists; b is the second one's from its end
+__device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b_reversed, int lane)
+{
+    uint64_t v = larger(a, b_reversed);
+#pragma unroll
+    for (int j = 32; j > 0; j >>= 1) v = merge_step(v, lane, j, true);
+    return v;
+}
+
+// The largest 64 of n keys, descending over wave 0's lanes: each wave sorts 64 at a time, the waves' lists are merged
+// through `list` [kWaves][64]. Every thread of the workgroup comes here.
+template <typename F>
+__device__ __forceinline__ uint64_t largest64(F key, int n, int k, uint64_t* list, int wave, int lane)
+{
+    uint64_t mine = 0;
+    for (int i0 = 64 * wave; i0 < n; i0 += 64 * kWaves) {
+        const uint64_t v = i0 + lane < n ? key(i0 + lane) : 0;
+        if (i0 == 64 * wave) {
+            mine = sort64(v, lane);
+        } else {
+            const uint64_t last = (uint64_t)__shfl((unsigned long long)mine, k - 1);
+            if (__any(v > last)) {
+                const uint64_t w = sort64(v, lane);
+                mine = merge64(mine, (uint64_t)__shfl((unsigned long long)w, 63 - lane), lane);
+            }
+        }
+    }
+    const int lists = min(kWaves, (n + 63) / 64);
+    if (wave < lists) list[64 * wave + lane] = mine;
+    __syncthreads();
+    for (int half = kWaves / 2; half > 0; half >>= 1) {
+        if (half >= lists) continue;                      // the same for every thread
+        if (wave < half && wave + half < lists) {
+            mine = merge64(mine, list[64 * (wave + half) + 63 - lane], lane);
+            list[64 * wave + lane] = mine;
         }
         __syncthreads();
-        if ((tid & 63) == 0) best[tid >> 6] = b;
-        __syncthreads();
-        for (int i = 0; i < kThreads / 64; i++) b = b > best[i] ? b : best[i];
-        last = b;
-        if (tid == 0) {
-            const int id = k < V ? (int)~(uint32_t)b : -1;
-            a.top_id[(size_t)row * a.top_k + k] = id;
-            a.top_logprob[(size_t)row * a.top_k + k] = id < 0 || none ? -INFINITY : x[id] - ref - ls;
+    }
+    return mine;
+}
+
+// A row's units joined by one wave: what log probabilities are measured from, and the tokens' and the entropy.
+__device__ __forceinline__ void join_units(const LogprobArgs& a, size_t row, int lane, float& ref, float& ls, bool& none)
+{
+    const f32x4* st = reinterpret_cast<const f32x4*>(a.stat) + row * a.units;
+    float m = -INFINITY;
+    for (int i = lane; i < a.units; i += 64) m = fmaxf(m, ld_global(st + i).x);
+    m = wave_max(m);
+    ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f, t = 0.f;
+    for (int i = lane; i < a.units; i += 64) {
+        const f32x4 u = ld_global(st + i);
+        const float d = u.x == -INFINITY ? 0.f : u.x - ref, e = __builtin_amdgcn_exp2f(d * kLog2e);
+        s = fmaf(u.y, e, s);
+        t += e == 0.f ? 0.f : fmaf(d, u.y, u.z) * e;      // d may be too far down for d * u.y
+    }
+    s = wave_sum(s);
+    t = wave_sum(t);
+    none = s == 0.f;
+    ls = logf(s);
+    if (lane == 0 && a.entropy) st_global(a.entropy + row, none ? 0.f : ls - t / s);
+    const float* x = a.logits + row * a.stride;
+    for (int i = lane; i < a.n_tok; i += 64) {
+        const int tok = ld_global(a.tokens + row * a.n_tok + i);
+        const bool there = tok >= 0 && tok < a.V;
+        st_global(a.logprob + row * a.n_tok + i, !there ? 0.f : none ? -INFINITY : ld_global(x + tok) - ref - ls);
+    }
+}
+
+__global__ __launch_bounds__(64) void logprob_row_kernel(const LogprobArgs a)
+{
+    float ref, ls;
+    bool none;
+    join_units(a, blockIdx.x, threadIdx.x, ref, ls, none);
+}
+
+__global__ __launch_bounds__(64 * kWaves) void logprob_top_kernel(const LogprobArgs a)
+{
+    __shared__ uint64_t list[64 * kWaves], found[kLogprobMaxTop * kPart];
+    __shared__ float norm[3];
+    __shared__ int count;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.top_k;
+    const size_t row = blockIdx.x;
+    if (wave == kWaves - 1) {
+        float ref, ls;
+        bool none;
+        join_units(a, row, lane, ref, ls, none);
+        if (lane == 0) {
+            norm[0] = ref;
+            norm[1] = ls;
+            norm[2] = none;
+            count = 0;
         }
+    }
+    const int parts = a.units * kParts;
+    const uint64_t* best = a.best + row * parts;
+    const uint64_t p = largest64([&](int i) { return ld_global(best + i); }, parts, k, list, wave, lane);
+    if (wave == 0) list[lane] = p;
+    __syncthreads();
+    const uint64_t least = list[k - 1] ? list[k - 1] : 1;
+    const float* x = a.logits + row * a.stride;
+    for (int q = wave; q < k; q += kWaves) {
+        const uint64_t key = list[q];
+        if (!key) continue;
+        const uint32_t at = ~(uint32_t)key;               // a part: 64 neighbours of each 256 of its unit
+        const int i0 = (at & ~(kUnit - 1u)) + kPart * (lane >> 4) + (at & 192u) + 4 * (lane & 15);
+        const f32x4 v = load4(x, i0, a.V);
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const uint64_t e = i0 + c < a.V ? key_of(order_bits(v[c]), i0 + c) : 0;
+            const uint64_t in = __ballot(e >= least);
+            if (!in) continue;
+            int base = 0;
+            if (lane == 0) base = atomicAdd(&count, __popcll(in));
+            base = __shfl(base, 0);
+            if (e >= least) found[base + __popcll(in & ((1ull << lane) - 1))] = e;
+        }
+    }
+    __syncthreads();
+    const int n = count;
+    const uint64_t top = largest64([&](int i) { return found[i]; }, n, k, list, wave, lane);
+    if (wave == 0 && lane < k) {
+        const bool none = norm[2] != 0.f;
+        st_global(a.top_id + row * k + lane, top ? (int)~(uint32_t)top : -1);
+        st_global(a.top_logprob + row * k + lane, !top || none ? -INFINITY : value_of(top) - norm[0] - norm[1]);
     }
 }
 
 }  // namespace
 
-hipError_t launch_token_logprobs(const LogprobArgs& a, hipStream_t stream)
+hipError_t launch_token_logprobs(LogprobArgs a, void* ws, size_t ws_bytes, hipStream_t stream)
 {
-    hipLaunchKernelGGL(token_logprobs_kernel, dim3(a.M), dim3(kThreads), 0, stream, a);
-    return hipGetLastError();
+    a.units = (a.V + kUnit - 1) / kUnit;
+    const size_t per = token_logprobs_bytes(1, a.V);
+    const int rows = (int)std::min<size_t>(a.M, ws_bytes / per);          // more rows go through the workspace in turn
+    a.stat = static_cast<float*>(ws);
+    a.best = reinterpret_cast<uint64_t*>(static_cast<char*>(ws) + (size_t)rows * a.units * 16);
+    const int M = a.M;
+    for (int m = 0; m < M; m += rows) {
+        a.M = std::min(rows, M - m);
+        const dim3 grid((a.units + 3) / 4, a.M);
+        if (a.top_k) {
+            hipLaunchKernelGGL(logprob_scan_kernel<true>, grid, dim3(256), 0, stream, a);
+            hipLaunchKernelGGL(logprob_top_kernel, dim3(a.M), dim3(64 * kWaves), 0, stream, a);
+        } else {
+            hipLaunchKernelGGL(logprob_scan_kernel<false>, grid, dim3(256), 0, stream, a);
+            hipLaunchKernelGGL(logprob_row_kernel, dim3(a.M), dim3(64), 0, stream, a);
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        a.logits += (size_t)a.M * a.stride;
+        a.tokens += (size_t)a.M * a.n_tok;
+        a.logprob += (size_t)a.M * a.n_tok;
+        if (a.entropy) a.entropy += a.M;
+        a.top_id += (size_t)a.M * a.top_k;
+        a.top_logprob += (size_t)a.M * a.top_k;
+    }
+    return hipSuccess;
 }
+
+// a unit's sums and its parts' largest
+uint64_t token_logprobs_bytes(int M, int V) { return (uint64_t)M * ((V + kUnit - 1) / kUnit) * (16 + 8 * kParts); }
 
 }  // namespace ql
