@@ -34,6 +34,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTreeWorkgroups = 512;     // two per CU
 constexpr int kTreeMaxSplit = 128;
+constexpr int kKeys = 32;                // keys of a block
 constexpr float kPScale = 16384.f;       // fp16 parts of P: 2^14 P
 constexpr float kMaxFinite = 3.4028235e38f;
 
@@ -42,16 +43,28 @@ __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x)
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return mfma_16x16x32_f16(a, b, c); }
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// x = p[0] + p[1] + p[2], each the nearest bf16 of what the ones before leave
+// x = p[0] + p[1] + p[2], exactly: each part the first eight bits of what the ones before leave (5.5 instructions a value; the
+// nearest ones instead of the first took 8.4, since conversions come in pairs)
 __device__ __forceinline__ void split_bf16(const float (&x)[8], bf16x8 (&p)[3])
 {
+    u32x4 w[3];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        p[0][e] = (__bf16)x[e];
-        const float r = x[e] - (float)p[0][e];
-        p[1][e] = (__bf16)r;
-        p[2][e] = (__bf16)(r - (float)p[1][e]);
+    for (int e = 0; e < 4; e++) {
+        uint32_t b[2][3];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            float r = x[2 * e + k];
+#pragma unroll
+            for (int i = 0; i < 3; i++) {
+                b[k][i] = __builtin_bit_cast(uint32_t, r);
+                if (i < 2) r -= __builtin_bit_cast(float, b[k][i] & 0xFFFF0000u);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 3; i++) w[i][e] = __builtin_amdgcn_perm(b[1][i], b[0][i], 0x07060302u);
     }
+#pragma unroll
+    for (int i = 0; i < 3; i++) p[i] = __builtin_bit_cast(bf16x8, w[i]);
 }
 
 // the six products of three parts, the small ones first; the largest is the caller's
@@ -67,9 +80,8 @@ __device__ __forceinline__ f32x4 small_products(const bf16x8 (&a)[3], const bf16
 template <typename T, int DP, int NT, bool FULL>
 struct TreeTile {
     static constexpr bool kHalf = std::is_same<T, _Float16>::value;
-    static constexpr int kKeys = 32;                        // keys of a block
     static constexpr bool kAhead = DP <= 128;               // a block's K is loaded before the last one's V is used, V before K is
-    static constexpr int kNK = kKeys / 16, kNH = kKeys / 32;
+    static constexpr int kNK = kKeys / 16, kNH = 1;
     static constexpr int kTD = DP / 32, kDT = DP / 16;
     static constexpr int kParts = kHalf ? 2 : 3;            // of q
     static constexpr int kCols = kHalf && DP >= 128 ? 8 : 4;   // columns of V a lane loads at once
@@ -87,37 +99,46 @@ struct TreeTile {
     static __device__ __forceinline__ int kcol(int t, int g, int e) { return kHalf ? 32 * t + 8 * g + e : 32 * t + 16 * (e >> 2) + 4 * g + (e & 3); }
 };
 
-// A block's first key, its number of keys, and which of them pair row m sees.
+// A block of up to 32 keys, all of them in the context or all drafted. It is read as the 32 keys from `at` on, which all
+// exist (the call has that many): where the last keys are fewer, those before them come along unseen.
 struct TreeBlock {
-    int base, n, j0;                                        // j0: the first drafted row, or -1 in the context
+    int base, n, j0, at;                                    // j0: the first drafted row, or -1 in the context
 };
-template <int KEYS>
 __device__ __forceinline__ TreeBlock tree_block(const TreeArgs& a, int b, int past_blocks)
 {
     TreeBlock k;
     if (b < past_blocks) {
-        k.base = b * KEYS;
-        k.n = min(KEYS, a.past - k.base);
+        k.base = b * kKeys;
+        k.n = min(kKeys, a.past - k.base);
         k.j0 = -1;
     } else {
-        k.j0 = (b - past_blocks) * KEYS;
+        k.j0 = (b - past_blocks) * kKeys;
         k.base = a.past + k.j0;
-        k.n = min(KEYS, a.M - k.j0);
+        k.n = min(kKeys, a.M - k.j0);
     }
+    k.at = min(k.base, a.past + a.M - kKeys);
     return k;
 }
-__device__ __forceinline__ uint64_t low_bits(int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; }
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : (1ull << n) - 1; }   // n < 64
+// which of the keys from k.base on query row m sees
 __device__ __forceinline__ uint64_t seen_bits(const TreeArgs& a, const TreeBlock& k, int m)
 {
     if (k.j0 < 0) return low_bits(k.n);
-    const uint64_t w = a.mask ? ld_global(a.mask + (size_t)m * a.words + (k.j0 >> 6)) >> (k.j0 & 63) : low_bits(m - k.j0 + 1);
+    const uint64_t w = a.mask ? ld_global(a.mask + (size_t)m * a.words + (k.j0 >> 6)) >> (k.j0 & 63) : low_bits(min(m - k.j0 + 1, kKeys));
     return w & low_bits(k.n);
+}
+// the row of q and out of pair r of kv head kvh, and its query row m
+__device__ __forceinline__ int pair_row(const TreeArgs& a, int kvh, int r, int& m)
+{
+    r = min(r, a.M * a.G - 1);
+    m = (int)(((float)r + 0.5f) * a.inv_g);                 // r / G, exact: r < 2^20
+    return m * a.H + kvh * a.G + (r - m * a.G);
 }
 
 // The wave's blocks on the VALU, in the layout of the kernel below.
 template <typename T, int DP, int NT, bool FULL>
-__device__ __attribute__((noinline)) void tree_again(const TreeArgs& a, int kvh, int first, int end, int past_blocks, const int (&qrow)[NT], const int (&qm)[NT],
-                                                     float (&mr)[NT], float (&l)[NT], f32x4 (&acc)[DP / 16][NT])
+__device__ __forceinline__ void tree_again(const TreeArgs& a, int kvh, int r0, int first, int end, int past_blocks, float (&mr)[NT], float (&l)[NT],
+                                                     f32x4 (&acc)[DP / 16][NT])
 {
     using C = TreeTile<T, DP, NT, FULL>;
     const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
@@ -132,11 +153,12 @@ __device__ __attribute__((noinline)) void tree_again(const TreeArgs& a, int kvh,
         for (int d = 0; d < C::kDT; d++) acc[d][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     for (int b = first; b < end; b += 4) {
-        const TreeBlock blk = tree_block<C::kKeys>(a, b, past_blocks);
+        const TreeBlock blk = tree_block(a, b, past_blocks);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const uint64_t seen = seen_bits(a, blk, qm[nt]);
-            const float* q = a.q + (size_t)qrow[nt] * a.D;
+            int m;
+            const float* q = a.q + (size_t)pair_row(a, kvh, r0 + 16 * nt + i16, m) * a.D;
+            const uint64_t seen = seen_bits(a, blk, m);
             // four of the block's keys per lane and 16; then each lane takes all of them to its columns
 #pragma unroll 1
             for (int kt = 0; kt < C::kNK; kt++) {
@@ -197,81 +219,104 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
     using C = TreeTile<T, DP, NT, FULL>;
     using Frag = typename C::Frag;
     __shared__ __attribute__((aligned(16))) char lds[C::kLds];
-    __shared__ float qscale[C::kRows], stat[2][4][C::kRows];
+    __shared__ float qmax[C::kHalf ? C::kTD : 1][C::kRows], stat[2][4][C::kRows], row_inv[C::kRows];
+    __shared__ int row_at[C::kRows];
     const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kvh = blockIdx.x % a.KV, split = blockIdx.x / a.KV, rg = blockIdx.y;
-    const int R = a.M * a.G, D = a.D, last_key = a.past + a.M - 1;
-    const int past_blocks = (a.past + C::kKeys - 1) / C::kKeys, blocks = past_blocks + (a.M + C::kKeys - 1) / C::kKeys;
-    const int per = (blocks + a.nsplit - 1) / a.nsplit;
-    const int b0 = min(blocks, split * per), b1 = min(blocks, b0 + per);
+    // Workgroups go to the eight XCDs in turn. The groups of pairs that read the same keys, (kv head, range) number p, are to
+    // share one's L2: x = 8 * group + p % 8, y = p / 8. A kv head's keys lie in a few of the L2's channels (row stride), so an
+    // XCD has ranges of all the kv heads (of one only: 24 rows after 4000 keys 44 us for 33).
+    const int p = 8 * blockIdx.y + (blockIdx.x & 7), rg = blockIdx.x >> 3;
+    if (p >= a.KV * a.nsplit) return;
+    const int kvh = __builtin_amdgcn_readfirstlane((int)(((float)p + 0.5f) * a.inv_nsplit)), split = p - kvh * a.nsplit;   // exact: p < 2^19
+    const int R = a.M * a.G, D = a.D;
+    const int past_blocks = a.past_blocks, blocks = a.blocks, b0 = split * a.per, b1 = min(blocks, b0 + a.per);
     const size_t row_len = (size_t)a.KV * D;
     const T* kb = static_cast<const T*>(a.k) + (size_t)kvh * D;
     const T* vb = static_cast<const T*>(a.v) + (size_t)kvh * D;
-    auto pair_row = [&](int r, int& m) {                    // pair r of this kv head as a row of q and out
-        m = r / a.G;
-        return m * a.H + kvh * a.G + (r - m * a.G);
-    };
 
+    // q's fragments (t, nt): a wave has some whole, lane (i, g) eight values of pair i's row
+    constexpr int kUnits = (C::kTD * NT + 3) / 4;
+    float qv[kUnits][8];
+#pragma unroll
+    for (int k = 0; k < kUnits; k++) {
+        const int u = wave + 4 * k, t = u / NT, nt = u % NT;
+        int m;
+        const float* q = a.q + (size_t)pair_row(a, kvh, rg * C::kRows + 16 * nt + i16, m) * D;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int d = C::kcol(t, g, 4 * h);
+            const f32x4 y = u < C::kTD * NT && (FULL || d < D) ? ld_global(reinterpret_cast<const f32x4*>(q + d)) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; e++) qv[k][4 * h + e] = y[e];
+        }
+    }
     // K of the wave's first block is on its way while q's parts are made
     typename std::conditional<C::kHalf, u32x4, f32x4>::type kraw[C::kNK][C::kTD * (C::kHalf ? 1 : 2)];
+    // from an address that the whole wave shares and a lane's own offset
+    const uint32_t row_bytes = (uint32_t)(row_len * sizeof(T));
+    const uint32_t k_lane = (uint32_t)i16 * row_bytes + (C::kHalf ? 8 : 4) * g * (uint32_t)sizeof(T);
+    const uint32_t v_lane = 4u * g * row_bytes + C::kCols * i16 * (uint32_t)sizeof(T);
     auto load_k = [&](const TreeBlock& blk, int from, int to) {
+        const char* base = reinterpret_cast<const char*>(kb + (size_t)blk.at * row_len);
 #pragma unroll
         for (int kt = from; kt < to; kt++) {
-            const T* p = kb + (size_t)min(blk.base + 16 * kt + i16, last_key) * row_len;
+            const char* p = base + (size_t)(16 * kt) * row_bytes;
 #pragma unroll
             for (int t = 0; t < C::kTD; t++)
                 if constexpr (C::kHalf) {
-                    const int d = 32 * t + 8 * g;
-                    kraw[kt][t] = FULL || d < D ? ld_global(reinterpret_cast<const u32x4*>(p + d)) : u32x4{0, 0, 0, 0};
+                    kraw[kt][t] = FULL || 32 * t + 8 * g < D ? ld_global(reinterpret_cast<const u32x4*>(p + 64 * t + k_lane)) : u32x4{0, 0, 0, 0};
                 } else {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int d = 32 * t + 16 * h + 4 * g;
-                        kraw[kt][2 * t + h] = FULL || d < D ? ld_global(reinterpret_cast<const f32x4*>(p + d)) : f32x4{0.f, 0.f, 0.f, 0.f};
-                    }
+                    for (int h = 0; h < 2; h++)
+                        kraw[kt][2 * t + h] = FULL || 32 * t + 16 * h + 4 * g < D ? ld_global(reinterpret_cast<const f32x4*>(p + 128 * t + 64 * h + k_lane))
+                                                                                 : f32x4{0.f, 0.f, 0.f, 0.f};
                 }
         }
     };
+    auto drop_k = [&](int from, int to) {                   // no value: the last block's is not carried along
+#pragma unroll
+        for (int kt = from; kt < to; kt++)
+#pragma unroll
+            for (auto& x : kraw[kt]) x = __builtin_nondeterministic_value(x);
+    };
     int b = b0 + wave;
-    TreeBlock blk = tree_block<C::kKeys>(a, min(b, blocks - 1), past_blocks);
+    TreeBlock blk = tree_block(a, min(b, blocks - 1), past_blocks);
     if (C::kAhead && b < b1) load_k(blk, 0, C::kNK);
 
-    // q's parts as fragments in LDS: unit (t, nt, part), lane (i, g)
+    // q's parts as fragments in LDS: (t, nt, part), lane (i, g)
     Frag* qf = reinterpret_cast<Frag*>(lds);
     if (C::kHalf) {
-        constexpr int P = 256 / C::kRows;                   // threads a row
-        int m;
-        const float* q = a.q + (size_t)pair_row(min(rg * C::kRows + tid / P, R - 1), m) * D;
-        float mx = 0.f;
-        for (int d = 4 * (tid % P); d < D; d += 4 * P) {
-            const f32x4 x = ld_global(reinterpret_cast<const f32x4*>(q + d));
-            mx = fmaxf(fmaxf(mx, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-        }
 #pragma unroll
-        for (int o = 1; o < P; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        if (tid % P == 0) qscale[tid / P] = mx > 0.f && mx <= kMaxFinite ? ldexpf(1.f, min(100, 14 - ilogbf(mx))) : 1.f;
+        for (int k = 0; k < kUnits; k++) {
+            const int u = wave + 4 * k;
+            float mx = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[k][e]));
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (g == 0 && u < C::kTD * NT) qmax[u / NT][16 * (u % NT) + i16] = mx;
+        }
         __syncthreads();
     }
-    for (int u = tid; u < C::kTD * NT * 64; u += 256) {
-        const int ln = u & 63, t = (u >> 6) / NT, nt = (u >> 6) % NT, row = 16 * nt + (ln & 15);
-        int m;
-        const float* q = a.q + (size_t)pair_row(min(rg * C::kRows + row, R - 1), m) * D;
-        float x[8];
+    // a row's power of two: its largest value to [2^14, 2^15)
+    auto q_scale = [&](int row) {
+        float mx = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int d = C::kcol(t, ln >> 4, 4 * h);
-            const f32x4 y = FULL || d < D ? ld_global(reinterpret_cast<const f32x4*>(q + d)) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < C::kTD; t++) mx = fmaxf(mx, qmax[t][row]);
+        return mx > 0.f && mx <= kMaxFinite ? ldexpf(1.f, min(100, 14 - ilogbf(mx))) : 1.f;
+    };
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[4 * h + e] = y[e];
-        }
-        Frag* dst = qf + (size_t)(u >> 6) * C::kParts * 64 + ln;
+    for (int k = 0; k < kUnits; k++) {
+        const int u = wave + 4 * k;
+        if (u >= C::kTD * NT) break;
+        Frag* dst = qf + (size_t)u * C::kParts * 64 + lane;
         if constexpr (C::kHalf) {
-            const float s = qscale[row];
+            const float s = q_scale(16 * (u % NT) + i16);
             f16x8 hi, lo;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float y = x[e] * s;
+                const float y = qv[k][e] * s;
                 hi[e] = (_Float16)y;
                 lo[e] = (_Float16)((y - (float)hi[e]) * 2048.f);
             }
@@ -279,15 +324,15 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
             dst[64] = lo;
         } else {
             bf16x8 p[3];
-            split_bf16(x, p);
+            split_bf16(qv[k], p);
             dst[0] = p[0];
             dst[64] = p[1];
             dst[128] = p[2];
         }
     }
-    int qrow[NT], qm[NT];
+    int qm[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) qrow[nt] = pair_row(min(rg * C::kRows + 16 * nt + i16, R - 1), qm[nt]);
+    for (int nt = 0; nt < NT; nt++) pair_row(a, kvh, rg * C::kRows + 16 * nt + i16, qm[nt]);
     __syncthreads();
 
     f32x4 acc[C::kDT][NT];
@@ -296,7 +341,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
     for (int nt = 0; nt < NT; nt++) {
         mr[nt] = -INFINITY;
         l[nt] = 0.f;
-        f[nt] = C::kHalf ? fmaxf(a.scale / qscale[16 * nt + i16], 1.17549435e-38f) : a.scale;
+        f[nt] = C::kHalf ? fmaxf(a.scale / q_scale(16 * nt + i16), 1.17549435e-38f) : a.scale;
 #pragma unroll
         for (int d = 0; d < C::kDT; d++) acc[d][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -304,18 +349,17 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
     for (; b < b1; b += 4) {
         typename C::VRaw vraw[C::kNH][8][C::kNC];           // [32 keys][element of the fragment][columns]
         auto load_v = [&](const TreeBlock& blk, int c0, int c1) {
+            const char* base = reinterpret_cast<const char*>(vb + (size_t)blk.at * row_len);
 #pragma unroll
-            for (int h = 0; h < C::kNH; h++)
+            for (int e = 0; e < 8; e++) {
+                const char* p = base + (size_t)(16 * (e >> 2) + (e & 3)) * row_bytes;      // 4 g keys more in group g
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const T* p = vb + (size_t)min(blk.base + 32 * h + 16 * (e >> 2) + 4 * g + (e & 3), last_key) * row_len;
-#pragma unroll
-                    for (int c = c0; c < c1; c++) {
-                        const int d = C::kChunk * c + C::kCols * i16;
-                        if (FULL || d < D) vraw[h][e][c] = ld_global(reinterpret_cast<const typename C::VRaw*>(p + d));
-                        else vraw[h][e][c] = typename C::VRaw{};
-                    }
+                for (int c = c0; c < c1; c++) {
+                    if (FULL || C::kChunk * c + C::kCols * i16 < D)
+                        vraw[0][e][c] = ld_global(reinterpret_cast<const typename C::VRaw*>(p + C::kChunk * c * sizeof(T) + v_lane));
+                    else vraw[0][e][c] = typename C::VRaw{};
                 }
+            }
         };
         f32x4 s[C::kNK][NT];
 #pragma unroll
@@ -323,7 +367,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
             if (!C::kAhead) load_k(blk, kt, kt + 1);
             if (C::kAhead && kt == 1) {
                 __builtin_amdgcn_sched_barrier(0);          // not before the first keys' registers are free
-                load_v(blk, 0, C::kNC);
+                load_v(blk, 0, 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (C::kHalf) {
@@ -360,6 +404,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
                         lo[nt] = small_products(kp, qp, lo[nt]);
                     }
                     kh[t] = kp[0];
+                    __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
@@ -373,19 +418,18 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
                 }
             }
         }
-        const TreeBlock now = blk;
-        if (b + 4 < b1) {
-            blk = tree_block<C::kKeys>(a, b + 4, past_blocks);
-            if (C::kAhead) {
-                __builtin_amdgcn_sched_barrier(0);
-                load_k(blk, 0, C::kNK);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        if (C::kAhead && C::kNC > 1) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(blk, 1, C::kNC);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (now.j0 >= 0 || now.n < C::kKeys) {
+        const TreeBlock now = blk;
+        const bool more = b + 4 < b1;
+        if (more) blk = tree_block(a, b + 4, past_blocks);
+        if (now.j0 >= 0 || now.n < kKeys) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const uint64_t seen = seen_bits(a, now, qm[nt]) >> (4 * g);
+                const uint32_t seen = (uint32_t)(seen_bits(a, now, qm[nt]) << (now.base - now.at)) >> (4 * g);
 #pragma unroll
                 for (int kt = 0; kt < C::kNK; kt++)
 #pragma unroll
@@ -441,6 +485,13 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
 #pragma unroll
         for (int c = 0; c < C::kNC; c++) {
             if (!C::kAhead) load_v(now, c, c + 1);
+            if (C::kAhead && c < 2) {                       // the next K: in halves, the second in the first columns' registers
+                constexpr bool whole = C::kNC == 1;
+                __builtin_amdgcn_sched_barrier(0);
+                if (c == 0 && more) load_k(blk, 0, whole ? 2 : 1);
+                else if (c == 0) drop_k(0, whole ? 2 : 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int j = 0; j < C::kCols; j++) {
                 f32x4 o[NT];
@@ -473,7 +524,13 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) acc[c * C::kCols + j][nt] += o[nt];
+                if (!C::kHalf) __builtin_amdgcn_sched_barrier(0);   // parts of more tiles at once would spill
             }
+        }
+        if (C::kAhead && C::kNC > 1) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_k(blk, 1, 2);
+            else drop_k(1, 2);
         }
     }
     float odd = 0.f;                                        // NaN if a sum is not finite
@@ -486,24 +543,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
             for (int r = 0; r < 4; r++) odd = fmaf(acc[d][nt][r], 0.f, odd);
     }
     const bool redo = __any(odd != 0.f);
-    if (redo) {                                             // through copies: the sums themselves stay in registers
-        int row[NT], m[NT];
-        float mx[NT], sum[NT];
-        f32x4 o[C::kDT][NT];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            row[nt] = qrow[nt];
-            m[nt] = qm[nt];
-        }
-        tree_again<T, DP, NT, FULL>(a, kvh, first, b1, past_blocks, row, m, mx, sum, o);
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            mr[nt] = mx[nt];
-            l[nt] = sum[nt];
-#pragma unroll
-            for (int d = 0; d < C::kDT; d++) acc[d][nt] = o[d][nt];
-        }
-    }
+    if (redo) tree_again<T, DP, NT, FULL>(a, kvh, rg * C::kRows, first, b1, past_blocks, mr, l, acc);
 
     // the four waves' states
     const float unit = C::kHalf && !redo ? 1.f / kPScale : 1.f;
@@ -523,9 +563,27 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
     for (int nt = 0; nt < NT; nt++) {
         const int r = 16 * nt + i16;
         const float mx = fmaxf(fmaxf(stat[0][0][r], stat[0][1][r]), fmaxf(stat[0][2][r], stat[0][3][r]));
-        w[nt] = mr[nt] == -INFINITY ? 0.f : ex2(mr[nt] - mx) * unit;
-        if (mr[nt] == -INFINITY && l[nt] != l[nt]) w[nt] = 1.f;   // scores that are all NaN
+        w[nt] = mr[nt] == -INFINITY ? (l[nt] != l[nt] ? 1.f : 0.f) : ex2(mr[nt] - mx) * unit;   // NaN: no score is a number
     }
+    if (tid < C::kRows) {                                   // what a row's sums are divided by, or its state, and its place
+        const int r = rg * C::kRows + tid;
+        const float mx = fmaxf(fmaxf(stat[0][0][tid], stat[0][1][tid]), fmaxf(stat[0][2][tid], stat[0][3][tid]));
+        float total = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float lk = stat[1][k][tid], mk = stat[0][k][tid];
+            total += mk == -INFINITY ? (lk != lk ? lk : 0.f) : lk * ex2(mk - mx);
+        }
+        int m;
+        const int at = pair_row(a, kvh, r, m);
+        row_at[tid] = r < R ? at : -1;
+        row_inv[tid] = a.nsplit > 1 ? 1.f : total == 0.f ? 0.f : 1.f / total;
+        if (a.nsplit > 1 && r < R) {
+            f32x2* st = reinterpret_cast<f32x2*>(a.ws + (size_t)a.M * a.H * a.nsplit * D) + (size_t)at * a.nsplit + split;
+            st_global(st, f32x2{mx, total});
+        }
+    }
+    float* const out = a.nsplit > 1 ? a.ws + (size_t)split * D : a.out;
 #pragma unroll
     for (int c = 0; c < C::kNC; c++) {
         if (c) __syncthreads();
@@ -543,35 +601,57 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
                 }
         }
         __syncthreads();
+#pragma unroll
         for (int u = tid; u < C::kRows * (C::kChunk / 4); u += 256) {
-            const int row = u / (C::kChunk / 4), c4 = u % (C::kChunk / 4), d = C::kChunk * c + 4 * c4, r = rg * C::kRows + row;
-            if (r >= R || (!FULL && d >= D)) continue;
+            const int row = u / (C::kChunk / 4), c4 = u % (C::kChunk / 4), d = C::kChunk * c + 4 * c4, at = row_at[row];
+            if (at < 0 || (!FULL && d >= D)) continue;
             f32x4 sum = *reinterpret_cast<const f32x4*>(merge + (size_t)row * C::kMergeStride + 4 * c4);
 #pragma unroll
             for (int k = 1; k < 4; k++) sum += *reinterpret_cast<const f32x4*>(merge + (size_t)(k * C::kRows + row) * C::kMergeStride + 4 * c4);
-            const float mx = fmaxf(fmaxf(stat[0][0][row], stat[0][1][row]), fmaxf(stat[0][2][row], stat[0][3][row]));
-            float total = 0.f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float lk = stat[1][k][row], mk = stat[0][k][row];
-                total += mk == -INFINITY ? (lk != lk ? lk : 0.f) : lk * ex2(mk - mx);
-            }
-            int m;
-            const size_t at = pair_row(r, m);
-            if (a.nsplit == 1) {
-                const float inv = total == 0.f ? 0.f : 1.f / total;
-                st_global(reinterpret_cast<f32x4*>(a.out + at * D + d), f32x4{sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv});
-            } else {
-                const size_t slot = at * a.nsplit + split;
-                st_global(reinterpret_cast<f32x4*>(a.ws + slot * D + d), sum);
-                if (d == 0) {
-                    float* st = a.ws + (size_t)a.M * a.H * a.nsplit * D + 2 * slot;
-                    st_global(st, mx);
-                    st_global(st + 1, total);
-                }
-            }
+            const float inv = row_inv[row];
+            st_global(reinterpret_cast<f32x4*>(out + (size_t)at * a.nsplit * D + d), f32x4{sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv});
         }
     }
+}
+
+// Fewer keys than a block: one wave per (row, head), a lane's own key for the scores, its own values of D for the sums
+template <typename T>
+__global__ __launch_bounds__(64) void attn_tree_row_kernel(const TreeArgs a)
+{
+    __shared__ float q[256];
+    const int h = blockIdx.x, m = blockIdx.y, lane = threadIdx.x, D = a.D, T0 = a.past + a.M, j = lane - a.past;
+    const size_t row = (size_t)m * a.H + h, row_len = (size_t)a.KV * D;
+    const T* k = static_cast<const T*>(a.k) + (size_t)(h / a.G) * D;
+    const T* v = static_cast<const T*>(a.v) + (size_t)(h / a.G) * D;
+    for (int d = lane; d < D; d += 64) q[d] = ld_global(a.q + row * D + d);
+    __syncthreads();
+    bool seen = lane < T0;
+    if (seen && j >= 0) seen = a.mask ? ld_global(a.mask + (size_t)m * a.words) >> j & 1 : j <= m;
+    float sc = -INFINITY;
+    if (seen) {
+        sc = 0.f;
+#pragma unroll 8
+        for (int d = 0; d < D; d++) sc = fmaf(q[d], (float)k[(size_t)lane * row_len + d], sc);
+        sc *= a.scale;
+    }
+    float mx = sc;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    const float p = seen ? ex2(sc - (mx == -INFINITY ? 0.f : mx)) : 0.f;
+    float l = p, acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+    const uint64_t all = __ballot(seen);
+    for (int s = 0; s < T0; s++) {
+        if (!(all >> s & 1)) continue;
+        const float w = __shfl(p, s);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (lane + 64 * i < D) acc[i] = fmaf(w, (float)v[(size_t)s * row_len + lane + 64 * i], acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (lane + 64 * i < D) st_global(a.out + row * D + lane + 64 * i, l == 0.f ? 0.f : acc[i] / l);
 }
 
 // out = sum_i acc_i 2^(m_i - m) / sum_i l_i 2^(m_i - m) over the key ranges, a workgroup a row: the ranges' weights in
@@ -644,22 +724,32 @@ TreeFn tree_fn(int D, int nt)
 
 uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes)
 {
-    const int R = a->M * a->G, keys = 32;
+    const int R = a->M * a->G;
+    a->nsplit = 1;
+    if (a->past + a->M < kKeys) return 0;
     a->nt = (a->D == 64 || a->D == 128) && R > 16 ? 2 : 1;
     a->groups = (R + 16 * a->nt - 1) / (16 * a->nt);
-    const int blocks = (a->past + keys - 1) / keys + (a->M + keys - 1) / keys;
+    a->past_blocks = (a->past + kKeys - 1) / kKeys;
+    const int blocks = a->blocks = a->past_blocks + (a->M + kKeys - 1) / kKeys;
     const size_t one = (size_t)a->M * a->H * (a->D + 2) * sizeof(float);
     // key ranges up to two workgroups a CU, of at least a block a wave, as many as the workspace holds
     const int s = std::max(1, std::min({kTreeWorkgroups / (a->groups * a->KV), (blocks + 3) / 4, kTreeMaxSplit, (int)std::min<size_t>(kTreeMaxSplit, ws_bytes / one)}));
-    const int per = (blocks + s - 1) / s;
-    a->nsplit = (blocks + per - 1) / per;
+    a->per = ((blocks + s - 1) / s + 3) / 4 * 4;            // as many for each of the waves
+    a->nsplit = (blocks + a->per - 1) / a->per;
+    a->inv_nsplit = 1.f / a->nsplit;
+    a->inv_g = 1.f / a->G;
     return a->nsplit == 1 ? 0 : a->nsplit * one;
 }
 
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t stream)
 {
+    if (a.past + a.M < kKeys) {
+        if (a.half) hipLaunchKernelGGL(attn_tree_row_kernel<_Float16>, dim3(a.H, a.M), dim3(64), 0, stream, a);
+        else hipLaunchKernelGGL(attn_tree_row_kernel<float>, dim3(a.H, a.M), dim3(64), 0, stream, a);
+        return hipGetLastError();
+    }
     const TreeFn fn = a.half ? tree_fn<_Float16>(a.D, a.nt) : tree_fn<float>(a.D, a.nt);
-    hipLaunchKernelGGL(fn, dim3(a.nsplit * a.KV, a.groups), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(fn, dim3(8 * a.groups, (a.KV * a.nsplit + 7) / 8), dim3(256), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
     hipLaunchKernelGGL(attn_tree_merge_kernel, dim3(a.H, a.M), dim3(256), 0, stream, a);

@@ -324,7 +324,9 @@ struct TreeArgs {
     float* ws;                 // key ranges' partials, as attn_kernel's
     int M, H, KV, G, D, past, words, half;
     float scale;               // fp32(log2(e) / sqrt(D))
-    int nt, groups, nsplit;    // plan_attention_tree: 16 nt pairs a workgroup, groups of them, key ranges
+    // plan_attention_tree fills these: 16 nt pairs a workgroup, groups of them; blocks of 32 keys, key ranges of `per` of them
+    int nt, groups, past_blocks, blocks, per, nsplit;
+    float inv_nsplit, inv_g;
 };
 uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes);   // the workspace it needs
 hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t stream);
