@@ -25,6 +25,7 @@
 #include "ql_device.h"
 #include "ql_digits.h"
 #include "ql_internal.h"
+#include "ql_lanes.h"
 
 namespace ql {
 
@@ -179,8 +180,7 @@ __device__ __forceinline__ void tree_again(const TreeArgs& a, int kvh, int r0, i
                     s[3] = r == 3 ? sc : s[3];
                     bm = fmaxf(bm, sc);
                 }
-                bm = fmaxf(bm, __shfl_xor(bm, 16));
-                bm = fmaxf(bm, __shfl_xor(bm, 32));
+                bm = pair_max<32>(pair_max<16>(bm));
                 const float mn = fmaxf(mr[nt], bm), ref = mn == -INFINITY ? 0.f : mn, al = ex2(mr[nt] - ref);
                 mr[nt] = mn;
                 l[nt] *= al;
@@ -293,8 +293,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
             float mx = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[k][e]));
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            mx = pair_max<32>(pair_max<16>(mx));
             if (g == 0 && u < C::kTD * NT) qmax[u / NT][16 * (u % NT) + i16] = mx;
         }
         __syncthreads();
@@ -446,8 +445,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
             for (int kt = 0; kt < C::kNK; kt++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) bm = fmaxf(bm, s[kt][nt][r]);
-            bm = fmaxf(bm, __shfl_xor(bm, 16));
-            bm = fmaxf(bm, __shfl_xor(bm, 32));
+            bm = pair_max<32>(pair_max<16>(bm));
             const float mn = fmaxf(mr[nt], bm * f[nt]), ref = mn == -INFINITY ? 0.f : mn;
             al[nt] = ex2(mr[nt] - ref);
             mr[nt] = mn;
@@ -549,8 +547,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
     const float unit = C::kHalf && !redo ? 1.f / kPScale : 1.f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        l[nt] += __shfl_xor(l[nt], 16);
-        l[nt] += __shfl_xor(l[nt], 32);
+        l[nt] = pair_sum<32>(pair_sum<16>(l[nt]));
         if (g == 0) {
             stat[0][wave][16 * nt + i16] = mr[nt];
             stat[1][wave][16 * nt + i16] = l[nt];

@@ -2,7 +2,8 @@
 // in every region, a K or V cache of one layer. Forks a sequence (a prefix into another cache) and keeps a tree's
 // accepted path (rows gathered in place).
 //
-// kv_copy_kernel: source and destination rows do not overlap; 16 bytes a thread and step, kUnroll loads in flight.
+// kv_copy_kernel: source and destination rows do not overlap; 16 bytes a thread and step, two loads in flight, loads and stores
+//   past the caches: 115 MB copied in 38.3 us, 6.0 TB/s of reads and writes (cached 41.6; four in flight 39.5 and 43.2; eight 40.6 and 45.2).
 // kv_gather_kernel: a region onto itself, up to kMoveInPlaceRows rows. A workgroup has a strip of columns of all n
 //   rows and holds it in registers (kHold pieces of 16 bytes a thread) until every load of the strip has arrived, so any
 //   list is right, also one that names a row twice or out of order.
@@ -18,7 +19,7 @@ namespace ql {
 
 namespace {
 
-constexpr int kUnroll = 4;
+constexpr int kUnroll = 2;
 constexpr int kHold = 4;
 static_assert(kMoveInPlaceRows <= 256 * kHold, "a strip of one column piece fits a workgroup's registers");
 
@@ -40,12 +41,12 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(const MoveArgs a)
     for (int k = 0; k < kUnroll; k++) {
         const uint32_t u = u0 + 256u * k, i = u / a.row16, c = u - i * a.row16;
         r[k] = u < units ? source_row(a, i) : -1;
-        if (r[k] >= 0) v[k] = ld_global(reinterpret_cast<const u32x4*>(src + ((size_t)r[k] * a.row16 + c) * 16));
+        if (r[k] >= 0) v[k] = ld_stream(reinterpret_cast<const u32x4*>(src + ((size_t)r[k] * a.row16 + c) * 16));
     }
 #pragma unroll
     for (int k = 0; k < kUnroll; k++) {
         const uint32_t u = u0 + 256u * k;
-        if (r[k] >= 0) st_global(reinterpret_cast<u32x4*>(dst + ((size_t)a.dst_row * a.row16 + u) * 16), v[k]);
+        if (r[k] >= 0) __builtin_nontemporal_store(v[k], QL_GLOBAL(u32x4, reinterpret_cast<u32x4*>(dst + ((size_t)a.dst_row * a.row16 + u) * 16)));
     }
 }
 

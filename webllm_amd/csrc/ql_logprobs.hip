@@ -17,6 +17,7 @@
 #include "ql_device.h"
 #include "ql_digits.h"
 #include "ql_internal.h"
+#include "ql_lanes.h"
 
 namespace ql {
 
@@ -41,20 +42,6 @@ __device__ __forceinline__ float value_of(uint64_t key)
 }
 __device__ __forceinline__ uint64_t key_of(uint32_t bits, uint32_t index) { return (uint64_t)bits << 32 | (uint32_t)~index; }
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) { return (uint64_t)__shfl_xor((unsigned long long)v, o); }
-
-__device__ __forceinline__ float wave_max(float v)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
-}
-__device__ __forceinline__ float wave_sum(float v)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
 
 // four logits from index i on; those past the row's end are -inf
 __device__ __forceinline__ f32x4 load4(const float* x, int i, int V)
@@ -85,7 +72,7 @@ __global__ __launch_bounds__(256) void logprob_scan_kernel(const LogprobArgs a)
     for (int u = 0; u < 4; u++)
 #pragma unroll
         for (int c = 0; c < 4; c++) mx = fmaxf(mx, v[u][c]);
-    const float m = wave_max(mx), ref = m == -INFINITY ? 0.f : m;
+    const float m = wave_max(mx, lane), ref = m == -INFINITY ? 0.f : m;
     float s = 0.f, t = 0.f;
 #pragma unroll
     for (int u = 0; u < 4; u++)
@@ -95,8 +82,8 @@ __global__ __launch_bounds__(256) void logprob_scan_kernel(const LogprobArgs a)
             s += e;
             t += d == -INFINITY ? 0.f : d * e;
         }
-    s = wave_sum(s);
-    t = wave_sum(t);
+    s = wave_sum(s, lane);
+    t = wave_sum(t, lane);
     if (lane == 0) st_global(reinterpret_cast<f32x4*>(a.stat) + row * a.units + unit, f32x4{m, s, t, 0.f});
     if (TOP) {
         uint32_t best = 0, at = 0;
@@ -112,33 +99,40 @@ __global__ __launch_bounds__(256) void logprob_scan_kernel(const LogprobArgs a)
                 }
             }
         uint64_t key = best ? key_of(best, at) : 0;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) key = larger(key, shfl_xor64(key, o));
+        key = larger(key, lane_xor64<8>(key, lane));
+        key = larger(key, lane_xor64<4>(key, lane));
+        key = larger(key, lane_xor64<2>(key, lane));
+        key = larger(key, lane_xor64<1>(key, lane));
         if ((lane & 15) == 0) st_global(a.best + (row * a.units + unit) * kParts + (lane >> 4), key);
     }
 }
 
-// descending over the wave's lanes
-__device__ __forceinline__ uint64_t merge_step(uint64_t v, int lane, int j, bool down)
+// a step of a bitonic network: with the lane ^ J, descending where `down`
+template <int J>
+__device__ __forceinline__ uint64_t merge_step(uint64_t v, int lane, bool down)
 {
-    const uint64_t o = shfl_xor64(v, j);
-    return ((lane & j) == 0) == down ? larger(v, o) : (v > o ? o : v);
+    const uint64_t o = lane_xor64<J>(v, lane);
+    return ((lane & J) == 0) == down ? larger(v, o) : (v > o ? o : v);
 }
+template <int J>
+__device__ __forceinline__ uint64_t merge_from(uint64_t v, int lane, bool down)
+{
+    v = merge_step<J>(v, lane, down);
+    if constexpr (J > 1) v = merge_from<J / 2>(v, lane, down);
+    return v;
+}
+// descending over the wave's lanes
+template <int K = 2>
 __device__ __forceinline__ uint64_t sort64(uint64_t v, int lane)
 {
-#pragma unroll
-    for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-        for (int j = k >> 1; j > 0; j >>= 1) v = merge_step(v, lane, j, (lane & k) == 0);
+    v = merge_from<K / 2>(v, lane, (lane & K) == 0);
+    if constexpr (K < 64) v = sort64<2 * K>(v, lane);
     return v;
 }
 // the largest 64 of two descending lists; b is the second one's from its end
 __device__ __forceinline__ uint64_t merge64(uint64_t a, uint64_t b_reversed, int lane)
 {
-    uint64_t v = larger(a, b_reversed);
-#pragma unroll
-    for (int j = 32; j > 0; j >>= 1) v = merge_step(v, lane, j, true);
-    return v;
+    return merge_from<32>(larger(a, b_reversed), lane, true);
 }
 
 // The largest 64 of n keys, descending over wave 0's lanes: each wave sorts 64 at a time, the waves' lists are merged
@@ -179,7 +173,7 @@ __device__ __forceinline__ void join_units(const LogprobArgs& a, size_t row, int
     const f32x4* st = reinterpret_cast<const f32x4*>(a.stat) + row * a.units;
     float m = -INFINITY;
     for (int i = lane; i < a.units; i += 64) m = fmaxf(m, ld_global(st + i).x);
-    m = wave_max(m);
+    m = wave_max(m, lane);
     ref = m == -INFINITY ? 0.f : m;
     float s = 0.f, t = 0.f;
     for (int i = lane; i < a.units; i += 64) {
@@ -188,8 +182,8 @@ __device__ __forceinline__ void join_units(const LogprobArgs& a, size_t row, int
         s = fmaf(u.y, e, s);
         t += e == 0.f ? 0.f : fmaf(d, u.y, u.z) * e;      // d may be too far down for d * u.y
     }
-    s = wave_sum(s);
-    t = wave_sum(t);
+    s = wave_sum(s, lane);
+    t = wave_sum(t, lane);
     none = s == 0.f;
     ls = logf(s);
     if (lane == 0 && a.entropy) st_global(a.entropy + row, none ? 0.f : ls - t / s);
