@@ -33,7 +33,6 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kTreeWorkgroups = 512;     // two per CU
 constexpr int kTreeMaxSplit = 128;
 constexpr int kKeys = 32;                // keys of a block
 constexpr float kPScale = 16384.f;       // fp16 parts of P: 2^14 P
@@ -94,8 +93,6 @@ struct TreeTile {
     static constexpr int kMergeStride = kChunk + 4;
     static constexpr int kMergeBytes = 4 * kRows * kMergeStride * 4;
     static constexpr int kLds = kQBytes > kMergeBytes ? kQBytes : kMergeBytes;
-    // the column of tile (c, j), index i
-    static __device__ __forceinline__ int col(int c, int j, int i) { return kChunk * c + kCols * i + j; }
     // the column of element e of step t of a K or Q fragment, group g
     static __device__ __forceinline__ int kcol(int t, int g, int e) { return kHalf ? 32 * t + 8 * g + e : 32 * t + 16 * (e >> 2) + 4 * g + (e & 3); }
 };
@@ -137,11 +134,11 @@ __device__ __forceinline__ int pair_row(const TreeArgs& a, int kvh, int r, int& 
 }
 
 // The wave's blocks on the VALU, in the layout of the kernel below.
-template <typename T, int DP, int NT, bool FULL>
-__device__ __forceinline__ void tree_again(const TreeArgs& a, int kvh, int r0, int first, int end, int past_blocks, float (&mr)[NT], float (&l)[NT],
-                                                     f32x4 (&acc)[DP / 16][NT])
+// Blocks first, first + step, ... before `end`; a lane's columns come COLS at a time.
+template <typename T, int DP, int NT, bool FULL, int COLS>
+__device__ __forceinline__ void tree_again(const TreeArgs& a, int kvh, int r0, int first, int end, int step, int past_blocks, float (&mr)[NT], float (&l)[NT],
+                                           f32x4 (&acc)[DP / 16][NT])
 {
-    using C = TreeTile<T, DP, NT, FULL>;
     const int lane = threadIdx.x & 63, i16 = lane & 15, g = lane >> 4;
     const size_t row_len = (size_t)a.KV * a.D;
     const T* kb = static_cast<const T*>(a.k) + (size_t)kvh * a.D;
@@ -151,9 +148,9 @@ __device__ __forceinline__ void tree_again(const TreeArgs& a, int kvh, int r0, i
         mr[nt] = -INFINITY;
         l[nt] = 0.f;
 #pragma unroll
-        for (int d = 0; d < C::kDT; d++) acc[d][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < DP / 16; d++) acc[d][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int b = first; b < end; b += 4) {
+    for (int b = first; b < end; b += step) {
         const TreeBlock blk = tree_block(a, b, past_blocks);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -162,7 +159,7 @@ __device__ __forceinline__ void tree_again(const TreeArgs& a, int kvh, int r0, i
             const uint64_t seen = seen_bits(a, blk, m);
             // four of the block's keys per lane and 16; then each lane takes all of them to its columns
 #pragma unroll 1
-            for (int kt = 0; kt < C::kNK; kt++) {
+            for (int kt = 0; kt < kKeys / 16; kt++) {
                 float s[4], bm = -INFINITY;
 #pragma unroll 1
                 for (int r = 0; r < 4; r++) {
@@ -185,7 +182,7 @@ __device__ __forceinline__ void tree_again(const TreeArgs& a, int kvh, int r0, i
                 mr[nt] = mn;
                 l[nt] *= al;
 #pragma unroll
-                for (int d = 0; d < C::kDT; d++) acc[d][nt] *= al;
+                for (int d = 0; d < DP / 16; d++) acc[d][nt] *= al;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     s[r] = seen >> (16 * kt + 4 * g + r) & 1 ? ex2(s[r] - ref) : 0.f;
@@ -199,13 +196,13 @@ __device__ __forceinline__ void tree_again(const TreeArgs& a, int kvh, int r0, i
                     if (!(seen >> (16 * kt + key) & 1)) continue;      // differs between lanes, but not between the four of a pair
                     const T* v = vb + (size_t)(blk.base + 16 * kt + key) * row_len;
 #pragma unroll
-                    for (int c = 0; c < C::kNC; c++)
+                    for (int c = 0; c < DP / (16 * COLS); c++)
 #pragma unroll
-                        for (int j = 0; j < C::kCols; j++)
+                        for (int j = 0; j < COLS; j++)
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
-                                const int d = C::col(c, j, 4 * g + e);
-                                if (FULL || d < a.D) acc[c * C::kCols + j][nt][e] = fmaf(p, (float)v[d], acc[c * C::kCols + j][nt][e]);
+                                const int d = 16 * COLS * c + COLS * (4 * g + e) + j;
+                                if (FULL || d < a.D) acc[c * COLS + j][nt][e] = fmaf(p, (float)v[d], acc[c * COLS + j][nt][e]);
                             }
                 }
             }
@@ -541,7 +538,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
             for (int r = 0; r < 4; r++) odd = fmaf(acc[d][nt][r], 0.f, odd);
     }
     const bool redo = __any(odd != 0.f);
-    if (redo) tree_again<T, DP, NT, FULL>(a, kvh, rg * C::kRows, first, b1, past_blocks, mr, l, acc);
+    if (redo) tree_again<T, DP, NT, FULL, C::kCols>(a, kvh, rg * C::kRows, first, b1, 4, past_blocks, mr, l, acc);
 
     // the four waves' states
     const float unit = C::kHalf && !redo ? 1.f / kPScale : 1.f;
@@ -729,8 +726,11 @@ uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes)
     a->past_blocks = (a->past + kKeys - 1) / kKeys;
     const int blocks = a->blocks = a->past_blocks + (a->M + kKeys - 1) / kKeys;
     const size_t one = (size_t)a->M * a->H * (a->D + 2) * sizeof(float);
-    // key ranges up to two workgroups a CU, of at least a block a wave, as many as the workspace holds
-    const int s = std::max(1, std::min({kTreeWorkgroups / (a->groups * a->KV), (blocks + 3) / 4, kTreeMaxSplit, (int)std::min<size_t>(kTreeMaxSplit, ws_bytes / one)}));
+    const int fit = (int)std::min<size_t>(kTreeMaxSplit, ws_bytes / one);
+    // key ranges that keep every XCD's 32 CUs within `each` workgroups: a (kv head, range)'s groups are on one of them
+    auto ranges = [&](int each) { return 8 * (32 * each / a->groups) / a->KV; };
+    // up to two workgroups a CU, at least a block a wave, as many as the workspace holds
+    const int s = std::max(1, std::min({ranges(2), (blocks + 3) / 4, fit}));
     a->per = ((blocks + s - 1) / s + 3) / 4 * 4;            // as many for each of the waves
     a->nsplit = (blocks + a->per - 1) / a->per;
     a->inv_nsplit = 1.f / a->nsplit;
