@@ -357,6 +357,11 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
                 }
             }
         };
+        const bool all_seen = blk.j0 < 0 && blk.n == kKeys;
+        uint32_t seen[NT];                                  // bit 16 kt + r: key 16 kt + 4 g + r; asked for before it is needed
+        if (!all_seen)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) seen[nt] = (uint32_t)(seen_bits(a, blk, qm[nt]) << (blk.base - blk.at)) >> (4 * g);
         f32x4 s[C::kNK][NT];
 #pragma unroll
         for (int kt = 0; kt < C::kNK; kt++) {
@@ -422,17 +427,14 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
         const TreeBlock now = blk;
         const bool more = b + 4 < b1;
         if (more) blk = tree_block(a, b + 4, past_blocks);
-        if (now.j0 >= 0 || now.n < kKeys) {
+        if (!all_seen)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const uint32_t seen = (uint32_t)(seen_bits(a, now, qm[nt]) << (now.base - now.at)) >> (4 * g);
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int kt = 0; kt < C::kNK; kt++)
 #pragma unroll
                     for (int r = 0; r < 4; r++)
-                        if (!(seen >> (16 * kt + r) & 1)) s[kt][nt][r] = -INFINITY;
-            }
-        }
+                        if (!(seen[nt] >> (16 * kt + r) & 1)) s[kt][nt][r] = -INFINITY;
         Frag pf[C::kNH][NT][C::kParts];
         float al[NT];
 #pragma unroll
@@ -654,42 +656,46 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const TreeArgs a)
 {
     __shared__ float wgt[kTreeMaxSplit];
     __shared__ f32x4 part[256];
+    constexpr int kFirst = 4;                               // ranges a thread has asked for before the weights are there
     const size_t row = (size_t)blockIdx.y * a.H + blockIdx.x;
-    const int t = threadIdx.x, S = a.nsplit, D = a.D;
+    const int t = threadIdx.x, lane = t & 63, S = a.nsplit, D = a.D;
+    const int nc = D / 4, P = 256 / nc, p = t / nc, c = t - p * nc;
+    const f32x4* src = reinterpret_cast<const f32x4*>(a.ws + row * S * D) + c;
+    f32x4 v[kFirst];
+#pragma unroll
+    for (int k = 0; k < kFirst; k++) v[k] = p < P && p + k * P < S ? ld_global(src + (size_t)(p + k * P) * nc) : f32x4{0.f, 0.f, 0.f, 0.f};
     if (t < 64) {
-        const float* st = a.ws + (size_t)a.M * a.H * S * D + 2 * row * S;
-        float mi[2], li[2];
+        const f32x2* st = reinterpret_cast<const f32x2*>(a.ws + (size_t)a.M * a.H * S * D) + row * S;
+        f32x2 s[2];
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int i = t + 64 * r;
-            mi[r] = i < S ? ld_global(st + 2 * i) : -INFINITY;
-            li[r] = i < S ? ld_global(st + 2 * i + 1) : 0.f;
-        }
-        float mx = fmaxf(mi[0], mi[1]);
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+        for (int r = 0; r < 2; r++) s[r] = t + 64 * r < S ? ld_global(st + t + 64 * r) : f32x2{-INFINITY, 0.f};
+        const float mx = wave_max(fmaxf(s[0].x, s[1].x), lane);
         float e[2], l = 0.f;
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-            e[r] = mi[r] == -INFINITY ? (li[r] != li[r] ? li[r] : 0.f) : ex2(mi[r] - mx);
-            l += li[r] * e[r];
+            const float mi = s[r].x, li = s[r].y;
+            e[r] = mi == -INFINITY ? (li != li ? li : 0.f) : ex2(mi - mx);
+            l += li * e[r];
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) l += __shfl_xor(l, o);
+        l = wave_sum(l, lane);
 #pragma unroll
         for (int r = 0; r < 2; r++) wgt[t + 64 * r] = l == 0.f ? 0.f : e[r] / l;
     }
     __syncthreads();
-    const int nc = D / 4, P = 256 / nc, c = t % nc, p = t / nc;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     if (p < P) {
-        const f32x4* src = reinterpret_cast<const f32x4*>(a.ws + row * S * D) + c;
-#pragma unroll 4
-        for (int i = p; i < S; i += P) {
-            const float w = wgt[i];
-            const f32x4 v = ld_global(src + (size_t)i * nc);
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = fmaf(w, v[e], o[e]);
+        for (int k = 0; k < kFirst; k++) {
+            const float w = p + k * P < S ? wgt[p + k * P] : 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(w, v[k][e], o[e]);
+        }
+#pragma unroll 4
+        for (int i = p + kFirst * P; i < S; i += P) {
+            const float w = wgt[i];
+            const f32x4 x = ld_global(src + (size_t)i * nc);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(w, x[e], o[e]);
         }
     }
     part[t] = o;
@@ -721,7 +727,11 @@ uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes)
     const int R = a->M * a->G;
     a->nsplit = 1;
     if (a->past + a->M < kKeys) return 0;
-    a->nt = (a->D == 64 || a->D == 128) && R > 16 ? 2 : 1;
+    // 32 pairs a workgroup where those fill the chip twice (fp16: four times) with ranges of a block a wave: a block is then split
+    // into parts half as often, but a wave's own chain is longer. 16 against 32, in us (28 / 4 heads of 128): 8 rows after 300 keys
+    // 11.3, 13.5, 4 after 4000 12.1, 14.2, 24 after 4000 29.0, 25.2; fp16 16 after 4000 14.4, 16.4, 24 after 4000 18.3 both.
+    const long full = (long)((R + 31) / 32) * a->KV * ((a->past + a->M + 4 * kKeys - 1) / (4 * kKeys));
+    a->nt = (a->D == 64 || a->D == 128) && full >= (a->half ? 1024 : 512) ? 2 : 1;
     a->groups = (R + 16 * a->nt - 1) / (16 * a->nt);
     a->past_blocks = (a->past + kKeys - 1) / kKeys;
     const int blocks = a->blocks = a->past_blocks + (a->M + kKeys - 1) / kKeys;
