@@ -199,7 +199,7 @@ class Tensor:
     pool: "ActivationArena | None" = None
 
     def read(self) -> np.ndarray:
-        dt = {"f32": np.float32, "f16": np.float16, "u8": np.uint8, "u32": np.uint32}[self.dtype]
+        dt = {"f32": np.float32, "f16": np.float16, "u8": np.uint8, "u32": np.uint32, "i32": np.int32, "u64": np.uint64}[self.dtype]
         return self.arena.read(self.offset, self.shape, dt)
 
     def write(self, data: np.ndarray):
@@ -215,7 +215,7 @@ class ActivationArena:
 
     def alloc(self, shape, dtype: str = "f32") -> Tensor:
         n = int(np.prod(shape))
-        size = n * {"f16": 2, "u8": 1}.get(dtype, 4)
+        size = n * {"f16": 2, "u8": 1, "u64": 8}.get(dtype, 4)
         off = self.layout.take(size)
         if self.layout.used > self.arena.size:
             raise ValueError(f"activation arena exhausted ({self.layout.used} > {self.arena.size})")
@@ -236,19 +236,27 @@ class ActivationArena:
 
 
 class KvCache:
-    """Per-layer fp32 K and V caches [block_size, n_kv_head * D] in one device arena, and the
-    decode attention over them: QwenGpt's kCache/vCache (qwen.ts:140-141, :200-205), kv store
-    (qwen.ts:427-428) and attention_gqa_cache dispatch (qwen.ts:429-440). Stream order replaces
-    the reference's pass breaks. The caller keeps the context length (the reference's cacheLen,
-    qwen.ts:142, :490) and passes it as pos0 / past_len."""
+    """Per-layer K and V caches [block_size, n_kv_head * D] in one device arena, and the attention over
+    them: QwenGpt's kCache/vCache (qwen.ts:140-141, :200-205), kv store (qwen.ts:427-428) and
+    attention_gqa_cache dispatch (qwen.ts:429-440). Stream order replaces the reference's pass breaks. The
+    caller keeps the context length (the reference's cacheLen, qwen.ts:142, :490) and passes it as pos0 / past_len.
 
-    def __init__(self, ctx: ql.Context, config: QwenConfig):
+    dtype "f32", or "f16": half the memory and its reads; store and attend take fp32 caches, rotate_store and
+    attend_tree both. A pass over drafted tokens (a tree, ql.tree_masks) runs rotate_store and attend_tree per layer, and
+    accept keeps the path that was accepted."""
+
+    def __init__(self, ctx: ql.Context, config: QwenConfig, dtype: str = "f32"):
+        if dtype not in ("f32", "f16"):
+            raise ValueError(f"kv cache: dtype {dtype}")
         self.ctx = ctx
         self.config = config
+        self.dtype = dtype
         self.D = qwen_head_dim(config)
         self.row_len = qwen_kv_dim(config)
-        self.region = -(-config.block_size * self.row_len * 4 // 256) * 256
+        self.row_bytes = self.row_len * (2 if dtype == "f16" else 4)
+        self.region = -(-config.block_size * self.row_bytes // 256) * 256
         self.arena = ctx.arena(2 * config.n_layer * self.region)
+        self.regions = ql.offsets([i * self.region for i in range(2 * config.n_layer)])
 
     def offsets(self, layer: int):
         if not 0 <= layer < self.config.n_layer:
@@ -256,8 +264,17 @@ class KvCache:
         base = 2 * layer * self.region
         return base, base + self.region
 
+    def _f32_only(self, what: str):
+        if self.dtype != "f32":
+            raise ValueError(f"{what}: an fp16 cache takes rotate_store and attend_tree")
+
+    @property
+    def _ql_dtype(self) -> int:
+        return ql.DTYPE_F16 if self.dtype == "f16" else ql.DTYPE_F32
+
     def store(self, layer: int, k: Tensor, v: Tensor, rows: int, pos0: int):
         """cache[pos0 + r] = k[r] / v[r] for r < rows (after RoPE on k, as the reference)."""
+        self._f32_only("kv store")
         if k.length < rows * self.row_len or v.length < rows * self.row_len:
             raise ValueError("kv store: k/v tensors smaller than [rows, n_kv_head * D]")
         ko, vo = self.offsets(layer)
@@ -267,6 +284,7 @@ class KvCache:
 
     def attend(self, layer: int, q: Tensor, out: Tensor, M: int, past_len: int):
         """out [M, n_head * D] = causal GQA attention of q's M rows at positions past_len + m."""
+        self._f32_only("attention")
         c = self.config
         if q.length < M * c.n_head * self.D or out.length < M * c.n_head * self.D:
             raise ValueError("attention: q/out smaller than [M, n_head * D]")
@@ -275,6 +293,63 @@ class KvCache:
         ko, vo = self.offsets(layer)
         self.ctx.attention_decode(q.arena, q.offset, self.arena, ko, vo, c.block_size, M, c.n_head,
                                   c.n_kv_head, self.D, past_len, out.offset)
+
+    def rotate_store(self, layer: int, model: "QuantLinearModel", q: Tensor, k: Tensor, v: Tensor, positions: Tensor, q_out: Tensor,
+                     M: int, slot0: int, rope: str = "rope", q_norm: str | None = None, k_norm: str | None = None, eps: float = 1e-6):
+        """q and k turned by their rows' positions (i32 [M]; qwen.ts:414-423, ropeHalfRef's pairs), normed per head first where
+        norm weights are named; q to q_out (q itself may be given), k and v to cache rows slot0 + m."""
+        c = self.config
+        if q.length < M * c.n_head * self.D or q_out.length < M * c.n_head * self.D:
+            raise ValueError("rotate_store: q/q_out smaller than [M, n_head * D]")
+        if k.length < M * self.row_len or v.length < M * self.row_len:
+            raise ValueError("rotate_store: k/v smaller than [M, n_kv_head * D]")
+        if positions.dtype != "i32" or positions.length < M:
+            raise ValueError("rotate_store: positions must be an i32 tensor of at least M")
+        if any(t.arena is not q.arena for t in (k, v, positions, q_out)):
+            raise ValueError("rotate_store: tensors must live in one activation arena")
+        table = model.f32.get(rope)
+        if table is None:
+            raise ValueError(f"missing rope table: {rope}")
+        norms = [None if n is None else model.f32.get(n) for n in (q_norm, k_norm)]
+        for name, w in zip((q_norm, k_norm), norms):
+            if name is not None and (w is None or w.length != self.D):
+                raise ValueError(f"missing f32 weight of {self.D} values: {name}")
+        desc = ql.make_rope(table.offset, table.shape[0], c.n_head, c.n_kv_head, self.D, rot_dim=table.shape[1],
+                            q_norm_off=None if norms[0] is None else norms[0].offset, k_norm_off=None if norms[1] is None else norms[1].offset,
+                            norm_eps=eps, cache_dtype=self._ql_dtype)
+        ko, vo = self.offsets(layer)
+        self.ctx.qk_norm_rope(desc, model.weights, q.arena, q.offset, k.offset, v.offset, positions.offset, M, q_out.offset, self.arena,
+                              ko, vo, c.block_size, slot0)
+
+    def attend_tree(self, layer: int, q: Tensor, out: Tensor, M: int, past_len: int, masks: Tensor | None = None):
+        """out [M, n_head * D] = GQA attention of M <= 256 drafted rows, stored at past_len + m, over the context and the rows that
+        their masks (u64 [M, ceil(M/64)], ql.tree_masks) name; without masks in order, causal."""
+        c = self.config
+        if q.length < M * c.n_head * self.D or out.length < M * c.n_head * self.D:
+            raise ValueError("attend_tree: q/out smaller than [M, n_head * D]")
+        if masks is not None and (masks.dtype != "u64" or masks.length < M * -(-M // 64)):
+            raise ValueError("attend_tree: masks must be a u64 tensor [M, ceil(M/64)]")
+        if q.arena is not out.arena or (masks is not None and masks.arena is not q.arena):
+            raise ValueError("attend_tree: q, out and masks must live in the same activation arena")
+        ko, vo = self.offsets(layer)
+        self.ctx.attention_tree(q.arena, q.offset, self.arena, ko, vo, self._ql_dtype, c.block_size, M, c.n_head, c.n_kv_head, self.D,
+                                past_len, None if masks is None else masks.offset, out.offset)
+
+    def accept(self, past_len: int, path: Tensor, n: int):
+        """Keeps an accepted path of the tree stored at past_len: row past_len + i of every layer becomes row past_len + path[i]
+        (i32, i < n)."""
+        if path.dtype != "i32" or path.length < n:
+            raise ValueError("accept: path must be an i32 tensor of at least n rows")
+        T = self.config.block_size
+        self.ctx.kv_move(self.arena, self.regions, T, self.arena, self.regions, T, self.row_bytes, past_len, past_len, n, path.arena,
+                         path.offset)
+
+    def fork(self, to: "KvCache", rows: int):
+        """The first rows of every layer into another cache of the same layers and heads (another sequence that continues them)."""
+        a, b = self.config, to.config
+        if (a.n_layer, self.row_len, self.dtype) != (b.n_layer, to.row_len, to.dtype):
+            raise ValueError("fork: the caches differ in layers, heads or dtype")
+        self.ctx.kv_move(to.arena, to.regions, b.block_size, self.arena, self.regions, a.block_size, self.row_bytes, 0, 0, rows)
 
     def release(self):
         self.arena.release()
@@ -412,6 +487,38 @@ class QuantLinearModel:
         if any(t.arena is not gate.arena for t in ts) or any(t.length < n for t in ts):
             raise ValueError("silu_mul: tensors must hold n values in one activation arena")
         self.ctx.silu_mul(gate.arena, gate.offset, up.offset, n, out.offset)
+
+    def make_rope_table(self, max_pos: int, rot_dim: int, theta: float, name: str = "rope"):
+        """Cosines and sines of positions 0 .. max_pos - 1 in the weight arena, for KvCache.rotate_store (qwen.ts ropeTheta)."""
+        if name in self.f32:
+            raise ValueError(f"weight already exists: {name}")
+        off = self.layout.take(max_pos * rot_dim * 4)
+        if self.layout.used > self.weights.size:
+            raise ValueError(f"weight arena exhausted ({self.layout.used} > {self.weights.size})")
+        self.ctx.rope_table(self.weights, off, max_pos, rot_dim, theta)
+        self.f32[name] = Tensor(self.weights, off, max_pos * rot_dim, (max_pos, rot_dim), "f32")
+
+    def token_logprobs(self, logits: Tensor, M: int, V: int, tokens: Tensor | None = None, logprobs: Tensor | None = None,
+                       entropy: Tensor | None = None, top_ids: Tensor | None = None, top_logprobs: Tensor | None = None):
+        """Over M rows of V logits (gemm's C for the lm_head): logprobs [M, T] of tokens (i32 [M, T]; -1: none), the rows' entropies
+        [M], and the top k alternatives (top_ids i32 and top_logprobs [M, k])."""
+        if (tokens is None) != (logprobs is None) or (top_ids is None) != (top_logprobs is None):
+            raise ValueError("token_logprobs: tokens come with logprobs, top_ids with top_logprobs")
+        given = [t for t in (tokens, logprobs, entropy, top_ids, top_logprobs) if t is not None]
+        if any(t.arena is not logits.arena for t in given):
+            raise ValueError("token_logprobs: tensors must live in the logits' arena")
+        if logits.dtype != "f32" or logits.length < M * V:
+            raise ValueError("token_logprobs: logits must be f32 [M, V]")
+        T = 0 if tokens is None else tokens.length // M
+        k = 0 if top_ids is None else top_ids.length // M
+        if (tokens is not None and (tokens.dtype != "i32" or logprobs.length < M * T)) or (entropy is not None and entropy.length < M) or \
+                (top_ids is not None and (top_ids.dtype != "i32" or top_logprobs.length < M * k)):
+            raise ValueError("token_logprobs: tokens and top_ids are i32, logprobs [M, T], entropy [M], top_logprobs [M, k]")
+
+        def off(t):
+            return 0 if t is None else t.offset
+        self.ctx.token_logprobs(logits.arena, logits.offset, V, M, V, off(tokens), T, k, off(logprobs),
+                                None if entropy is None else entropy.offset, off(top_ids), off(top_logprobs))
 
     def _gemm_f16(self, A: Tensor, weight: str, C: Tensor, bias: str | None, M: int, N: int, K: int):
         """C[M,N] = A[M,K] @ W^T (+ bias) over an fp16 weight [N,K] (the tied lm_head `embed`,

@@ -77,15 +77,16 @@ export interface GptqInt4Params {
 /** quant.ts dequantizeGptqInt4, computed on the GPU: fp32 [outFeatures, inFeatures], for any f32 scales. */
 export function dequantizeGptqInt4(params: GptqInt4Params, ctx?: Context): Float32Array;
 
+export type TensorDtype = 'f32' | 'f16' | 'u32' | 'i32' | 'u64';
 export class Tensor {
     readonly arena: Arena; readonly offset: number; readonly length: number;
-    readonly shape: number[]; readonly dtype: 'f32' | 'f16' | 'u32';
-    read(): Float32Array | Uint16Array | Uint32Array;
+    readonly shape: number[]; readonly dtype: TensorDtype;
+    read(): Float32Array | Uint16Array | Uint32Array | Int32Array | BigUint64Array;
     write(data: ArrayBufferView): void;
 }
 export class ActivationArena {
     constructor(ctx: Context, bytes: number);
-    alloc(shape: number[], dtype?: 'f32' | 'f16' | 'u32'): Tensor;
+    alloc(shape: number[], dtype?: TensorDtype): Tensor;
     scratchOffset(nbytes: number): number;
     reset(): void;
     release(): void;
@@ -110,6 +111,12 @@ export class QuantLinearModel {
             residual?: Tensor | null, sumOut?: Tensor | null): void;
     /** out = silu(gate) * up (ql_silu_mul). */
     siluMul(gate: Tensor, up: Tensor, out: Tensor, n: number): void;
+    /** cosines and sines of positions 0 .. maxPos - 1 in the weight arena (ql_rope_table), named 'rope' by default */
+    makeRopeTable(maxPos: number, rotDim: number, theta: number, name?: string): void;
+    /** log probabilities of given tokens, entropies and top alternatives of M rows of V logits (ql_token_logprobs) */
+    tokenLogprobs(logits: Tensor, M: number, V: number, o: {
+        tokens?: Tensor | null; logprobs?: Tensor | null; entropy?: Tensor | null; topIds?: Tensor | null; topLogprobs?: Tensor | null;
+    }): void;
     unpackF16(name: string, out: Tensor): void;
     /** fp16 [N,K] copies of many weights in a few launches (ql_unpack_f16_batch). */
     unpackAllF16(names: string[], outs: Tensor[]): void;
@@ -117,13 +124,25 @@ export class QuantLinearModel {
     release(): void;
 }
 
-/** Per-layer fp32 K/V caches and decode attention (qwen.ts:200-205, :427-440). */
+/** masks (ceil(M/64) words a row) and depths of a drafted tree; parents[m] is -1 or an earlier row (ql_tree_masks) */
+export function treeMasks(parents: ArrayLike<number>): { masks: BigUint64Array; depths: Int32Array };
+
+/** Per-layer K/V caches and attention (qwen.ts:200-205, :427-440); 'f16' caches take rotateStore and attendTree only. */
 export class KvCache {
-    constructor(ctx: Context, config: QwenConfig);
+    constructor(ctx: Context, config: QwenConfig, dtype?: 'f32' | 'f16');
     readonly D: number;
     readonly rowLen: number;
     store(layer: number, k: Tensor, v: Tensor, rows: number, pos0: number): void;
     attend(layer: number, q: Tensor, out: Tensor, M: number, pastLen: number): void;
+    /** norms (where named), rotation by positions (i32) and cache store in one launch (ql_qk_norm_rope) */
+    rotateStore(layer: number, model: QuantLinearModel, q: Tensor, k: Tensor, v: Tensor, positions: Tensor, qOut: Tensor, M: number,
+                slot0: number, options?: { rope?: string; qNorm?: string; kNorm?: string; eps?: number }): void;
+    /** attention of M <= 256 drafted rows (ql_attention_tree); masks: treeMasks' words, or none for causal rows */
+    attendTree(layer: number, q: Tensor, out: Tensor, M: number, pastLen: number, masks?: Tensor | null): void;
+    /** keeps an accepted path (i32 rows of the tree at pastLen) in every layer (ql_kv_move) */
+    accept(pastLen: number, path: Tensor, n: number): void;
+    /** the first rows of every layer into another cache (ql_kv_move) */
+    fork(to: KvCache, rows: number): void;
     release(): void;
 }
 

@@ -324,7 +324,7 @@ class Tensor {
         this.dtype = dtype; this.pool = pool || null;
     }
     read() {
-        const T = this.dtype === 'f16' ? Uint16Array : (this.dtype === 'u32' ? Uint32Array : Float32Array);
+        const T = { f32: Float32Array, f16: Uint16Array, u32: Uint32Array, i32: Int32Array, u64: BigUint64Array }[this.dtype];
         return this.arena.read(this.offset, new T(this.length));
     }
     write(data) { this.arena.write(this.offset, data); }
@@ -339,7 +339,7 @@ class ActivationArena {
     alloc(shape, dtype) {
         const dt = dtype || 'f32';
         const n = shape.reduce((a, b) => a * b, 1);
-        const off = this.layout.take(n * (dt === 'f16' ? 2 : 4));
+        const off = this.layout.take(n * (dt === 'f16' ? 2 : dt === 'u64' ? 8 : 4));
         if (this.layout.used > this.arena.size) throw new Error('activation arena exhausted');
         return new Tensor(this.arena, off, n, shape.slice(), dt, this);
     }
@@ -456,6 +456,31 @@ class QuantLinearModel {
     siluMul(gate, up, out, n) {
         if (gate.arena !== up.arena || gate.arena !== out.arena) throw new Error('siluMul: tensors must share one arena');
         addon.siluMul(this.ctx.handle, gate.arena.handle, gate.offset, up.offset, n, out.offset);
+    }
+    /** Cosines and sines of positions 0 .. maxPos - 1 in the weight arena, for KvCache.rotateStore. */
+    makeRopeTable(maxPos, rotDim, theta, name) {
+        const key = name || 'rope';
+        if (this.f32Weights.has(key)) throw new Error(`weight already exists: ${key}`);
+        const off = this.layout.take(maxPos * rotDim * 4);
+        if (this.layout.used > this.weights.size) throw new Error(`weight arena exhausted (${this.layout.used} > ${this.weights.size})`);
+        addon.ropeTable(this.ctx.handle, this.weights.handle, off, maxPos, rotDim, theta);
+        this.f32Weights.set(key, new Tensor(this.weights, off, maxPos * rotDim, [maxPos, rotDim], 'f32'));
+    }
+    /**
+     * Over M rows of V logits: logprobs [M, T] of tokens (i32 [M, T]; -1: none), entropy [M], topIds (i32) and topLogprobs
+     * [M, k]; each may be left out (tokens with logprobs, topIds with topLogprobs).
+     */
+    tokenLogprobs(logits, M, V, o) {
+        if (!o.tokens !== !o.logprobs || !o.topIds !== !o.topLogprobs) throw new Error('tokenLogprobs: tokens come with logprobs, topIds with topLogprobs');
+        for (const t of [o.tokens, o.logprobs, o.entropy, o.topIds, o.topLogprobs]) {
+            if (t && t.arena !== logits.arena) throw new Error('tokenLogprobs: tensors must share one arena');
+        }
+        const T = o.tokens ? Math.floor(o.tokens.length / M) : 0, k = o.topIds ? Math.floor(o.topIds.length / M) : 0;
+        if (logits.length < M * V || (o.tokens && (o.tokens.dtype !== 'i32' || o.logprobs.length < M * T)) || (o.entropy && o.entropy.length < M) ||
+            (o.topIds && (o.topIds.dtype !== 'i32' || o.topLogprobs.length < M * k))) throw new Error('tokenLogprobs: a tensor is too small or of another type');
+        const off = (t) => (t ? t.offset : 0);
+        addon.tokenLogprobs(this.ctx.handle, logits.arena.handle, logits.offset, V, M, V, off(o.tokens), T, k, off(o.logprobs),
+            o.entropy ? o.entropy.offset : null, off(o.topIds), off(o.topLogprobs));
     }
     /** Several linears on one input in one launch (q/k/v, gate/up; qwen.ts:411-413, :464-465). */
     gemmBatch(A, weights, Cs, M) {
@@ -639,35 +664,98 @@ async function loadQwenWeights(ctx, model, options) {
     return { gpuBytes: model.weightBytes, tensorCount, fileBytes: raw.byteLength, layer: kept, embedRows, storedZeros };
 }
 
+/** {masks: BigUint64Array [M, ceil(M/64)], depths: Int32Array} of a drafted tree: parents[m] is -1 or an earlier row. */
+function treeMasks(parents) {
+    const p = Int32Array.from(parents), M = p.length;
+    const masks = new BigUint64Array(M * Math.ceil(M / 64)), depths = new Int32Array(M);
+    addon.treeMasks(p, masks, depths);
+    return { masks, depths };
+}
+
 /**
- * Per-layer fp32 K and V caches [blockSize, nKvHead * headDim] and the decode attention over them:
+ * Per-layer K and V caches [blockSize, nKvHead * headDim] and the attention over them:
  * QwenGpt's kCache/vCache (qwen.ts:140-141, :200-205), kv_store (:427-428), attention_gqa_cache (:429-440).
+ * dtype 'f32', or 'f16' (rotateStore and attendTree only). A pass over drafted tokens (treeMasks) runs rotateStore and
+ * attendTree per layer; accept keeps the accepted path.
  */
 class KvCache {
-    constructor(ctx, config) {
+    constructor(ctx, config, dtype) {
         this.ctx = ctx;
         this.config = config;
+        this.dtype = dtype || 'f32';
+        if (this.dtype !== 'f32' && this.dtype !== 'f16') throw new Error(`kv cache: dtype ${dtype}`);
         this.D = qwenHeadDim(config);
         this.rowLen = qwenKvDim(config);
-        this.region = Math.ceil(config.blockSize * this.rowLen * 4 / 256) * 256;
+        this.rowBytes = this.rowLen * (this.dtype === 'f16' ? 2 : 4);
+        this.region = Math.ceil(config.blockSize * this.rowBytes / 256) * 256;
         this.arena = ctx.arena(2 * config.nLayer * this.region);
+        this.regions = Array.from({ length: 2 * config.nLayer }, (_, i) => i * this.region);
     }
     offsets(layer) {
         if (layer < 0 || layer >= this.config.nLayer) throw new Error(`layer ${layer} out of range`);
         return [2 * layer * this.region, (2 * layer + 1) * this.region];
     }
+    _f32Only(what) {
+        if (this.dtype !== 'f32') throw new Error(`${what}: an fp16 cache takes rotateStore and attendTree`);
+    }
     store(layer, k, v, rows, pos0) {
+        this._f32Only('store');
         const [ko, vo] = this.offsets(layer);
         if (k.arena !== v.arena) throw new Error('store: k and v must share one arena');
         addon.kvStore(this.ctx.handle, k.arena.handle, k.offset, this.arena.handle, ko, this.config.blockSize, rows, this.rowLen, pos0);
         addon.kvStore(this.ctx.handle, v.arena.handle, v.offset, this.arena.handle, vo, this.config.blockSize, rows, this.rowLen, pos0);
     }
     attend(layer, q, out, M, pastLen) {
+        this._f32Only('attend');
         const c = this.config;
         if (q.arena !== out.arena) throw new Error('attend: q and out must share one arena');
         const [ko, vo] = this.offsets(layer);
         addon.attention(this.ctx.handle, q.arena.handle, q.offset, this.arena.handle, ko, vo, c.blockSize, M,
             c.nHead, c.nKvHead, this.D, pastLen, out.offset);
+    }
+    /** q and k turned by positions (i32 [M]) and normed per head where weights are named; q to qOut, k and v to rows slot0 + m. */
+    rotateStore(layer, model, q, k, v, positions, qOut, M, slot0, options) {
+        const o = options || {}, c = this.config;
+        if ([k, v, positions, qOut].some((t) => t.arena !== q.arena)) throw new Error('rotateStore: tensors must share one arena');
+        if (q.length < M * c.nHead * this.D || qOut.length < M * c.nHead * this.D || k.length < M * this.rowLen || v.length < M * this.rowLen ||
+            positions.dtype !== 'i32' || positions.length < M) throw new Error('rotateStore: a tensor is too small or of another type');
+        const weight = (name, length) => {
+            const w = model.f32Weights.get(name);
+            if (!w || (length && w.length !== length)) throw new Error(`missing f32 weight: ${name}`);
+            return w;
+        };
+        const table = weight(o.rope || 'rope');
+        const [ko, vo] = this.offsets(layer);
+        addon.qkNormRope(this.ctx.handle, {
+            tableOff: table.offset, maxPos: table.shape[0], nHead: c.nHead, nKvHead: c.nKvHead, D: this.D, rotDim: table.shape[1], interleaved: 0,
+            qNormOff: o.qNorm ? weight(o.qNorm, this.D).offset : null, kNormOff: o.kNorm ? weight(o.kNorm, this.D).offset : null,
+            normEps: o.eps === undefined ? 1e-6 : o.eps, qStride: 0, kStride: 0, vStride: 0, cacheDtype: this.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32,
+        }, model.weights.handle, q.arena.handle, q.offset, k.offset, v.offset, positions.offset, M, qOut.offset, this.arena.handle, ko, vo,
+        c.blockSize, slot0);
+    }
+    /** GQA attention of M <= 256 drafted rows at pastLen + m; masks: a u64 tensor of treeMasks' words, or null for causal rows. */
+    attendTree(layer, q, out, M, pastLen, masks) {
+        const c = this.config;
+        if (q.arena !== out.arena || (masks && masks.arena !== q.arena)) throw new Error('attendTree: q, out and masks must share one arena');
+        if (q.length < M * c.nHead * this.D || out.length < M * c.nHead * this.D || (masks && (masks.dtype !== 'u64' || masks.length < M * Math.ceil(M / 64))))
+            throw new Error('attendTree: a tensor is too small or of another type');
+        const [ko, vo] = this.offsets(layer);
+        addon.attentionTree(this.ctx.handle, q.arena.handle, q.offset, this.arena.handle, ko, vo, this.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32,
+            c.blockSize, M, c.nHead, c.nKvHead, this.D, pastLen, masks ? masks.offset : null, out.offset);
+    }
+    /** Row pastLen + i of every layer becomes row pastLen + path[i] (i32, i < n): an accepted path of the tree at pastLen. */
+    accept(pastLen, path, n) {
+        if (path.dtype !== 'i32' || path.length < n) throw new Error('accept: path must be an i32 tensor of at least n rows');
+        const T = this.config.blockSize;
+        addon.kvMove(this.ctx.handle, this.arena.handle, this.regions, T, this.arena.handle, this.regions, T, this.rowBytes, pastLen, pastLen, n,
+            path.arena.handle, path.offset);
+    }
+    /** The first rows of every layer into another cache of the same layers, heads and dtype. */
+    fork(to, rows) {
+        if (to.config.nLayer !== this.config.nLayer || to.rowLen !== this.rowLen || to.dtype !== this.dtype)
+            throw new Error('fork: the caches differ in layers, heads or dtype');
+        addon.kvMove(this.ctx.handle, to.arena.handle, to.regions, to.config.blockSize, this.arena.handle, this.regions, this.config.blockSize,
+            this.rowBytes, 0, 0, rows, null, null);
     }
     release() { this.arena.release(); }
 }
@@ -678,5 +766,5 @@ module.exports = {
     expectTensor, f16BitsToF32, readTensorBytes, readTensorF32, ArenaLayout, Arena, Context,
     makeDesc, dequantizeGptqInt4, Tensor, ActivationArena, QuantLinearModel,
     qwenLinearShapes, loadQwenWeights, KvCache, QWEN_LOCAL_DIR, urlToPath, readF16Rows, checkGIdx,
-    countStoredZeros,
+    countStoredZeros, treeMasks,
 };

@@ -497,6 +497,140 @@ static napi_value js_kv_store(napi_env env, napi_callback_info info)
     return NULL;
 }
 
+/* ropeTable(ctx, weights, tableOff, maxPos, rotDim, theta) */
+static napi_value js_rope_table(napi_env env, napi_callback_info info)
+{
+    napi_value argv[6];
+    void *ctx, *w;
+    uint64_t off;
+    int32_t max_pos, rot;
+    double theta;
+    if (get_args(env, info, 6, argv) || get_ptr(env, argv[0], &ctx) || get_ptr(env, argv[1], &w) || get_u64(env, argv[2], &off, 0) ||
+        get_i32(env, argv[3], &max_pos) || get_i32(env, argv[4], &rot))
+        return NULL;
+    CHECK_NAPI(env, napi_get_value_double(env, argv[5], &theta));
+    throw_rc(env, ql_rope_table((ql_ctx*)ctx, (ql_arena*)w, off, max_pos, rot, theta));
+    return NULL;
+}
+
+/* {tableOff, maxPos, nHead, nKvHead, D, rotDim, interleaved, qNormOff|null, kNormOff|null, normEps, qStride, kStride, vStride,
+ *  cacheDtype} -> ql_rope_desc */
+static int get_rope(napi_env env, napi_value obj, ql_rope_desc* d)
+{
+    const struct {
+        const char* name;
+        int32_t* out;
+    } ints[] = {{"maxPos", &d->max_pos}, {"nHead", &d->n_head}, {"nKvHead", &d->n_kv_head}, {"D", &d->D}, {"rotDim", &d->rot_dim},
+                {"interleaved", &d->interleaved}, {"qStride", &d->q_stride}, {"kStride", &d->k_stride}, {"vStride", &d->v_stride},
+                {"cacheDtype", &d->cache_dtype}};
+    napi_value v;
+    double eps;
+    memset(d, 0, sizeof *d);
+    if (prop(env, obj, "tableOff", &v) || get_u64(env, v, &d->table_off, 0)) return 1;
+    if (prop(env, obj, "qNormOff", &v) || get_u64(env, v, &d->q_norm_off, 1)) return 1;
+    if (prop(env, obj, "kNormOff", &v) || get_u64(env, v, &d->k_norm_off, 1)) return 1;
+    for (size_t i = 0; i < sizeof ints / sizeof ints[0]; i++)
+        if (prop(env, obj, ints[i].name, &v) || get_i32(env, v, ints[i].out)) return 1;
+    if (prop(env, obj, "normEps", &v) || napi_get_value_double(env, v, &eps) != napi_ok) {
+        napi_throw_type_error(env, "QL_E_INVALID", "normEps");
+        return 1;
+    }
+    d->norm_eps = (float)eps;
+    return 0;
+}
+
+/* qkNormRope(ctx, rope, weights, act, qOff, kOff, vOff, posOff, M, qOutOff, cache, kCacheOff, vCacheOff, maxT, slot0) */
+static napi_value js_qk_norm_rope(napi_env env, napi_callback_info info)
+{
+    napi_value argv[15];
+    void *ctx, *w, *act, *cache;
+    ql_rope_desc d;
+    uint64_t q, k, v, pos, out, kc, vc;
+    int32_t M, max_t, slot0;
+    if (get_args(env, info, 15, argv) || get_ptr(env, argv[0], &ctx) || get_rope(env, argv[1], &d) || get_ptr(env, argv[2], &w) ||
+        get_ptr(env, argv[3], &act) || get_u64(env, argv[4], &q, 0) || get_u64(env, argv[5], &k, 0) || get_u64(env, argv[6], &v, 0) ||
+        get_u64(env, argv[7], &pos, 0) || get_i32(env, argv[8], &M) || get_u64(env, argv[9], &out, 0) || get_ptr(env, argv[10], &cache) ||
+        get_u64(env, argv[11], &kc, 0) || get_u64(env, argv[12], &vc, 0) || get_i32(env, argv[13], &max_t) || get_i32(env, argv[14], &slot0))
+        return NULL;
+    throw_rc(env, ql_qk_norm_rope((ql_ctx*)ctx, &d, (ql_arena*)w, (ql_arena*)act, q, k, v, pos, M, out, (ql_arena*)cache, kc, vc, max_t, slot0));
+    return NULL;
+}
+
+/* treeMasks(parents Int32Array, masks BigUint64Array [M, ceil(M/64)], depths Int32Array [M]): fills both */
+static napi_value js_tree_masks(napi_env env, napi_callback_info info)
+{
+    napi_value argv[3];
+    void *p, *m, *d;
+    size_t np, nm, nd;
+    if (get_args(env, info, 3, argv) || get_bytes(env, argv[0], &p, &np) || get_bytes(env, argv[1], &m, &nm) ||
+        get_bytes(env, argv[2], &d, &nd))
+        return NULL;
+    const size_t M = np / 4;
+    if (nd < 4 * M || nm < M * ((M + 63) / 64) * 8) {
+        napi_throw_error(env, "QL_E_INVALID", "QL_E_INVALID: masks or depths too short for the parents");
+        return NULL;
+    }
+    throw_rc(env, ql_tree_masks(M > 0x7fffffff ? -1 : (int32_t)M, (const int32_t*)p, (uint64_t*)m, (int32_t*)d));
+    return NULL;
+}
+
+/* attentionTree(ctx, act, qOff, cache, kOff, vOff, cacheDtype, maxT, M, nHead, nKvHead, D, pastLen, maskOff|null, outOff) */
+static napi_value js_attention_tree(napi_env env, napi_callback_info info)
+{
+    napi_value argv[15];
+    void *ctx, *act, *cache;
+    uint64_t q, k, v, mask, out;
+    int32_t i[7];
+    if (get_args(env, info, 15, argv) || get_ptr(env, argv[0], &ctx) || get_ptr(env, argv[1], &act) || get_u64(env, argv[2], &q, 0) ||
+        get_ptr(env, argv[3], &cache) || get_u64(env, argv[4], &k, 0) || get_u64(env, argv[5], &v, 0) || get_u64(env, argv[13], &mask, 1) ||
+        get_u64(env, argv[14], &out, 0))
+        return NULL;
+    for (int n = 0; n < 7; n++)
+        if (get_i32(env, argv[6 + n], &i[n])) return NULL;
+    throw_rc(env, ql_attention_tree((ql_ctx*)ctx, (ql_arena*)act, q, (ql_arena*)cache, k, v, i[0], i[1], i[2], i[3], i[4], i[5], i[6], mask, out));
+    return NULL;
+}
+
+/* tokenLogprobs(ctx, act, logitsOff, stride, M, V, tokensOff, nTok, topK, logprobOff, entropyOff|null, topIdOff, topLogprobOff) */
+static napi_value js_token_logprobs(napi_env env, napi_callback_info info)
+{
+    napi_value argv[13];
+    void *ctx, *act;
+    uint64_t x, tok, lp, ent, id, tlp;
+    int32_t stride, M, V, T, k;
+    if (get_args(env, info, 13, argv) || get_ptr(env, argv[0], &ctx) || get_ptr(env, argv[1], &act) || get_u64(env, argv[2], &x, 0) ||
+        get_i32(env, argv[3], &stride) || get_i32(env, argv[4], &M) || get_i32(env, argv[5], &V) || get_u64(env, argv[6], &tok, 0) ||
+        get_i32(env, argv[7], &T) || get_i32(env, argv[8], &k) || get_u64(env, argv[9], &lp, 0) || get_u64(env, argv[10], &ent, 1) ||
+        get_u64(env, argv[11], &id, 0) || get_u64(env, argv[12], &tlp, 0))
+        return NULL;
+    throw_rc(env, ql_token_logprobs((ql_ctx*)ctx, (ql_arena*)act, x, stride, M, V, tok, T, k, lp, ent, id, tlp));
+    return NULL;
+}
+
+/* kvMove(ctx, dst, dstOffs, dstMaxT, src, srcOffs, srcMaxT, rowBytes, dstRow, srcRow, n, act|null, rowsOff|null) */
+static napi_value js_kv_move(napi_env env, napi_callback_info info)
+{
+    napi_value argv[13];
+    void *ctx, *dst, *src, *act = NULL;
+    uint64_t d[256], s[256], rows;
+    uint32_t count;
+    int32_t dt, st, rb, dr, sr, n;
+    napi_valuetype at;
+    if (get_args(env, info, 13, argv) || get_ptr(env, argv[0], &ctx) || get_ptr(env, argv[1], &dst) || get_i32(env, argv[3], &dt) ||
+        get_ptr(env, argv[4], &src) || get_i32(env, argv[6], &st) || get_i32(env, argv[7], &rb) || get_i32(env, argv[8], &dr) ||
+        get_i32(env, argv[9], &sr) || get_i32(env, argv[10], &n) || get_u64(env, argv[12], &rows, 1))
+        return NULL;
+    CHECK_NAPI(env, napi_typeof(env, argv[11], &at));
+    if (at != napi_null && at != napi_undefined && get_ptr(env, argv[11], &act)) return NULL;
+    if (napi_get_array_length(env, argv[2], &count) != napi_ok || count == 0 || count > 256) {
+        napi_throw_type_error(env, "QL_E_INVALID", "expected an array of 1..256 offsets");
+        return NULL;
+    }
+    if (get_u64_array(env, argv[2], d, count) || get_u64_array(env, argv[5], s, count)) return NULL;
+    throw_rc(env, ql_kv_move((ql_ctx*)ctx, (ql_arena*)dst, d, dt, (ql_arena*)src, s, st, (int32_t)count, rb, dr, sr, n, (ql_arena*)act, rows));
+    return NULL;
+}
+
 /* attention(ctx, act, qOff, cache, kOff, vOff, maxT, M, nHead, nKvHead, D, pastLen, outOff) */
 static napi_value js_attention(napi_env env, napi_callback_info info)
 {
@@ -834,6 +968,16 @@ static napi_value init(napi_env env, napi_value exports)
             napi_set_named_property(env, exports, fns[i].name, f) != napi_ok)
             return NULL;
     }
+    /* speculative decoding, which the reference lacks: not among the enumerable exports, which are its path's */
+    const napi_property_descriptor more[] = {
+        {"ropeTable", NULL, js_rope_table, NULL, NULL, NULL, napi_default, NULL},
+        {"qkNormRope", NULL, js_qk_norm_rope, NULL, NULL, NULL, napi_default, NULL},
+        {"treeMasks", NULL, js_tree_masks, NULL, NULL, NULL, napi_default, NULL},
+        {"attentionTree", NULL, js_attention_tree, NULL, NULL, NULL, napi_default, NULL},
+        {"tokenLogprobs", NULL, js_token_logprobs, NULL, NULL, NULL, napi_default, NULL},
+        {"kvMove", NULL, js_kv_move, NULL, NULL, NULL, napi_default, NULL},
+    };
+    if (napi_define_properties(env, exports, sizeof more / sizeof more[0], more) != napi_ok) return NULL;
     return exports;
 }
 
