@@ -331,6 +331,14 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
     for (int nt = 0; nt < NT; nt++) pair_row(a, kvh, rg * C::kRows + 16 * nt + i16, qm[nt]);
     __syncthreads();
 
+    f16x8 qr[NT][C::kTD][2];                                // fp16 caches leave the registers for q
+    if constexpr (C::kHalf && C::kAhead)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int t = 0; t < C::kTD; t++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) qr[nt][t][i] = qf[(size_t)((t * NT + nt) * 2 + i) * 64 + lane];
     f32x4 acc[C::kDT][NT];
     float mr[NT], l[NT], f[NT];
 #pragma unroll
@@ -377,10 +385,13 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
                     f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int t = 0; t < C::kTD; t++) {
-                        const f16x8* q = qf + (size_t)(t * NT + nt) * 128 + lane;
                         const f16x8 k = __builtin_bit_cast(f16x8, kraw[kt][t]);
-                        lo = mfma(k, q[64], lo);
-                        hi = mfma(k, q[0], hi);
+                        if constexpr (!C::kAhead) {
+#pragma unroll
+                            for (int i = 0; i < 2; i++) qr[nt][t][i] = qf[(size_t)((t * NT + nt) * 2 + i) * 64 + lane];
+                        }
+                        lo = mfma(k, qr[nt][t][1], lo);
+                        hi = mfma(k, qr[nt][t][0], hi);
                     }
 #pragma unroll
                     for (int r = 0; r < 4; r++) s[kt][nt][r] = fmaf(lo[r], 1.f / 2048.f, hi[r]);
