@@ -229,6 +229,28 @@ def test_values_far_apart(ql, ctx, half):
         run(ql, ctx, M, 6, 2, 64, past, half, masks, 18, edit=wide)
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("D", [8, 40, 64, 80, 128, 200, 256])
+def test_short_contexts(ql, ctx, D, half):
+    """A few blocks of keys, every head width, from the first length that has a wave for each of them on."""
+    for M, past in ((1, 128), (9, 150), (9, 225), (40, 190), (1, 470), (16, 500)):
+        print(D, M, past, flush=True)
+        run(ql, ctx, M, 6, 2, D, past, half, ql.tree_masks(tree(M, M))[0], M + past)
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_scores_that_rise(ql, ctx, half):
+    """Scores that rise along the context, slowly and by leaps, and fall: the largest is met last, first or in between."""
+    M, past, D = 9, 1500, 64
+    masks, _ = ql.tree_masks(tree(M, 5))
+    at = np.arange(past + M)
+    for line in (at / 60, at / 5, (past - at) / 60, np.where(at % 200 == 199, at / 20, 0), 12 * np.sin(at / 40)):
+        def edit(c):
+            c.q[:, :, 0] = 4
+            c.k[:, :, 0] = (line * 2).astype(c.k.dtype)[:, None]             # score 1 line
+        run(ql, ctx, M, 4, 2, D, past, half, masks, 20, edit=edit)
+
+
 def test_equal_scores(ql, ctx):
     """A query of zeros: the mean of what is seen, over a long context."""
     for half in (False, True):

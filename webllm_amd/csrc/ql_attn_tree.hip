@@ -4,7 +4,7 @@
 // over the cache's past positions and the drafted rows j (at past + j) whose bit is set in row m's mask. A row that sees
 // nothing is zero; what it does not see it takes nothing from, not even 0 * V.
 //
-// attn_tree_kernel: a workgroup has 16 NT (row, head) pairs of one kv head and a range of key blocks; its four waves take
+// attn_tree_kernel: a workgroup has 16 NT (row, head) pairs of one kv head and a range of key blocks; its four or eight waves take
 // the blocks in turn, so that K and V go from memory to the registers of one wave, with no shared memory and no barrier
 // on the way, and each is split into parts once for 16 NT pairs. Scores are computed transposed, S^T = K Q^T (lane = pair, registers =
 // keys), which leaves a lane with the B fragment of O^T = V^T P^T. V's fragment needs eight keys of one column in a lane: a lane loads
@@ -14,7 +14,7 @@
 //
 // fp32 caches: an operand enters as three bf16 parts, 24 bits with fp32's own range, so no value depends on its neighbours' size; a
 // product is the six largest of the nine (v_mfma_f32_16x16x32_bf16: 6/16 of the fp32 MFMA's time).
-// fp16 caches: K and V enter as they are; q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^14 P. Two products.
+// fp16 caches: K and V enter as they are; q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P. Two products.
 //
 // What the parts cannot carry is not finite: an infinity's remainder is a NaN, and 0 * V is one where V is not. A wave whose sums
 // end that way does its blocks again on the VALU from q, K and V themselves, skipping what a pair does not see (again()).
@@ -35,7 +35,8 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTreeMaxSplit = 128;
 constexpr int kKeys = 32;                // keys of a block
-constexpr float kPScale = 16384.f;       // fp16 parts of P: 2^14 P
+constexpr float kRaise = 7.f;            // log2 that scores may rise above the running reference before it is raised
+constexpr float kPScale = 256.f;         // fp16 parts of P: 2^8 P, at most 2^15
 constexpr float kMaxFinite = 3.4028235e38f;
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -77,7 +78,7 @@ __device__ __forceinline__ f32x4 small_products(const bf16x8 (&a)[3], const bf16
     return mfma(a[0], b[1], c);
 }
 
-template <typename T, int DP, int NT, bool FULL>
+template <typename T, int DP, int NT, bool FULL, int WAVES>
 struct TreeTile {
     static constexpr bool kHalf = std::is_same<T, _Float16>::value;
     static constexpr bool kAhead = DP <= 128;               // a block's K is loaded before the last one's V is used, V before K is
@@ -91,7 +92,7 @@ struct TreeTile {
     typedef typename std::conditional<kHalf, typename std::conditional<kCols == 8, u32x4, u32x2>::type, f32x4>::type VRaw;
     static constexpr int kQBytes = kTD * NT * kParts * 64 * 16;
     static constexpr int kMergeStride = kChunk + 4;
-    static constexpr int kMergeBytes = 4 * kRows * kMergeStride * 4;
+    static constexpr int kMergeBytes = WAVES * kRows * kMergeStride * 4;
     static constexpr int kLds = kQBytes > kMergeBytes ? kQBytes : kMergeBytes;
     // the column of element e of step t of a K or Q fragment, group g
     static __device__ __forceinline__ int kcol(int t, int g, int e) { return kHalf ? 32 * t + 8 * g + e : 32 * t + 16 * (e >> 2) + 4 * g + (e & 3); }
@@ -210,13 +211,13 @@ __device__ __forceinline__ void tree_again(const TreeArgs& a, int kvh, int r0, i
     }
 }
 
-template <typename T, int DP, int NT, bool FULL>
-__global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
+template <typename T, int DP, int NT, bool FULL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs a)
 {
-    using C = TreeTile<T, DP, NT, FULL>;
+    using C = TreeTile<T, DP, NT, FULL, WAVES>;
     using Frag = typename C::Frag;
     __shared__ __attribute__((aligned(16))) char lds[C::kLds];
-    __shared__ float qmax[C::kHalf ? C::kTD : 1][C::kRows], stat[2][4][C::kRows], row_inv[C::kRows];
+    __shared__ float qmax[C::kHalf ? C::kTD : 1][C::kRows], stat[2][WAVES][C::kRows], row_inv[C::kRows];
     __shared__ int row_at[C::kRows];
     const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -233,11 +234,11 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
     const T* vb = static_cast<const T*>(a.v) + (size_t)kvh * D;
 
     // q's fragments (t, nt): a wave has some whole, lane (i, g) eight values of pair i's row
-    constexpr int kUnits = (C::kTD * NT + 3) / 4;
+    constexpr int kUnits = (C::kTD * NT + WAVES - 1) / WAVES;
     float qv[kUnits][8];
 #pragma unroll
     for (int k = 0; k < kUnits; k++) {
-        const int u = wave + 4 * k, t = u / NT, nt = u % NT;
+        const int u = wave + WAVES * k, t = u / NT, nt = u % NT;
         int m;
         const float* q = a.q + (size_t)pair_row(a, kvh, rg * C::kRows + 16 * nt + i16, m) * D;
 #pragma unroll
@@ -286,7 +287,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
     if (C::kHalf) {
 #pragma unroll
         for (int k = 0; k < kUnits; k++) {
-            const int u = wave + 4 * k;
+            const int u = wave + WAVES * k;
             float mx = 0.f;
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(qv[k][e]));
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
     };
 #pragma unroll
     for (int k = 0; k < kUnits; k++) {
-        const int u = wave + 4 * k;
+        const int u = wave + WAVES * k;
         if (u >= C::kTD * NT) break;
         Frag* dst = qf + (size_t)u * C::kParts * 64 + lane;
         if constexpr (C::kHalf) {
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
         for (int d = 0; d < C::kDT; d++) acc[d][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     const int first = b;
-    for (; b < b1; b += 4) {
+    for (; b < b1; b += WAVES) {
         typename C::VRaw vraw[C::kNH][8][C::kNC];           // [32 keys][element of the fragment][columns]
         auto load_v = [&](const TreeBlock& blk, int c0, int c1) {
             const char* base = reinterpret_cast<const char*>(vb + (size_t)blk.at * row_len);
@@ -436,8 +437,8 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
             __builtin_amdgcn_sched_barrier(0);
         }
         const TreeBlock now = blk;
-        const bool more = b + 4 < b1;
-        if (more) blk = tree_block(a, b + 4, past_blocks);
+        const bool more = b + WAVES < b1;
+        if (more) blk = tree_block(a, b + WAVES, past_blocks);
         if (!all_seen)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -446,27 +447,41 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
 #pragma unroll
                     for (int r = 0; r < 4; r++)
                         if (!(seen[nt] >> (16 * kt + r) & 1)) s[kt][nt][r] = -INFINITY;
-        Frag pf[C::kNH][NT][C::kParts];
-        float al[NT];
+        // The exponentials are taken from a reference, a maximum of earlier blocks, and the sums rescaled only where a score has
+        // risen far above it: a maximum over 32 pairs rises a little in almost every block (256 rows after 8000 keys: fp32 212
+        // -> 207 us, fp16 92.2 -> 90.8).
+        float bm[NT];
+        bool up = false;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            float bm = s[0][nt][0];
+            bm[nt] = s[0][nt][0];
 #pragma unroll
             for (int kt = 0; kt < C::kNK; kt++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) bm = fmaxf(bm, s[kt][nt][r]);
-            bm = pair_max<32>(pair_max<16>(bm));
-            const float mn = fmaxf(mr[nt], bm * f[nt]), ref = mn == -INFINITY ? 0.f : mn;
-            al[nt] = ex2(mr[nt] - ref);
-            mr[nt] = mn;
-            float sum = 0.f;
+                for (int r = 0; r < 4; r++) bm[nt] = fmaxf(bm[nt], s[kt][nt][r]);
+            bm[nt] = pair_max<32>(pair_max<16>(bm[nt])) * f[nt];
+            up = up || bm[nt] > mr[nt] + kRaise;
+        }
+        if (__any(up))
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const float mn = fmaxf(mr[nt], bm[nt]), al = ex2(mr[nt] - (mn == -INFINITY ? 0.f : mn));
+                mr[nt] = mn;
+                l[nt] *= al;
+#pragma unroll
+                for (int d = 0; d < C::kDT; d++) acc[d][nt] *= al;
+            }
+        Frag pf[C::kNH][NT][C::kParts];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const float ref = mr[nt] == -INFINITY ? 0.f : mr[nt];
 #pragma unroll
             for (int h = 0; h < C::kNH; h++) {
                 float p[8];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     p[e] = ex2(fmaf(s[2 * h + (e >> 2)][nt][e & 3], f[nt], -ref));
-                    sum += p[e];
+                    l[nt] += p[e];
                 }
                 if constexpr (C::kHalf) {
 #pragma unroll
@@ -479,16 +494,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
                     split_bf16(p, pf[h][nt]);
                 }
             }
-            l[nt] = l[nt] * al[nt] + sum;
         }
-        bool moved = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) moved = moved || al[nt] != 1.f;
-        if (__any(moved))
-#pragma unroll
-            for (int d = 0; d < C::kDT; d++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) acc[d][nt] *= al[nt];
         // a block's sums start from zero and are added to the others by the VALU: the matrix unit carries no long sum
 #pragma unroll
         for (int c = 0; c < C::kNC; c++) {
@@ -551,7 +557,7 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
             for (int r = 0; r < 4; r++) odd = fmaf(acc[d][nt][r], 0.f, odd);
     }
     const bool redo = __any(odd != 0.f);
-    if (redo) tree_again<T, DP, NT, FULL, C::kCols>(a, kvh, rg * C::kRows, first, b1, 4, past_blocks, mr, l, acc);
+    if (redo) tree_again<T, DP, NT, FULL, C::kCols>(a, kvh, rg * C::kRows, first, b1, WAVES, past_blocks, mr, l, acc);
 
     // the four waves' states
     const float unit = C::kHalf && !redo ? 1.f / kPScale : 1.f;
@@ -569,15 +575,19 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         const int r = 16 * nt + i16;
-        const float mx = fmaxf(fmaxf(stat[0][0][r], stat[0][1][r]), fmaxf(stat[0][2][r], stat[0][3][r]));
+        float mx = stat[0][0][r];
+#pragma unroll
+        for (int k = 1; k < WAVES; k++) mx = fmaxf(mx, stat[0][k][r]);
         w[nt] = mr[nt] == -INFINITY ? (l[nt] != l[nt] ? 1.f : 0.f) : ex2(mr[nt] - mx) * unit;   // NaN: no score is a number
     }
     if (tid < C::kRows) {                                   // what a row's sums are divided by, or its state, and its place
         const int r = rg * C::kRows + tid;
-        const float mx = fmaxf(fmaxf(stat[0][0][tid], stat[0][1][tid]), fmaxf(stat[0][2][tid], stat[0][3][tid]));
+        float mx = stat[0][0][tid];
+#pragma unroll
+        for (int k = 1; k < WAVES; k++) mx = fmaxf(mx, stat[0][k][tid]);
         float total = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < WAVES; k++) {
             const float lk = stat[1][k][tid], mk = stat[0][k][tid];
             total += mk == -INFINITY ? (lk != lk ? lk : 0.f) : lk * ex2(mk - mx);
         }
@@ -609,12 +619,12 @@ __global__ __launch_bounds__(256, 2) void attn_tree_kernel(const TreeArgs a)
         }
         __syncthreads();
 #pragma unroll
-        for (int u = tid; u < C::kRows * (C::kChunk / 4); u += 256) {
+        for (int u = tid; u < C::kRows * (C::kChunk / 4); u += 64 * WAVES) {
             const int row = u / (C::kChunk / 4), c4 = u % (C::kChunk / 4), d = C::kChunk * c + 4 * c4, at = row_at[row];
             if (at < 0 || (!FULL && d >= D)) continue;
             f32x4 sum = *reinterpret_cast<const f32x4*>(merge + (size_t)row * C::kMergeStride + 4 * c4);
 #pragma unroll
-            for (int k = 1; k < 4; k++) sum += *reinterpret_cast<const f32x4*>(merge + (size_t)(k * C::kRows + row) * C::kMergeStride + 4 * c4);
+            for (int k = 1; k < WAVES; k++) sum += *reinterpret_cast<const f32x4*>(merge + (size_t)(k * C::kRows + row) * C::kMergeStride + 4 * c4);
             const float inv = row_inv[row];
             st_global(reinterpret_cast<f32x4*>(out + (size_t)at * a.nsplit * D + d), f32x4{sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv});
         }
@@ -721,14 +731,14 @@ __global__ __launch_bounds__(256) void attn_tree_merge_kernel(const TreeArgs a)
 typedef void (*TreeFn)(TreeArgs);
 
 template <typename T>
-TreeFn tree_fn(int D, int nt)
+TreeFn tree_fn(int D, int nt, int waves)
 {
-    if (D == 64) return nt == 2 ? attn_tree_kernel<T, 64, 2, true> : attn_tree_kernel<T, 64, 1, true>;
-    if (D == 128) return nt == 2 ? attn_tree_kernel<T, 128, 2, true> : attn_tree_kernel<T, 128, 1, true>;
-    if (D == 256) return attn_tree_kernel<T, 256, 1, true>;
-    if (D < 64) return attn_tree_kernel<T, 64, 1, false>;
-    if (D < 128) return attn_tree_kernel<T, 128, 1, false>;
-    return attn_tree_kernel<T, 256, 1, false>;
+    if (D == 64) return waves == 8 ? attn_tree_kernel<T, 64, 1, true, 8> : nt == 2 ? attn_tree_kernel<T, 64, 2, true, 4> : attn_tree_kernel<T, 64, 1, true, 4>;
+    if (D == 128) return waves == 8 ? attn_tree_kernel<T, 128, 1, true, 8> : nt == 2 ? attn_tree_kernel<T, 128, 2, true, 4> : attn_tree_kernel<T, 128, 1, true, 4>;
+    if (D == 256) return waves == 8 ? attn_tree_kernel<T, 256, 1, true, 8> : attn_tree_kernel<T, 256, 1, true, 4>;
+    if (D < 64) return waves == 8 ? attn_tree_kernel<T, 64, 1, false, 8> : attn_tree_kernel<T, 64, 1, false, 4>;
+    if (D < 128) return waves == 8 ? attn_tree_kernel<T, 128, 1, false, 8> : attn_tree_kernel<T, 128, 1, false, 4>;
+    return waves == 8 ? attn_tree_kernel<T, 256, 1, false, 8> : attn_tree_kernel<T, 256, 1, false, 4>;
 }
 
 }  // namespace
@@ -743,16 +753,23 @@ uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes)
     // 11.3, 13.5, 4 after 4000 12.1, 14.2, 24 after 4000 29.0, 25.2; fp16 16 after 4000 14.4, 16.4, 24 after 4000 18.3 both.
     const long full = (long)((R + 31) / 32) * a->KV * ((a->past + a->M + 4 * kKeys - 1) / (4 * kKeys));
     a->nt = (a->D == 64 || a->D == 128) && full >= (a->half ? 1024 : 512) ? 2 : 1;
-    a->groups = (R + 16 * a->nt - 1) / (16 * a->nt);
     a->past_blocks = (a->past + kKeys - 1) / kKeys;
     const int blocks = a->blocks = a->past_blocks + (a->M + kKeys - 1) / kKeys;
+    // Short contexts: one range of 8 waves and no merge launch, while a wave has two blocks or (keys of over 256 bytes) one and
+    // an XCD, which then has whole kv heads only, has a workgroup a CU. Eight waves against four with ranges, in us: 5 rows
+    // after 300 keys (14 / 2 heads of 64, fp32) 8.1, 9.5, 40 after 200 (fp16) 6.1, 8.8; 28 / 4 heads of 128: 16 after 200
+    // (fp32) 10.7, 12.0, 64 after 100 10.2, 12.8, and beyond these limits 8 after 300 12.6, 11.8, 8 after 700 (fp16) 11.0, 9.5,
+    // 128 after 100 20.7, 17.9, 128 after none 16.8, 11.5.
+    a->waves = 4;
+    if (blocks > 4 && blocks <= (a->D * (a->half ? 2 : 4) > 256 ? 8 : 16) && (R + 15) / 16 * ((a->KV + 7) / 8) <= 32) a->waves = 8, a->nt = 1;
+    a->groups = (R + 16 * a->nt - 1) / (16 * a->nt);
     const size_t one = (size_t)a->M * a->H * (a->D + 2) * sizeof(float);
     const int fit = (int)std::min<size_t>(kTreeMaxSplit, ws_bytes / one);
     // key ranges that keep every XCD's 32 CUs within `each` workgroups: a (kv head, range)'s groups are on one of them
     auto ranges = [&](int each) { return 8 * (32 * each / a->groups) / a->KV; };
     // up to two workgroups a CU, at least a block a wave, as many as the workspace holds
-    const int s = std::max(1, std::min({ranges(2), (blocks + 3) / 4, fit}));
-    a->per = ((blocks + s - 1) / s + 3) / 4 * 4;            // as many for each of the waves
+    const int s = a->waves == 8 ? 1 : std::max(1, std::min({ranges(2), (blocks + 3) / 4, fit}));
+    a->per = ((blocks + s - 1) / s + a->waves - 1) / a->waves * a->waves;            // as many for each of the waves
     a->nsplit = (blocks + a->per - 1) / a->per;
     a->inv_nsplit = 1.f / a->nsplit;
     a->inv_g = 1.f / a->G;
@@ -766,8 +783,8 @@ hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t stream)
         else hipLaunchKernelGGL(attn_tree_row_kernel<float>, dim3(a.H, a.M), dim3(64), 0, stream, a);
         return hipGetLastError();
     }
-    const TreeFn fn = a.half ? tree_fn<_Float16>(a.D, a.nt) : tree_fn<float>(a.D, a.nt);
-    hipLaunchKernelGGL(fn, dim3(8 * a.groups, (a.KV * a.nsplit + 7) / 8), dim3(256), 0, stream, a);
+    const TreeFn fn = a.half ? tree_fn<_Float16>(a.D, a.nt, a.waves) : tree_fn<float>(a.D, a.nt, a.waves);
+    hipLaunchKernelGGL(fn, dim3(8 * a.groups, (a.KV * a.nsplit + 7) / 8), dim3(64 * a.waves), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
     hipLaunchKernelGGL(attn_tree_merge_kernel, dim3(a.H, a.M), dim3(256), 0, stream, a);

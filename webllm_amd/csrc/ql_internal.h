@@ -326,6 +326,7 @@ struct TreeArgs {
     float scale;               // fp32(log2(e) / sqrt(D))
     // plan_attention_tree fills these: 16 nt pairs a workgroup, groups of them; blocks of 32 keys, key ranges of `per` of them
     int nt, groups, past_blocks, blocks, per, nsplit;
+    int waves;                 // of a workgroup
     float inv_nsplit, inv_g;
 };
 uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes);   // the workspace it needs
