@@ -293,8 +293,8 @@ int ql_rope_table(ql_ctx* ctx, ql_arena* weights, uint64_t table_off, int32_t ma
 /* q and k RMSNormed per head (where the descriptor has weights) and turned by pos[m], q to q_out [M, n_head, D], k and v
  * to rows slot0 + m of the caches [max_t, n_kv_head * D] (fp16: rounded once). pos is int32 [M] in `act`. A row whose position
  * is not in 0..max_pos-1 is padding: its q_out row and its cache rows stay as they were. q_out may be q itself (same
- * offset, dense rows); any other overlap of what is written with what is read fails with QL_E_INVALID. M = 1..65535;
- * slot0 + M > max_t fails with QL_E_RANGE. Offsets 16-byte aligned (pos: 4). */
+ * offset, dense rows); any other overlap of what is written with what is read fails with QL_E_INVALID. M = 1..65535,
+ * M * (n_head + 2 n_kv_head) <= 2^26; slot0 + M > max_t fails with QL_E_RANGE. Offsets 16-byte aligned (pos: 4). */
 int ql_qk_norm_rope(ql_ctx* ctx, const ql_rope_desc* desc, const ql_arena* weights, ql_arena* act, uint64_t q_off, uint64_t k_off,
                     uint64_t v_off, uint64_t pos_off, int32_t M, uint64_t q_out_off, ql_arena* cache, uint64_t k_cache_off,
                     uint64_t v_cache_off, int32_t max_t, int32_t slot0);

@@ -217,6 +217,8 @@ def test_refusals(ql, ctx):
     for bad in ((16, 12, 1e4), (16, 264, 1e4), (16, 32, 0.0), (16, 32, float("inf")), (1 << 20, 32, 1e4)):
         with pytest.raises(ql.QlError):
             ctx.rope_table(w.arena, 0, *bad)
+    for change in ({"n_head": 1024}, {"n_kv_head": 4096}):                   # heads of all rows past 2^26
+        refused("QL_E_INVALID", at={7: 65535, 12: 1 << 20}, **change)
     ctx.qk_norm_rope(*args)                                                  # the unchanged call runs
     for b in boxes:
         b.release()

@@ -2650,6 +2650,7 @@ int ql_qk_norm_rope(ql_ctx* ctx, const ql_rope_desc* d, const ql_arena* weights,
     if (!ctx || !d || !weights || !act || !cache) return fail(QL_E_INVALID, "null context, descriptor or arena");
     if (M < 1 || M > 65535) return fail(QL_E_INVALID, "M must be 1..65535 (got %d)", M);
     if (d->n_head < 1 || d->n_head > 4096 || d->n_kv_head < 1 || d->n_kv_head > 4096) return fail(QL_E_INVALID, "n_head and n_kv_head must be 1..4096");
+    if ((int64_t)M * (d->n_head + 2 * d->n_kv_head) > ql::kRopeMaxHeads) return fail(QL_E_INVALID, "M x (n_head + 2 n_kv_head) above %d", ql::kRopeMaxHeads);
     if (d->D < 8 || d->D > ql::kRopeMaxD || d->D % 8) return fail(QL_E_INVALID, "head dim must be 8..%d, a multiple of 8 (got %d)", ql::kRopeMaxD, d->D);
     if (d->rot_dim < 8 || d->rot_dim > d->D || d->rot_dim % 8) return fail(QL_E_INVALID, "rot_dim must be 8..D, a multiple of 8 (got %d)", d->rot_dim);
     if (d->max_pos < 1 || (d->interleaved & ~1) || d->reserved) return fail(QL_E_INVALID, "max_pos must be positive, interleaved 0 or 1, reserved 0");

@@ -301,6 +301,7 @@ hipError_t launch_kv_store(const float* src, float* dst, int rows, int row_len, 
 // Speculative decoding: rotation and store, attention of a drafted tree, log probabilities, cache rows moved.
 
 constexpr int kRopeMaxD = 256;
+constexpr int kRopeMaxHeads = 1 << 26;           // of a call, all rows': 32 lanes each are counted in 32 bits
 struct RopeArgs {
     const float *q, *k, *v;    // rows of H or KV heads, strides in values
     const float *q_norm, *k_norm;   // [D] or nullptr

@@ -8,9 +8,12 @@
 // logprob_scan_kernel reads the logits, once: a wave has a unit of 1024 of a row in registers, and leaves the unit's (m, S, sum (x - m)
 // e^(x - m)) and, where alternatives are wanted, the largest (value, index) of each of its four parts of 256. No LDS, no barrier.
 // logprob_row_kernel joins a row's units, and finds the top k exactly from the parts' largest: a part whose largest is not
-// among the k largest of those has none of the top k (k others are larger), so the k parts that are hold them all; what
-// lies below the smallest of those k is left out, and the rest is sorted. Whatever the logits, that is k * 256 of them at most.
-// Bound: 4 bytes a logit from memory; with few rows the two launches and their chains of loads.
+// among the k largest of those has none of the top k (k others are larger), so the k parts that are hold them all, and what
+// lies below the smallest of those k is left out. Where more than 256 are left (a masked row's are all alike) the same is done once
+// more with the threads' largest, of eight each, which leaves 8 k at most; the rest is sorted.
+// Bound: 4 bytes a logit from memory: 512 rows of 152064 take 55.4 us, 5.6 TB/s. With few rows the two launches and their chains
+// of loads: 1 row 7.2 us, with alternatives 9.9; 24 rows 8.0, with 20 alternatives 13.7, and 17.6 where a row is masked whole
+// (22.2 with one sort of all that is alike).
 #include <algorithm>
 #include <cmath>
 
@@ -170,28 +173,47 @@ __device__ __forceinline__ uint64_t largest64(F key, int n, int k, uint64_t* lis
 // A row's units joined by one wave: what log probabilities are measured from, and the tokens' and the entropy.
 __device__ __forceinline__ void join_units(const LogprobArgs& a, size_t row, int lane, float& ref, float& ls, bool& none)
 {
+    constexpr int kFirst = 4;                             // units a lane has at once, the first with the first token's logit
     const f32x4* st = reinterpret_cast<const f32x4*>(a.stat) + row * a.units;
+    const float* x = a.logits + row * a.stride;
+    const f32x4 empty = {-INFINITY, 0.f, 0.f, 0.f};
+    f32x4 u[kFirst];
+#pragma unroll
+    for (int i = 0; i < kFirst; i++) u[i] = lane + 64 * i < a.units ? ld_global(st + lane + 64 * i) : empty;
+    auto logit = [&](int i, bool& there) {
+        const int tok = ld_global(a.tokens + row * a.n_tok + i);
+        there = tok >= 0 && tok < a.V;
+        return there ? ld_global(x + tok) : 0.f;
+    };
+    bool there = false;
+    const float xt = lane < a.n_tok ? logit(lane, there) : 0.f;
     float m = -INFINITY;
-    for (int i = lane; i < a.units; i += 64) m = fmaxf(m, ld_global(st + i).x);
+#pragma unroll
+    for (int i = 0; i < kFirst; i++) m = fmaxf(m, u[i].x);
+    for (int i = lane + 64 * kFirst; i < a.units; i += 64) m = fmaxf(m, ld_global(st + i).x);
     m = wave_max(m, lane);
     ref = m == -INFINITY ? 0.f : m;
     float s = 0.f, t = 0.f;
-    for (int i = lane; i < a.units; i += 64) {
-        const f32x4 u = ld_global(st + i);
+    auto add = [&](const f32x4& u) {
         const float d = u.x == -INFINITY ? 0.f : u.x - ref, e = __builtin_amdgcn_exp2f(d * kLog2e);
         s = fmaf(u.y, e, s);
         t += e == 0.f ? 0.f : fmaf(d, u.y, u.z) * e;      // d may be too far down for d * u.y
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < kFirst; i++) add(u[i]);
+    for (int i = lane + 64 * kFirst; i < a.units; i += 64) add(ld_global(st + i));
     s = wave_sum(s, lane);
     t = wave_sum(t, lane);
     none = s == 0.f;
     ls = logf(s);
     if (lane == 0 && a.entropy) st_global(a.entropy + row, none ? 0.f : ls - t / s);
-    const float* x = a.logits + row * a.stride;
-    for (int i = lane; i < a.n_tok; i += 64) {
-        const int tok = ld_global(a.tokens + row * a.n_tok + i);
-        const bool there = tok >= 0 && tok < a.V;
-        st_global(a.logprob + row * a.n_tok + i, !there ? 0.f : none ? -INFINITY : ld_global(x + tok) - ref - ls);
+    auto put = [&](int i, bool there, float x) {
+        st_global(a.logprob + row * a.n_tok + i, !there ? 0.f : none ? -INFINITY : x - ref - ls);
+    };
+    if (lane < a.n_tok) put(lane, there, xt);
+    for (int i = lane + 64; i < a.n_tok; i += 64) {
+        const float xi = logit(i, there);
+        put(i, there, xi);
     }
 }
 
@@ -204,9 +226,11 @@ __global__ __launch_bounds__(64) void logprob_row_kernel(const LogprobArgs a)
 
 __global__ __launch_bounds__(64 * kWaves) void logprob_top_kernel(const LogprobArgs a)
 {
-    __shared__ uint64_t list[64 * kWaves], found[kLogprobMaxTop * kPart];
+    constexpr int kOwn = (kLogprobMaxTop + kWaves - 1) / kWaves, kKeysOwn = 4 * kOwn;   // parts of a wave, logits of a thread
+    constexpr int kFound = kLogprobMaxTop * kKeysOwn;
+    __shared__ uint64_t list[64 * kWaves], found[kFound];
     __shared__ float norm[3];
-    __shared__ int count;
+    __shared__ int count[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.top_k;
     const size_t row = blockIdx.x;
     if (wave == kWaves - 1) {
@@ -217,7 +241,7 @@ __global__ __launch_bounds__(64 * kWaves) void logprob_top_kernel(const LogprobA
             norm[0] = ref;
             norm[1] = ls;
             norm[2] = none;
-            count = 0;
+            count[0] = count[1] = 0;
         }
     }
     const int parts = a.units * kParts;
@@ -225,27 +249,47 @@ __global__ __launch_bounds__(64 * kWaves) void logprob_top_kernel(const LogprobA
     const uint64_t p = largest64([&](int i) { return ld_global(best + i); }, parts, k, list, wave, lane);
     if (wave == 0) list[lane] = p;
     __syncthreads();
-    const uint64_t least = list[k - 1] ? list[k - 1] : 1;
     const float* x = a.logits + row * a.stride;
-    for (int q = wave; q < k; q += kWaves) {
-        const uint64_t key = list[q];
-        if (!key) continue;
+    uint64_t e[kKeysOwn], most = 0;
+#pragma unroll
+    for (int o = 0; o < kOwn; o++) {
+        const uint64_t key = wave + o * kWaves < k ? list[wave + o * kWaves] : 0;
         const uint32_t at = ~(uint32_t)key;               // a part: 64 neighbours of each 256 of its unit
         const int i0 = (at & ~(kUnit - 1u)) + kPart * (lane >> 4) + (at & 192u) + 4 * (lane & 15);
-        const f32x4 v = load4(x, i0, a.V);
+        const f32x4 v = key ? load4(x, i0, a.V) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < 4; c++) {
-            const uint64_t e = i0 + c < a.V ? key_of(order_bits(v[c]), i0 + c) : 0;
-            const uint64_t in = __ballot(e >= least);
-            if (!in) continue;
-            int base = 0;
-            if (lane == 0) base = atomicAdd(&count, __popcll(in));
-            base = __shfl(base, 0);
-            if (e >= least) found[base + __popcll(in & ((1ull << lane) - 1))] = e;
+            e[4 * o + c] = key && i0 + c < a.V ? key_of(order_bits(v[c]), i0 + c) : 0;
+            most = larger(most, e[4 * o + c]);
         }
     }
+    uint64_t least = list[k - 1] ? list[k - 1] : 1;
+    // the wave's logits from `least` on, and their place behind the other waves'
+    auto place = [&](int* total) {
+        int mine = 0;
+#pragma unroll
+        for (int c = 0; c < kKeysOwn; c++) mine += __popcll(__ballot(e[c] >= least));
+        int base = 0;
+        if (lane == 0 && mine) base = atomicAdd(total, mine);
+        return __builtin_amdgcn_readfirstlane(base);
+    };
+    int base = place(&count[0]);
     __syncthreads();
-    const int n = count;
+    int n = count[0];
+    if (n > kFound) {                                     // many are alike: once more, from the threads' largest
+        largest64([&](int) { return most; }, 64 * kWaves, k, list, wave, lane);
+        least = list[k - 1];
+        base = place(&count[1]);
+        __syncthreads();
+        n = count[1];
+    }
+#pragma unroll
+    for (int c = 0; c < kKeysOwn; c++) {
+        const uint64_t in = __ballot(e[c] >= least);
+        if (e[c] >= least) found[base + __popcll(in & ((1ull << lane) - 1))] = e[c];
+        base += __popcll(in);
+    }
+    __syncthreads();
     const uint64_t top = largest64([&](int i) { return found[i]; }, n, k, list, wave, lane);
     if (wave == 0 && lane < k) {
         const bool none = norm[2] != 0.f;
