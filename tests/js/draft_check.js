@@ -74,6 +74,11 @@ function gpu(dir) {
         errors.path = message(() => kv.accept(0, P, c.path + 1));
         errors.missing = message(() => kv.rotateStore(1, model, Q, K, V, pos, QR, M, 0, { kNorm: 'nothing' }));
         errors.pair = message(() => model.tokenLogprobs(X, M, c.V, { tokens: tok }));
+        const H = pool.alloc([M, cfg.nEmbd], 'f16');
+        errors.half = message(() => kv.attendTree(0, H, O, M, 0, W));
+        errors.halfOut = message(() => kv.rotateStore(1, model, Q, K, V, pos, H, M, 0));
+        errors.regions = message(() => q.addon.kvMove(ctx.handle, kv.arena.handle, [0, kv.region], cfg.blockSize, other.arena.handle, [0], cfg.blockSize,
+            kv.rowBytes, 0, 0, 1, null, null));
         kv.release();
         other.release();
         pool.reset();

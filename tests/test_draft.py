@@ -92,6 +92,7 @@ def test_node_drafted_pass(tmp_path):
     assert "fp16 cache" in errors["store"] and "fp16 cache" in errors["attend"] and "another type" in errors["type"]
     assert "QL_E_RANGE" in errors["range"] and "at least n" in errors["path"] and "missing f32 weight" in errors["missing"]
     assert "come with" in errors["pair"] and "dtype" in errors["dtype"]
+    assert "another type" in errors["half"] and "another type" in errors["halfOut"] and "as many source offsets" in errors["regions"]
 
 
 # ------------------------------------------------------------------ a model's pass, from embedding to accepted path
@@ -266,4 +267,24 @@ def test_host_refusals(ctx):
     with pytest.raises(ql.QlError):
         kv.rotate_store(0, model, q, k, k, pos, o, 4, CFG.block_size - 3)
     for x in (kv, half, pool.arena, model):
+        x.release()
+
+
+@pytest.mark.gpu
+def test_types_of_a_drafted_pass(ctx):
+    """Tensors of another type than the calls read and write are refused before anything runs."""
+    kv, pool, model = gptq.KvCache(ctx, CFG), gptq.ActivationArena(ctx, 4 << 20), gptq.QuantLinearModel(ctx, 1 << 20)
+    C, KVD = CFG.n_embd, gptq.qwen_kv_dim(CFG)
+    q, k, o, pos, half, word = (pool.alloc(s, t) for s, t in (((4, C), "f32"), ((4, KVD), "f32"), ((4, C), "f32"), ((4,), "i32"), ((4, C), "f16"), ((4, C), "u32")))
+    model.make_rope_table(64, 64, 1e4)
+    model.f32["line"] = gptq.Tensor(model.weights, 0, 64, (64,), "f32")
+    bad = [lambda: kv.rotate_store(0, model, half, k, k, pos, o, 4, 0), lambda: kv.rotate_store(0, model, q, half, k, pos, o, 4, 0),
+           lambda: kv.rotate_store(0, model, q, k, word, pos, o, 4, 0), lambda: kv.rotate_store(0, model, q, k, k, pos, half, 4, 0),
+           lambda: kv.rotate_store(0, model, q, k, k, pos, o, 4, 0, rope="line"), lambda: kv.attend_tree(0, half, o, 4, 0),
+           lambda: kv.attend_tree(0, q, half, 4, 0), lambda: model.token_logprobs(q, 4, C, entropy=half),
+           lambda: model.token_logprobs(q, 4, C, tokens=pos, logprobs=half), lambda: model.token_logprobs(q, 0, C, tokens=pos, logprobs=o)]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    for x in (kv, pool.arena, model):
         x.release()

@@ -204,6 +204,23 @@ def test_not_finite_in_the_context(ql, ctx, half):
 
 
 @pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("past", [4, 40, 300, 3000])
+def test_scores_all_minus_infinity(ql, ctx, past, half):
+    """No score above -inf: the row is zero, as one that sees nothing; rows of other heads are as the formula has them."""
+    M = 3
+    def edit(c):
+        c.q[:, 2:] = np.abs(c.q[:, 2:])
+        c.k[:, 1] = -np.inf
+    c = Call(ql, ctx, M, 4, 2, 64, past, half, None, 21, edit=edit)
+    ctx.attention_tree(*c.args)
+    want, tol = formula(c.q[:, :2], c.k[:, :1], c.v[:, :1], seen_of(None, M, past))
+    got = c.out().astype(np.float64)
+    assert (got[:, 2:] == 0).all()
+    assert (np.abs(got[:, :2] - want) <= tol).all()
+    c.release()
+
+
+@pytest.mark.parametrize("half", [False, True])
 def test_values_far_apart(ql, ctx, half):
     """Scores that one key decides, large and small values side by side in q, K and V."""
     M, past = 10, 500

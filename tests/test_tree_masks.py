@@ -52,3 +52,9 @@ def test_null_handles(ql):
     assert L.ql_token_logprobs(None, None, 0, 1, 1, 1, 0, 0, 0, 0, 0, 0, 0) == -10
     assert L.ql_kv_move(None, None, None, 1, None, None, 1, 1, 16, 0, 0, 1, None, none) == -10
     assert ctypes.sizeof(ql.RopeDesc) == 3 * 8 + 12 * 4
+
+
+def test_parents_past_32_bits(ql):
+    for parents in (np.array([-1, 2**32 - 1]), np.array([-1, 2**32]), np.array([-(2**40), 0])):
+        with pytest.raises(ql.QlError):
+            ql.tree_masks(parents)

@@ -303,12 +303,14 @@ class KvCache:
             raise ValueError("rotate_store: q/q_out smaller than [M, n_head * D]")
         if k.length < M * self.row_len or v.length < M * self.row_len:
             raise ValueError("rotate_store: k/v smaller than [M, n_kv_head * D]")
+        if any(t.dtype != "f32" for t in (q, k, v, q_out)):
+            raise ValueError("rotate_store: q, k, v and q_out must be f32")
         if positions.dtype != "i32" or positions.length < M:
             raise ValueError("rotate_store: positions must be an i32 tensor of at least M")
         if any(t.arena is not q.arena for t in (k, v, positions, q_out)):
             raise ValueError("rotate_store: tensors must live in one activation arena")
         table = model.f32.get(rope)
-        if table is None:
+        if table is None or len(table.shape) != 2:
             raise ValueError(f"missing rope table: {rope}")
         norms = [None if n is None else model.f32.get(n) for n in (q_norm, k_norm)]
         for name, w in zip((q_norm, k_norm), norms):
@@ -327,6 +329,8 @@ class KvCache:
         c = self.config
         if q.length < M * c.n_head * self.D or out.length < M * c.n_head * self.D:
             raise ValueError("attend_tree: q/out smaller than [M, n_head * D]")
+        if q.dtype != "f32" or out.dtype != "f32":
+            raise ValueError("attend_tree: q and out must be f32")
         if masks is not None and (masks.dtype != "u64" or masks.length < M * -(-M // 64)):
             raise ValueError("attend_tree: masks must be a u64 tensor [M, ceil(M/64)]")
         if q.arena is not out.arena or (masks is not None and masks.arena is not q.arena):
@@ -507,7 +511,9 @@ class QuantLinearModel:
         given = [t for t in (tokens, logprobs, entropy, top_ids, top_logprobs) if t is not None]
         if any(t.arena is not logits.arena for t in given):
             raise ValueError("token_logprobs: tensors must live in the logits' arena")
-        if logits.dtype != "f32" or logits.length < M * V:
+        if any(t.dtype != "f32" for t in (logprobs, entropy, top_logprobs) if t is not None):
+            raise ValueError("token_logprobs: results are f32, top_ids i32")
+        if M < 1 or logits.dtype != "f32" or logits.length < M * V:
             raise ValueError("token_logprobs: logits must be f32 [M, V]")
         T = 0 if tokens is None else tokens.length // M
         k = 0 if top_ids is None else top_ids.length // M

@@ -476,7 +476,7 @@ class QuantLinearModel {
             if (t && t.arena !== logits.arena) throw new Error('tokenLogprobs: tensors must share one arena');
         }
         const T = o.tokens ? Math.floor(o.tokens.length / M) : 0, k = o.topIds ? Math.floor(o.topIds.length / M) : 0;
-        if (logits.length < M * V || (o.tokens && (o.tokens.dtype !== 'i32' || o.logprobs.length < M * T)) || (o.entropy && o.entropy.length < M) ||
+        if (!(M >= 1) || logits.dtype !== 'f32' || [o.logprobs, o.entropy, o.topLogprobs].some((t) => t && t.dtype !== 'f32') || logits.length < M * V || (o.tokens && (o.tokens.dtype !== 'i32' || o.logprobs.length < M * T)) || (o.entropy && o.entropy.length < M) ||
             (o.topIds && (o.topIds.dtype !== 'i32' || o.topLogprobs.length < M * k))) throw new Error('tokenLogprobs: a tensor is too small or of another type');
         const off = (t) => (t ? t.offset : 0);
         addon.tokenLogprobs(this.ctx.handle, logits.arena.handle, logits.offset, V, M, V, off(o.tokens), T, k, off(o.logprobs),
@@ -718,10 +718,10 @@ class KvCache {
         const o = options || {}, c = this.config;
         if ([k, v, positions, qOut].some((t) => t.arena !== q.arena)) throw new Error('rotateStore: tensors must share one arena');
         if (q.length < M * c.nHead * this.D || qOut.length < M * c.nHead * this.D || k.length < M * this.rowLen || v.length < M * this.rowLen ||
-            positions.dtype !== 'i32' || positions.length < M) throw new Error('rotateStore: a tensor is too small or of another type');
+            [q, k, v, qOut].some((t) => t.dtype !== 'f32') || positions.dtype !== 'i32' || positions.length < M) throw new Error('rotateStore: a tensor is too small or of another type');
         const weight = (name, length) => {
             const w = model.f32Weights.get(name);
-            if (!w || (length && w.length !== length)) throw new Error(`missing f32 weight: ${name}`);
+            if (!w || (length ? w.length !== length : w.shape.length !== 2)) throw new Error(`missing f32 weight: ${name}`);
             return w;
         };
         const table = weight(o.rope || 'rope');
@@ -737,7 +737,7 @@ class KvCache {
     attendTree(layer, q, out, M, pastLen, masks) {
         const c = this.config;
         if (q.arena !== out.arena || (masks && masks.arena !== q.arena)) throw new Error('attendTree: q, out and masks must share one arena');
-        if (q.length < M * c.nHead * this.D || out.length < M * c.nHead * this.D || (masks && (masks.dtype !== 'u64' || masks.length < M * Math.ceil(M / 64))))
+        if (q.dtype !== 'f32' || out.dtype !== 'f32' || q.length < M * c.nHead * this.D || out.length < M * c.nHead * this.D || (masks && (masks.dtype !== 'u64' || masks.length < M * Math.ceil(M / 64))))
             throw new Error('attendTree: a tensor is too small or of another type');
         const [ko, vo] = this.offsets(layer);
         addon.attentionTree(this.ctx.handle, q.arena.handle, q.offset, this.arena.handle, ko, vo, this.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32,

@@ -613,7 +613,7 @@ static napi_value js_kv_move(napi_env env, napi_callback_info info)
     napi_value argv[13];
     void *ctx, *dst, *src, *act = NULL;
     uint64_t d[256], s[256], rows;
-    uint32_t count;
+    uint32_t count, ns;
     int32_t dt, st, rb, dr, sr, n;
     napi_valuetype at;
     if (get_args(env, info, 13, argv) || get_ptr(env, argv[0], &ctx) || get_ptr(env, argv[1], &dst) || get_i32(env, argv[3], &dt) ||
@@ -624,6 +624,10 @@ static napi_value js_kv_move(napi_env env, napi_callback_info info)
     if (at != napi_null && at != napi_undefined && get_ptr(env, argv[11], &act)) return NULL;
     if (napi_get_array_length(env, argv[2], &count) != napi_ok || count == 0 || count > 256) {
         napi_throw_type_error(env, "QL_E_INVALID", "expected an array of 1..256 offsets");
+        return NULL;
+    }
+    if (napi_get_array_length(env, argv[5], &ns) != napi_ok || ns != count) {
+        napi_throw_type_error(env, "QL_E_INVALID", "expected as many source offsets as destination offsets");
         return NULL;
     }
     if (get_u64_array(env, argv[2], d, count) || get_u64_array(env, argv[5], s, count)) return NULL;

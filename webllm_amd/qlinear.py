@@ -229,7 +229,7 @@ def plan_attention(max_t: int, M: int, n_head: int, n_kv_head: int, D: int, past
 def tree_masks(parents) -> tuple[np.ndarray, np.ndarray]:
     """(masks uint64 [M, ceil(M/64)], depths int32 [M]) of a drafted tree: parents[m] is -1 (continues the context) or an earlier
     row (host only)."""
-    p = np.ascontiguousarray(parents, dtype=np.int32)
+    p = np.ascontiguousarray(np.clip(parents, -2, 2**31 - 1), dtype=np.int32)
     M = p.size
     masks, depths = np.empty((M, (M + 63) // 64), np.uint64), np.empty(M, np.int32)
     _check(lib().ql_tree_masks(M, p.ctypes.data, masks.ctypes.data, depths.ctypes.data))
