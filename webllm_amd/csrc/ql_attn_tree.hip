@@ -5,7 +5,7 @@
 // nothing is zero; what it does not see it takes nothing from, not even 0 * V.
 //
 // attn_tree_kernel: a workgroup has 16 NT (row, head) pairs of one kv head and a range of key blocks; its four or eight waves take
-// the blocks in turn, so that K and V go from memory to the registers of one wave, with no shared memory and no barrier
+// the blocks in turn, so that K and V go from memory to the registers of one wave, with no barrier
 // on the way, and each is split into parts once for 16 NT pairs. Scores are computed transposed, S^T = K Q^T (lane = pair, registers =
 // keys), which leaves a lane with the B fragment of O^T = V^T P^T. V's fragment needs eight keys of one column in a lane: a lane loads
 // four (fp16: eight) neighbouring columns of eight keys, and the tile of MFMA j takes the j-th of each, so the tile's
@@ -93,7 +93,12 @@ struct TreeTile {
     static constexpr int kQBytes = kTD * NT * kParts * 64 * 16;
     static constexpr int kMergeStride = kChunk + 4;
     static constexpr int kMergeBytes = WAVES * kRows * kMergeStride * 4;
-    static constexpr int kLds = kQBytes > kMergeBytes ? kQBytes : kMergeBytes;
+    // K of kAhead: 16 bytes a lane, whole rows; units of a row, rows of a load, loads of 16 keys, a row's bytes in LDS
+    static constexpr int kRowUnits = DP * (int)sizeof(T) / 16, kLoadRows = 64 / kRowUnits, kLoads = 16 / kLoadRows;
+    static constexpr int kTurnStride = 16 * kRowUnits + 16;
+    static constexpr int kTurnBytes = kAhead ? 16 * kTurnStride : 0;
+    static constexpr int kLoopBytes = kQBytes + WAVES * kTurnBytes;
+    static constexpr int kLds = kLoopBytes > kMergeBytes ? kLoopBytes : kMergeBytes;
     // the column of element e of step t of a K or Q fragment, group g
     static __device__ __forceinline__ int kcol(int t, int g, int e) { return kHalf ? 32 * t + 8 * g + e : 32 * t + 16 * (e >> 2) + 4 * g + (e & 3); }
 };
@@ -250,16 +255,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
         }
     }
     // K of the wave's first block is on its way while q's parts are made
-    typename std::conditional<C::kHalf, u32x4, f32x4>::type kraw[C::kNK][C::kTD * (C::kHalf ? 1 : 2)];
+    typedef typename std::conditional<C::kHalf, u32x4, f32x4>::type KRaw;
+    KRaw kraw[C::kNK][C::kTD * (C::kHalf ? 1 : 2)];
     // from an address that the whole wave shares and a lane's own offset
     const uint32_t row_bytes = (uint32_t)(row_len * sizeof(T));
-    const uint32_t k_lane = (uint32_t)i16 * row_bytes + (C::kHalf ? 8 : 4) * g * (uint32_t)sizeof(T);
+    const uint32_t k_lane = C::kAhead ? lane / C::kRowUnits * row_bytes + 16 * (lane % C::kRowUnits)
+                                      : (uint32_t)i16 * row_bytes + (C::kHalf ? 8 : 4) * g * (uint32_t)sizeof(T);
     const uint32_t v_lane = 4u * g * row_bytes + C::kCols * i16 * (uint32_t)sizeof(T);
     auto load_k = [&](const TreeBlock& blk, int from, int to) {
         const char* base = reinterpret_cast<const char*>(kb + (size_t)blk.at * row_len);
 #pragma unroll
         for (int kt = from; kt < to; kt++) {
             const char* p = base + (size_t)(16 * kt) * row_bytes;
+            if constexpr (C::kAhead) {
+#pragma unroll
+                for (int r = 0; r < C::kLoads; r++)
+                    kraw[kt][r] = FULL || 16 / (int)sizeof(T) * (lane % C::kRowUnits) < D ? ld_global(reinterpret_cast<const KRaw*>(p + (size_t)(C::kLoadRows * r) * row_bytes + k_lane))
+                                                                                          : KRaw{};
+                continue;
+            }
 #pragma unroll
             for (int t = 0; t < C::kTD; t++)
                 if constexpr (C::kHalf) {
@@ -272,6 +286,20 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
                 }
         }
     };
+    // A fragment is 16 keys' rows, 64 bytes of each: K is loaded as whole rows, which the L1 serves faster, and turned in a part of
+    // LDS that is the wave's own (5 rows after 300 keys 8.1 -> 7.4 us, 24 after 4000 25.2 -> 23.6, fp16 17.3 -> 15.1, 16 after 200
+    // 7.0 -> 5.9; where LDS is busy with q's parts, 256 after 8000 in fp32, 207 -> 214).
+    char* const turn = lds + C::kQBytes + wave * C::kTurnBytes;
+    auto turn_k = [&](int kt) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < C::kLoads; r++)
+            *reinterpret_cast<KRaw*>(turn + (lane / C::kRowUnits + C::kLoadRows * r) * C::kTurnStride + 16 * (lane % C::kRowUnits)) = kraw[kt][r];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    auto turned = [&](int r) { return *reinterpret_cast<const KRaw*>(turn + i16 * C::kTurnStride + 16 * g + 64 * r); };
     auto drop_k = [&](int from, int to) {                   // no value: the last block's is not carried along
 #pragma unroll
         for (int kt = from; kt < to; kt++)
@@ -366,6 +394,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
                 }
             }
         };
+        const bool more = b + WAVES < b1;
+        const TreeBlock next = tree_block(a, more ? b + WAVES : b, past_blocks);
         const bool all_seen = blk.j0 < 0 && blk.n == kKeys;
         uint32_t seen[NT];                                  // bit 16 kt + r: key 16 kt + 4 g + r; asked for before it is needed
         if (!all_seen)
@@ -380,50 +410,58 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
                 load_v(blk, 0, 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if (C::kAhead) turn_k(kt);
             if constexpr (C::kHalf) {
+                f16x8 keys[C::kTD];
+#pragma unroll
+                for (int t = 0; t < C::kTD; t++) keys[t] = __builtin_bit_cast(f16x8, C::kAhead ? turned(t) : kraw[kt][t]);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int t = 0; t < C::kTD; t++) {
-                        const f16x8 k = __builtin_bit_cast(f16x8, kraw[kt][t]);
                         if constexpr (!C::kAhead) {
 #pragma unroll
                             for (int i = 0; i < 2; i++) qr[nt][t][i] = qf[(size_t)((t * NT + nt) * 2 + i) * 64 + lane];
                         }
-                        lo = mfma(k, qr[nt][t][1], lo);
-                        hi = mfma(k, qr[nt][t][0], hi);
+                        lo = mfma(keys[t], qr[nt][t][1], lo);
+                        hi = mfma(keys[t], qr[nt][t][0], hi);
                     }
 #pragma unroll
                     for (int r = 0; r < 4; r++) s[kt][nt][r] = fmaf(lo[r], 1.f / 2048.f, hi[r]);
                 }
             } else {
                 // the small products first: the sum takes its full size only in the last ones, and half of those apart
-                bf16x8 kh[C::kTD];
+                bf16x8 kh[C::kTD], qh[C::kTD][NT];
                 f32x4 lo[NT], hi[NT];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) lo[nt] = hi[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+                f32x4 y[2];                                 // the next step's, on their way from LDS
+                auto key = [&](int r) { return C::kAhead ? turned(r) : kraw[kt][r]; };
+                y[0] = key(0), y[1] = key(1);
 #pragma unroll
                 for (int t = 0; t < C::kTD; t++) {
-                    float x[8];
+                    const float x[8] = {y[0].x, y[0].y, y[0].z, y[0].w, y[1].x, y[1].y, y[1].z, y[1].w};
+                    if (t + 1 < C::kTD) y[0] = key(2 * t + 2), y[1] = key(2 * t + 3);
+                    bf16x8 qp[NT][3];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = kraw[kt][2 * t + (e >> 2)][e & 3];
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int i = 0; i < 3; i++) qp[nt][i] = qf[(size_t)((t * NT + nt) * 3 + i) * 64 + lane];
                     bf16x8 kp[3];
                     split_bf16(x, kp);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        const bf16x8* q = qf + (size_t)(t * NT + nt) * 192 + lane;
-                        const bf16x8 qp[3] = {q[0], q[64], q[128]};
-                        lo[nt] = small_products(kp, qp, lo[nt]);
-                    }
+                    for (int nt = 0; nt < NT; nt++) lo[nt] = small_products(kp, qp[nt], lo[nt]);
                     kh[t] = kp[0];
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) qh[t][nt] = qp[nt][0];
                     __builtin_amdgcn_sched_barrier(0);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
                     for (int t = 0; t < C::kTD; t++) {
-                        const bf16x8 q = qf[(size_t)(t * NT + nt) * 192 + lane];
+                        const bf16x8 q = qh[t][nt];
                         if (t < C::kTD / 2) lo[nt] = mfma(kh[t], q, lo[nt]);
                         else hi[nt] = mfma(kh[t], q, hi[nt]);
                     }
@@ -437,8 +475,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
             __builtin_amdgcn_sched_barrier(0);
         }
         const TreeBlock now = blk;
-        const bool more = b + WAVES < b1;
-        if (more) blk = tree_block(a, b + WAVES, past_blocks);
+        blk = next;
         if (!all_seen)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
