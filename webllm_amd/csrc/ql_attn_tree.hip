@@ -792,13 +792,15 @@ uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes)
     a->nt = (a->D == 64 || a->D == 128) && full >= (a->half ? 1024 : 512) ? 2 : 1;
     a->past_blocks = (a->past + kKeys - 1) / kKeys;
     const int blocks = a->blocks = a->past_blocks + (a->M + kKeys - 1) / kKeys;
-    // Short contexts: one range of 8 waves and no merge launch, while a wave has two blocks or (keys of over 256 bytes) one and
-    // an XCD, which then has whole kv heads only, has a workgroup a CU. Eight waves against four with ranges, in us: 5 rows
-    // after 300 keys (14 / 2 heads of 64, fp32) 8.1, 9.5, 40 after 200 (fp16) 6.1, 8.8; 28 / 4 heads of 128: 16 after 200
-    // (fp32) 10.7, 12.0, 64 after 100 10.2, 12.8, and beyond these limits 8 after 300 12.6, 11.8, 8 after 700 (fp16) 11.0, 9.5,
-    // 128 after 100 20.7, 17.9, 128 after none 16.8, 11.5.
+    // Short contexts: one range of 8 waves and no merge launch, while an XCD, which then has whole kv heads only, has a workgroup
+    // a CU (fp16: two) and a wave has two blocks or (keys of over 256 bytes) one, and more where the merge would have many rows.
+    // Eight waves against four with ranges, in us: 5 rows after 300 keys (14 / 2 heads of 64, fp32) 7.4, 8.5, 40 after 200 (fp16)
+    // 5.4, 9.1; 28 / 4 heads of 128: 8 after 200 (fp32) 8.9, 10.8, 64 after 200 11.7, 13.6, 64 after 450 (fp16) 8.5, 12.3, 128 after
+    // 100 (fp16) 11.2, 13.3; beyond these limits 8 after 300 (fp32) 11.3, 10.4, 8 after 700 (fp16) 8.9, 8.4, 128 after 100 (fp32)
+    // 17.6, 16.3.
+    const int per_xcd = (R + 15) / 16 * ((a->KV + 7) / 8);
     a->waves = 4;
-    if (blocks > 4 && blocks <= (a->D * (a->half ? 2 : 4) > 256 ? 8 : 16) && (R + 15) / 16 * ((a->KV + 7) / 8) <= 32) a->waves = 8, a->nt = 1;
+    if (blocks > 4 && per_xcd <= (a->half ? 64 : 32) && blocks <= (a->D * (a->half ? 2 : 4) > 256 ? 8 : 16) + per_xcd / 8) a->waves = 8, a->nt = 1;
     a->groups = (R + 16 * a->nt - 1) / (16 * a->nt);
     const size_t one = (size_t)a->M * a->H * (a->D + 2) * sizeof(float);
     const int fit = (int)std::min<size_t>(kTreeMaxSplit, ws_bytes / one);
