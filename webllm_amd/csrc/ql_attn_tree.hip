@@ -785,11 +785,15 @@ uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes)
     const int R = a->M * a->G;
     a->nsplit = 1;
     if (a->past + a->M < kKeys) return 0;
-    // 32 pairs a workgroup where those fill the chip twice (fp16: four times) with ranges of a block a wave: a block is then split
-    // into parts half as often, but a wave's own chain is longer. 16 against 32, in us (28 / 4 heads of 128): 8 rows after 300 keys
-    // 11.3, 13.5, 4 after 4000 12.1, 14.2, 24 after 4000 29.0, 25.2; fp16 16 after 4000 14.4, 16.4, 24 after 4000 18.3 both.
+    // 32 pairs a workgroup where those fill the chip three times (fp16: eight) with ranges of a block a wave: a block is then split
+    // into parts half as often, but a wave's own chain is longer. Also where 16 would be more than two workgroups a CU (fp16: and 32
+    // fill it four times). 16 against 32, in us (28 / 4 heads of 128): 16 rows after 4000 keys 18.9, 19.5, 24 after 4000 26.1, 23.6,
+    // fp16 24 after 8000 19.8, 21.1, 64 after 8000 32.8, 31.1, 256 after none 15.5, 21.2; 14 / 2 heads of 64: 256 after 200 22.8,
+    // 15.1, fp16 256 after 200 11.5, 13.7, after 2000 35.9, 19.6.
     const long full = (long)((R + 31) / 32) * a->KV * ((a->past + a->M + 4 * kKeys - 1) / (4 * kKeys));
-    a->nt = (a->D == 64 || a->D == 128) && full >= (a->half ? 1024 : 512) ? 2 : 1;
+    const int per_xcd = (R + 15) / 16 * ((a->KV + 7) / 8);              // workgroups of 16 pairs, in a range
+    const bool crowded = per_xcd > 64, wide = a->half ? full >= (crowded ? 1024 : 2048) : full >= 768 || crowded;
+    a->nt = (a->D == 64 || a->D == 128) && wide ? 2 : 1;
     a->past_blocks = (a->past + kKeys - 1) / kKeys;
     const int blocks = a->blocks = a->past_blocks + (a->M + kKeys - 1) / kKeys;
     // Short contexts: one range of 8 waves and no merge launch, while an XCD, which then has whole kv heads only, has a workgroup
@@ -798,7 +802,6 @@ uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes)
     // 5.4, 9.1; 28 / 4 heads of 128: 8 after 200 (fp32) 8.9, 10.8, 64 after 200 11.7, 13.6, 64 after 450 (fp16) 8.5, 12.3, 128 after
     // 100 (fp16) 11.2, 13.3; beyond these limits 8 after 300 (fp32) 11.3, 10.4, 8 after 700 (fp16) 8.9, 8.4, 128 after 100 (fp32)
     // 17.6, 16.3.
-    const int per_xcd = (R + 15) / 16 * ((a->KV + 7) / 8);
     a->waves = 4;
     if (blocks > 4 && per_xcd <= (a->half ? 64 : 32) && blocks <= (a->D * (a->half ? 2 : 4) > 256 ? 8 : 16) + per_xcd / 8) a->waves = 8, a->nt = 1;
     a->groups = (R + 16 * a->nt - 1) / (16 * a->nt);
