@@ -708,60 +708,64 @@ __global__ __launch_bounds__(64) void attn_tree_row_kernel(const TreeArgs a)
         if (lane + 64 * i < D) st_global(a.out + row * D + lane + 64 * i, l == 0.f ? 0.f : acc[i] / l);
 }
 
-// out = sum_i acc_i 2^(m_i - m) / sum_i l_i 2^(m_i - m) over the key ranges, a workgroup a row: the ranges' weights in
-// LDS, then thread (part p, four columns c) adds ranges p, p + P, ... in order, and the P parts are added in order
-__global__ __launch_bounds__(256) void attn_tree_merge_kernel(const TreeArgs a)
+// out = sum_i acc_i 2^(m_i - m) / sum_i l_i 2^(m_i - m) over the key ranges. A workgroup has `rows` rows and a power of two `parts` of threads a
+// column of each: the ranges' weights go to LDS, a wave a row, then thread (row, part p, four columns c) adds ranges p, p + parts, ... in
+// order, and the parts are added in order.
+constexpr int kMergeFirst = 4;                              // ranges a thread has asked for before the weights are there
+__global__ __launch_bounds__(256) void attn_tree_merge_kernel(const TreeArgs a, int rows, int log_parts)
 {
-    __shared__ float wgt[kTreeMaxSplit];
+    __shared__ float wgt[512];                              // rows * nsplit: 4 * (256 / (D / 4)), or one row's
     __shared__ f32x4 part[256];
-    constexpr int kFirst = 4;                               // ranges a thread has asked for before the weights are there
-    const size_t row = (size_t)blockIdx.y * a.H + blockIdx.x;
-    const int t = threadIdx.x, lane = t & 63, S = a.nsplit, D = a.D;
-    const int nc = D / 4, P = 256 / nc, p = t / nc, c = t - p * nc;
+    const int t = threadIdx.x, lane = t & 63, S = a.nsplit, D = a.D, R = a.M * a.H, row0 = blockIdx.x * rows;
+    const int nc = D / 4, slot = t / nc, c = t - slot * nc, parts = 1 << log_parts, r = slot >> log_parts, p = slot - (r << log_parts);
+    const size_t row = (size_t)row0 + r;
+    const bool here = r < rows && row < (size_t)R;
     const f32x4* src = reinterpret_cast<const f32x4*>(a.ws + row * S * D) + c;
-    f32x4 v[kFirst];
+    f32x4 v[kMergeFirst];
 #pragma unroll
-    for (int k = 0; k < kFirst; k++) v[k] = p < P && p + k * P < S ? ld_global(src + (size_t)(p + k * P) * nc) : f32x4{0.f, 0.f, 0.f, 0.f};
-    if (t < 64) {
-        const f32x2* st = reinterpret_cast<const f32x2*>(a.ws + (size_t)a.M * a.H * S * D) + row * S;
+    for (int k = 0; k < kMergeFirst; k++) v[k] = here && p + k * parts < S ? ld_global(src + (size_t)(p + k * parts) * nc) : f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = t >> 6; i < rows && row0 + i < R; i += 4) {
+        const f32x2* st = reinterpret_cast<const f32x2*>(a.ws + (size_t)R * S * D) + (size_t)(row0 + i) * S;
         f32x2 s[2];
 #pragma unroll
-        for (int r = 0; r < 2; r++) s[r] = t + 64 * r < S ? ld_global(st + t + 64 * r) : f32x2{-INFINITY, 0.f};
+        for (int k = 0; k < 2; k++) s[k] = lane + 64 * k < S ? ld_global(st + lane + 64 * k) : f32x2{-INFINITY, 0.f};
         const float mx = wave_max(fmaxf(s[0].x, s[1].x), lane);
         float e[2], l = 0.f;
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const float mi = s[r].x, li = s[r].y;
-            e[r] = mi == -INFINITY ? (li != li ? li : 0.f) : ex2(mi - mx);
-            l += li * e[r];
+        for (int k = 0; k < 2; k++) {
+            const float mi = s[k].x, li = s[k].y;
+            e[k] = mi == -INFINITY ? (li != li ? li : 0.f) : ex2(mi - mx);
+            l += li * e[k];
         }
         l = wave_sum(l, lane);
 #pragma unroll
-        for (int r = 0; r < 2; r++) wgt[t + 64 * r] = l == 0.f ? 0.f : e[r] / l;
+        for (int k = 0; k < 2; k++)
+            if (lane + 64 * k < S) wgt[i * S + lane + 64 * k] = l == 0.f ? 0.f : e[k] / l;
     }
     __syncthreads();
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    if (p < P) {
+    if (here) {
+        const float* w = wgt + r * S;
 #pragma unroll
-        for (int k = 0; k < kFirst; k++) {
-            const float w = p + k * P < S ? wgt[p + k * P] : 0.f;
+        for (int k = 0; k < kMergeFirst; k++) {
+            const float wk = p + k * parts < S ? w[p + k * parts] : 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = fmaf(w, v[k][e], o[e]);
+            for (int e = 0; e < 4; e++) o[e] = fmaf(wk, v[k][e], o[e]);
         }
 #pragma unroll 4
-        for (int i = p + kFirst * P; i < S; i += P) {
-            const float w = wgt[i];
+        for (int i = p + kMergeFirst * parts; i < S; i += parts) {
             const f32x4 x = ld_global(src + (size_t)i * nc);
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = fmaf(w, x[e], o[e]);
+            for (int e = 0; e < 4; e++) o[e] = fmaf(w[i], x[e], o[e]);
         }
     }
-    part[t] = o;
-    __syncthreads();
-    if (t < nc) {
-        f32x4 r = part[t];
-        for (int k = 1; k < P; k++) r += part[k * nc + t];
-        st_global(reinterpret_cast<f32x4*>(a.out + row * D) + t, r);
+    if (parts > 1) {
+        part[t] = o;
+        __syncthreads();
+    }
+    if (here && p == 0) {
+        for (int k = 1; k < parts; k++) o += part[t + k * nc];
+        st_global(reinterpret_cast<f32x4*>(a.out + row * D) + c, o);
     }
 }
 
@@ -829,7 +833,13 @@ hipError_t launch_attention_tree(const TreeArgs& a, hipStream_t stream)
     hipLaunchKernelGGL(fn, dim3(8 * a.groups, (a.KV * a.nsplit + 7) / 8), dim3(64 * a.waves), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.nsplit == 1) return e;
-    hipLaunchKernelGGL(attn_tree_merge_kernel, dim3(a.H, a.M), dim3(256), 0, stream, a);
+    // a thread's columns of four ranges, more where a row has more than the workgroup's; rows as fit (a row a workgroup: 256 rows
+    // after 8000 keys, two ranges, 9.2 us of 90)
+    const int slots = 256 / (a.D / 4);
+    int log_parts = 0;
+    while (kMergeFirst << log_parts < a.nsplit && 2 << log_parts <= slots) log_parts++;
+    const int rows = slots >> log_parts;
+    hipLaunchKernelGGL(attn_tree_merge_kernel, dim3((a.M * a.H + rows - 1) / rows), dim3(256), 0, stream, a, rows, log_parts);
     return hipGetLastError();
 }
 
