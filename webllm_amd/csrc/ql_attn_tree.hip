@@ -9,15 +9,21 @@
 // on the way, and each is split into parts once for 16 NT pairs. Scores are computed transposed, S^T = K Q^T (lane = pair, registers =
 // keys), which leaves a lane with the B fragment of O^T = V^T P^T. V's fragment needs eight keys of one column in a lane: a lane loads
 // four (fp16: eight) neighbouring columns of eight keys, and the tile of MFMA j takes the j-th of each, so the tile's
-// columns are 4 i + j, and nothing crosses lanes. The softmax keeps its running maximum and sum in fp32; the waves' states are
-// merged through LDS, the key ranges' (where the pairs do not fill the chip) by attn_tree_merge_*.
+// columns are 4 i + j, and nothing crosses lanes. The softmax keeps its running reference and sum in fp32; the waves' states are
+// merged through LDS, the key ranges' (where the pairs do not fill the chip) by attn_tree_merge_kernel. Contexts of fewer keys than
+// a block: attn_tree_row_kernel, a wave a (row, head).
 //
 // fp32 caches: an operand enters as three bf16 parts, 24 bits with fp32's own range, so no value depends on its neighbours' size; a
 // product is the six largest of the nine (v_mfma_f32_16x16x32_bf16: 6/16 of the fp32 MFMA's time).
 // fp16 caches: K and V enter as they are; q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P. Two products.
 //
 // What the parts cannot carry is not finite: an infinity's remainder is a NaN, and 0 * V is one where V is not. A wave whose sums
-// end that way does its blocks again on the VALU from q, K and V themselves, skipping what a pair does not see (again()).
+// end that way does its blocks again on the VALU from q, K and V themselves, skipping what a pair does not see (tree_again).
+//
+// us, of them the merge, and what bounds it (28 / 4 heads of 128): 1 row after 32000 fp16 keys 17.1, 4, memory (65.5 MB); 24 rows after
+// 4000 fp32 keys 23.5, 4, the parts' VALU work and the matrix unit in turn; 256 after 8000 fp16 keys 87.4, 5, issue: two waves a SIMD
+// fit its registers, the VALU is busy half of the cycles, the matrix unit 27 %. 14 / 2 heads of 64: 5 rows after 300 fp32 keys 7.3,
+// one launch and its chain of loads.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

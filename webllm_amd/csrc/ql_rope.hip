@@ -11,7 +11,7 @@
 // butterfly over the 8 to 32 lanes of the head) crosses lanes, and q may be rotated in place. The angles come from
 // the table, since t in fp32 is off by position * 2^-24 and fp64 sines a row cost more than 4 rot bytes from L2.
 // Bytes: q, k and v read once, q, k and v written once: 2048 rows (28 / 4 heads of 128, norms, fp32) 13.2 us, 5.8 TB/s; up to some
-// 24 rows one launch and a chain of loads, 4.7 us.
+// 24 rows one launch and a chain of loads, 4.4 us.
 #include <cmath>
 
 #include "ql_device.h"
