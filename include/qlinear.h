@@ -305,8 +305,8 @@ int ql_tree_masks(int32_t M, const int32_t* parents, uint64_t* masks, int32_t* d
 /* out[m, h, :] = softmax_s(q[m, h] . K[s, h / (n_head / n_kv_head)] / sqrt(D)) V[s, ...] over s < past_len and the drafted rows
  * s = past_len + j whose bit j is set in row m of mask (uint64 [M, ceil(M/64)] at mask_off in `act`; bits from M on are ignored;
  * QL_NONE: j <= m, causal rows). A row that sees nothing, or no score above -inf, is zero. What a row does not see adds nothing to it,
- * infinities and NaN included. M = 1..256, D = 8..256 (a multiple of 8), past_len + M <= max_t (the cache may be longer
- * than ql_attention_decode's 8192); fp32 q and out, sums and softmax in fp32; caches fp32 or fp16. Offsets 16-byte
+ * infinities and NaN included. M = 1..256, D = 8..256 (a multiple of 8), past_len <= 2^30, past_len + M <= max_t (the cache may be
+ * longer than ql_attention_decode's 8192); fp32 q and out, sums and softmax in fp32; caches fp32 or fp16. Offsets 16-byte
  * aligned (mask: 8). Uses the context's 64 MiB workspace, as ql_attention_decode. */
 int ql_attention_tree(ql_ctx* ctx, ql_arena* act, uint64_t q_off, const ql_arena* cache, uint64_t k_off, uint64_t v_off,
                       int32_t cache_dtype, int32_t max_t, int32_t M, int32_t n_head, int32_t n_kv_head, int32_t D, int32_t past_len,

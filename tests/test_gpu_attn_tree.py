@@ -380,3 +380,15 @@ def test_refusals(ql, ctx):
     ctx.attention_tree(*a)
     c.check()
     c.release()
+
+
+def test_refuses_more_keys_than_it_counts(ql, ctx):
+    c = Call(ql, ctx, 4, 4, 2, 32, 10, False, None, 1)
+    a = list(c.args)
+    a[6] = (1 << 31) - 1
+    for past in ((1 << 30) + 1, (1 << 31) - 8):
+        a[11] = past
+        with pytest.raises(ql.QlError) as e:
+            ctx.attention_tree(*a)
+        assert e.value.name == "QL_E_INVALID"
+    c.release()

@@ -2750,6 +2750,7 @@ int ql_attention_tree(ql_ctx* ctx, ql_arena* act, uint64_t q_off, const ql_arena
     if (!ctx || !act || !cache) return fail(QL_E_INVALID, "null context or arena");
     if (M < 1 || M > ql::kTreeMaxRows) return fail(QL_E_INVALID, "M must be 1..%d (got %d)", ql::kTreeMaxRows, M);
     if (n_head < 1 || n_head > 4096 || n_kv_head < 1 || past_len < 0 || max_t < 1) return fail(QL_E_INVALID, "bad attention dimensions");
+    if (past_len > ql::kTreeMaxPast) return fail(QL_E_INVALID, "past_len above %d", ql::kTreeMaxPast);
     if (n_head % n_kv_head) return fail(QL_E_INVALID, "n_head (%d) must be a multiple of n_kv_head (%d)", n_head, n_kv_head);
     if (D < 8 || D > ql::kAttnMaxD || D % 8) return fail(QL_E_INVALID, "head dim must be 8..%d, a multiple of 8 (got %d)", ql::kAttnMaxD, D);
     uint64_t cb;

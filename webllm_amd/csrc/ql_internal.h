@@ -317,6 +317,7 @@ hipError_t launch_qk_norm_rope(const RopeArgs& a, hipStream_t stream);
 hipError_t launch_rope_table(float* table, int max_pos, int rot, double theta, hipStream_t stream);
 
 constexpr int kTreeMaxRows = 256;
+constexpr int kTreeMaxPast = 1 << 30;            // its keys are counted in 31 bits
 struct TreeArgs {
     const float* q;            // [M, H, D]
     const void *k, *v;         // cache [max_t, KV * D], fp32 or fp16 (half)
