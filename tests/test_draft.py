@@ -288,3 +288,62 @@ def test_types_of_a_drafted_pass(ctx):
             call()
     for x in (kv, pool.arena, model):
         x.release()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_captured_pass(ctx, dtype):
+    """A pass's operators captured once and replayed on new inputs, between the context's own calls of other sizes: the same bits
+    as uncaptured, in the outputs and in the cache."""
+    g, C, KVD, past, M, V = np.random.default_rng(6), CFG.n_embd, gptq.qwen_kv_dim(CFG), 170, 9, 3000
+    model, pool = gptq.QuantLinearModel(ctx, 1 << 20), gptq.ActivationArena(ctx, 8 << 20)
+    model.make_rope_table(CFG.block_size, 64, 1e4)
+    parents = tree(M, 2)
+    masks, depths = ql.tree_masks(parents)
+    a, b = (gptq.KvCache(ctx, CFG, dtype) for _ in range(2))
+    context = [(pool.alloc((past, C)), pool.alloc((past, KVD)), pool.alloc((past, KVD)), pool.alloc((past,), "i32"))]
+    for t in context[0][:3]:
+        t.write(g.standard_normal(t.shape).astype(np.float32))
+    context[0][3].write(np.arange(past, dtype=np.int32))
+    q, k, v, x = pool.alloc((M, C)), pool.alloc((M, KVD)), pool.alloc((M, KVD)), pool.alloc((M, V))
+    pos, words, tok, path = pool.alloc((M,), "i32"), pool.alloc(masks.shape, "u64"), pool.alloc((M, 2), "i32"), pool.alloc((3,), "i32")
+    pos.write((past + depths).astype(np.int32))
+    words.write(masks)
+    tok.write(g.integers(0, V, (M, 2)).astype(np.int32))
+    sets = [[pool.alloc(s, t) for s, t in (((M, C), "f32"), ((M, C), "f32"), ((M, 2), "f32"), ((M,), "f32"), ((M, 20), "i32"), ((M, 20), "f32"))] for _ in range(2)]
+
+    def run(cache, out):
+        for layer in range(CFG.n_layer):
+            cache.rotate_store(layer, model, q, k, v, pos, out[0], M, past)
+            cache.attend_tree(layer, out[0], out[1], M, past, words)
+        model.token_logprobs(x, M, V, tok, out[2], out[3], out[4], out[5])
+        cache.accept(past, path, 3)
+
+    def other_work():
+        b.attend_tree(0, context[0][0], pool_out, past, 0)
+        model.token_logprobs(x, M - 1, V, entropy=sets[1][3])
+
+    pool_out = pool.alloc((past, C))
+    for cache in (a, b):
+        for layer in range(CFG.n_layer):
+            cache.rotate_store(layer, model, context[0][0], *context[0][1:], pool_out, past, 0)
+    ctx.graph_begin()
+    run(a, sets[0])
+    graph = ctx.graph_end()
+    for i in range(4):
+        for t in (q, k, v, x):
+            t.write((2 * g.standard_normal(t.shape)).astype(np.float32))
+        path.write(np.array([[0, 2, 5], [1, 3, 8], [4, 4, 0], [8, 7, 6]][i], np.int32))
+        other_work()
+        graph.launch()
+        other_work()
+        run(b, sets[1])
+        ctx.sync()
+        for s, t in zip(*sets):
+            assert np.array_equal(s.read(), t.read(), equal_nan=True)
+        rows = [c.arena.read(0, (2 * CFG.n_layer, c.region), np.uint8)[:, :(past + M) * c.row_bytes] for c in (a, b)]
+        assert np.array_equal(*rows)
+    graph.destroy()
+    for r in (a, b, model):
+        r.release()
+    pool.arena.release()
