@@ -294,7 +294,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
     };
     // A fragment is 16 keys' rows, 64 bytes of each: K is loaded as whole rows, which the L1 serves faster, and turned in a part of
     // LDS that is the wave's own (5 rows after 300 keys 8.1 -> 7.4 us, 24 after 4000 25.2 -> 23.6, fp16 17.3 -> 15.1, 16 after 200
-    // 7.0 -> 5.9; where LDS is busy with q's parts, 256 after 8000 in fp32, 207 -> 214).
+    // 7.0 -> 5.9; 256 after 8000 in fp32, where LDS is busy with q's parts, 207 either way).
     char* const turn = lds + C::kQBytes + wave * C::kTurnBytes;
     auto turn_k = [&](int kt) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -454,6 +454,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int i = 0; i < 3; i++) qp[nt][i] = qf[(size_t)((t * NT + nt) * 3 + i) * 64 + lane];
+                    __builtin_amdgcn_sched_barrier(0);      // asked for before the parts are made (256 rows after 8000: 207 -> 203 us)
                     bf16x8 kp[3];
                     split_bf16(x, kp);
 #pragma unroll
