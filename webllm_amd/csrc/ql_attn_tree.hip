@@ -808,13 +808,14 @@ uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes)
     a->past_blocks = (a->past + kKeys - 1) / kKeys;
     const int blocks = a->blocks = a->past_blocks + (a->M + kKeys - 1) / kKeys;
     // Short contexts: one range of 8 waves and no merge launch, while an XCD, which then has whole kv heads only, has a workgroup
-    // a CU (fp16: two) and a wave has two blocks or (keys of over 256 bytes) one, and more where the merge would have many rows.
-    // Eight waves against four with ranges, in us: 5 rows after 300 keys (14 / 2 heads of 64, fp32) 7.4, 8.5, 40 after 200 (fp16)
-    // 5.4, 9.1; 28 / 4 heads of 128: 8 after 200 (fp32) 8.9, 10.8, 64 after 200 11.7, 13.6, 64 after 450 (fp16) 8.5, 12.3, 128 after
-    // 100 (fp16) 11.2, 13.3; beyond these limits 8 after 300 (fp32) 11.3, 10.4, 8 after 700 (fp16) 8.9, 8.4, 128 after 100 (fp32)
-    // 17.6, 16.3.
+    // a CU (fp16: two) and a wave has one block (keys of 512 bytes), two or (128 bytes) four, and more where the merge would have
+    // many rows. Eight waves against four with ranges, in us: 14 / 2 heads of 64: 5 rows after 300 keys (fp32) 7.4, 8.5, 5 after 800
+    // (fp16) 7.2, 8.4; 28 / 4 heads of 128: 8 after 200 (fp32) 8.9, 10.8, 64 after 200 11.7, 13.6, 64 after 450 (fp16) 8.5, 12.3, 128
+    // after 100 (fp16) 11.2, 13.3; beyond these limits 8 after 300 (fp32) 11.3, 10.4, 8 after 700 (fp16) 8.9, 8.4, 128 after 100
+    // (fp32) 17.6, 16.3.
+    const int key_bytes = (a->D <= 64 ? 64 : a->D <= 128 ? 128 : 256) * (a->half ? 2 : 4);
     a->waves = 4;
-    if (blocks > 4 && per_xcd <= (a->half ? 64 : 32) && blocks <= (a->D * (a->half ? 2 : 4) > 256 ? 8 : 16) + per_xcd / 8) a->waves = 8, a->nt = 1;
+    if (blocks > 4 && per_xcd <= (a->half ? 64 : 32) && blocks <= std::max(8, 4096 / key_bytes) + per_xcd / 8) a->waves = 8, a->nt = 1;
     a->groups = (R + 16 * a->nt - 1) / (16 * a->nt);
     const size_t one = (size_t)a->M * a->H * (a->D + 2) * sizeof(float);
     const int fit = (int)std::min<size_t>(kTreeMaxSplit, ws_bytes / one);
