@@ -243,3 +243,13 @@ def test_refusals(ql, ctx):
         refused("QL_E_INVALID", **at)
     ctx.token_logprobs(*a)
     c.box.release()
+
+
+@pytest.mark.parametrize("V", [16384, 70000, 151936, 262145, 600001])
+def test_few_alternatives(ql, ctx, V):
+    """Numbers of alternatives about the one at which the parts' largest are joined at once, over few and many parts."""
+    g = np.random.default_rng(V)
+    x = (3 * g.standard_normal((2, V))).astype(np.float32)
+    x[1, g.integers(0, V, 40)] = 20.0                                        # equal ones in many parts
+    for top in (1, 3, 4, 5, 6, 7, 8, 12, 13):
+        run(ql, ctx, x, g.integers(0, V, (2, 1)), top)
