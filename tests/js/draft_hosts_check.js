@@ -1,0 +1,48 @@
+'use strict';
+/**
+ * Drives the Node host's speculative decoding for tests/test_draft_hosts.py; prints one JSON line.
+ *
+ *   node draft_hosts_check.js widths   no GPU: tensors of log probabilities that are taken and refused
+ *   node draft_hosts_check.js gpu      log probabilities into buffers of more rows than the pass has
+ */
+const q = require('../../webllm_amd/js');
+
+function message(fn) {
+    try { fn(); return null; } catch (e) { return e.message; }
+}
+
+const arena = { handle: {} };
+const tensor = (shape, dtype) => new q.Tensor(arena, 0, shape.reduce((a, b) => a * b, 1), shape, dtype || 'f32');
+
+function widths() {
+    const model = Object.assign(Object.create(q.QuantLinearModel.prototype), { ctx: { handle: {} } });
+    const x = tensor([256, 100]), ent = tensor([256]);
+    const call = (M, o) => message(() => model.tokenLogprobs(x, M, 100, o));
+    const pair = (a, b) => ({ tokens: tensor(a, 'i32'), logprobs: tensor(b) });
+    const top = (a, b) => ({ topIds: tensor(a, 'i32'), topLogprobs: tensor(b) });
+    return {
+        taken: [call(256, pair([256, 4], [256, 4])), call(100, top([256, 5], [256, 5])), call(24, pair([24], [24, 1])), call(256, pair([256, 4], [1024]))],
+        refused: [call(128, { entropy: ent, ...pair([3, 4], [256, 4]) }), call(128, pair([512], [1024])), call(128, pair([24], [24, 1])),
+            call(128, pair([256, 4], [256, 3])), call(128, top([256, 4], [256, 5])), call(128, pair([256, 4], [24, 1])), call(128, { tokens: tensor([128], 'u32'), logprobs: tensor([128]) })],
+    };
+}
+
+function gpu() {
+    const ctx = new q.Context(0);
+    const model = new q.QuantLinearModel(ctx, 1 << 20), pool = new q.ActivationArena(ctx, 1 << 20);
+    const x = pool.alloc([4, 20]), ids = pool.alloc([4, 2], 'i32'), tlp = pool.alloc([4, 2]);
+    const logits = new Float32Array(80);
+    for (let m = 0; m < 4; m++) { logits[20 * m + 2] = 5; logits[20 * m + 9] = 3; }
+    x.write(logits);
+    ids.write(new Int32Array(8).fill(-7));
+    tlp.write(new Float32Array(8).fill(7));
+    model.tokenLogprobs(x, 3, 20, { topIds: ids, topLogprobs: tlp });
+    const i = ids.read(), l = tlp.read();
+    const r = { ids: [0, 1, 2, 3].map((m) => Array.from(i.subarray(2 * m, 2 * m + 2))), behind: Array.from(l.subarray(6)) };
+    pool.release();
+    model.release();
+    ctx.destroy();
+    return r;
+}
+
+console.log(JSON.stringify({ widths, gpu }[process.argv[2]]()));

@@ -505,21 +505,32 @@ class QuantLinearModel:
     def token_logprobs(self, logits: Tensor, M: int, V: int, tokens: Tensor | None = None, logprobs: Tensor | None = None,
                        entropy: Tensor | None = None, top_ids: Tensor | None = None, top_logprobs: Tensor | None = None):
         """Over M rows of V logits (gemm's C for the lm_head): logprobs [M, T] of tokens (i32 [M, T]; -1: none), the rows' entropies
-        [M], and the top k alternatives (top_ids i32 and top_logprobs [M, k])."""
+        [M], and the top k alternatives (top_ids i32 and top_logprobs [M, k]). T and k are the tensors' second dimension, so that
+        tensors of more rows serve smaller passes (their first M rows); tensors of one dimension hold one value a row."""
         if (tokens is None) != (logprobs is None) or (top_ids is None) != (top_logprobs is None):
             raise ValueError("token_logprobs: tokens come with logprobs, top_ids with top_logprobs")
         given = [t for t in (tokens, logprobs, entropy, top_ids, top_logprobs) if t is not None]
         if any(t.arena is not logits.arena for t in given):
             raise ValueError("token_logprobs: tensors must live in the logits' arena")
-        if any(t.dtype != "f32" for t in (logprobs, entropy, top_logprobs) if t is not None):
-            raise ValueError("token_logprobs: results are f32, top_ids i32")
+        if any(t.dtype != "f32" for t in (logprobs, entropy, top_logprobs) if t is not None) or \
+                any(t.dtype != "i32" for t in (tokens, top_ids) if t is not None):
+            raise ValueError("token_logprobs: results are f32, tokens and top_ids i32")
         if M < 1 or logits.dtype != "f32" or logits.length < M * V:
             raise ValueError("token_logprobs: logits must be f32 [M, V]")
-        T = 0 if tokens is None else tokens.length // M
-        k = 0 if top_ids is None else top_ids.length // M
-        if (tokens is not None and (tokens.dtype != "i32" or logprobs.length < M * T)) or (entropy is not None and entropy.length < M) or \
-                (top_ids is not None and (top_ids.dtype != "i32" or top_logprobs.length < M * k)):
-            raise ValueError("token_logprobs: tokens and top_ids are i32, logprobs [M, T], entropy [M], top_logprobs [M, k]")
+        if entropy is not None and entropy.length < M:
+            raise ValueError("token_logprobs: entropy must hold M values")
+
+        def width(t, same):
+            """values a row of two tensors that belong together"""
+            if t is None:
+                return 0
+            if len(t.shape) != 2 and (len(t.shape) != 1 or t.length != M):
+                raise ValueError("token_logprobs: tokens and top_ids must be [rows, values a row] or [M]")
+            w = t.shape[1] if len(t.shape) == 2 else 1
+            if t.length < M * w or same.length < M * w or (len(same.shape) == 2 and same.shape[1] != w):
+                raise ValueError("token_logprobs: tokens and logprobs must be [M, T] alike, top_ids and top_logprobs [M, k]")
+            return w
+        T, k = width(tokens, logprobs), width(top_ids, top_logprobs)
 
         def off(t):
             return 0 if t is None else t.offset

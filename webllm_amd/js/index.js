@@ -468,16 +468,29 @@ class QuantLinearModel {
     }
     /**
      * Over M rows of V logits: logprobs [M, T] of tokens (i32 [M, T]; -1: none), entropy [M], topIds (i32) and topLogprobs
-     * [M, k]; each may be left out (tokens with logprobs, topIds with topLogprobs).
+     * [M, k]; each may be left out (tokens with logprobs, topIds with topLogprobs). T and k are the tensors' second dimension:
+     * tensors of more rows serve smaller passes. Tensors of one dimension hold one value a row.
      */
     tokenLogprobs(logits, M, V, o) {
         if (!o.tokens !== !o.logprobs || !o.topIds !== !o.topLogprobs) throw new Error('tokenLogprobs: tokens come with logprobs, topIds with topLogprobs');
         for (const t of [o.tokens, o.logprobs, o.entropy, o.topIds, o.topLogprobs]) {
             if (t && t.arena !== logits.arena) throw new Error('tokenLogprobs: tensors must share one arena');
         }
-        const T = o.tokens ? Math.floor(o.tokens.length / M) : 0, k = o.topIds ? Math.floor(o.topIds.length / M) : 0;
-        if (!(M >= 1) || logits.dtype !== 'f32' || [o.logprobs, o.entropy, o.topLogprobs].some((t) => t && t.dtype !== 'f32') || logits.length < M * V || (o.tokens && (o.tokens.dtype !== 'i32' || o.logprobs.length < M * T)) || (o.entropy && o.entropy.length < M) ||
-            (o.topIds && (o.topIds.dtype !== 'i32' || o.topLogprobs.length < M * k))) throw new Error('tokenLogprobs: a tensor is too small or of another type');
+        const bad = (t, dtype) => t && t.dtype !== dtype;
+        if (!(M >= 1) || logits.dtype !== 'f32' || logits.length < M * V || (o.entropy && o.entropy.length < M) ||
+            [o.logprobs, o.entropy, o.topLogprobs].some((t) => bad(t, 'f32')) || [o.tokens, o.topIds].some((t) => bad(t, 'i32')))
+            throw new Error('tokenLogprobs: a tensor is too small or of another type');
+        // values a row of two tensors that belong together
+        const width = (t, same) => {
+            if (!t) return 0;
+            if (t.shape.length !== 2 && !(t.shape.length === 1 && t.length === M))
+                throw new Error('tokenLogprobs: tokens and topIds must be [rows, values a row] or [M]');
+            const w = t.shape.length === 2 ? t.shape[1] : 1;
+            if (t.length < M * w || same.length < M * w || (same.shape.length === 2 && same.shape[1] !== w))
+                throw new Error('tokenLogprobs: tokens and logprobs must be [M, T] alike, topIds and topLogprobs [M, k]');
+            return w;
+        };
+        const T = width(o.tokens, o.logprobs), k = width(o.topIds, o.topLogprobs);
         const off = (t) => (t ? t.offset : 0);
         addon.tokenLogprobs(this.ctx.handle, logits.arena.handle, logits.offset, V, M, V, off(o.tokens), T, k, off(o.logprobs),
             o.entropy ? o.entropy.offset : null, off(o.topIds), off(o.topLogprobs));
