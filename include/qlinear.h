@@ -329,7 +329,7 @@ int ql_token_logprobs(ql_ctx* ctx, ql_arena* act, uint64_t logits_off, int32_t s
  * row as it was. A region may be moved onto itself (same arena and offset; n <= 256): every row is read before any is
  * written, so the list may have any order and name a row twice. Any other overlap of a written row with a source region, with
  * rows, or with another written row fails with QL_E_INVALID. count 1..256, n 0..2^24 (0: nothing is done), row_bytes a multiple of 16,
- * offsets 16-byte aligned (rows: 4). */
+ * offsets 16-byte aligned (rows: 4). Ordered on ctx's stream only: where another context works on dst or src, the caller syncs. */
 int ql_kv_move(ql_ctx* ctx, ql_arena* dst, const uint64_t* dst_offs, int32_t dst_max_t, const ql_arena* src, const uint64_t* src_offs,
                int32_t src_max_t, int32_t count, int32_t row_bytes, int32_t dst_row, int32_t src_row, int32_t n, const ql_arena* act,
                uint64_t rows_off);

@@ -3,6 +3,7 @@
  * Drives the Node host's speculative decoding for tests/test_draft_hosts.py; prints one JSON line.
  *
  *   node draft_hosts_check.js widths   no GPU: tensors of log probabilities that are taken and refused
+ *   node draft_hosts_check.js fork     no GPU: which contexts a fork waits for
  *   node draft_hosts_check.js gpu      log probabilities into buffers of more rows than the pass has
  */
 const q = require('../../webllm_amd/js');
@@ -27,6 +28,17 @@ function widths() {
     };
 }
 
+function fork() {
+    const config = { nLayer: 2, nHead: 2, nKvHead: 1, nEmbd: 128, blockSize: 32 }, log = [];
+    const context = (name) => ({ name, handle: {}, arena: () => ({ handle: {} }), sync: () => log.push(name) });
+    const one = context('one'), two = context('two');
+    const a = new q.KvCache(one, config), b = new q.KvCache(two, config), c = new q.KvCache(one, config);
+    message(() => a.fork(b, 5));                               // ends at the library: no device
+    const before = log.splice(0);
+    message(() => a.fork(c, 5));
+    return { before, same: log };
+}
+
 function gpu() {
     const ctx = new q.Context(0);
     const model = new q.QuantLinearModel(ctx, 1 << 20), pool = new q.ActivationArena(ctx, 1 << 20);
@@ -45,4 +57,4 @@ function gpu() {
     return r;
 }
 
-console.log(JSON.stringify({ widths, gpu }[process.argv[2]]()));
+console.log(JSON.stringify({ widths, fork, gpu }[process.argv[2]]()));

@@ -85,6 +85,74 @@ def test_node_widths_of_logprobs():
     assert all(e and e.startswith("tokenLogprobs:") for e in r["refused"]), r["refused"]
 
 
+def cache_of(ctx, log):
+    """A KvCache whose context only notes what it is asked for."""
+    cfg = gptq.QwenConfig(vocab_size=64, block_size=32, n_layer=2, n_head=2, n_kv_head=1, n_embd=128, intermediate=64, rope_theta=1e4)
+    c = gptq.KvCache(ctx, cfg)
+    log.clear()
+    return c
+
+
+def test_fork_between_contexts_is_ordered():
+    """Each context has a stream of its own: nothing of the other's may still use the cache when the copy begins, and the copy is
+    done when the other may use it again. On one context its stream's order is enough."""
+    log = []
+    one, two = Recorder(log, "one"), Recorder(log, "two")
+    a, b, c = cache_of(one, log), cache_of(two, log), cache_of(one, log)
+    a.fork(b, 5)
+    calls = [(name, call) for name, call, _ in log]
+    copy = calls.index(("one", "kv_move"))
+    assert ("two", "sync") in calls[:copy] and ("one", "sync") in calls[copy:] and calls.count(("one", "kv_move")) == 1
+    log.clear()
+    a.fork(c, 5)
+    assert [(name, call) for name, call, _ in log] == [("one", "kv_move")]
+
+
+def test_fork_between_contexts_refuses_before_it_copies():
+    """A context that is being captured cannot be waited for: nothing is recorded."""
+    log = []
+
+    class Capturing(Recorder):
+        def sync(self):
+            raise ql.QlError(-14, "ql_sync during graph capture")
+    a, b = cache_of(Capturing(log, "one"), log), cache_of(Recorder(log, "two"), log)
+    for x, y in ((a, b), (b, a)):
+        with pytest.raises(ql.QlError):
+            x.fork(y, 5)
+    assert not any(call == "kv_move" for _, call, _ in log)
+
+
+@needs_node
+def test_node_fork_between_contexts_is_ordered():
+    r = node("fork")
+    assert sorted(r["before"]) == ["one", "two"] and r["same"] == []
+
+
+@pytest.mark.gpu
+def test_fork_between_contexts(ql):
+    """A prefix copied into another context's cache, whose own stream reads it at once."""
+    g, a, b = np.random.default_rng(8), ql.Context(0), ql.Context(0)
+    cfg = gptq.QwenConfig(vocab_size=64, block_size=2048, n_layer=3, n_head=4, n_kv_head=2, n_embd=256, intermediate=64, rope_theta=1e4)
+    one, two = gptq.KvCache(a, cfg), gptq.KvCache(b, cfg)
+    for layer in range(cfg.n_layer):
+        for off in one.offsets(layer):
+            one.arena.write(off, g.standard_normal((2048, 128)).astype(np.float32))
+    pool, own = gptq.ActivationArena(b, 1 << 20), gptq.ActivationArena(a, 1 << 20)
+    q, o, q1, o1 = pool.alloc((4, 256)), pool.alloc((4, 256)), own.alloc((4, 256)), own.alloc((4, 256))
+    x = g.standard_normal((4, 256)).astype(np.float32)
+    q.write(x)
+    q1.write(x)
+    one.attend_tree(2, q1, o1, 4, 1500)
+    want = o1.read()
+    for _ in range(5):
+        two.arena.write(0, np.zeros(2 * cfg.n_layer * two.region, np.uint8))
+        one.fork(two, 1504)
+        two.attend_tree(2, q, o, 4, 1500)
+        assert np.array_equal(o.read(), want)
+    a.destroy()
+    b.destroy()
+
+
 @pytest.mark.gpu
 def test_buffers_of_more_rows(ctx):
     """Buffers of 256 rows in passes of 128 and 100: the rows lie where the tensors' shapes say."""

@@ -349,11 +349,19 @@ class KvCache:
                          path.offset)
 
     def fork(self, to: "KvCache", rows: int):
-        """The first rows of every layer into another cache of the same layers and heads (another sequence that continues them)."""
+        """The first rows of every layer into another cache of the same layers and heads (another sequence that continues them).
+        A cache of another context: the copy runs on this one's stream, and the host waits for what the other stream has still to do
+        with the cache before it, and for the copy after it."""
         a, b = self.config, to.config
         if (a.n_layer, self.row_len, self.dtype) != (b.n_layer, to.row_len, to.dtype):
             raise ValueError("fork: the caches differ in layers, heads or dtype")
+        apart = to.ctx is not self.ctx
+        if apart:
+            self.ctx.sync()
+            to.ctx.sync()
         self.ctx.kv_move(to.arena, to.regions, b.block_size, self.arena, self.regions, a.block_size, self.row_bytes, 0, 0, rows)
+        if apart:
+            self.ctx.sync()
 
     def release(self):
         self.arena.release()

@@ -141,7 +141,7 @@ export class KvCache {
     attendTree(layer: number, q: Tensor, out: Tensor, M: number, pastLen: number, masks?: Tensor | null): void;
     /** keeps an accepted path (i32 rows of the tree at pastLen) in every layer (ql_kv_move) */
     accept(pastLen: number, path: Tensor, n: number): void;
-    /** the first rows of every layer into another cache (ql_kv_move) */
+    /** the first rows of every layer into another cache (ql_kv_move); one of another context: waits for its stream and for the copy */
     fork(to: KvCache, rows: number): void;
     release(): void;
 }

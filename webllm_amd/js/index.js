@@ -763,12 +763,18 @@ class KvCache {
         addon.kvMove(this.ctx.handle, this.arena.handle, this.regions, T, this.arena.handle, this.regions, T, this.rowBytes, pastLen, pastLen, n,
             path.arena.handle, path.offset);
     }
-    /** The first rows of every layer into another cache of the same layers, heads and dtype. */
+    /**
+     * The first rows of every layer into another cache of the same layers, heads and dtype. A cache of another context: the copy
+     * runs on this one's stream, and the host waits for the other stream before it and for the copy after it.
+     */
     fork(to, rows) {
         if (to.config.nLayer !== this.config.nLayer || to.rowLen !== this.rowLen || to.dtype !== this.dtype)
             throw new Error('fork: the caches differ in layers, heads or dtype');
+        const apart = to.ctx !== this.ctx;
+        if (apart) { this.ctx.sync(); to.ctx.sync(); }
         addon.kvMove(this.ctx.handle, to.arena.handle, to.regions, to.config.blockSize, this.arena.handle, this.regions, this.config.blockSize,
             this.rowBytes, 0, 0, rows, null, null);
+        if (apart) this.ctx.sync();
     }
     release() { this.arena.release(); }
 }
