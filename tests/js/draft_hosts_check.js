@@ -4,6 +4,7 @@
  *
  *   node draft_hosts_check.js widths   no GPU: tensors of log probabilities that are taken and refused
  *   node draft_hosts_check.js fork     no GPU: which contexts a fork waits for
+ *   node draft_hosts_check.js trees    no GPU: parents of drafted trees
  *   node draft_hosts_check.js gpu      log probabilities into buffers of more rows than the pass has
  */
 const q = require('../../webllm_amd/js');
@@ -39,6 +40,19 @@ function fork() {
     return { before, same: log };
 }
 
+function trees() {
+    const bad = [[-1, 4294967295], [-1, 4294967296], [-1, NaN], [-1, undefined], [-1, 0.7], [-1, null], [-1, '0'], [-1, 0n], [-1, , 0], [-1, -4294967296],
+        Float64Array.from([-1, 0.5])];
+    const { masks, depths } = q.treeMasks(Float32Array.from([-1, 0, 0, 1]));
+    const p = new Int32Array([-1, 0]), m = new BigUint64Array(2), d = new Int32Array(2);
+    return {
+        refused: bad.map((b) => message(() => q.treeMasks(b))),
+        kinds: [[Float32Array.from([-1, 0]), m, d], [p.buffer, m, d], [[-1, 0], m, d], [p, new Float64Array(2), d], [p, m, new Float32Array(2)], [p, m, new Uint32Array(2)]]
+            .map((a) => message(() => q.addon.treeMasks(...a))),
+        masks: Array.from(masks, String), depths: Array.from(depths),
+    };
+}
+
 function gpu() {
     const ctx = new q.Context(0);
     const model = new q.QuantLinearModel(ctx, 1 << 20), pool = new q.ActivationArena(ctx, 1 << 20);
@@ -57,4 +71,4 @@ function gpu() {
     return r;
 }
 
-console.log(JSON.stringify({ widths, fork, gpu }[process.argv[2]]()));
+console.log(JSON.stringify({ widths, fork, trees, gpu }[process.argv[2]]()));

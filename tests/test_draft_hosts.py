@@ -128,6 +128,15 @@ def test_node_fork_between_contexts_is_ordered():
     assert sorted(r["before"]) == ["one", "two"] and r["same"] == []
 
 
+@needs_node
+def test_node_parents_that_are_no_rows():
+    """What an Int32Array would wrap or round to a row, and arrays of other kinds at the addon."""
+    r = node("trees")
+    assert all(e and "QL_E_INVALID" in e for e in r["refused"]), r["refused"]
+    assert all(e and "expected a" in e for e in r["kinds"]), r["kinds"]
+    assert r["masks"] == ["1", "3", "5", "11"] and r["depths"] == [0, 1, 1, 2]
+
+
 @pytest.mark.gpu
 def test_fork_between_contexts(ql):
     """A prefix copied into another context's cache, whose own stream reads it at once."""

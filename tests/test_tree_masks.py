@@ -58,3 +58,14 @@ def test_parents_past_32_bits(ql):
     for parents in (np.array([-1, 2**32 - 1]), np.array([-1, 2**32]), np.array([-(2**40), 0])):
         with pytest.raises(ql.QlError):
             ql.tree_masks(parents)
+
+
+def test_parents_that_are_no_rows(ql):
+    """Fractions and NaN, which a cast would make row 0 or -1 of; whole numbers in any type are rows."""
+    for parents in ([-1, 0.7], [-1, -0.5], [-1, 0, float("nan")], [-1, float("inf")], np.array([-1, 0, 0.999], np.float32)):
+        with pytest.raises(ql.QlError) as e:
+            ql.tree_masks(parents)
+        assert e.value.name == "QL_E_INVALID"
+    for parents in ([-1.0, 0.0, 1.0], np.array([-1, 0, 1], np.int64), np.array([-1, 0, 1], np.int8), (-1, 0, 1)):
+        masks, depths = ql.tree_masks(parents)
+        assert [int(w) for w in masks[:, 0]] == [1, 3, 7] and list(depths) == [0, 1, 2]

@@ -679,9 +679,12 @@ async function loadQwenWeights(ctx, model, options) {
 
 /** {masks: BigUint64Array [M, ceil(M/64)], depths: Int32Array} of a drafted tree: parents[m] is -1 or an earlier row. */
 function treeMasks(parents) {
-    const p = Int32Array.from(parents), M = p.length;
+    const list = Array.from(parents), M = list.length;
+    list.forEach((p, m) => {                                  // before an Int32Array wraps or rounds them
+        if (!Number.isInteger(p) || p < -1 || p >= m) throw libError('QL_E_INVALID', `the parent of row ${m} must be -1 or an earlier row (got ${p})`);
+    });
     const masks = new BigUint64Array(M * Math.ceil(M / 64)), depths = new Int32Array(M);
-    addon.treeMasks(p, masks, depths);
+    addon.treeMasks(Int32Array.from(list), masks, depths);
     return { masks, depths };
 }
 

@@ -556,14 +556,27 @@ static napi_value js_qk_norm_rope(napi_env env, napi_callback_info info)
     return NULL;
 }
 
+/* bytes of a typed array of one kind */
+static int get_typed(napi_env env, napi_value v, napi_typedarray_type want, const char* message, void** data, size_t* len)
+{
+    bool is = false;
+    napi_typedarray_type type;
+    if (napi_is_typedarray(env, v, &is) != napi_ok || !is || napi_get_typedarray_info(env, v, &type, NULL, NULL, NULL, NULL) != napi_ok || type != want) {
+        napi_throw_type_error(env, "QL_E_INVALID", message);
+        return 1;
+    }
+    return get_bytes(env, v, data, len);
+}
+
 /* treeMasks(parents Int32Array, masks BigUint64Array [M, ceil(M/64)], depths Int32Array [M]): fills both */
 static napi_value js_tree_masks(napi_env env, napi_callback_info info)
 {
     napi_value argv[3];
     void *p, *m, *d;
     size_t np, nm, nd;
-    if (get_args(env, info, 3, argv) || get_bytes(env, argv[0], &p, &np) || get_bytes(env, argv[1], &m, &nm) ||
-        get_bytes(env, argv[2], &d, &nd))
+    if (get_args(env, info, 3, argv) || get_typed(env, argv[0], napi_int32_array, "parents: expected an Int32Array", &p, &np) ||
+        get_typed(env, argv[1], napi_biguint64_array, "masks: expected a BigUint64Array", &m, &nm) ||
+        get_typed(env, argv[2], napi_int32_array, "depths: expected an Int32Array", &d, &nd))
         return NULL;
     const size_t M = np / 4;
     if (nd < 4 * M || nm < M * ((M + 63) / 64) * 8) {

@@ -229,7 +229,12 @@ def plan_attention(max_t: int, M: int, n_head: int, n_kv_head: int, D: int, past
 def tree_masks(parents) -> tuple[np.ndarray, np.ndarray]:
     """(masks uint64 [M, ceil(M/64)], depths int32 [M]) of a drafted tree: parents[m] is -1 (continues the context) or an earlier
     row (host only)."""
-    p = np.ascontiguousarray(np.clip(parents, -2, 2**31 - 1), dtype=np.int32)
+    given = np.asarray(parents)
+    whole = given == np.floor(given)                                         # not NaN, no fractions, which a cast would drop
+    if not np.all(whole):
+        m = int(np.argmin(whole))
+        raise QlError(-10, f"the parent of row {m} must be -1 or an earlier row (got {given.flat[m]})")
+    p = np.ascontiguousarray(np.clip(given, -2, 2**31 - 1), dtype=np.int32)
     M = p.size
     masks, depths = np.empty((M, (M + 63) // 64), np.uint64), np.empty(M, np.int32)
     _check(lib().ql_tree_masks(M, p.ctypes.data, masks.ctypes.data, depths.ctypes.data))
