@@ -5,6 +5,7 @@
  *   node draft_hosts_check.js widths   no GPU: tensors of log probabilities that are taken and refused
  *   node draft_hosts_check.js fork     no GPU: which contexts a fork waits for
  *   node draft_hosts_check.js trees    no GPU: parents of drafted trees
+ *   node draft_hosts_check.js table    no GPU: rope tables that are refused
  *   node draft_hosts_check.js gpu      log probabilities into buffers of more rows than the pass has
  */
 const q = require('../../webllm_amd/js');
@@ -53,6 +54,19 @@ function trees() {
     };
 }
 
+function table() {
+    let syncs = 0;
+    const model = Object.assign(Object.create(q.QuantLinearModel.prototype),
+        { ctx: { handle: {}, sync: () => { syncs++; } }, weights: { handle: {}, size: 1 << 20 }, layout: new q.ArenaLayout(), f32Weights: new Map() });
+    model.layout.take(256);
+    const used = [model.layout.used];
+    const long = message(() => model.makeRopeTable(1 << 20, 64, 1e4));
+    used.push(model.layout.used);
+    const bad = message(() => model.makeRopeTable(100, 64, 1e4));          // refused by the library: no handle
+    used.push(model.layout.used);
+    return { used, long, bad, syncs };
+}
+
 function gpu() {
     const ctx = new q.Context(0);
     const model = new q.QuantLinearModel(ctx, 1 << 20), pool = new q.ActivationArena(ctx, 1 << 20);
@@ -71,4 +85,4 @@ function gpu() {
     return r;
 }
 
-console.log(JSON.stringify({ widths, fork, trees, gpu }[process.argv[2]]()));
+console.log(JSON.stringify({ widths, fork, trees, table, gpu }[process.argv[2]]()));

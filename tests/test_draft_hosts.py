@@ -137,6 +137,58 @@ def test_node_parents_that_are_no_rows():
     assert r["masks"] == ["1", "3", "5", "11"] and r["depths"] == [0, 1, 1, 2]
 
 
+def test_rope_table_is_a_weight():
+    """Filled when the call returns, as an upload is, so that any context may read it; a refused one takes none of the arena."""
+    log = []
+    m = model_of(Recorder(log))
+    m.weights.size = 1 << 20
+    m.make_rope_table(100, 64, 1e4)
+    calls = [call for _, call, _ in log]
+    assert "sync" in calls[calls.index("rope_table"):] and m.f32["rope"].shape == (100, 64)
+    used = m.layout.used
+    with pytest.raises(ValueError, match="exhausted"):
+        m.make_rope_table(1 << 20, 64, 1e4, "long")
+    assert m.layout.used == used
+
+    class Refusing(Recorder):
+        def rope_table(self, *args):
+            raise ql.QlError(-10, "rot_dim")
+    m.ctx = Refusing(log)
+    for max_pos, rot in ((100, 12), (-5, 64)):
+        with pytest.raises(ql.QlError):
+            m.make_rope_table(max_pos, rot, 1e4, "bad")
+        assert m.layout.used == used and "bad" not in m.f32
+
+    class Capturing(Recorder):
+        def sync(self):
+            raise ql.QlError(-14, "ql_sync during graph capture")
+    log.clear()
+    m.ctx = Capturing(log)
+    with pytest.raises(ql.QlError):
+        m.make_rope_table(100, 64, 1e4, "late")
+    assert m.layout.used == used and not log
+
+
+@needs_node
+def test_node_rope_table_is_a_weight():
+    r = node("table")
+    assert r["used"] == [256, 256, 256] and "exhausted" in r["long"] and "handle" in r["bad"] and r["syncs"] >= 1
+
+
+@pytest.mark.gpu
+def test_weights_after_a_refused_table(ctx):
+    model = gptq.QuantLinearModel(ctx, 1 << 16)
+    with pytest.raises(ValueError, match="exhausted"):
+        model.make_rope_table(1 << 16, 64, 1e4)
+    with pytest.raises(ql.QlError):
+        model.make_rope_table(64, 12, 1e4)
+    model.make_rope_table(64, 64, 1e4)
+    model.upload_f32("w", np.arange(64, dtype=np.float32))
+    t = model.f32["rope"].read()
+    assert np.abs(t[:, 0] - np.cos(np.arange(64))).max() < 1e-6 and np.array_equal(model.f32["w"].read(), np.arange(64, dtype=np.float32))
+    model.release()
+
+
 @pytest.mark.gpu
 def test_fork_between_contexts(ql):
     """A prefix copied into another context's cache, whose own stream reads it at once."""

@@ -501,13 +501,21 @@ class QuantLinearModel:
         self.ctx.silu_mul(gate.arena, gate.offset, up.offset, n, out.offset)
 
     def make_rope_table(self, max_pos: int, rot_dim: int, theta: float, name: str = "rope"):
-        """Cosines and sines of positions 0 .. max_pos - 1 in the weight arena, for KvCache.rotate_store (qwen.ts ropeTheta)."""
+        """Cosines and sines of positions 0 .. max_pos - 1 in the weight arena, for KvCache.rotate_store (qwen.ts ropeTheta). As an
+        uploaded weight, the table is there when this returns, for any context; a refused one takes no room."""
         if name in self.f32:
             raise ValueError(f"weight already exists: {name}")
+        self.ctx.sync()                          # not during a capture, which would keep the fill for its replays
+        start = self.layout.used
         off = self.layout.take(max_pos * rot_dim * 4)
-        if self.layout.used > self.weights.size:
-            raise ValueError(f"weight arena exhausted ({self.layout.used} > {self.weights.size})")
-        self.ctx.rope_table(self.weights, off, max_pos, rot_dim, theta)
+        try:
+            if self.layout.used > self.weights.size:
+                raise ValueError(f"weight arena exhausted ({self.layout.used} > {self.weights.size})")
+            self.ctx.rope_table(self.weights, off, max_pos, rot_dim, theta)
+            self.ctx.sync()
+        except Exception:
+            self.layout.used = start
+            raise
         self.f32[name] = Tensor(self.weights, off, max_pos * rot_dim, (max_pos, rot_dim), "f32")
 
     def token_logprobs(self, logits: Tensor, M: int, V: int, tokens: Tensor | None = None, logprobs: Tensor | None = None,

@@ -457,13 +457,24 @@ class QuantLinearModel {
         if (gate.arena !== up.arena || gate.arena !== out.arena) throw new Error('siluMul: tensors must share one arena');
         addon.siluMul(this.ctx.handle, gate.arena.handle, gate.offset, up.offset, n, out.offset);
     }
-    /** Cosines and sines of positions 0 .. maxPos - 1 in the weight arena, for KvCache.rotateStore. */
+    /**
+     * Cosines and sines of positions 0 .. maxPos - 1 in the weight arena, for KvCache.rotateStore. As an uploaded weight, the table
+     * is there when this returns, for any context; a refused one takes no room.
+     */
     makeRopeTable(maxPos, rotDim, theta, name) {
         const key = name || 'rope';
         if (this.f32Weights.has(key)) throw new Error(`weight already exists: ${key}`);
+        this.ctx.sync();                                       // not during a capture, which would keep the fill for its replays
+        const start = this.layout.used;
         const off = this.layout.take(maxPos * rotDim * 4);
-        if (this.layout.used > this.weights.size) throw new Error(`weight arena exhausted (${this.layout.used} > ${this.weights.size})`);
-        addon.ropeTable(this.ctx.handle, this.weights.handle, off, maxPos, rotDim, theta);
+        try {
+            if (this.layout.used > this.weights.size) throw new Error(`weight arena exhausted (${this.layout.used} > ${this.weights.size})`);
+            addon.ropeTable(this.ctx.handle, this.weights.handle, off, maxPos, rotDim, theta);
+            this.ctx.sync();
+        } catch (e) {
+            this.layout.used = start;
+            throw e;
+        }
         this.f32Weights.set(key, new Tensor(this.weights, off, maxPos * rotDim, [maxPos, rotDim], 'f32'));
     }
     /**
