@@ -6,6 +6,7 @@
  *   node draft_hosts_check.js fork     no GPU: which contexts a fork waits for
  *   node draft_hosts_check.js trees    no GPU: parents of drafted trees
  *   node draft_hosts_check.js table    no GPU: rope tables that are refused
+ *   node draft_hosts_check.js read     no GPU: arrays that tensors read into
  *   node draft_hosts_check.js gpu      log probabilities into buffers of more rows than the pass has
  */
 const q = require('../../webllm_amd/js');
@@ -67,6 +68,11 @@ function table() {
     return { used, long, bad, syncs };
 }
 
+function read() {
+    const from = { read: (offset, out) => out };
+    return [undefined, 'f32', 'bytes', 'f16', 'u32', 'i32', 'u64'].map((dtype) => new q.Tensor(from, 0, 2, [2], dtype).read().constructor.name);
+}
+
 function gpu() {
     const ctx = new q.Context(0);
     const model = new q.QuantLinearModel(ctx, 1 << 20), pool = new q.ActivationArena(ctx, 1 << 20);
@@ -85,4 +91,4 @@ function gpu() {
     return r;
 }
 
-console.log(JSON.stringify({ widths, fork, trees, table, gpu }[process.argv[2]]()));
+console.log(JSON.stringify({ widths, fork, trees, table, read, gpu }[process.argv[2]]()));

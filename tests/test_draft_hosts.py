@@ -137,6 +137,12 @@ def test_node_parents_that_are_no_rows():
     assert r["masks"] == ["1", "3", "5", "11"] and r["depths"] == [0, 1, 1, 2]
 
 
+@needs_node
+def test_node_tensors_without_a_type():
+    """A tensor whose type is left out, or is none of those with an array of their own, reads as fp32."""
+    assert node("read") == ["Float32Array", "Float32Array", "Float32Array", "Uint16Array", "Uint32Array", "Int32Array", "BigUint64Array"]
+
+
 def test_rope_table_is_a_weight():
     """Filled when the call returns, as an upload is, so that any context may read it; a refused one takes none of the arena."""
     log = []

@@ -324,7 +324,7 @@ class Tensor {
         this.dtype = dtype; this.pool = pool || null;
     }
     read() {
-        const T = { f32: Float32Array, f16: Uint16Array, u32: Uint32Array, i32: Int32Array, u64: BigUint64Array }[this.dtype];
+        const T = { f16: Uint16Array, u32: Uint32Array, i32: Int32Array, u64: BigUint64Array }[this.dtype] || Float32Array;
         return this.arena.read(this.offset, new T(this.length));
     }
     write(data) { this.arena.write(this.offset, data); }
