@@ -253,3 +253,44 @@ def test_few_alternatives(ql, ctx, V):
     x[1, g.integers(0, V, 40)] = 20.0                                        # equal ones in many parts
     for top in (1, 3, 4, 5, 6, 7, 8, 12, 13):
         run(ql, ctx, x, g.integers(0, V, (2, 1)), top)
+
+
+def sure(x):
+    """(log probabilities [V], entropy) of a row with few logits far above the others: the rest's terms R are summed apart from the n
+    largest ones, so that 64 bits hold ln S = ln n + ln(1 + R / n) to 2^-50 of itself."""
+    d = x.astype(np.float64) - x.max()
+    rest = d < 0
+    n, R = (~rest).sum(), np.exp(d[rest]).sum()
+    ls = np.log(n) + np.log1p(R / n)
+    return d - ls, ls - (d[rest] * np.exp(d[rest])).sum() / (n + R)
+
+
+@pytest.mark.parametrize("gap", [3, 8, 12, 17, 24, 30])
+@pytest.mark.parametrize("V", [2, 50, 1001, 30000, 151936])
+def test_sure_rows(ql, ctx, V, gap):
+    """One logit far above the others, or several alike: a log probability and an entropy far below 1, to their own rounding.
+    A term e^d is off by (2.3 |d| + 4) u (the difference's rounding, log2 e's and the product's, two exponentials), d at most gap + 6 here;
+    R's additions and the product with d by some 50 u: (2.3 (gap + 6) + 54) u of ln S and of the entropy, and one rounding."""
+    g = np.random.default_rng(V + gap)
+    x = np.zeros((6, V), np.float32)
+    x[:3] = np.clip(g.standard_normal((3, V)), -3, 3)
+    at = [V // 2, 0, V - 1, V // 3, 0, V - 1]
+    for m in range(6):
+        x[m, at[m]] = x[m].max() + gap if m < 3 else gap
+    x[4, V - 1] = gap                                                        # two alike, far apart
+    x[5, ::7] = gap                                                          # many alike
+    tokens = np.stack([at, [(a + 1) % V for a in at]], 1)
+    top = min(V, 3)
+    c = Call(ql, ctx, x, tokens, top)
+    ctx.token_logprobs(*c.args)
+    lp, ent, ids, tlp = (a.astype(np.float64) for a in c.results())
+    for m in range(6):
+        want, H = sure(x[m])
+        r = (2.3 * (gap + 6) + 56) * U
+        ls = -want.max()
+        assert abs(ent[m] - H) <= r * H, (m, ent[m], H)
+        assert (np.abs(lp[m] - want[tokens[m]]) <= r * ls + U * np.abs(want[tokens[m]])).all()
+        order = np.argsort(-x[m], kind="stable")[:top]
+        assert np.array_equal(ids[m], order)
+        assert (np.abs(tlp[m] - want[order]) <= r * ls + U * np.abs(want[order])).all()
+    c.box.release()

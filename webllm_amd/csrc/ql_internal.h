@@ -345,7 +345,7 @@ struct LogprobArgs {
     int M, V, n_tok, top_k;
     // launch_token_logprobs fills these
     int units;                 // of 1024 logits
-    float* stat;               // [M, units, 4]
+    float* stat;               // [M, units, 4]: largest, sum of the others' terms, entropy's sum, how many are the largest
     uint64_t* best;            // [M, units, 4]
 };
 uint64_t token_logprobs_bytes(int M, int V);   // workspace of M rows in one go; a row needs 48 bytes per 1024 logits

@@ -4,15 +4,17 @@
 //   lse = m + ln sum e^(x - m),  log p(t) = x_t - lse,  H = ln S - (sum (x - m) e^(x - m)) / S,  S = sum e^(x - m)
 // with m the row's largest logit, so nothing cancels however large the logits are; -inf logits (a mask) add nothing. A
 // row without any other: log p = -inf, H = 0. Alternatives are ordered by value, equal ones by index.
+// S = n + R: the n logits that are m are counted, R is the sum of the others' terms. A sure row's R is far below the last bit of an
+// fp32 S, and its log probability and entropy are made of nothing else: ln S = ln n + ln(1 + R / n).
 //
-// logprob_scan_kernel reads the logits, once: a wave has a unit of 1024 of a row in registers, and leaves the unit's (m, S, sum (x - m)
-// e^(x - m)) and, where alternatives are wanted, the largest (value, index) of each of its four parts of 256. No LDS, no barrier.
+// logprob_scan_kernel reads the logits, once: a wave has a unit of 1024 of a row in registers, and leaves the unit's (m, R, sum (x - m)
+// e^(x - m), n) and, where alternatives are wanted, the largest (value, index) of each of its four parts of 256. No LDS, no barrier.
 // logprob_row_kernel joins a row's units, and finds the top k exactly from the parts' largest: a part whose largest is not
 // among the k largest of those has none of the top k (k others are larger), so the k parts that are hold them all, and what
 // lies below the smallest of those k is left out. Where more than 256 are left (a masked row's are all alike) the same is done once
 // more with the threads' largest, of eight each, which leaves 8 k at most; the rest is sorted.
-// Bound: 4 bytes a logit from memory: 512 rows of 152064 take 55.4 us, 5.6 TB/s. With few rows the two launches and their chains
-// of loads: 1 row 7.2 us, with alternatives 9.8; 24 rows 8.0, with 20 alternatives 13.7, and 17.6 where a row is masked whole
+// Bound: 4 bytes a logit from memory: 512 rows of 151936 take 55.7 us, 5.6 TB/s. With few rows the two launches and their chains
+// of loads: 1 row 7.2 us, with alternatives 9.6; 24 rows 8.0, with 20 alternatives 13.9, and 17.8 where a row is masked whole
 // (22.2 with one sort of all that is alike).
 #include <algorithm>
 #include <cmath>
@@ -28,7 +30,7 @@ namespace {
 
 constexpr int kUnit = 1024, kPart = 256, kParts = kUnit / kPart;   // logits of a wave, of its 16-lane rows
 constexpr int kWaves = 16;                                          // of a row's workgroup where alternatives are wanted
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kMaxFinite = 3.4028235e38f;
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // rows start at any multiple of 4 bytes
 
@@ -77,17 +79,19 @@ __global__ __launch_bounds__(256) void logprob_scan_kernel(const LogprobArgs a)
         for (int c = 0; c < 4; c++) mx = fmaxf(mx, v[u][c]);
     const float m = wave_max(mx, lane), ref = m == -INFINITY ? 0.f : m;
     float s = 0.f, t = 0.f;
+    int n = 0;                                            // the wave's
 #pragma unroll
     for (int u = 0; u < 4; u++)
 #pragma unroll
         for (int c = 0; c < 4; c++) {
             const float d = v[u][c] - ref, e = __builtin_amdgcn_exp2f(d * kLog2e);
-            s += e;
-            t += d == -INFINITY ? 0.f : d * e;
+            n += __popcll(__ballot(d == 0.f));
+            s += d == 0.f ? 0.f : e;
+            t = fmaf(fmaxf(d, -kMaxFinite), e, t);        // -inf: e is 0
         }
     s = wave_sum(s, lane);
     t = wave_sum(t, lane);
-    if (lane == 0) st_global(reinterpret_cast<f32x4*>(a.stat) + row * a.units + unit, f32x4{m, s, t, 0.f});
+    if (lane == 0) st_global(reinterpret_cast<f32x4*>(a.stat) + row * a.units + unit, f32x4{m, s, t, (float)n});
     if (TOP) {
         uint32_t best = 0, at = 0;
 #pragma unroll
@@ -177,8 +181,8 @@ __device__ __forceinline__ uint64_t largest64(F key, int n, int k, uint64_t* lis
     return mine;
 }
 
-// A row's units joined by one wave: its largest logit and ln S, and the tokens' log probabilities and the entropy. The logarithm and the last
-// subtractions are in 64 bits, so they add no rounding but the last (512 rows' entropies off by 2.8e-8 for 3.7e-8 in 32 bits, as fast).
+// A row's units joined by one wave: its largest logit and ln S, and the tokens' log probabilities and the entropy. The logarithm, the
+// division and the last subtractions are in 64 bits: what is rounded before them are the sums.
 __device__ __forceinline__ void join_units(const LogprobArgs& a, size_t row, int lane, float& ref, double& ls, bool& none)
 {
     constexpr int kFirst = 4;                             // units a lane has at once, the first with the first token's logit
@@ -201,20 +205,24 @@ __device__ __forceinline__ void join_units(const LogprobArgs& a, size_t row, int
     for (int i = lane + 64 * kFirst; i < a.units; i += 64) m = fmaxf(m, ld_global(st + i).x);
     m = wave_max(m, lane);
     ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f, t = 0.f;
+    float n = 0.f, s = 0.f, t = 0.f;
     auto add = [&](const f32x4& u) {
-        const float d = u.x == -INFINITY ? 0.f : u.x - ref, e = __builtin_amdgcn_exp2f(d * kLog2e);
-        s = fmaf(u.y, e, s);
-        t += e == 0.f ? 0.f : fmaf(d, u.y, u.z) * e;      // d may be too far down for d * u.y
+        const float d = u.x == -INFINITY ? 0.f : u.x - ref, e = __builtin_amdgcn_exp2f(d * kLog2e), all = u.y + u.w;
+        n += d == 0.f ? u.w : 0.f;                        // the unit's largest are the row's
+        s = d == 0.f ? s + u.y : fmaf(all, e, s);
+        t += e == 0.f ? 0.f : fmaf(d, all, u.z) * e;      // d may be too far down for d * all
     };
 #pragma unroll
     for (int i = 0; i < kFirst; i++) add(u[i]);
     for (int i = lane + 64 * kFirst; i < a.units; i += 64) add(ld_global(st + i));
+    n = wave_sum(n, lane);
     s = wave_sum(s, lane);
     t = wave_sum(t, lane);
-    none = s == 0.f;
-    ls = log((double)s);
-    if (lane == 0 && a.entropy) st_global(a.entropy + row, none ? 0.f : (float)(ls - t / s));
+    none = n + s == 0.f;
+    const bool sure = s < n * 0x1p-20f;                   // ln(1 + r) = r - r^2 / 2 to 2^-41 of itself
+    const double all = (double)n + s, r = sure ? s / n : 0.f;
+    ls = log(sure ? (double)n : all) + (r - 0.5 * r * r);
+    if (lane == 0 && a.entropy) st_global(a.entropy + row, none ? 0.f : (float)(ls - t / all));
     auto put = [&](int i, bool there, float x) {
         st_global(a.logprob + row * a.n_tok + i, !there ? 0.f : none ? -INFINITY : (float)((double)x - ref - ls));
     };
