@@ -311,6 +311,17 @@ int ql_tree_masks(int32_t M, const int32_t* parents, uint64_t* masks, int32_t* d
 int ql_attention_tree(ql_ctx* ctx, ql_arena* act, uint64_t q_off, const ql_arena* cache, uint64_t k_off, uint64_t v_off,
                       int32_t cache_dtype, int32_t max_t, int32_t M, int32_t n_head, int32_t n_kv_head, int32_t D, int32_t past_len,
                       uint64_t mask_off, uint64_t out_off);
+/* The launch shape ql_attention_tree picks for these dimensions (host only, with the same checks): `pairs` (row, head) pairs of a
+ * kv head share a workgroup of `waves` waves and its reads of K and V; nsplit key ranges (1: no merge launch). */
+typedef struct ql_tree_info {
+    int32_t pairs;
+    int32_t waves;
+    int32_t nsplit;
+    int32_t keys_per_split;
+    int32_t workgroups;    /* of the attention launch */
+} ql_tree_info;
+int ql_plan_attention_tree(int32_t cache_dtype, int32_t max_t, int32_t M, int32_t n_head, int32_t n_kv_head, int32_t D, int32_t past_len,
+                           ql_tree_info* info);
 /* Log probabilities over M rows of V fp32 logits (stride values apart, stride >= V; ql_gemv_f16w's y has stride V), natural
  * logarithms, no temperature:
  *   logprob [M, n_tok] fp32    of tokens [M, n_tok] int32; 0 for an id outside 0..V-1 (a padding entry)

@@ -392,3 +392,144 @@ def test_refuses_more_keys_than_it_counts(ql, ctx):
             ctx.attention_tree(*a)
         assert e.value.name == "QL_E_INVALID"
     c.release()
+
+
+def many(q, k, v, seen):
+    """formula()'s results for a head's rows at once."""
+    M, H, D = q.shape
+    T, KV, _ = k.shape
+    q, k, v = (a.astype(np.float64) for a in (q, k, v))
+    out, tol = np.zeros((M, H, D)), np.zeros((M, H, D))
+    with np.errstate(all="ignore"):
+        for h in range(H):
+            kh, vh = k[:, h // (H // KV)], v[:, h // (H // KV)]
+            score = np.where(seen, q[:, h] @ kh.T / np.sqrt(D), -np.inf)
+            p = np.exp(score - score.max(1, keepdims=True))
+            total = p.sum(1, keepdims=True)
+            fine = np.isfinite(vh)
+            o = p @ np.where(fine, vh, 0)
+            for key, d in np.argwhere(~fine):
+                o[:, d] += np.where(seen[:, key], p[:, key] * vh[key, d], 0)
+            a = np.where(seen, np.abs(q[:, h]) @ np.where(np.isfinite(kh), np.abs(kh), 0).T, 0).max(1, keepdims=True) / np.sqrt(D)
+            bad = (np.isnan(score) | (score == np.inf)).any(1)
+            any_seen = seen.any(1)
+            out[:, h] = np.where(any_seen[:, None], np.where(bad[:, None], np.nan, o / total), 0)
+            tol[:, h] = np.where(any_seen[:, None], (32 * a + 32 + 2 * np.sqrt(T)) * U * (p @ np.where(fine, np.abs(vh), 0)) / total, 0)
+    return out, tol
+
+
+def run_many(ql, ctx, M, H, KV, D, past, half, masks, seed, **kw):
+    c = Call(ql, ctx, M, H, KV, D, past, half, masks, seed, **kw)
+    ctx.attention_tree(*c.args)
+    c.check(many(c.q, c.k, c.v, seen_of(masks, M, past)))
+    c.release()
+
+
+# Shapes of the instances with 32 pairs a workgroup, and of more than 64 key ranges, whose merge has two weights a lane.
+PLANS = [
+    # M, H, KV, D, past, half, (pairs, waves, key ranges), label
+    (251, 5, 1, 64, 40, False, (32, 4, 3), "1255 pairs of a kv head, a last group of 7"),
+    (140, 9, 1, 128, 33, False, (32, 4, 2), "heads of 128, a last group of 12"),
+    (25, 28, 4, 128, 3980, False, (32, 4, 16), "a tree after a long context, a last group of 15"),
+    (65, 33, 1, 64, 1950, True, (32, 4, 1), "a half cache, a last group of 1"),
+    (129, 17, 1, 128, 2000, True, (32, 4, 1), "a half cache, heads of 128, a last group of 17"),
+    (40, 40, 1, 64, 3200, True, (32, 4, 7), "a half cache, ranges that are merged"),
+    (1, 28, 4, 128, 20000, False, (16, 4, 79), "more than 64 key ranges"),
+    (1, 28, 4, 128, 20000, True, (16, 4, 79), "more than 64 key ranges of a half cache"),
+    (3, 6, 2, 200, 32700, True, (16, 4, 128), "as many key ranges as there are"),
+]
+
+
+@pytest.mark.parametrize("M,H,KV,D,past,half,plan,label", PLANS)
+def test_planned_instances(ql, ctx, M, H, KV, D, past, half, plan, label):
+    print(label, flush=True)
+    info = ql.plan_attention_tree(ql.DTYPE_F16 if half else ql.DTYPE_F32, past + M, M, H, KV, D, past)
+    assert (info.pairs, info.waves, info.nsplit) == plan
+    c = Call(ql, ctx, M, H, KV, D, past, half, ql.tree_masks(tree(M, M))[0], past)
+    ctx.attention_tree(*c.args)
+    first = c.check(many(c.q, c.k, c.v, seen_of(c.masks, M, past)))
+    for _ in range(3):
+        ctx.attention_tree(*c.args)
+    assert np.array_equal(c.out(), first.astype(np.float32))
+    c.release()
+
+
+WIDE = [p[:6] for p in PLANS if p[6][0] == 32 and p[4] < 3000]
+
+
+@pytest.mark.parametrize("M,H,KV,D,past,half", WIDE)
+def test_32_pairs_without_a_mask(ql, ctx, M, H, KV, D, past, half):
+    """Causal rows: with the chain's mask the bits are the same."""
+    c = Call(ql, ctx, M, H, KV, D, past, half, None, M)
+    ctx.attention_tree(*c.args)
+    got = c.check(many(c.q, c.k, c.v, seen_of(None, M, past)))
+    d = Call(ql, ctx, M, H, KV, D, past, half, ql.tree_masks(np.arange(-1, M - 1))[0], M)
+    ctx.attention_tree(*d.args)
+    assert np.array_equal(d.out(), got)
+    c.release()
+    d.release()
+
+
+@pytest.mark.parametrize("M,H,KV,D,past,half", WIDE)
+@pytest.mark.parametrize("what,value", [("k", np.nan), ("v", np.inf), ("k", -np.inf)])
+def test_32_pairs_of_what_is_not_finite(ql, ctx, M, H, KV, D, past, half, what, value):
+    """In a drafted row that a few see, and (a second call) in the context: on the VALU again, both tiles of a wave. Some rows see
+    nothing of the tree."""
+    masks, _ = ql.tree_masks(tree(M, 3))
+    masks[[0, M // 2]] = 0
+    for key in (past + 2 * M // 3, past // 2):
+        def edit(c):
+            getattr(c, what)[key, :, 5] = value
+        run_many(ql, ctx, M, H, KV, D, past, half, masks, 11, edit=edit)
+
+
+@pytest.mark.parametrize("M,H,KV,D,half", [(256, 5, 1, 64, False), (128, 9, 1, 128, False), (256, 64, 1, 64, True), (256, 64, 1, 128, True)])
+def test_32_pairs_that_see_nothing(ql, ctx, M, H, KV, D, half):
+    """No context, masks of any bits and of none: rows of zeros among the others, whole workgroups of them at the end."""
+    assert ql.plan_attention_tree(ql.DTYPE_F16 if half else ql.DTYPE_F32, M, M, H, KV, D, 0).pairs == 32
+    g = np.random.default_rng(M)
+    masks = g.integers(0, 2**63, (M, M // 64)).astype(np.uint64)
+    masks[::7] = 0
+    masks[M - 40:] = 0
+    run_many(ql, ctx, M, H, KV, D, 0, half, masks, 5)
+
+
+@pytest.mark.parametrize("M,H,KV,D,past,half", WIDE)
+def test_32_pairs_with_scores_that_rise(ql, ctx, M, H, KV, D, past, half):
+    """Along the context, slowly and by leaps, for one tile of a wave and not for the other."""
+    masks, _ = ql.tree_masks(tree(M, 5))
+    at = np.arange(past + M)
+    for line in (at / 40, np.where(at % 90 == 89, at / 9, 0), (past - at) / 40):
+        def edit(c):
+            c.q[:, :, 0] = np.where(np.arange(M)[:, None] % 5 == 0, 4, 0.01)
+            c.k[:, :, 0] = (line * 2).astype(c.k.dtype)[:, None]
+        run_many(ql, ctx, M, H, KV, D, past, half, masks, 20, edit=edit)
+
+
+@pytest.mark.parametrize("past,low", [(40000, 20), (300000, 22), (300000, 24)])
+def test_long_tails_of_small_weights(ql, ctx, past, low):
+    """One key far above all the others over a long half cache: V is 0 at the key and 1 elsewhere, so the result is the others' part,
+    t / (1 + t) with t = (T - 1) e^-low. Its relative error: the scores' 16 u A twice, A = low, and the sums' (32 + 2 sqrt(T)) u. A weight's
+    two parts end at half a step of 2^-24 of 2^8 of it: 2^-33 of the reference, which T weights lose at most T times."""
+    M, H, KV, D = 2, 2, 1, 64
+    g = np.random.default_rng(past)
+    act, cache = Box(ql, ctx), Box(ql, ctx)
+    T = past + M
+    q = np.zeros((M, H, D), np.float32)
+    q[:, :, 0] = low * 8                                                     # sqrt(D): a key's first value times `low` is its score
+    k, v = np.zeros((T, KV, D), np.float16), np.ones((T, KV, D), np.float16)
+    at = int(g.integers(past))
+    k[at, :, 0], v[at] = 1, 0
+    act.put("q", q)
+    act.put("out", np.zeros((M, H, D), np.float32))
+    cache.put("k", k)
+    cache.put("v", v)
+    act.place()
+    cache.place()
+    ctx.attention_tree(act.arena, act.off("q"), cache.arena, cache.off("k"), cache.off("v"), ql.DTYPE_F16, T, M, H, KV, D, past, None, act.off("out"))
+    for m, row in enumerate(act.get("out").astype(np.float64)):
+        t = (past + m // H) * np.exp(-np.float64(low))
+        want = t / (1 + t)
+        assert np.abs(row - want).max() <= (32 * low + 32 + 2 * np.sqrt(T)) * U * want + T * 2.0 ** -33
+    act.release()
+    cache.release()

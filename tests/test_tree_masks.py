@@ -69,3 +69,42 @@ def test_parents_that_are_no_rows(ql):
     for parents in ([-1.0, 0.0, 1.0], np.array([-1, 0, 1], np.int64), np.array([-1, 0, 1], np.int8), (-1, 0, 1)):
         masks, depths = ql.tree_masks(parents)
         assert [int(w) for w in masks[:, 0]] == [1, 3, 7] and list(depths) == [0, 1, 2]
+
+
+def test_plans_of_tree_attention(ql):
+    """ql_plan_attention_tree (host only): the GPU tests' instances, ranges that cover the keys, the call's refusals."""
+    from tests.test_gpu_attn_tree import PLANS, SHAPES
+
+    for M, H, KV, D, past, half, want, label in PLANS:
+        p = ql.plan_attention_tree(int(half), past + M, M, H, KV, D, past)
+        assert (p.pairs, p.waves, p.nsplit) == want, label
+    seen = set()
+    for M, H, KV, D, past, label in SHAPES:
+        for half in (0, 1):
+            p = ql.plan_attention_tree(half, past + M, M, H, KV, D, past)
+            seen.add((p.pairs, p.waves))
+            assert p.nsplit * p.keys_per_split >= past + M and p.workgroups * p.pairs >= M * H * p.nsplit, label
+    assert seen == {(1, 1), (16, 4), (16, 8)}
+    for bad in ((2, 64, 4, 4, 2, 64, 10), (0, 13, 4, 4, 2, 64, 10), (0, 64, 0, 4, 2, 64, 10), (0, 64, 257, 4, 2, 64, 10), (0, 64, 4, 4, 3, 64, 10),
+                (0, 64, 4, 4, 2, 68, 10), (0, 64, 4, 4, 2, 264, 10), (0, 64, 4, 4, 2, 64, -1), (0, 2**31 - 1, 4, 4, 2, 64, 2**30 + 1)):
+        with pytest.raises(ql.QlError):
+            ql.plan_attention_tree(*bad)
+    assert ql.lib().ql_plan_attention_tree(0, 64, 4, 4, 2, 64, 10, None) == -10
+
+
+def test_rows_at_once_are_the_formula(ql):
+    """The GPU tests' two forms of the formula agree, with rows that see nothing, NaN and infinities in seen and unseen keys."""
+    from tests.test_gpu_attn_tree import formula, many, seen_of, tree
+
+    g, M, past = np.random.default_rng(1), 9, 20
+    masks, _ = ql.tree_masks(tree(M, 2))
+    masks[4] = 0
+    for p in (0, past):
+        for what, value in ((None, 0), ("k", np.nan), ("k", np.inf), ("k", -np.inf), ("v", np.nan), ("v", np.inf), ("v", -np.inf)):
+            q, k, v = (g.standard_normal(s).astype(np.float32) for s in ((M, 4, 8), (p + M, 2, 8), (p + M, 2, 8)))
+            if what:
+                (k if what == "k" else v)[[p + 3, p + M - 1], :, 5] = value
+            a, b = formula(q, k, v, seen_of(masks, M, p)), many(q, k, v, seen_of(masks, M, p))
+            assert np.allclose(a[0], b[0], rtol=1e-12, atol=1e-12, equal_nan=True)
+            at = np.isfinite(a[0]) & (a[0] != 0)
+            assert np.allclose(a[1][at], b[1][at], rtol=1e-9)

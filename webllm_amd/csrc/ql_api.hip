@@ -2626,6 +2626,28 @@ bool dtype_bytes(int32_t dtype, uint64_t* bytes)
     return dtype == QL_DTYPE_F16 || dtype == QL_DTYPE_F32;
 }
 
+// the dimensions of ql_attention_tree and its plan, in `a`; `bytes` of a cache value
+int tree_args(int32_t cache_dtype, int32_t max_t, int32_t M, int32_t n_head, int32_t n_kv_head, int32_t D, int32_t past_len, ql::TreeArgs* a, uint64_t* bytes)
+{
+    if (M < 1 || M > ql::kTreeMaxRows) return fail(QL_E_INVALID, "M must be 1..%d (got %d)", ql::kTreeMaxRows, M);
+    if (n_head < 1 || n_head > 4096 || n_kv_head < 1 || past_len < 0 || max_t < 1) return fail(QL_E_INVALID, "bad attention dimensions");
+    if (past_len > ql::kTreeMaxPast) return fail(QL_E_INVALID, "past_len above %d", ql::kTreeMaxPast);
+    if (n_head % n_kv_head) return fail(QL_E_INVALID, "n_head (%d) must be a multiple of n_kv_head (%d)", n_head, n_kv_head);
+    if (D < 8 || D > ql::kAttnMaxD || D % 8) return fail(QL_E_INVALID, "head dim must be 8..%d, a multiple of 8 (got %d)", ql::kAttnMaxD, D);
+    if (!dtype_bytes(cache_dtype, bytes)) return fail(QL_E_INVALID, "bad cache_dtype %d", cache_dtype);
+    if ((int64_t)past_len + M > max_t) return fail(QL_E_RANGE, "context length %lld exceeds the cache's %d positions", (long long)past_len + M, max_t);
+    a->M = M;
+    a->H = n_head;
+    a->KV = n_kv_head;
+    a->G = n_head / n_kv_head;
+    a->D = D;
+    a->past = past_len;
+    a->words = (M + 63) / 64;
+    a->half = *bytes == 2;
+    a->scale = (float)(1.4426950408889634 / std::sqrt((double)D));
+    return QL_OK;
+}
+
 }  // namespace
 
 int ql_rope_table(ql_ctx* ctx, ql_arena* weights, uint64_t table_off, int32_t max_pos, int32_t rot_dim, double theta)
@@ -2743,22 +2765,33 @@ int ql_tree_masks(int32_t M, const int32_t* parents, uint64_t* masks, int32_t* d
     return QL_OK;
 }
 
+int ql_plan_attention_tree(int32_t cache_dtype, int32_t max_t, int32_t M, int32_t n_head, int32_t n_kv_head, int32_t D, int32_t past_len, ql_tree_info* info)
+{
+    if (!info) return fail(QL_E_INVALID, "null info");
+    ql::TreeArgs a;
+    uint64_t cb;
+    const int rc = tree_args(cache_dtype, max_t, M, n_head, n_kv_head, D, past_len, &a, &cb);
+    if (rc) return rc;
+    ql::plan_attention_tree(&a, ql::kAttnTileWsBytes);
+    const bool few = past_len + M < ql::kTreeKeys;
+    info->pairs = few ? 1 : 16 * a.nt;
+    info->waves = few ? 1 : a.waves;
+    info->nsplit = a.nsplit;
+    info->keys_per_split = few ? past_len + M : a.per * ql::kTreeKeys;
+    info->workgroups = few ? M * n_head : a.groups * a.KV * a.nsplit;
+    return QL_OK;
+}
+
 int ql_attention_tree(ql_ctx* ctx, ql_arena* act, uint64_t q_off, const ql_arena* cache, uint64_t k_off, uint64_t v_off,
                       int32_t cache_dtype, int32_t max_t, int32_t M, int32_t n_head, int32_t n_kv_head, int32_t D, int32_t past_len,
                       uint64_t mask_off, uint64_t out_off)
 {
     if (!ctx || !act || !cache) return fail(QL_E_INVALID, "null context or arena");
-    if (M < 1 || M > ql::kTreeMaxRows) return fail(QL_E_INVALID, "M must be 1..%d (got %d)", ql::kTreeMaxRows, M);
-    if (n_head < 1 || n_head > 4096 || n_kv_head < 1 || past_len < 0 || max_t < 1) return fail(QL_E_INVALID, "bad attention dimensions");
-    if (past_len > ql::kTreeMaxPast) return fail(QL_E_INVALID, "past_len above %d", ql::kTreeMaxPast);
-    if (n_head % n_kv_head) return fail(QL_E_INVALID, "n_head (%d) must be a multiple of n_kv_head (%d)", n_head, n_kv_head);
-    if (D < 8 || D > ql::kAttnMaxD || D % 8) return fail(QL_E_INVALID, "head dim must be 8..%d, a multiple of 8 (got %d)", ql::kAttnMaxD, D);
+    ql::TreeArgs a;
     uint64_t cb;
-    if (!dtype_bytes(cache_dtype, &cb)) return fail(QL_E_INVALID, "bad cache_dtype %d", cache_dtype);
-    if ((int64_t)past_len + M > max_t) return fail(QL_E_RANGE, "context length %lld exceeds the cache's %d positions", (long long)past_len + M, max_t);
-    int rc = check_devices(ctx, act, cache, nullptr);
-    if (rc) return rc;
-    const int words = (M + 63) / 64;
+    int rc = tree_args(cache_dtype, max_t, M, n_head, n_kv_head, D, past_len, &a, &cb);
+    if (rc || (rc = check_devices(ctx, act, cache, nullptr))) return rc;
+    const int words = a.words;
     const uint64_t qo = (uint64_t)M * n_head * D * 4, row = (uint64_t)n_kv_head * D * cb, seen = (uint64_t)(past_len + M) * row;
     const bool masked = mask_off != QL_NONE;
     const Span out = {act, out_off, qo};
@@ -2772,21 +2805,11 @@ int ql_attention_tree(ql_ctx* ctx, ql_arena* act, uint64_t q_off, const ql_arena
         return fail(QL_E_ALIGN, "offsets must be 16-byte aligned (mask 8-byte)");
     if (any_meet(&out, 1, reads, 4)) return fail(QL_E_INVALID, "out overlaps an input");
     if ((rc = set_device(ctx))) return rc;
-    ql::TreeArgs a;
     a.q = reinterpret_cast<const float*>(act->base + q_off);
     a.k = cache->base + k_off;
     a.v = cache->base + v_off;
     a.mask = masked ? reinterpret_cast<const uint64_t*>(act->base + mask_off) : nullptr;
     a.out = reinterpret_cast<float*>(act->base + out_off);
-    a.M = M;
-    a.H = n_head;
-    a.KV = n_kv_head;
-    a.G = n_head / n_kv_head;
-    a.D = D;
-    a.past = past_len;
-    a.words = words;
-    a.half = cb == 2;
-    a.scale = (float)(1.4426950408889634 / std::sqrt((double)D));
     const uint64_t bytes = ql::plan_attention_tree(&a, ql::kAttnTileWsBytes);
     std::lock_guard<std::mutex> guard(ctx->ws_lock);
     void* ws;

@@ -40,7 +40,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTreeMaxSplit = 128;
-constexpr int kKeys = 32;                // keys of a block
+constexpr int kKeys = kTreeKeys;         // keys of a block
 constexpr float kRaise = 7.f;            // log2 that scores may rise above the running reference before it is raised
 constexpr float kPScale = 256.f;         // fp16 parts of P: 2^8 P, at most 2^15
 constexpr float kMaxFinite = 3.4028235e38f;

@@ -317,6 +317,7 @@ hipError_t launch_qk_norm_rope(const RopeArgs& a, hipStream_t stream);
 hipError_t launch_rope_table(float* table, int max_pos, int rot, double theta, hipStream_t stream);
 
 constexpr int kTreeMaxRows = 256;
+constexpr int kTreeKeys = 32;                    // keys of a block; contexts of fewer take attn_tree_row_kernel
 constexpr int kTreeMaxPast = 1 << 30;            // its keys are counted in 31 bits
 struct TreeArgs {
     const float* q;            // [M, H, D]
@@ -326,7 +327,7 @@ struct TreeArgs {
     float* ws;                 // key ranges' partials, as attn_kernel's
     int M, H, KV, G, D, past, words, half;
     float scale;               // fp32(log2(e) / sqrt(D))
-    // plan_attention_tree fills these: 16 nt pairs a workgroup, groups of them; blocks of 32 keys, key ranges of `per` of them
+    // plan_attention_tree fills these: 16 nt pairs a workgroup, groups of them; blocks of kTreeKeys keys, key ranges of `per` of them
     int nt, groups, past_blocks, blocks, per, nsplit;
     int waves;                 // of a workgroup
     float inv_nsplit, inv_g;

@@ -97,6 +97,11 @@ class AttnInfo(ctypes.Structure):
                 ("workgroups", ctypes.c_int32), ("keys_per_split", ctypes.c_int32)]
 
 
+class TreeInfo(ctypes.Structure):
+    """The launch shape ql_attention_tree picks (ql_tree_info)."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("pairs", "waves", "nsplit", "keys_per_split", "workgroups")]
+
+
 class RopeDesc(ctypes.Structure):
     """Heads, rotation and cache type of Context.qk_norm_rope (ql_rope_desc)."""
     _fields_ = [("q_norm_off", ctypes.c_uint64), ("k_norm_off", ctypes.c_uint64), ("table_off", ctypes.c_uint64),
@@ -165,6 +170,7 @@ def lib():
         "ql_rope_table": (I, [P, P, U64, I, I, ctypes.c_double]),
         "ql_qk_norm_rope": (I, [P, ctypes.POINTER(RopeDesc), P, P, U64, U64, U64, U64, I, U64, P, U64, U64, I, I]),
         "ql_tree_masks": (I, [I, P, P, P]),
+        "ql_plan_attention_tree": (I, [I, I, I, I, I, I, I, ctypes.POINTER(TreeInfo)]),
         "ql_attention_tree": (I, [P, P, U64, P, U64, U64, I, I, I, I, I, I, I, U64, U64]),
         "ql_token_logprobs": (I, [P, P, U64, I, I, I, U64, I, I, U64, U64, U64, U64]),
         "ql_kv_move": (I, [P, P, ctypes.POINTER(U64), I, P, ctypes.POINTER(U64), I, I, I, I, I, I, P, U64]),
@@ -223,6 +229,13 @@ def plan_attention(max_t: int, M: int, n_head: int, n_kv_head: int, D: int, past
     """The launch shape of ql_attention_decode for these dimensions (host only)."""
     info = AttnInfo()
     _check(lib().ql_plan_attention(max_t, M, n_head, n_kv_head, D, past_len, ctypes.byref(info)))
+    return info
+
+
+def plan_attention_tree(cache_dtype: int, max_t: int, M: int, n_head: int, n_kv_head: int, D: int, past_len: int) -> TreeInfo:
+    """The launch shape of ql_attention_tree for these dimensions (host only)."""
+    info = TreeInfo()
+    _check(lib().ql_plan_attention_tree(cache_dtype, max_t, M, n_head, n_kv_head, D, past_len, ctypes.byref(info)))
     return info
 
 
