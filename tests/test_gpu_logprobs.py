@@ -294,3 +294,34 @@ def test_sure_rows(ql, ctx, V, gap):
         assert np.array_equal(ids[m], order)
         assert (np.abs(tlp[m] - want[order]) <= r * ls + U * np.abs(want[order])).all()
     c.box.release()
+
+
+def test_rows_that_pass_through_the_workspace_in_turn(ql, ctx):
+    """More rows than 64 MiB of partial sums hold at once: 48 bytes per 1024 logits, 9383 rows of 151936. 97 different rows take turns,
+    so that a row's place shows in its results on both sides of the border."""
+    g = np.random.default_rng(12)
+    V, M, N = 151936, 9383 + 20, 97
+    assert (64 << 20) // (48 * -(-V // 1024)) == M - 20
+    x = (2 * g.standard_normal((N, V))).astype(np.float32)
+    x[5] = -np.inf
+    x[7, 3] = np.nan
+    tokens = g.integers(-1, V, (N, 2))
+    lp, ent, ids, tlp = reference(x, tokens, 3)
+    lay, size = ql.ArenaLayout(), 4 * V * M
+    off = {n: lay.take(b) for n, b in (("x", size), ("tok", 8 * M), ("lp", 8 * M + 64), ("ent", 4 * M + 64), ("ids", 12 * M + 64), ("tlp", 12 * M + 64))}
+    arena = ctx.arena(lay.used)
+    for m in range(0, M, N):
+        n = min(N, M - m)
+        arena.write(off["x"] + 4 * V * m, x[:n])
+    at = np.arange(M) % N
+    arena.write(off["tok"], tokens[at].astype(np.int32))
+    for n in ("lp", "ent", "ids", "tlp"):
+        arena.write(off[n], np.full(3 * M + 16 if n in ("ids", "tlp") else 2 * M + 16 if n == "lp" else M + 16, 5, np.float32))
+    ctx.token_logprobs(arena, off["x"], V, M, V, off["tok"], 2, 3, off["lp"], off["ent"], off["ids"], off["tlp"])
+    close(arena.read(off["lp"], (M, 2), np.float32), lp[at], ((100 + 3 * np.abs(lp)) * U)[at])
+    close(arena.read(off["ent"], (M,), np.float32), ent[at], ((200 + 103 * np.abs(ent)) * U)[at])
+    assert np.array_equal(arena.read(off["ids"], (M, 3), np.int32), ids[at])
+    close(arena.read(off["tlp"], (M, 3), np.float32), tlp[at], ((100 + 3 * np.abs(tlp)) * U)[at])
+    for n, size in (("lp", 8 * M), ("ent", 4 * M), ("ids", 12 * M), ("tlp", 12 * M)):
+        assert (arena.read(off[n] + size, (16,), np.float32) == 5).all()
+    arena.release()
