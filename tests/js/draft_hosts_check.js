@@ -7,6 +7,7 @@
  *   node draft_hosts_check.js trees    no GPU: parents of drafted trees
  *   node draft_hosts_check.js table    no GPU: rope tables that are refused
  *   node draft_hosts_check.js read     no GPU: arrays that tensors read into
+ *   node draft_hosts_check.js exports  no GPU: the addon's functions
  *   node draft_hosts_check.js gpu      log probabilities into buffers of more rows than the pass has
  */
 const q = require('../../webllm_amd/js');
@@ -73,6 +74,11 @@ function read() {
     return [undefined, 'f32', 'bytes', 'f16', 'u32', 'i32', 'u64'].map((dtype) => new q.Tensor(from, 0, 2, [2], dtype).read().constructor.name);
 }
 
+function addonExports() {
+    const all = Object.getOwnPropertyNames(q.addon).filter((n) => typeof q.addon[n] === 'function').sort();
+    return { all, hidden: all.filter((n) => !Object.keys(q.addon).includes(n)) };
+}
+
 function gpu() {
     const ctx = new q.Context(0);
     const model = new q.QuantLinearModel(ctx, 1 << 20), pool = new q.ActivationArena(ctx, 1 << 20);
@@ -91,4 +97,4 @@ function gpu() {
     return r;
 }
 
-console.log(JSON.stringify({ widths, fork, trees, table, read, gpu }[process.argv[2]]()));
+console.log(JSON.stringify({ widths, fork, trees, table, read, exports: addonExports, gpu }[process.argv[2]]()));

@@ -138,6 +138,18 @@ def test_node_parents_that_are_no_rows():
 
 
 @needs_node
+def test_every_addon_function_is_a_declared_one():
+    """The addon's functions, those of a drafted pass among them (which are not enumerable), and the C functions they forward to."""
+    from tests.test_node_host import BINDING
+
+    draft = {"ropeTable": "ql_rope_table", "qkNormRope": "ql_qk_norm_rope", "treeMasks": "ql_tree_masks", "attentionTree": "ql_attention_tree",
+             "tokenLogprobs": "ql_token_logprobs", "kvMove": "ql_kv_move"}
+    r = node("exports")
+    assert r["all"] == sorted({**BINDING, **draft}) and r["hidden"] == sorted(draft)
+    assert set(draft.values()) <= set(ql.header_functions())
+
+
+@needs_node
 def test_node_tensors_without_a_type():
     """A tensor whose type is left out, or is none of those with an array of their own, reads as fp32."""
     assert node("read") == ["Float32Array", "Float32Array", "Float32Array", "Uint16Array", "Uint32Array", "Int32Array", "BigUint64Array"]
