@@ -40,7 +40,8 @@ function fork() {
     message(() => a.fork(b, 5));                               // ends at the library: no device
     const before = log.splice(0);
     message(() => a.fork(c, 5));
-    return { before, same: log };
+    const d = new q.KvCache(one, { ...config, nHead: 4, nKvHead: 2 });
+    return { before, same: log, heads: message(() => a.fork(d, 3)) };
 }
 
 function trees() {

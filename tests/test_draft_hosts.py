@@ -85,9 +85,9 @@ def test_node_widths_of_logprobs():
     assert all(e and e.startswith("tokenLogprobs:") for e in r["refused"]), r["refused"]
 
 
-def cache_of(ctx, log):
+def cache_of(ctx, log, n_head=2, n_kv_head=1):
     """A KvCache whose context only notes what it is asked for."""
-    cfg = gptq.QwenConfig(vocab_size=64, block_size=32, n_layer=2, n_head=2, n_kv_head=1, n_embd=128, intermediate=64, rope_theta=1e4)
+    cfg = gptq.QwenConfig(vocab_size=64, block_size=32, n_layer=2, n_head=n_head, n_kv_head=n_kv_head, n_embd=128, intermediate=64, rope_theta=1e4)
     c = gptq.KvCache(ctx, cfg)
     log.clear()
     return c
@@ -122,9 +122,22 @@ def test_fork_between_contexts_refuses_before_it_copies():
     assert not any(call == "kv_move" for _, call, _ in log)
 
 
+def test_fork_between_other_heads():
+    """One head of 64 and two of 32 have rows of the same bytes, which mean other keys."""
+    log = []
+    ctx = Recorder(log)
+    a, b = cache_of(ctx, log), cache_of(ctx, log, n_head=4, n_kv_head=2)
+    assert a.row_len == b.row_len
+    for x, y in ((a, b), (b, a)):
+        with pytest.raises(ValueError, match="heads"):
+            x.fork(y, 3)
+    assert log == []
+
+
 @needs_node
 def test_node_fork_between_contexts_is_ordered():
     r = node("fork")
+    assert "heads" in r["heads"]
     assert sorted(r["before"]) == ["one", "two"] and r["same"] == []
 
 

@@ -353,7 +353,7 @@ class KvCache:
         A cache of another context: the copy runs on this one's stream, and the host waits for what the other stream has still to do
         with the cache before it, and for the copy after it."""
         a, b = self.config, to.config
-        if (a.n_layer, self.row_len, self.dtype) != (b.n_layer, to.row_len, to.dtype):
+        if (a.n_layer, a.n_kv_head, self.D, self.dtype) != (b.n_layer, b.n_kv_head, to.D, to.dtype):
             raise ValueError("fork: the caches differ in layers, heads or dtype")
         apart = to.ctx is not self.ctx
         if apart:

@@ -782,7 +782,7 @@ class KvCache {
      * runs on this one's stream, and the host waits for the other stream before it and for the copy after it.
      */
     fork(to, rows) {
-        if (to.config.nLayer !== this.config.nLayer || to.rowLen !== this.rowLen || to.dtype !== this.dtype)
+        if (to.config.nLayer !== this.config.nLayer || to.config.nKvHead !== this.config.nKvHead || to.D !== this.D || to.dtype !== this.dtype)
             throw new Error('fork: the caches differ in layers, heads or dtype');
         const apart = to.ctx !== this.ctx;
         if (apart) { this.ctx.sync(); to.ctx.sync(); }
