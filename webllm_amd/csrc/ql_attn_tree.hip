@@ -16,14 +16,18 @@
 // fp32 caches: an operand enters as three bf16 parts, 24 bits with fp32's own range, so no value depends on its neighbours' size; a
 // product is the six largest of the nine (v_mfma_f32_16x16x32_bf16: 6/16 of the fp32 MFMA's time).
 // fp16 caches: K and V enter as they are; q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P. Two products.
+// P's parts hold 22 bits of a weight down to 2^-10 of the running reference, below that to half a step of 2^-24, 2^-33 of the reference: T
+// keys of a wave are off by T 2^-33 of the largest |V| at most, a sixteenth of what their T / 32 fp32 additions may be. Finer parts,
+// and what 256 rows after 8000 keys took for 91.0 us: lo as 2^-11 lo in a sum of its own (2^-44 of the reference) 96.0, a reference
+// raised at 2^1 in place of 2^7 and 2^14 P (2^-39) 93.9, at 2^3 and 2^12 P (2^-37) 91.8.
 //
 // What the parts cannot carry is not finite: an infinity's remainder is a NaN, and 0 * V is one where V is not. A wave whose sums
 // end that way does its blocks again on the VALU from q, K and V themselves, skipping what a pair does not see (tree_again).
 //
-// us, of them the merge, and what bounds it (28 / 4 heads of 128): 1 row after 32000 fp16 keys 17.1, 4, memory (65.5 MB); 24 rows after
-// 4000 fp32 keys 23.3, 4, the parts' VALU work and the matrix unit in turn; 256 after 8000 fp16 keys 85.1, 5, issue: two waves a SIMD
-// fit its registers, the VALU is busy half of the cycles, the matrix unit 27 %. 14 / 2 heads of 64: 5 rows after 300 fp32 keys 7.4,
-// one launch and its chain of loads.
+// us, of them the merge, and what bounds it (28 / 4 heads of 128): 1 row after 32000 fp16 keys 17.1, 4, memory (65.5 MB; fp32 35.2); 24 rows
+// after 4000 fp32 keys 23.3, 4, the parts' VALU work and the matrix unit in turn, on CUs that have one or two workgroups: they are
+// busy 55 % of the time; 256 after 8000 fp16 keys 86.4, 5, issue: two waves a SIMD fit its registers, the VALU is busy half of the
+// cycles, the matrix unit 28 %; fp32 205.8. 14 / 2 heads of 64: 5 rows after 300 fp32 keys 7.4, one launch and its chain of loads.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -88,7 +92,7 @@ template <typename T, int DP, int NT, bool FULL, int WAVES>
 struct TreeTile {
     static constexpr bool kHalf = std::is_same<T, _Float16>::value;
     static constexpr bool kAhead = DP <= 128;               // a block's K is loaded before the last one's V is used, V before K is
-    static constexpr int kNK = kKeys / 16, kNH = 1;
+    static constexpr int kNK = kKeys / 16;
     static constexpr int kTD = DP / 32, kDT = DP / 16;
     static constexpr int kParts = kHalf ? 2 : 3;            // of q
     static constexpr int kCols = kHalf && DP >= 128 ? 8 : 4;   // columns of V a lane loads at once
@@ -386,7 +390,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
     }
     const int first = b;
     for (; b < b1; b += WAVES) {
-        typename C::VRaw vraw[C::kNH][8][C::kNC];           // [32 keys][element of the fragment][columns]
+        typename C::VRaw vraw[8][C::kNC];                   // [element of the fragment][columns]
         auto load_v = [&](const TreeBlock& blk, int c0, int c1) {
             const char* base = reinterpret_cast<const char*>(vb + (size_t)blk.at * row_len);
 #pragma unroll
@@ -395,8 +399,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
 #pragma unroll
                 for (int c = c0; c < c1; c++) {
                     if (FULL || C::kChunk * c + C::kCols * i16 < D)
-                        vraw[0][e][c] = ld_global(reinterpret_cast<const typename C::VRaw*>(p + C::kChunk * c * sizeof(T) + v_lane));
-                    else vraw[0][e][c] = typename C::VRaw{};
+                        vraw[e][c] = ld_global(reinterpret_cast<const typename C::VRaw*>(p + C::kChunk * c * sizeof(T) + v_lane));
+                    else vraw[e][c] = typename C::VRaw{};
                 }
             }
         };
@@ -515,28 +519,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
 #pragma unroll
                 for (int d = 0; d < C::kDT; d++) acc[d][nt] *= al;
             }
-        Frag pf[C::kNH][NT][C::kParts];
+        Frag pf[NT][C::kParts];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const float ref = mr[nt] == -INFINITY ? 0.f : mr[nt];
+            float p[8];
 #pragma unroll
-            for (int h = 0; h < C::kNH; h++) {
-                float p[8];
+            for (int e = 0; e < 8; e++) {
+                p[e] = ex2(fmaf(s[e >> 2][nt][e & 3], f[nt], -ref));
+                l[nt] += p[e];
+            }
+            if constexpr (C::kHalf) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    p[e] = ex2(fmaf(s[2 * h + (e >> 2)][nt][e & 3], f[nt], -ref));
-                    l[nt] += p[e];
+                    const float y = p[e] * kPScale;
+                    pf[nt][0][e] = (_Float16)y;
+                    pf[nt][1][e] = (_Float16)(y - (float)pf[nt][0][e]);
                 }
-                if constexpr (C::kHalf) {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float y = p[e] * kPScale;
-                        pf[h][nt][0][e] = (_Float16)y;
-                        pf[h][nt][1][e] = (_Float16)(y - (float)pf[h][nt][0][e]);
-                    }
-                } else {
-                    split_bf16(p, pf[h][nt]);
-                }
+            } else {
+                split_bf16(p, pf[nt]);
             }
         }
         // a block's sums start from zero and are added to the others by the VALU: the matrix unit carries no long sum
@@ -556,29 +557,23 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) o[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if constexpr (C::kHalf) {
-                    f16x8 v[C::kNH];
+                    u32x4 w;
 #pragma unroll
-                    for (int h = 0; h < C::kNH; h++) {
-                        u32x4 w;
-#pragma unroll
-                        for (int e = 0; e < 4; e++)         // column j of keys 2 e and 2 e + 1
-                            w[e] = __builtin_amdgcn_perm(vraw[h][2 * e + 1][c][j / 2], vraw[h][2 * e][c][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
-                        v[h] = __builtin_bit_cast(f16x8, w);
-                    }
+                    for (int e = 0; e < 4; e++)             // column j of keys 2 e and 2 e + 1
+                        w[e] = __builtin_amdgcn_perm(vraw[2 * e + 1][c][j / 2], vraw[2 * e][c][j / 2], j & 1 ? 0x07060302u : 0x05040100u);
+                    const f16x8 v = __builtin_bit_cast(f16x8, w);
 #pragma unroll
                     for (int part = 1; part >= 0; part--)
 #pragma unroll
-                        for (int h = 0; h < C::kNH; h++)
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) o[nt] = mfma(v[h], pf[h][nt][part], o[nt]);
+                        for (int nt = 0; nt < NT; nt++) o[nt] = mfma(v, pf[nt][part], o[nt]);
                 } else {
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = vraw[0][e][c][j];
+                    for (int e = 0; e < 8; e++) x[e] = vraw[e][c][j];
                     bf16x8 vp[3];
                     split_bf16(x, vp);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) o[nt] = mfma(vp[0], pf[0][nt][0], small_products(vp, pf[0][nt], o[nt]));
+                    for (int nt = 0; nt < NT; nt++) o[nt] = mfma(vp[0], pf[nt][0], small_products(vp, pf[nt], o[nt]));
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) acc[c * C::kCols + j][nt] += o[nt];
@@ -603,7 +598,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_tree_kernel(const TreeArgs
     const bool redo = __any(odd != 0.f);
     if (redo) tree_again<T, DP, NT, FULL, C::kCols>(a, kvh, rg * C::kRows, first, b1, WAVES, past_blocks, mr, l, acc);
 
-    // the four waves' states
+    // the waves' states
     const float unit = C::kHalf && !redo ? 1.f / kPScale : 1.f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
@@ -800,7 +795,10 @@ uint64_t plan_attention_tree(TreeArgs* a, size_t ws_bytes)
     // into parts half as often, but a wave's own chain is longer. Also where 16 would be more than two workgroups a CU (fp16: and 32
     // fill it four times). 16 against 32, in us (28 / 4 heads of 128): 16 rows after 4000 keys 18.9, 19.5, 24 after 4000 26.1, 23.6,
     // fp16 24 after 8000 19.8, 21.1, 64 after 8000 32.8, 31.1, 256 after none 15.5, 21.2; 14 / 2 heads of 64: 256 after 200 22.8,
-    // 15.1, fp16 256 after 200 11.5, 13.7, after 2000 35.9, 19.6.
+    // 15.1, fp16 256 after 200 11.5, 13.7, after 2000 35.9, 19.6. About the border in fp32, by `full`: 576 21.7, 22.4 (24 after 3000), 640
+    // 22.2, 22.7 (20 after 4000), 672 22.3, 23.4 (32 after 3000), 744 26.0, 23.2 (24 after 3900), 748 22.4, 23.9 (48 after 2000), 756 25.9, 22.4
+    // (12 after 8000), 868 26.6, 24.5 (32 after 3900), 960 26.7, 24.1 (20 after 6000), 1056 27.6, 29.5 (48 after 3000), 1364 34.8, 34.9 (48 after
+    // 4000): `full` is a measure of the work, and what decides between 700 and 1100 is how evenly the ranges lie on the CUs.
     const long full = (long)((R + 31) / 32) * a->KV * ((a->past + a->M + 4 * kKeys - 1) / (4 * kKeys));
     const int per_xcd = (R + 15) / 16 * ((a->KV + 7) / 8);              // workgroups of 16 pairs, in a range
     const bool crowded = per_xcd > 64, wide = a->half ? full >= (crowded ? 1024 : 2048) : full >= 768 || crowded;

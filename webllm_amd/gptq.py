@@ -297,7 +297,9 @@ class KvCache:
     def rotate_store(self, layer: int, model: "QuantLinearModel", q: Tensor, k: Tensor, v: Tensor, positions: Tensor, q_out: Tensor,
                      M: int, slot0: int, rope: str = "rope", q_norm: str | None = None, k_norm: str | None = None, eps: float = 1e-6):
         """q and k turned by their rows' positions (i32 [M]; qwen.ts:414-423, ropeHalfRef's pairs), normed per head first where
-        norm weights are named; q to q_out (q itself may be given), k and v to cache rows slot0 + m."""
+        norm weights are named; q to q_out (q itself may be given), k and v to cache rows slot0 + m. A row whose position the table
+        does not have is padding: its q_out and cache rows stay as they were (q_out = q: unturned), so the table needs as many
+        positions as the text may have."""
         c = self.config
         if q.length < M * c.n_head * self.D or q_out.length < M * c.n_head * self.D:
             raise ValueError("rotate_store: q/q_out smaller than [M, n_head * D]")

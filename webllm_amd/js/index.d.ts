@@ -134,7 +134,7 @@ export class KvCache {
     readonly rowLen: number;
     store(layer: number, k: Tensor, v: Tensor, rows: number, pos0: number): void;
     attend(layer: number, q: Tensor, out: Tensor, M: number, pastLen: number): void;
-    /** norms (where named), rotation by positions (i32) and cache store in one launch (ql_qk_norm_rope) */
+    /** norms (where named), rotation by positions (i32; outside the table: padding, left out) and cache store in one launch (ql_qk_norm_rope) */
     rotateStore(layer: number, model: QuantLinearModel, q: Tensor, k: Tensor, v: Tensor, positions: Tensor, qOut: Tensor, M: number,
                 slot0: number, options?: { rope?: string; qNorm?: string; kNorm?: string; eps?: number }): void;
     /** attention of M <= 256 drafted rows (ql_attention_tree); masks: treeMasks' words, or none for causal rows */

@@ -740,12 +740,17 @@ class KvCache {
         addon.attention(this.ctx.handle, q.arena.handle, q.offset, this.arena.handle, ko, vo, c.blockSize, M,
             c.nHead, c.nKvHead, this.D, pastLen, out.offset);
     }
-    /** q and k turned by positions (i32 [M]) and normed per head where weights are named; q to qOut, k and v to rows slot0 + m. */
+    /**
+     * q and k turned by positions (i32 [M]) and normed per head where weights are named; q to qOut, k and v to rows slot0 + m. A row
+     * whose position the table does not have is padding: its qOut and cache rows stay as they were (qOut = q: unturned), so the
+     * table needs as many positions as the text may have.
+     */
     rotateStore(layer, model, q, k, v, positions, qOut, M, slot0, options) {
         const o = options || {}, c = this.config;
         if ([k, v, positions, qOut].some((t) => t.arena !== q.arena)) throw new Error('rotateStore: tensors must share one arena');
         if (q.length < M * c.nHead * this.D || qOut.length < M * c.nHead * this.D || k.length < M * this.rowLen || v.length < M * this.rowLen ||
-            [q, k, v, qOut].some((t) => t.dtype !== 'f32') || positions.dtype !== 'i32' || positions.length < M) throw new Error('rotateStore: a tensor is too small or of another type');
+            [q, k, v, qOut].some((t) => t.dtype !== 'f32') || positions.dtype !== 'i32' || positions.length < M)
+            throw new Error('rotateStore: a tensor is too small or of another type');
         const weight = (name, length) => {
             const w = model.f32Weights.get(name);
             if (!w || (length ? w.length !== length : w.shape.length !== 2)) throw new Error(`missing f32 weight: ${name}`);
@@ -764,7 +769,8 @@ class KvCache {
     attendTree(layer, q, out, M, pastLen, masks) {
         const c = this.config;
         if (q.arena !== out.arena || (masks && masks.arena !== q.arena)) throw new Error('attendTree: q, out and masks must share one arena');
-        if (q.dtype !== 'f32' || out.dtype !== 'f32' || q.length < M * c.nHead * this.D || out.length < M * c.nHead * this.D || (masks && (masks.dtype !== 'u64' || masks.length < M * Math.ceil(M / 64))))
+        if (q.dtype !== 'f32' || out.dtype !== 'f32' || q.length < M * c.nHead * this.D || out.length < M * c.nHead * this.D ||
+            (masks && (masks.dtype !== 'u64' || masks.length < M * Math.ceil(M / 64))))
             throw new Error('attendTree: a tensor is too small or of another type');
         const [ko, vo] = this.offsets(layer);
         addon.attentionTree(this.ctx.handle, q.arena.handle, q.offset, this.arena.handle, ko, vo, this.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32,
