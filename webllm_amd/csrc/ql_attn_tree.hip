@@ -25,8 +25,8 @@
 // end that way does its blocks again on the VALU from q, K and V themselves, skipping what a pair does not see (tree_again).
 //
 // us, of them the merge, and what bounds it (28 / 4 heads of 128): 1 row after 32000 fp16 keys 17.1, 4, memory (65.5 MB; fp32 35.2); 24 rows
-// after 4000 fp32 keys 23.3, 4, the parts' VALU work and the matrix unit in turn, on CUs that have one or two workgroups: they are
-// busy 55 % of the time; 256 after 8000 fp16 keys 86.4, 5, issue: two waves a SIMD fit its registers, the VALU is busy half of the
+// after 4000 fp32 keys 23.3, 4, the parts' VALU work and the matrix unit in turn, on CUs that have one or two workgroups;
+// 256 after 8000 fp16 keys 86.4, 5, issue: two waves a SIMD fit its registers, the VALU is busy half of the
 // cycles, the matrix unit 28 %; fp32 205.8. 14 / 2 heads of 64: 5 rows after 300 fp32 keys 7.4, one launch and its chain of loads.
 #include <algorithm>
 #include <cmath>
