@@ -113,7 +113,8 @@ export class QuantLinearModel {
     siluMul(gate: Tensor, up: Tensor, out: Tensor, n: number): void;
     /** cosines and sines of positions 0 .. maxPos - 1 in the weight arena (ql_rope_table), named 'rope' by default */
     makeRopeTable(maxPos: number, rotDim: number, theta: number, name?: string): void;
-    /** log probabilities of given tokens, entropies and top alternatives of M rows of V logits (ql_token_logprobs) */
+    /** log probabilities of given tokens, entropies and top alternatives of M rows of V logits (ql_token_logprobs); T and k are the
+     * tensors' second dimension */
     tokenLogprobs(logits: Tensor, M: number, V: number, o: {
         tokens?: Tensor | null; logprobs?: Tensor | null; entropy?: Tensor | null; topIds?: Tensor | null; topLogprobs?: Tensor | null;
     }): void;
