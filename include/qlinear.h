@@ -64,6 +64,7 @@ extern "C" {
 
 #define QL_DTYPE_F32 0
 #define QL_DTYPE_F16 1
+#define QL_DTYPE_F8 2 /* e4m3 values (largest 448) under powers of two: paged caches only */
 
 /* kernel families returned by ql_plan_linear */
 #define QL_KIND_GEMV_MFMA 1   /* M <= 16: packed-int4 GEMV on MFMA, hi/lo split activations */
@@ -344,6 +345,80 @@ int ql_token_logprobs(ql_ctx* ctx, ql_arena* act, uint64_t logits_off, int32_t s
 int ql_kv_move(ql_ctx* ctx, ql_arena* dst, const uint64_t* dst_offs, int32_t dst_max_t, const ql_arena* src, const uint64_t* src_offs,
                int32_t src_max_t, int32_t count, int32_t row_bytes, int32_t dst_row, int32_t src_row, int32_t n, const ql_arena* act,
                uint64_t rows_off);
+
+/* ---- a pass over many requests at once: paged caches, a batch's rows of several sequences, low-rank adapters.
+ * The order of a layer: linears over all M rows, ql_lora_add where requests have adapters, ql_paged_append,
+ * ql_paged_attention, linears.
+ *
+ * A batch has n_seq sequences, whose rows lie one behind the other: sequence s has rows row_start[s] .. row_start[s + 1] - 1, one
+ * of a request that decodes, many of a prompt or a piece of one. kv_len[s] counts its tokens with those of this pass: the last of its n
+ * rows is token kv_len[s] - 1, the first kv_len[s] - n, and a row's position is its token. Token t lies in page pages[s][t / page_size].
+ * The tables are int32 in `act` and read on the device, so a captured graph serves every pass of its sizes. What they may not say is
+ * skipped, not followed: a sequence with row_start descending or outside 0..M, with more than max_rows rows, or with kv_len outside n..max_len has no
+ * rows at all; a token whose page is outside 0..n_page - 1 is not stored, and no row sees it. Rows behind the last sequence are padding.
+ * Rows of q_out and out that belong to no sequence stay as they were. No two sequences may append to one page; they may share pages that they
+ * only read. */
+typedef struct ql_batch_desc {
+    uint64_t row_start_off; /* int32 [n_seq + 1], ascending */
+    uint64_t kv_len_off;    /* int32 [n_seq] */
+    uint64_t pages_off;     /* int32 [n_seq, max_pages] */
+    int32_t n_seq;          /* 1..4096 */
+    int32_t max_pages;      /* pages of a sequence's list */
+    int32_t max_rows;       /* most rows that a sequence has in this pass, and the most tokens that one has: at most max_pages * page_size. */
+    int32_t max_len;        /* They choose the launches; bounds near what the tables hold serve best */
+} ql_batch_desc;
+/* A layer's paged cache, regions of n_page pages in a cache arena, offsets 16-byte aligned. A page holds page_size tokens of all kv heads, each
+ * head's behind the other. D is a multiple of 16, u = 16 bytes of values: 8 (fp16) or 16 (e4m3).
+ *   K  [n_page, n_kv_head, page_size / 16, D / u, 16, u]: value d of token t at (t / 16, d / u, t % 16, d % u)
+ *   V  [n_page, n_kv_head, page_size / 4u, D / 16, 4, 16, u]: at (t / 4u, d / 16, t / 4 % 4, d % 16, t / 16 % (u / 4) * 4 + t % 4)
+ *   QL_DTYPE_F8: fp32 scales [n_page, n_kv_head, page_size / 16] of K and of V, powers of two 2^-120 .. 2^120; a value is its e4m3
+ *   number times the scale of its 16 tokens.
+ * Pages are copied with ql_kv_move: a page is a row of n_kv_head * page_size * D values. */
+typedef struct ql_paged_desc {
+    uint64_t k_off, v_off;
+    uint64_t k_scale_off, v_scale_off;   /* QL_DTYPE_F8 (otherwise ignored) */
+    int32_t n_page;
+    int32_t page_size;      /* 64, 128 or 256 */
+    int32_t n_kv_head;
+    int32_t D;              /* 16..256, a multiple of 16 */
+    int32_t cache_dtype;    /* QL_DTYPE_F16 or QL_DTYPE_F8 */
+    int32_t reserved;       /* 0 */
+} ql_paged_desc;
+/* ql_qk_norm_rope over a batch's rows: q and k RMSNormed per head (where the descriptor has weights) and turned by their positions, q to
+ * q_out [M, n_head, D] in q_dtype (fp32, or fp16 rounded once), k and v to their tokens' places in the cache. `rope` is ql_qk_norm_rope's
+ * descriptor, with the cache's n_kv_head, D and cache_dtype, and max_pos at least max_len.
+ * fp16: rounded once; beyond 65504 infinite. e4m3: a group of 16 tokens of a head has one scale. Where the pass brings the group's first token, it is the smallest
+ * 2^e (e >= -120) under which its largest new value is at most 448; otherwise that or the one the group has, whichever is larger, and
+ * where it grows, the group's earlier tokens are rounded anew under it (exact but for values below 2^-6 of the new scale). Each value is rounded
+ * once to e4m3; an infinity or NaN is stored as NaN and does not enter the scale.
+ * q_out may be q itself (fp32, same offset, dense rows); any other overlap of what is written with what is read, tables included, fails with
+ * QL_E_INVALID. M = 1..65535 rows of the buffers, M * (n_head + 2 n_kv_head) <= 2^26. Offsets 16-byte aligned (tables: 4). */
+int ql_paged_append(ql_ctx* ctx, const ql_rope_desc* rope, const ql_arena* weights, ql_arena* act, uint64_t q_off, uint64_t k_off,
+                    uint64_t v_off, const ql_batch_desc* batch, int32_t M, uint64_t q_out_off, int32_t q_dtype, ql_arena* cache,
+                    const ql_paged_desc* paged);
+/* out[m, h, :] = softmax_t(q[m, h] . K[t, h / (n_head / n_kv_head)] / sqrt(D)) V[t, ...] over the tokens t <= the row's own of its
+ * sequence, which the cache holds (ql_paged_append has run). q and out are [M, n_head, D] in `act`, both of q_dtype: fp32 (q as two fp16
+ * parts of about 22 bits under its row's exponent, probabilities likewise), or fp16 (probabilities rounded once to fp16, as the result is). Sums and softmax in
+ * fp32. A row that sees nothing, or no score above -inf, is zero. What a row does not see adds nothing to it, infinities and NaN included;
+ * a value of q that is not finite makes its head's row NaN. max_len <= 2^30. Offsets 16-byte aligned. Uses the context's 64 MiB workspace. */
+int ql_paged_attention(ql_ctx* ctx, ql_arena* act, uint64_t q_off, int32_t q_dtype, const ql_arena* cache, const ql_paged_desc* paged,
+                       const ql_batch_desc* batch, int32_t M, int32_t n_head, uint64_t out_off);
+/* Low-rank adapters of one projection, all n_adapter of them, in `weights`. */
+typedef struct ql_lora_desc {
+    uint64_t a_off;         /* fp16 [n_adapter, rank, K] */
+    uint64_t b_off;         /* fp16 [n_adapter, N, rank] */
+    uint64_t scale_off;     /* fp32 [n_adapter], or QL_NONE: 1 */
+    int32_t K, N;           /* the projection's; K a multiple of 8, N of 4 */
+    int32_t rank;           /* 8..128, a multiple of 8; an adapter of a lower rank has zeros behind its own */
+    int32_t n_adapter;      /* 1..65536 */
+} ql_lora_desc;
+/* For each of `count` (1..8) projections: y[m, :] = base[m, :] + scale[a] * (x[m, :] . A_a^T) . B_a^T, a = ids[m]; y = base where ids[m] is outside
+ * 0..n_adapter - 1 (-1: a row without an adapter). ids is int32 [M] in `act`; x [M, K] in x_dtype (fp32 or fp16), base and y fp32 [M, N] at
+ * x_offs[i], base_offs[i], y_offs[i] in `act`. y_offs[i] may be base_offs[i] (a row without an adapter is not touched);
+ * any other overlap of what is written with what is read fails with QL_E_INVALID. Products and sums in fp32 (fp16 x: exact products).
+ * M = 1..65535. Offsets 16-byte aligned (ids, scales: 4). Uses the context's 64 MiB workspace. */
+int ql_lora_add(ql_ctx* ctx, int32_t count, const ql_lora_desc* descs, const ql_arena* weights, ql_arena* act, uint64_t ids_off,
+                const uint64_t* x_offs, int32_t x_dtype, int32_t M, const uint64_t* base_offs, const uint64_t* y_offs);
 
 /* several independent linears in one launch (e.g. q/k/v on one input, gate/up on another);
  * linear i reads x_offs[i] and writes y_offs[i]; scratch for all of them starts at scratch_off

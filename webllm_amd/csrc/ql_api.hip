@@ -2917,6 +2917,243 @@ int ql_kv_move(ql_ctx* ctx, ql_arena* dst, const uint64_t* dst_offs, int32_t dst
     return QL_OK;
 }
 
+// ---- a pass over many requests
+
+namespace {
+
+// a cache of pages, checked; *read: its regions and scales
+int paged_regions(const ql_paged_desc* p, const ql_arena* cache, uint64_t* value_bytes, Span read[4])
+{
+    if (p->cache_dtype != QL_DTYPE_F16 && p->cache_dtype != QL_DTYPE_F8) return fail(QL_E_INVALID, "bad cache_dtype %d", p->cache_dtype);
+    if (p->n_page < 1 || p->reserved) return fail(QL_E_INVALID, "n_page must be positive, reserved 0");
+    if (p->page_size != 64 && p->page_size != 128 && p->page_size != 256) return fail(QL_E_INVALID, "page_size must be 64, 128 or 256 (got %d)", p->page_size);
+    if (p->n_kv_head < 1 || p->n_kv_head > 4096) return fail(QL_E_INVALID, "n_kv_head must be 1..4096");
+    if (p->D < 16 || p->D > ql::kAttnMaxD || p->D % 16) return fail(QL_E_INVALID, "head dim must be 16..%d, a multiple of 16 (got %d)", ql::kAttnMaxD, p->D);
+    const bool f8 = p->cache_dtype == QL_DTYPE_F8;
+    *value_bytes = f8 ? 1 : 2;
+    const uint64_t tokens = (uint64_t)p->n_kv_head * p->page_size, values = (uint64_t)p->n_page * (tokens * p->D * *value_bytes);
+    const uint64_t scales = f8 ? (uint64_t)p->n_page * (tokens / 4) : 0;
+    read[0] = {cache, p->k_off, values};
+    read[1] = {cache, p->v_off, values};
+    read[2] = {cache, f8 ? p->k_scale_off : 0, scales};
+    read[3] = {cache, f8 ? p->v_scale_off : 0, scales};
+    for (int i = 0; i < 4; i++) {
+        if (!in_range(read[i].off, read[i].bytes, cache->size)) return fail(QL_E_RANGE, "pages or their scales outside the cache arena");
+        if (read[i].off % 16) return fail(QL_E_ALIGN, "cache offsets must be 16-byte aligned");
+    }
+    return QL_OK;
+}
+
+// a batch's tables, checked; *read: their ranges
+int batch_tables(const ql_batch_desc* b, const ql_paged_desc* p, const ql_arena* act, int32_t M, ql::PagedBatch* out, Span read[3])
+{
+    if (M < 1 || M > 65535) return fail(QL_E_INVALID, "M must be 1..65535 (got %d)", M);
+    if (b->n_seq < 1 || b->n_seq > ql::kPagedMaxSeqs) return fail(QL_E_INVALID, "n_seq must be 1..%d (got %d)", ql::kPagedMaxSeqs, b->n_seq);
+    if (b->max_pages < 1 || b->max_rows < 1 || b->max_len < 1) return fail(QL_E_INVALID, "max_pages, max_rows and max_len must be positive");
+    if (b->max_len > ql::kPagedMaxLen) return fail(QL_E_INVALID, "max_len above %d", ql::kPagedMaxLen);
+    if (b->max_len > (int64_t)b->max_pages * p->page_size) return fail(QL_E_RANGE, "max_len %d exceeds %d pages of %d tokens", b->max_len, b->max_pages, p->page_size);
+    read[0] = {act, b->row_start_off, (uint64_t)(b->n_seq + 1) * 4};
+    read[1] = {act, b->kv_len_off, (uint64_t)b->n_seq * 4};
+    read[2] = {act, b->pages_off, (uint64_t)b->n_seq * b->max_pages * 4};
+    for (int i = 0; i < 3; i++) {
+        if (!in_range(read[i].off, read[i].bytes, act->size)) return fail(QL_E_RANGE, "row_start, kv_len or pages outside the activation arena");
+        if (read[i].off % 4) return fail(QL_E_ALIGN, "the batch's tables must be 4-byte aligned");
+    }
+    out->row_start = reinterpret_cast<const int32_t*>(act->base + b->row_start_off);
+    out->kv_len = reinterpret_cast<const int32_t*>(act->base + b->kv_len_off);
+    out->pages = reinterpret_cast<const int32_t*>(act->base + b->pages_off);
+    out->S = b->n_seq;
+    out->M = M;
+    out->max_pages = b->max_pages;
+    out->max_rows = std::min(b->max_rows, M);
+    out->max_len = b->max_len;
+    out->n_page = p->n_page;
+    out->log_page = p->page_size == 64 ? 6 : p->page_size == 128 ? 7 : 8;
+    return QL_OK;
+}
+
+}  // namespace
+
+int ql_paged_append(ql_ctx* ctx, const ql_rope_desc* d, const ql_arena* weights, ql_arena* act, uint64_t q_off, uint64_t k_off, uint64_t v_off,
+                    const ql_batch_desc* batch, int32_t M, uint64_t q_out_off, int32_t q_dtype, ql_arena* cache, const ql_paged_desc* paged)
+{
+    if (!ctx || !d || !weights || !act || !batch || !cache || !paged) return fail(QL_E_INVALID, "null context, descriptor or arena");
+    ql::PagedAppendArgs a;
+    Span reads[10], pages[4];
+    uint64_t cb, qb;
+    int rc = paged_regions(paged, cache, &cb, pages);
+    if (rc || (rc = batch_tables(batch, paged, act, M, &a.b, reads + 1))) return rc;
+    if (d->n_head < 1 || d->n_head > 4096) return fail(QL_E_INVALID, "n_head must be 1..4096");
+    if (d->n_kv_head != paged->n_kv_head || d->D != paged->D || d->cache_dtype != paged->cache_dtype)
+        return fail(QL_E_INVALID, "n_kv_head, D or cache_dtype differ between the rotation and the cache");
+    if ((int64_t)M * (d->n_head + 2 * d->n_kv_head) > ql::kRopeMaxHeads) return fail(QL_E_INVALID, "M x (n_head + 2 n_kv_head) above %d", ql::kRopeMaxHeads);
+    if (d->rot_dim < 8 || d->rot_dim > d->D || d->rot_dim % 8) return fail(QL_E_INVALID, "rot_dim must be 8..D, a multiple of 8 (got %d)", d->rot_dim);
+    if ((d->interleaved & ~1) || d->reserved) return fail(QL_E_INVALID, "interleaved must be 0 or 1, reserved 0");
+    if (d->max_pos < batch->max_len) return fail(QL_E_RANGE, "max_len %d exceeds the rope table's %d positions", batch->max_len, d->max_pos);
+    if (!dtype_bytes(q_dtype, &qb)) return fail(QL_E_INVALID, "bad q_dtype %d", q_dtype);
+    if (!(d->norm_eps >= 0.f)) return fail(QL_E_INVALID, "norm_eps must be >= 0");
+    const uint64_t D = (uint64_t)d->D, hq = d->n_head * D, hk = d->n_kv_head * D;
+    const int32_t strides[3] = {d->q_stride, d->k_stride, d->v_stride};
+    uint64_t stride[3];
+    for (int i = 0; i < 3; i++) {
+        const uint64_t dense = i ? hk : hq;
+        stride[i] = strides[i] ? (uint64_t)strides[i] : dense;
+        if (strides[i] < 0 || stride[i] < dense || stride[i] % 4) return fail(QL_E_INVALID, "row strides must be 0 or at least a row's values, a multiple of 4");
+    }
+    if ((rc = check_devices(ctx, weights, act, cache))) return rc;
+    const uint64_t rows = (uint64_t)M - 1, offs[3] = {q_off, k_off, v_off};
+    for (int i = 0; i < 3; i++) {
+        Span& r = reads[i ? 3 + i : 0];
+        r = {act, offs[i], (rows * stride[i] + (i ? hk : hq)) * 4};
+        if (!in_range(r.off, r.bytes, act->size)) return fail(QL_E_RANGE, "q, k or v rows outside the activation arena");
+        if (r.off % 16) return fail(QL_E_ALIGN, "q, k and v offsets must be 16-byte aligned");
+    }
+    reads[6] = {weights, d->table_off, (uint64_t)d->max_pos * d->rot_dim * 4};
+    reads[7] = {weights, d->q_norm_off, d->q_norm_off == QL_NONE ? 0 : D * 4};
+    reads[8] = {weights, d->k_norm_off, d->k_norm_off == QL_NONE ? 0 : D * 4};
+    for (int i = 6; i < 9; i++) {
+        if (reads[i].bytes == 0) continue;
+        if (!in_range(reads[i].off, reads[i].bytes, weights->size)) return fail(QL_E_RANGE, "table or norm weight outside the weight arena");
+        if (reads[i].off % 16) return fail(QL_E_ALIGN, "table and norm weight offsets must be 16-byte aligned");
+    }
+    const Span writes[5] = {{act, q_out_off, (uint64_t)M * hq * qb}, pages[0], pages[1], pages[2], pages[3]};
+    if (!in_range(q_out_off, writes[0].bytes, act->size)) return fail(QL_E_RANGE, "q_out [M, n_head, D] outside the activation arena");
+    if (q_out_off % 16) return fail(QL_E_ALIGN, "the q_out offset must be 16-byte aligned");
+    const bool in_place = q_out_off == q_off && stride[0] == hq && qb == 4;
+    if (any_meet(writes, 5, reads + 1, 8) || any_meet(writes + (in_place ? 1 : 0), in_place ? 4 : 5, reads, 1))
+        return fail(QL_E_INVALID, "q_out or the cache overlap an input, each other or themselves");
+    if ((rc = set_device(ctx))) return rc;
+    a.r.q = reinterpret_cast<const float*>(act->base + q_off);
+    a.r.k = reinterpret_cast<const float*>(act->base + k_off);
+    a.r.v = reinterpret_cast<const float*>(act->base + v_off);
+    a.r.q_norm = reads[7].bytes ? reinterpret_cast<const float*>(weights->base + d->q_norm_off) : nullptr;
+    a.r.k_norm = reads[8].bytes ? reinterpret_cast<const float*>(weights->base + d->k_norm_off) : nullptr;
+    a.r.table = reinterpret_cast<const float*>(weights->base + d->table_off);
+    a.r.pos = nullptr;
+    a.r.q_out = nullptr;
+    a.r.k_cache = cache->base + paged->k_off;
+    a.r.v_cache = cache->base + paged->v_off;
+    a.r.q_stride = stride[0];
+    a.r.k_stride = stride[1];
+    a.r.v_stride = stride[2];
+    a.r.M = M;
+    a.r.H = d->n_head;
+    a.r.KV = d->n_kv_head;
+    a.r.D = d->D;
+    a.r.rot = d->rot_dim;
+    a.r.interleaved = d->interleaved;
+    a.r.max_pos = d->max_pos;
+    a.r.half = cb == 2;
+    a.r.slot0 = 0;
+    a.r.eps = d->norm_eps;
+    a.q_out = act->base + q_out_off;
+    a.q_half = qb == 2;
+    a.k_scale = cb == 1 ? reinterpret_cast<float*>(cache->base + paged->k_scale_off) : nullptr;
+    a.v_scale = cb == 1 ? reinterpret_cast<float*>(cache->base + paged->v_scale_off) : nullptr;
+    QL_HIP(ql::launch_paged_append(a, ctx->stream));
+    return QL_OK;
+}
+
+int ql_paged_attention(ql_ctx* ctx, ql_arena* act, uint64_t q_off, int32_t q_dtype, const ql_arena* cache, const ql_paged_desc* paged,
+                       const ql_batch_desc* batch, int32_t M, int32_t n_head, uint64_t out_off)
+{
+    if (!ctx || !act || !cache || !paged || !batch) return fail(QL_E_INVALID, "null context, descriptor or arena");
+    ql::PagedAttnArgs a;
+    Span reads[8];
+    uint64_t cb, qb;
+    int rc = paged_regions(paged, cache, &cb, reads);
+    if (rc || (rc = batch_tables(batch, paged, act, M, &a.b, reads + 4))) return rc;
+    if (n_head < 1 || n_head > 4096 || n_head % paged->n_kv_head) return fail(QL_E_INVALID, "n_head (%d) must be 1..4096, a multiple of n_kv_head (%d)", n_head, paged->n_kv_head);
+    if (!dtype_bytes(q_dtype, &qb)) return fail(QL_E_INVALID, "bad q_dtype %d", q_dtype);
+    if ((rc = check_devices(ctx, act, cache, nullptr))) return rc;
+    const uint64_t qo = (uint64_t)M * n_head * paged->D * qb;
+    reads[7] = {act, q_off, qo};
+    const Span out = {act, out_off, qo};
+    if (!in_range(q_off, qo, act->size)) return fail(QL_E_RANGE, "q [M, n_head, D] outside the activation arena");
+    if (!in_range(out_off, qo, act->size)) return fail(QL_E_RANGE, "out [M, n_head, D] outside the activation arena");
+    if (q_off % 16 || out_off % 16) return fail(QL_E_ALIGN, "offsets must be 16-byte aligned");
+    if (any_meet(&out, 1, reads, 8)) return fail(QL_E_INVALID, "out overlaps an input");
+    if ((rc = set_device(ctx))) return rc;
+    a.q = act->base + q_off;
+    a.out = act->base + out_off;
+    a.k = cache->base + paged->k_off;
+    a.v = cache->base + paged->v_off;
+    a.k_scale = cb == 1 ? reinterpret_cast<const float*>(cache->base + paged->k_scale_off) : nullptr;
+    a.v_scale = cb == 1 ? reinterpret_cast<const float*>(cache->base + paged->v_scale_off) : nullptr;
+    a.H = n_head;
+    a.KV = paged->n_kv_head;
+    a.G = n_head / paged->n_kv_head;
+    a.D = paged->D;
+    a.half = qb == 2;
+    a.scale = (float)(1.4426950408889634 / std::sqrt((double)paged->D));
+    const uint64_t bytes = ql::plan_paged_attention(&a, ql::kAttnTileWsBytes);
+    std::lock_guard<std::mutex> guard(ctx->ws_lock);
+    void* ws;
+    QL_HIP(workspace(ctx, ctx->tile_ws, bytes, &ws));
+    a.ws = static_cast<float*>(ws);
+    QL_HIP(ql::launch_paged_attention(a, ctx->stream));
+    return QL_OK;
+}
+
+int ql_lora_add(ql_ctx* ctx, int32_t count, const ql_lora_desc* descs, const ql_arena* weights, ql_arena* act, uint64_t ids_off,
+                const uint64_t* x_offs, int32_t x_dtype, int32_t M, const uint64_t* base_offs, const uint64_t* y_offs)
+{
+    if (!ctx || !descs || !weights || !act || !x_offs || !base_offs || !y_offs) return fail(QL_E_INVALID, "null context, descriptors, arena or offsets");
+    if (count < 1 || count > ql::kMaxBatch) return fail(QL_E_INVALID, "count must be 1..%d (got %d)", ql::kMaxBatch, count);
+    if (M < 1 || M > 65535) return fail(QL_E_INVALID, "M must be 1..65535 (got %d)", M);
+    uint64_t xb;
+    if (!dtype_bytes(x_dtype, &xb)) return fail(QL_E_INVALID, "bad x_dtype %d", x_dtype);
+    int rc = check_devices(ctx, weights, act, nullptr);
+    if (rc) return rc;
+    Span reads[1 + 5 * ql::kMaxBatch], writes[ql::kMaxBatch];
+    reads[0] = {act, ids_off, (uint64_t)M * 4};
+    if (!in_range(ids_off, reads[0].bytes, act->size)) return fail(QL_E_RANGE, "ids [M] outside the activation arena");
+    if (ids_off % 4) return fail(QL_E_ALIGN, "ids must be 4-byte aligned");
+    ql::LoraArgs a;
+    for (int i = 0; i < count; i++) {
+        const ql_lora_desc& d = descs[i];
+        if (d.K < 8 || d.K % 8 || d.N < 4 || d.N % 4 || d.K > (1 << 24) || d.N > (1 << 24)) return fail(QL_E_DIMS, "K must be a positive multiple of 8, N of 4, at most 2^24 (got %d, %d)", d.K, d.N);
+        if (d.rank < 8 || d.rank > ql::kLoraMaxRank || d.rank % 8) return fail(QL_E_INVALID, "rank must be 8..%d, a multiple of 8 (got %d)", ql::kLoraMaxRank, d.rank);
+        if (d.n_adapter < 1 || d.n_adapter > 65536) return fail(QL_E_INVALID, "n_adapter must be 1..65536 (got %d)", d.n_adapter);
+        const uint64_t n = d.n_adapter, mn = (uint64_t)M * d.N * 4;
+        Span* r = reads + 1 + 5 * i;
+        r[0] = {act, x_offs[i], (uint64_t)M * d.K * xb};
+        r[1] = {weights, d.a_off, n * d.rank * d.K * 2};
+        r[2] = {weights, d.b_off, n * d.rank * d.N * 2};
+        r[3] = {weights, d.scale_off, d.scale_off == QL_NONE ? 0 : n * 4};
+        r[4] = {act, base_offs[i], mn};
+        writes[i] = {act, y_offs[i], mn};
+        if (!in_range(r[0].off, r[0].bytes, act->size) || !in_range(r[4].off, mn, act->size) || !in_range(y_offs[i], mn, act->size))
+            return fail(QL_E_RANGE, "x [M, K], base or y [M, N] of projection %d outside the activation arena", i);
+        for (int k = 1; k < 4; k++)
+            if (r[k].bytes && !in_range(r[k].off, r[k].bytes, weights->size)) return fail(QL_E_RANGE, "adapters of projection %d outside the weight arena", i);
+        if (r[0].off % 16 || r[1].off % 16 || r[2].off % 16 || r[4].off % 16 || y_offs[i] % 16 || (r[3].bytes && r[3].off % 4))
+            return fail(QL_E_ALIGN, "offsets must be 16-byte aligned (scales 4-byte)");
+        a.p[i] = {reinterpret_cast<const uint16_t*>(weights->base + d.a_off), reinterpret_cast<const uint16_t*>(weights->base + d.b_off),
+                  r[3].bytes ? reinterpret_cast<const float*>(weights->base + d.scale_off) : nullptr, act->base + x_offs[i],
+                  reinterpret_cast<const float*>(act->base + base_offs[i]), reinterpret_cast<float*>(act->base + y_offs[i]), d.K, d.N, d.rank, d.n_adapter};
+    }
+    for (int i = 0; i < count; i++) {
+        for (int k = 0; k < 1 + 5 * count; k++)
+            if (meet(writes[i], reads[k]) && !(k == 5 + 5 * i && writes[i].off == reads[k].off))
+                return fail(QL_E_INVALID, "y of projection %d overlaps an input", i);
+        for (int k = 0; k < i; k++)
+            if (meet(writes[i], writes[k])) return fail(QL_E_INVALID, "y of projection %d overlaps that of projection %d", i, k);
+    }
+    if ((rc = set_device(ctx))) return rc;
+    a.ids = reinterpret_cast<const int32_t*>(act->base + ids_off);
+    a.count = count;
+    a.M = M;
+    a.half = xb == 2;
+    const uint64_t bytes = ql::plan_lora(&a, ql::kAttnTileWsBytes);
+    std::lock_guard<std::mutex> guard(ctx->ws_lock);
+    void* ws;
+    QL_HIP(workspace(ctx, ctx->tile_ws, bytes, &ws));
+    a.ws = static_cast<float*>(ws);
+    QL_HIP(ql::launch_lora(a, ctx->stream));
+    return QL_OK;
+}
+
 int ql_plan_batch(int32_t count, const ql_gptq_desc* descs, int32_t M, uint64_t* scratch_bytes)
 {
     if (!descs || !scratch_bytes || count <= 0 || count > ql::kMaxBatch)

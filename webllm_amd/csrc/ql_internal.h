@@ -366,6 +366,56 @@ struct MoveArgs {
 hipError_t launch_kv_move(MoveArgs& a, hipStream_t stream);
 
 // ----------------------------------------------------------------------------------------------
+// A pass over many requests: append to a paged cache, attention over it, low-rank adapters.
+
+constexpr int kPagedMaxSeqs = 4096;
+constexpr int kPagedMaxLen = 1 << 30;
+// a batch's tables on the device and their bounds
+struct PagedBatch {
+    const int32_t *row_start, *kv_len, *pages;   // [S + 1], [S], [S, max_pages]
+    int S, M, max_pages, max_rows, max_len;
+    int n_page, log_page;
+};
+struct PagedAppendArgs {
+    RopeArgs r;                // pos, q_out, slot0, half unused
+    PagedBatch b;
+    void* q_out;               // [M, H, D], fp32 or fp16 (q_half)
+    float *k_scale, *v_scale;  // e4m3 caches, otherwise nullptr
+    int q_half, jobs;          // jobs: most groups of 16 tokens that a pass of M rows brings tokens to
+};
+hipError_t launch_paged_append(PagedAppendArgs a, hipStream_t stream);
+
+struct PagedAttnArgs {
+    const void* q;             // [M, H, D], fp32 or fp16 (half)
+    void* out;
+    const void *k, *v;
+    const float *k_scale, *v_scale;   // e4m3 caches, otherwise nullptr
+    float* ws;
+    PagedBatch b;
+    int H, KV, G, D, half;
+    float scale;               // fp32(log2(e) / sqrt(D))
+};
+uint64_t plan_paged_attention(PagedAttnArgs* a, size_t ws_bytes);   // the workspace it needs
+hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
+
+constexpr int kLoraMaxRank = 128;
+struct LoraArgs {
+    struct One {
+        const uint16_t *a, *b; // fp16 [n, rank, K], [n, N, rank]
+        const float* scale;    // [n] or nullptr
+        const void* x;         // [M, K]
+        const float* base;     // [M, N]
+        float* y;
+        int K, N, rank, n;
+    } p[kMaxBatch];
+    const int32_t* ids;        // [M]
+    float* ws;
+    int count, M, half;        // half: x is fp16
+};
+uint64_t plan_lora(LoraArgs* a, size_t ws_bytes);
+hipError_t launch_lora(const LoraArgs& a, hipStream_t stream);
+
+// ----------------------------------------------------------------------------------------------
 // Linear sequences: many decode linears (M <= 16) in one persistent launch. Linear i may read the
 // output of an earlier linear; the kernel orders them on the device.
 

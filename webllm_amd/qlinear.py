@@ -24,6 +24,7 @@ QL_NONE = (1 << 64) - 1
 NOALLOC_SCRATCH_BYTES = 8 << 20   # QL_NOALLOC_SCRATCH_BYTES
 DTYPE_F32 = 0
 DTYPE_F16 = 1
+DTYPE_F8 = 2                      # e4m3 under powers of two: paged caches
 KIND_NAMES = {1: "gemv_mfma", 2: "gemv_simple", 3: "gemm_mfma", 4: "gemm_simple"}
 
 ERROR_NAMES = {
@@ -119,6 +120,39 @@ def make_rope(table_off: int, max_pos: int, n_head: int, n_kv_head: int, D: int,
                     norm_eps, 0)
 
 
+class BatchDesc(ctypes.Structure):
+    """A batch's rows of several sequences: where its tables lie, and their bounds (ql_batch_desc)."""
+    _fields_ = [("row_start_off", ctypes.c_uint64), ("kv_len_off", ctypes.c_uint64), ("pages_off", ctypes.c_uint64),
+                ("n_seq", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("max_rows", ctypes.c_int32), ("max_len", ctypes.c_int32)]
+
+
+class PagedDesc(ctypes.Structure):
+    """A layer's paged cache (ql_paged_desc)."""
+    _fields_ = [("k_off", ctypes.c_uint64), ("v_off", ctypes.c_uint64), ("k_scale_off", ctypes.c_uint64), ("v_scale_off", ctypes.c_uint64),
+                ("n_page", ctypes.c_int32), ("page_size", ctypes.c_int32), ("n_kv_head", ctypes.c_int32), ("D", ctypes.c_int32),
+                ("cache_dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class LoraDesc(ctypes.Structure):
+    """The low-rank adapters of one projection (ql_lora_desc)."""
+    _fields_ = [("a_off", ctypes.c_uint64), ("b_off", ctypes.c_uint64), ("scale_off", ctypes.c_uint64), ("K", ctypes.c_int32),
+                ("N", ctypes.c_int32), ("rank", ctypes.c_int32), ("n_adapter", ctypes.c_int32)]
+
+
+def make_batch(row_start_off: int, kv_len_off: int, pages_off: int, n_seq: int, max_pages: int, max_rows: int, max_len: int) -> BatchDesc:
+    return BatchDesc(row_start_off, kv_len_off, pages_off, n_seq, max_pages, max_rows, max_len)
+
+
+def make_paged(k_off: int, v_off: int, n_page: int, page_size: int, n_kv_head: int, D: int, cache_dtype: int = DTYPE_F16,
+               k_scale_off: int | None = None, v_scale_off: int | None = None) -> PagedDesc:
+    return PagedDesc(k_off, v_off, QL_NONE if k_scale_off is None else k_scale_off, QL_NONE if v_scale_off is None else v_scale_off,
+                     n_page, page_size, n_kv_head, D, cache_dtype, 0)
+
+
+def make_lora(a_off: int, b_off: int, K: int, N: int, rank: int, n_adapter: int, scale_off: int | None = None) -> LoraDesc:
+    return LoraDesc(a_off, b_off, QL_NONE if scale_off is None else scale_off, K, N, rank, n_adapter)
+
+
 _lib = None
 
 
@@ -174,6 +208,10 @@ def lib():
         "ql_attention_tree": (I, [P, P, U64, P, U64, U64, I, I, I, I, I, I, I, U64, U64]),
         "ql_token_logprobs": (I, [P, P, U64, I, I, I, U64, I, I, U64, U64, U64, U64]),
         "ql_kv_move": (I, [P, P, ctypes.POINTER(U64), I, P, ctypes.POINTER(U64), I, I, I, I, I, I, P, U64]),
+        "ql_paged_append": (I, [P, ctypes.POINTER(RopeDesc), P, P, U64, U64, U64, ctypes.POINTER(BatchDesc), I, U64, I, P,
+                                ctypes.POINTER(PagedDesc)]),
+        "ql_paged_attention": (I, [P, P, U64, I, P, ctypes.POINTER(PagedDesc), ctypes.POINTER(BatchDesc), I, I, U64]),
+        "ql_lora_add": (I, [P, I, ctypes.POINTER(LoraDesc), P, P, U64, ctypes.POINTER(U64), I, I, ctypes.POINTER(U64), ctypes.POINTER(U64)]),
         "ql_linear": (I, [P, ctypes.POINTER(GptqDesc), P, P, U64, I, I, U64, U64]),
         "ql_linear_noalloc": (I, [P, ctypes.POINTER(GptqDesc), P, P, U64, I, I, U64]),
         "ql_plan_batch": (I, [I, ctypes.POINTER(GptqDesc), I, ctypes.POINTER(U64)]),
@@ -255,8 +293,13 @@ def tree_masks(parents) -> tuple[np.ndarray, np.ndarray]:
 
 
 def offsets(offs):
-    """Offsets as the array that ql_kv_move takes; a program that moves often keeps it."""
+    """Offsets as the array that ql_kv_move and ql_lora_add take; a program that calls often keeps it."""
     return offs if isinstance(offs, ctypes.Array) else (ctypes.c_uint64 * len(offs))(*offs)
+
+
+def lora_descs(descs):
+    """Adapters of several projections as the array that ql_lora_add takes; a program keeps it."""
+    return descs if isinstance(descs, ctypes.Array) else (LoraDesc * len(descs))(*descs)
 
 
 def plan_batch(descs: list[GptqDesc], M: int) -> int:
@@ -494,6 +537,25 @@ class Context:
             raise ValueError(f"{len(d)} destination regions for {len(s)} source regions")
         _check(lib().ql_kv_move(self.handle, dst.handle, d, dst_max_t, src.handle, s, src_max_t, len(d), row_bytes, dst_row, src_row, n,
                                 None if act is None else act.handle, QL_NONE if rows_off is None else rows_off))
+
+    def paged_append(self, rope: RopeDesc, weights: Arena, act: Arena, q_off: int, k_off: int, v_off: int, batch: BatchDesc, M: int,
+                     q_out_off: int, q_dtype: int, cache: Arena, paged: PagedDesc):
+        """A batch's q and k normed per head and turned by their rows' positions; q to q_out, k and v to their tokens' places in the pages."""
+        _check(lib().ql_paged_append(self.handle, ctypes.byref(rope), weights.handle, act.handle, q_off, k_off, v_off,
+                                     ctypes.byref(batch), M, q_out_off, q_dtype, cache.handle, ctypes.byref(paged)))
+
+    def paged_attention(self, act: Arena, q_off: int, q_dtype: int, cache: Arena, paged: PagedDesc, batch: BatchDesc, M: int, n_head: int,
+                        out_off: int):
+        """Causal GQA attention of a batch's rows over their sequences' pages; q and out in q_dtype."""
+        _check(lib().ql_paged_attention(self.handle, act.handle, q_off, q_dtype, cache.handle, ctypes.byref(paged), ctypes.byref(batch),
+                                        M, n_head, out_off))
+
+    def lora_add(self, descs, weights: Arena, act: Arena, ids_off: int, x_offs, x_dtype: int, M: int, base_offs, y_offs):
+        """y = base + scale * (x . A^T) . B^T by each row's adapter (ids; -1: none), for up to 8 projections."""
+        d, x, b, y = lora_descs(descs), offsets(x_offs), offsets(base_offs), offsets(y_offs)
+        if not len(d) == len(x) == len(b) == len(y):
+            raise ValueError(f"lora_add: {len(d)} projections, {len(x)} inputs, {len(b)} bases, {len(y)} outputs")
+        _check(lib().ql_lora_add(self.handle, len(d), d, weights.handle, act.handle, ids_off, x, x_dtype, M, b, y))
 
     def unpack_f32(self, desc: GptqDesc, weights: Arena, out: Arena, out_off: int,
                    scales_dtype: int = DTYPE_F16):
