@@ -365,7 +365,7 @@ typedef struct ql_batch_desc {
     int32_t n_seq;          /* 1..4096 */
     int32_t max_pages;      /* pages of a sequence's list */
     int32_t max_rows;       /* most rows that a sequence has in this pass, and the most tokens that one has: at most max_pages * page_size. */
-    int32_t max_len;        /* They choose the launches; bounds near what the tables hold serve best */
+    int32_t max_len;        /* and 2^26. They choose the launches; bounds near what the tables hold serve best */
 } ql_batch_desc;
 /* A layer's paged cache, regions of n_page pages in a cache arena, offsets 16-byte aligned. A page holds page_size tokens of all kv heads, each
  * head's behind the other. D is a multiple of 16, u = 16 bytes of values: 8 (fp16) or 16 (e4m3).
@@ -400,7 +400,7 @@ int ql_paged_append(ql_ctx* ctx, const ql_rope_desc* rope, const ql_arena* weigh
  * sequence, which the cache holds (ql_paged_append has run). q and out are [M, n_head, D] in `act`, both of q_dtype: fp32 (q as two fp16
  * parts of about 22 bits under its row's exponent, probabilities likewise), or fp16 (probabilities rounded once to fp16, as the result is). Sums and softmax in
  * fp32. A row that sees nothing, or no score above -inf, is zero. What a row does not see adds nothing to it, infinities and NaN included;
- * a value of q that is not finite makes its head's row NaN. max_len <= 2^30. Offsets 16-byte aligned. Uses the context's 64 MiB workspace. */
+ * a value of q that is not finite makes its head's row NaN. Offsets 16-byte aligned. Uses the context's 64 MiB workspace. */
 int ql_paged_attention(ql_ctx* ctx, ql_arena* act, uint64_t q_off, int32_t q_dtype, const ql_arena* cache, const ql_paged_desc* paged,
                        const ql_batch_desc* batch, int32_t M, int32_t n_head, uint64_t out_off);
 /* Low-rank adapters of one projection, all n_adapter of them, in `weights`. */

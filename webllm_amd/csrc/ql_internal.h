@@ -369,7 +369,7 @@ hipError_t launch_kv_move(MoveArgs& a, hipStream_t stream);
 // A pass over many requests: append to a paged cache, attention over it, low-rank adapters.
 
 constexpr int kPagedMaxSeqs = 4096;
-constexpr int kPagedMaxLen = 1 << 30;
+constexpr int kPagedMaxLen = 1 << 26;            // blocks of 64 sequences at a time are counted in 32 bits
 // a batch's tables on the device and their bounds
 struct PagedBatch {
     const int32_t *row_start, *kv_len, *pages;   // [S + 1], [S], [S, max_pages]
@@ -394,6 +394,9 @@ struct PagedAttnArgs {
     PagedBatch b;
     int H, KV, G, D, half;
     float scale;               // fp32(log2(e) / sqrt(D))
+    // plan_paged_attention fills these: most (row, head) pairs of a sequence of few rows, most tiles of 16 of them that such sequences have,
+    // whether each tile is one workgroup's, or all their blocks are dealt to `ranges` workgroups a kv head
+    int few, units, whole, ranges;
 };
 uint64_t plan_paged_attention(PagedAttnArgs* a, size_t ws_bytes);   // the workspace it needs
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);

@@ -21,7 +21,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int s)
 // Unit number j of the units that the sequences have, count(sequence) of each, in order: its sequence s and its number in it. Every
 // lane of a wave takes part and gets the same; false beyond the last one.
 template <typename F>
-__device__ __forceinline__ bool paged_unit(const PagedBatch& b, int j, F count, int& s, int& local, PagedSeq& q)
+__device__ __forceinline__ bool paged_unit(const PagedBatch& b, long long j, F count, int& s, int& local, PagedSeq& q)
 {
     const int lane = threadIdx.x & 63;
     long long before = 0;
@@ -48,6 +48,23 @@ __device__ __forceinline__ bool paged_unit(const PagedBatch& b, int j, F count, 
     return false;
 }
 
+// The units of all sequences, or of those before the first `upto`
+template <typename F>
+__device__ __forceinline__ long long paged_total(const PagedBatch& b, F count, int upto = kPagedMaxSeqs)
+{
+    const int lane = threadIdx.x & 63, S = min(b.S, upto);
+    long long total = 0;
+    for (int s0 = 0; s0 < S; s0 += 64) {
+        PagedSeq me = {0, 0, 0};
+        if (s0 + lane < S) me = paged_seq(b, s0 + lane);
+        int c = me.n ? count(me) : 0;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o);
+        total += c;
+    }
+    return total;
+}
+
 // The sequence of a row, for a whole wave; false: padding.
 __device__ __forceinline__ bool paged_row(const PagedBatch& b, int row, int& s, PagedSeq& q)
 {
@@ -64,6 +81,13 @@ __device__ __forceinline__ int paged_page(const PagedBatch& b, int s, int t)
 {
     const int p = ld_global(b.pages + (size_t)s * b.max_pages + (t >> b.log_page));
     return (uint32_t)p < (uint32_t)b.n_page ? p : -1;
+}
+
+__device__ __forceinline__ void paged_out(float* to, f32x4 x) { st_global(reinterpret_cast<f32x4*>(to), x); }
+__device__ __forceinline__ void paged_out(_Float16* to, f32x4 x)
+{
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    st_global(reinterpret_cast<f16x4*>(to), __builtin_convertvector(x, f16x4));
 }
 
 // Layout (of one kv head's part of a page, in values of SIZE bytes)

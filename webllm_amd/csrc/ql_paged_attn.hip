@@ -1,23 +1,476 @@
 // Attention of a batch's rows over their sequences' pages (ql_paged_attention):
 //   out[m, h] = sum_t p_t V[t] / sum_t p_t,  p_t = exp(q[m, h] . K[t] / sqrt(D) - max)   over the tokens t up to the row's own.
 //
-// A workgroup a (row, head); its four waves take blocks of 64 tokens in turn, a lane a token's score, then a lane its columns; running
-// maximum and sum; the waves' states are merged through LDS.
+// paged_decode_kernel: sequences of few rows. A workgroup has 16 (row, head) pairs of one kv head and a range of blocks of 64 tokens; its
+// four waves take the blocks in turn, K and V from memory to the registers of one wave. The cache lies as the matrix instructions take it: a load
+// is 16 bytes a lane and 1 KB in a row. Scores are computed transposed, S^T = K Q^T (lane = pair, registers = tokens), and what a lane then has of P is the
+// B fragment of O^T = V^T P^T, with nothing crossing lanes: tile kt of S is the block's tokens 16 kt + 4 g + r (g: lane / 16, r: register), and the
+// tokens of V that a lane reads together are 16 b + 4 g + r. Softmax in fp32 with a running reference, raised by leaps only; the waves' states are
+// merged through LDS.
+// Sequences differ in length, so the blocks of all of them, one behind the other, are dealt to the workgroups in equal ranges; a workgroup goes through
+// the sequences that its range meets. Where a sequence's range is cut, paged_merge_kernel joins the parts. Every workgroup finds its range from
+// the tables by itself: lengths stay on the device.
+//
+// Numbers: K and V enter as they are (e4m3 is exact in fp16), K's scales multiply scores, V's the probabilities, relative to the block's largest, which multiplies
+// the block's sum. fp32 rows: q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P: about 22 bits. fp16 rows: q as it
+// is, 2^8 P rounded once. A product of an infinity's parts is a NaN, and 0 * V is one where V is not finite: a wave whose sums end that way does its blocks
+// again on the VALU from q, K and V themselves, skipping what a pair does not see (paged_again).
+#include <algorithm>
 #include <type_traits>
 
+#include "ql_lanes.h"
 #include "ql_paged.h"
 
 namespace ql {
 
 namespace {
 
+constexpr int kBlock = 64;               // tokens of a block; pages are whole blocks
+constexpr int kPairs = 16;
+constexpr float kRaise = 7.f;            // log2 that scores may rise above the running reference before it is raised
+constexpr float kPScale = 256.f;         // parts of P: 2^8 P, at most 2^15
+constexpr float kMaxFinite = 3.4028235e38f;
+
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 template <bool F8>
 __device__ __forceinline__ float value_at(const void* p, size_t i)
 {
-    if (F8) return __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(p)[i], 0);
-    return (float)static_cast<const _Float16*>(p)[i];
+    if (F8) return __builtin_amdgcn_cvt_f32_fp8(ld_global(static_cast<const uint8_t*>(p) + i), 0);
+    return (float)ld_global(static_cast<const _Float16*>(p) + i);
+}
+
+// eight e4m3 values, exactly
+__device__ __forceinline__ f16x8 f8_to_f16(uint32_t lo, uint32_t hi)
+{
+    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.f, true);
+    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.f, true);
+    return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// What a workgroup goes through: pairs r0 .. r0 + 15 of sequence s, blocks b0 .. b1 - 1 of nb
+struct Piece {
+    int s, r0, b0, b1, nb;
+    PagedSeq q;
+};
+
+__device__ __forceinline__ bool few(const PagedAttnArgs& a, const PagedSeq& q) { return q.n * a.G <= a.few; }
+__device__ __forceinline__ int tiles_of(const PagedAttnArgs& a, const PagedSeq& q) { return (q.n * a.G + kPairs - 1) / kPairs; }
+__device__ __forceinline__ int blocks_of(const PagedSeq& q) { return (q.len + kBlock - 1) / kBlock; }
+
+// A wave's blocks on the VALU, into the sums' own layout: lane (i, g) has pair i, columns 16 ct + 4 g + r. The four lanes of a pair share a dot product.
+template <bool F8, typename Q, int CT>
+__device__ __forceinline__ void paged_again(const PagedAttnArgs& a, const Piece& p, int kvh, size_t q_row, int last, int first, int step, float& mr, float& l, f32x4 (&acc)[CT])
+{
+    typedef PagedLayout<F8 ? 1 : 2> Lay;
+    const int g = threadIdx.x >> 4 & 3, D = a.D;
+    const Q* q = static_cast<const Q*>(a.q) + q_row;
+    mr = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int c = 0; c < CT; c++) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int b = first; b < p.b1; b += step) {
+        const int t0 = b * kBlock, page = paged_page(a.b, p.s, t0), in_page = t0 & ((1 << a.b.log_page) - 1);
+        if (page < 0) continue;
+        const size_t head = (size_t)page * a.KV + kvh, base = (head << a.b.log_page) * D, sc0 = (head << (a.b.log_page - 4)) + (in_page >> 4);
+#pragma unroll 1
+        for (int i = 0; i < kBlock && t0 + i < p.q.len; i++) {
+            const bool seen = t0 + i <= last;
+            float sc = 0.f;
+#pragma unroll 1
+            for (int d = g * (D / 4); d < (g + 1) * (D / 4); d++) sc = fmaf((float)q[d], value_at<F8>(a.k, base + Lay::k_at(D, in_page + i, d / Lay::kUnit) + d % Lay::kUnit), sc);
+            sc = pair_sum<32>(pair_sum<16>(sc)) * (a.scale * (F8 ? ld_global(a.k_scale + sc0 + i / 16) : 1.f));
+            if (!seen) sc = -INFINITY;
+            const float mn = fmaxf(mr, sc), ref = mn == -INFINITY ? 0.f : mn, al = ex2(mr - ref), e = seen ? ex2(sc - ref) : 0.f;
+            mr = mn;
+            l = l * al + (g == 0 ? e : 0.f);
+            const float ev = e * (F8 ? ld_global(a.v_scale + sc0 + i / 16) : 1.f);
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    acc[c][r] *= al;
+                    if (seen && 16 * c < D) acc[c][r] = fmaf(ev, value_at<F8>(a.v, base + Lay::v_at(D, in_page + i / 4 * 4, 16 * c + 4 * g + r) + i % 4), acc[c][r]);
+                }
+            }
+        }
+    }
+}
+
+template <bool F8, typename Q, int DP>
+struct DecodeTile {
+    static constexpr bool kHalf = std::is_same<Q, _Float16>::value;
+    static constexpr int kParts = kHalf ? 1 : 2;                 // of q and of P
+    static constexpr int kUnits = DP / (F8 ? 64 : 32);           // 16-byte loads of a token's K, of 16 tokens
+    static constexpr int kSteps = DP / 32;                       // matrix instructions along D
+    static constexpr int kCT = DP / 16;                          // tiles of 16 columns
+    static constexpr int kVB = F8 ? 1 : 2;                       // parts of a block whose tokens of V lie together
+    static constexpr int kMerge = DP + 4;                        // floats of a row of the merge buffer
+    // the column of element e of step t of a K or Q fragment, lane group g
+    static __device__ __forceinline__ int col(int t, int g) { return F8 ? 64 * (t >> 1) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g; }
+};
+
+template <bool F8, typename Q, int DP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_kernel(const PagedAttnArgs a)
+{
+    using C = DecodeTile<F8, Q, DP>;
+    typedef PagedLayout<F8 ? 1 : 2> Lay;
+    __shared__ __attribute__((aligned(16))) float merge[WAVES * kPairs * C::kMerge];
+    __shared__ float stat[2][WAVES][kPairs], row_inv[kPairs];
+    __shared__ int row_at[kPairs];
+    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4, D = a.D;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const PagedBatch& b = a.b;
+    const int kvh = blockIdx.x % a.KV, w = blockIdx.x / a.KV;
+
+    // this workgroup's range [at, end) of all sequences' blocks, or of their tiles where each is done whole (a.whole)
+    auto count = [&](const PagedSeq& q) { return few(a, q) ? tiles_of(a, q) * (a.whole ? 1 : blocks_of(q)) : 0; };
+    long long at, end;
+    if (a.whole) {
+        at = w;
+        end = w + 1;
+    } else {
+        const long long total = paged_total(b, count);
+        const long long per = (max((total + a.ranges - 1) / a.ranges, 1ll) + WAVES - 1) / WAVES * WAVES;
+        at = w * per;
+        end = min(at + per, total);
+    }
+    while (at < end) {
+        Piece p;
+        int local;
+        if (!paged_unit(b, at, count, p.s, local, p.q)) return;
+        p.nb = blocks_of(p.q);
+        if (a.whole) {
+            p.r0 = kPairs * local;
+            p.b0 = 0;
+            p.b1 = p.nb;
+            at++;
+        } else {
+            const int tile = local / p.nb;
+            p.r0 = kPairs * tile;
+            p.b0 = local - tile * p.nb;
+            p.b1 = (int)min((long long)p.nb, p.b0 + (end - at));
+            at += p.b1 - p.b0;
+        }
+        const int R = p.q.n * a.G, r = min(p.r0 + i16, R - 1), row = r / a.G;
+        const size_t q_row = ((size_t)(p.q.row0 + row) * a.H + kvh * a.G + (r - row * a.G)) * D;
+        const int last = p.q.len - p.q.n + row;             // the lane's pair sees the tokens up to it
+        const int all = p.q.len - p.q.n;                    // every row of the sequence sees the tokens up to it
+
+        f16x8 qf[C::kSteps][C::kParts];
+        float f = a.scale;
+        {
+            const Q* q = static_cast<const Q*>(a.q) + q_row;
+            if constexpr (C::kHalf) {
+#pragma unroll
+                for (int t = 0; t < C::kSteps; t++) {
+                    const int d = C::col(t, g);
+                    qf[t][0] = d < D ? __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(q + d))) : f16x8{};
+                }
+            } else {
+                f32x4 x[C::kSteps][2];
+                float mx = 0.f;
+#pragma unroll
+                for (int t = 0; t < C::kSteps; t++)
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int d = C::col(t, g) + 4 * k;
+                        x[t][k] = d < D ? ld_global(reinterpret_cast<const f32x4*>(q + d)) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[t][k][e]));
+                    }
+                mx = pair_max<32>(pair_max<16>(mx));
+                // the row's power of two: its largest value to [2^14, 2^15)
+                const float s = mx > 0.f && mx <= kMaxFinite ? ldexpf(1.f, min(100, 14 - ilogbf(mx))) : 1.f;
+                f = fmaxf(a.scale / s, 1.17549435e-38f);
+#pragma unroll
+                for (int t = 0; t < C::kSteps; t++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float y = x[t][e >> 2][e & 3] * s;
+                        const _Float16 hi = (_Float16)y;
+                        qf[t][0][e] = hi;
+                        qf[t][C::kParts - 1][e] = (_Float16)((y - (float)hi) * 2048.f);
+                    }
+            }
+        }
+        f32x4 acc[C::kCT];
+        float mr = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int c = 0; c < C::kCT; c++) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+        // The wave's blocks first, first + WAVES, ...; lane j knows the page of number (base + j) of them
+        const int first = p.b0 + wave, mine = first < p.b1 ? (p.b1 - first + WAVES - 1) / WAVES : 0;
+        int pages = 0;
+        u32x4 kraw[4][C::kUnits], vraw[C::kVB][C::kCT];
+        float ks[4], vs[4];
+        struct At {
+            size_t head;
+            int in_page, t0, lim;                           // lim: tokens of the block that a row may see
+        };
+        auto block = [&](int k) {
+            if ((k & 63) == 0) pages = k + lane < mine ? paged_page(b, p.s, (first + (k + lane) * WAVES) * kBlock) : -1;
+            const int page = __builtin_amdgcn_readlane(pages, k & 63);
+            At x;
+            x.t0 = (first + k * WAVES) * kBlock;
+            x.in_page = x.t0 & ((1 << b.log_page) - 1);
+            x.lim = page < 0 ? 0 : min(kBlock, p.q.len - x.t0);
+            x.head = (size_t)max(page, 0) * a.KV + kvh;
+            return x;
+        };
+        auto load_k = [&](const At& x) {
+            const u32x4* k = reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k) + ((x.head << b.log_page) + x.in_page) * D * (F8 ? 1 : 2));
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int c = 0; c < C::kUnits; c++) {
+                    const int unit = 4 * c + g;             // D / kUnit units of 16 tokens
+                    kraw[kt][c] = unit * Lay::kUnit < D ? ld_global(k + kt * 16 * (D / Lay::kUnit) + unit * 16 + i16) : u32x4{0, 0, 0, 0};
+                }
+            if constexpr (F8) {
+                const float* s = a.k_scale + (x.head << (b.log_page - 4)) + (x.in_page >> 4);
+                const float* v = a.v_scale + (x.head << (b.log_page - 4)) + (x.in_page >> 4);
+#pragma unroll
+                for (int i = 0; i < 4; i++) ks[i] = ld_global(s + i), vs[i] = ld_global(v + i);
+            }
+        };
+        auto load_v = [&](const At& x) {
+            const u32x4* v = reinterpret_cast<const u32x4*>(static_cast<const char*>(a.v) + ((x.head << b.log_page) + x.in_page) * D * (F8 ? 1 : 2));
+#pragma unroll
+            for (int h = 0; h < C::kVB; h++)
+#pragma unroll
+                for (int c = 0; c < C::kCT; c++)
+                    if (16 * c < D) vraw[h][c] = ld_global(v + h * 4 * D + c * 64 + lane);
+        };
+        At now = block(0);
+        if (mine > 0) load_k(now);
+        for (int k = 0; k < mine; k++) {
+            const At x = now;
+            load_v(x);
+            float fk[4], rv[4], vtop = 1.f;
+            if constexpr (F8) {
+                // groups without a token the sequence has may hold anything
+                vtop = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    fk[i] = f * ks[i];
+                    if (16 * i < x.lim) vtop = fmaxf(vtop, vs[i]);
+                }
+                const float inv = vtop > 0.f ? 1.f / vtop : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) rv[i] = 16 * i < x.lim ? vs[i] * inv : 0.f;
+            }
+            f32x4 s[4];
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++) {
+                f32x4 hi = {0.f, 0.f, 0.f, 0.f}, lo = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int t = 0; t < C::kSteps; t++) {
+                    f16x8 y;
+                    if constexpr (F8) {
+                        const u32x4 w = kraw[kt][t >> 1];
+                        y = t & 1 ? f8_to_f16(w[2], w[3]) : f8_to_f16(w[0], w[1]);
+                    } else {
+                        y = __builtin_bit_cast(f16x8, kraw[kt][t]);
+                    }
+                    if constexpr (!C::kHalf) lo = mfma_16x16x32_f16(y, qf[t][1], lo);
+                    hi = mfma_16x16x32_f16(y, qf[t][0], hi);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[kt][i] = (C::kHalf ? hi[i] : fmaf(lo[i], 1.f / 2048.f, hi[i])) * (F8 ? fk[kt] : f);
+            }
+            if (k + 1 < mine) {
+                now = block(k + 1);
+                load_k(now);
+            }
+            if (x.lim < kBlock || x.t0 + kBlock - 1 > all) {
+                const int see = min(x.lim, last - x.t0 + 1);
+#pragma unroll
+                for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (16 * kt + 4 * g + i >= see) s[kt][i] = -INFINITY;
+            }
+            float bm = s[0][0];
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) bm = fmaxf(bm, s[kt][i]);
+            bm = pair_max<32>(pair_max<16>(bm));
+            if (__any(bm > mr + kRaise)) {
+                const float mn = fmaxf(mr, bm), al = ex2(mr - (mn == -INFINITY ? 0.f : mn));
+                mr = mn;
+                l *= al;
+#pragma unroll
+                for (int c = 0; c < C::kCT; c++) acc[c] *= al;
+            }
+            const float ref = mr == -INFINITY ? 0.f : mr;
+            f16x8 pf[2][C::kParts];
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float e = ex2(s[kt][i] - ref);
+                    l += e;
+                    const float y = e * (F8 ? kPScale * rv[kt] : kPScale);
+                    const _Float16 hi = (_Float16)y;
+                    pf[kt >> 1][0][4 * (kt & 1) + i] = hi;
+                    if constexpr (!C::kHalf) pf[kt >> 1][1][4 * (kt & 1) + i] = (_Float16)(y - (float)hi);
+                }
+            if (x.lim < kBlock) {                           // what no row sees may hold anything: zero
+#pragma unroll
+                for (int h = 0; h < C::kVB; h++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        // word j: four tokens of group j (e4m3), or two of group 2 h + j / 2
+                        const int there = x.lim - (F8 ? 16 * j + 4 * g : 32 * h + 16 * (j >> 1) + 4 * g + 2 * (j & 1)), n = min(max(there, 0), F8 ? 4 : 2);
+                        const uint32_t keep = n == (F8 ? 4 : 2) ? ~0u : (1u << (n * (F8 ? 8 : 16))) - 1;
+#pragma unroll
+                        for (int c = 0; c < C::kCT; c++) vraw[h][c][j] &= keep;
+                    }
+            }
+            // a block's sums start from zero and are added to the others by the VALU: the matrix unit carries no long sum
+#pragma unroll
+            for (int c = 0; c < C::kCT; c++) {
+                if (16 * c >= D) continue;
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    f16x8 v;
+                    if constexpr (F8) v = f8_to_f16(vraw[0][c][2 * h], vraw[0][c][2 * h + 1]);
+                    else v = __builtin_bit_cast(f16x8, vraw[h][c]);
+#pragma unroll
+                    for (int part = C::kParts - 1; part >= 0; part--) o = mfma_16x16x32_f16(v, pf[h][part], o);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[c][i] = F8 ? fmaf(o[i], vtop, acc[c][i]) : acc[c][i] + o[i];
+            }
+        }
+        float odd = l * 0.f;                                // NaN if a sum is not finite
+#pragma unroll
+        for (int c = 0; c < C::kCT; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) odd = fmaf(acc[c][i], 0.f, odd);
+        const bool redo = __any(odd != 0.f);
+        if (redo) paged_again<F8, Q, C::kCT>(a, p, kvh, q_row, last, first, WAVES, mr, l, acc);
+
+        // the waves' states
+        const float unit = redo ? 1.f : 1.f / kPScale;
+        l = pair_sum<32>(pair_sum<16>(l));
+        __syncthreads();                                    // the last piece's are read
+        if (g == 0) {
+            stat[0][wave][i16] = mr;
+            stat[1][wave][i16] = l;
+        }
+        __syncthreads();
+        float mx = stat[0][0][i16];
+#pragma unroll
+        for (int k = 1; k < WAVES; k++) mx = fmaxf(mx, stat[0][k][i16]);
+        const float wt = mr == -INFINITY ? (l != l ? 1.f : 0.f) : ex2(mr - mx) * unit;   // NaN: no score is a number
+#pragma unroll
+        for (int c = 0; c < C::kCT; c++) {
+            f32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = wt == 0.f ? 0.f : acc[c][i] * wt;
+            *reinterpret_cast<f32x4*>(merge + (wave * kPairs + i16) * C::kMerge + 16 * c + 4 * g) = v;
+        }
+        const bool cut = p.b0 > 0 || p.b1 < p.nb;
+        float* const part = a.ws + ((size_t)blockIdx.x * 2 + (p.b0 == 0)) * (kPairs * (D + 2));
+        if (tid < kPairs) {
+            float top = stat[0][0][tid], total = 0.f;
+#pragma unroll
+            for (int k = 1; k < WAVES; k++) top = fmaxf(top, stat[0][k][tid]);
+#pragma unroll
+            for (int k = 0; k < WAVES; k++) {
+                const float lk = stat[1][k][tid], mk = stat[0][k][tid];
+                total += mk == -INFINITY ? (lk != lk ? lk : 0.f) : lk * ex2(mk - top);
+            }
+            row_at[tid] = p.r0 + tid < R ? 1 : 0;
+            row_inv[tid] = cut ? 1.f : total == 0.f ? 0.f : 1.f / total;
+            if (cut) st_global(reinterpret_cast<f32x2*>(part + kPairs * D) + tid, f32x2{top, total});
+        }
+        __syncthreads();
+        for (int u = tid; u < kPairs * (D / 4); u += 64 * WAVES) {
+            const int pair = u / (D / 4), d = 4 * (u - pair * (D / 4));
+            if (!row_at[pair]) continue;
+            f32x4 sum = *reinterpret_cast<const f32x4*>(merge + pair * C::kMerge + d);
+#pragma unroll
+            for (int k = 1; k < WAVES; k++) sum += *reinterpret_cast<const f32x4*>(merge + (k * kPairs + pair) * C::kMerge + d);
+            const float inv = row_inv[pair];
+            sum = f32x4{sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+            if (cut) {
+                st_global(reinterpret_cast<f32x4*>(part + pair * D + d), sum);
+            } else {
+                const int rr = p.r0 + pair, m = rr / a.G;
+                paged_out(static_cast<Q*>(a.out) + ((size_t)(p.q.row0 + m) * a.H + kvh * a.G + (rr - m * a.G)) * D + d, sum);
+            }
+        }
+    }
+}
+
+// The parts of the pairs whose blocks more than one workgroup had: out = sum_i acc_i 2^(m_i - m) / sum_i l_i 2^(m_i - m). A workgroup a pair;
+// the parts lie with the workgroups of the kv head in a row, the first part in its workgroup's second place, the others in their first.
+template <typename Q, int WAVES>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttnArgs a)
+{
+    __shared__ float wgt[256];
+    __shared__ float red[4][2];
+    __shared__ f32x4 sums[256];
+    const PagedBatch& b = a.b;
+    const int pair = blockIdx.x, kvh = blockIdx.z, tid = threadIdx.x, lane = tid & 63, D = a.D;
+    auto tiles = [&](const PagedSeq& q) { return few(a, q) ? tiles_of(a, q) : 0; };
+    auto count = [&](const PagedSeq& q) { return few(a, q) ? tiles_of(a, q) * blocks_of(q) : 0; };
+    int s, tile;
+    PagedSeq q;
+    if (!paged_unit(b, blockIdx.y, tiles, s, tile, q)) return;
+    const int r = kPairs * tile + pair;
+    if (r >= q.n * a.G) return;
+    const long long total = paged_total(b, count), before = paged_total(b, count, s) + (long long)tile * blocks_of(q);
+    const long long per = (max((total + a.ranges - 1) / a.ranges, 1ll) + WAVES - 1) / WAVES * WAVES;
+    const int w0 = (int)(before / per), w1 = (int)((before + blocks_of(q) - 1) / per), n = w1 - w0 + 1;
+    if (n == 1) return;
+    // part i of pair: state at .., sums at ..
+    const size_t stride = (size_t)kPairs * (D + 2);
+    auto part = [&](int i) { return a.ws + ((size_t)((w0 + i) * a.KV + kvh) * 2 + (i == 0)) * stride; };
+    const int nc = D / 4, slot = tid / nc, c = tid - slot * nc, slots = 256 / nc;
+    float top = -INFINITY;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    // 256 parts at a time, each with the reference of all so far
+    for (int i0 = 0; i0 < n; i0 += 256) {
+        const int here = min(256, n - i0);
+        const f32x2 st = tid < here ? ld_global(reinterpret_cast<const f32x2*>(part(i0 + tid) + kPairs * D) + pair) : f32x2{-INFINITY, 0.f};
+        float mx = wave_max(st.x, lane);
+        __syncthreads();
+        if (lane == 0) red[tid >> 6][0] = mx;
+        __syncthreads();
+        mx = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
+        const float now = fmaxf(top, mx), ref = now == -INFINITY ? 0.f : now, al = top == -INFINITY ? (l != l ? 1.f : 0.f) : ex2(top - ref);
+        const float mi = st.x, li = st.y, e = mi == -INFINITY ? (li != li ? 1.f : 0.f) : ex2(mi - ref);
+        wgt[tid] = e;
+        const float sum = wave_sum(e == 0.f ? 0.f : li * e, lane);
+        if (lane == 0) red[tid >> 6][1] = sum;
+        __syncthreads();
+        l = (al == 0.f ? 0.f : l * al) + ((red[0][1] + red[1][1]) + (red[2][1] + red[3][1]));
+        o *= al;
+        if (slot < slots)
+            for (int i = slot; i < here; i += slots) {
+                const float wi = wgt[i];
+                if (wi == 0.f) continue;
+                const f32x4 x = ld_global(reinterpret_cast<const f32x4*>(part(i0 + i) + pair * D) + c);
+#pragma unroll
+                for (int k = 0; k < 4; k++) o[k] = fmaf(wi, x[k], o[k]);
+            }
+        top = now;
+    }
+    sums[tid] = o;
+    __syncthreads();
+    if (tid >= nc) return;
+    for (int i = 1; i < slots; i++) o += sums[tid + i * nc];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int m = r / a.G;
+    paged_out(static_cast<Q*>(a.out) + ((size_t)(q.row0 + m) * a.H + kvh * a.G + (r - m * a.G)) * D + 4 * tid, f32x4{o.x * inv, o.y * inv, o.z * inv, o.w * inv});
 }
 
 template <bool F8, typename Q>
@@ -29,7 +482,7 @@ __global__ __launch_bounds__(256) void paged_row_kernel(const PagedAttnArgs a)
     const PagedBatch& b = a.b;
     int s;
     PagedSeq seq;
-    if (!paged_row(b, m, s, seq)) return;
+    if (!paged_row(b, m, s, seq) || few(a, seq)) return;
     const int last = seq.len - seq.n + m - seq.row0;
     const size_t row = ((size_t)m * a.H + h) * D;
     if (tid < D) q[tid] = (float)static_cast<const Q*>(a.q)[row + tid];
@@ -88,19 +541,36 @@ __global__ __launch_bounds__(256) void paged_row_kernel(const PagedAttnArgs a)
 
 }  // namespace
 
-uint64_t plan_paged_attention(PagedAttnArgs*, size_t) { return 0; }
+uint64_t plan_paged_attention(PagedAttnArgs* a, size_t)
+{
+    a->few = 4 * kPairs;
+    const int most = std::min<long long>(4ll * a->b.S, a->b.S + (long long)a->b.M * a->G / kPairs);
+    a->units = most;
+    a->whole = a->b.max_len <= 1024;
+    a->ranges = std::max(1, 512 / a->KV);
+    return a->whole || a->ranges == 1 ? 0 : (uint64_t)a->ranges * a->KV * 2 * kPairs * (a->D + 2) * sizeof(float);
+}
+
+namespace {
+
+template <bool F8, typename Q>
+hipError_t launch(const PagedAttnArgs& a, hipStream_t stream)
+{
+    const dim3 grid((a.whole ? a.units : a.ranges) * a.KV);
+    if (a.D <= 64) hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 64, 4>), grid, dim3(256), 0, stream, a);
+    else if (a.D <= 128) hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 128, 4>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 256, 4>), grid, dim3(256), 0, stream, a);
+    if (!a.whole && a.ranges > 1) hipLaunchKernelGGL((paged_merge_kernel<Q, 4>), dim3(kPairs, a.units, a.KV), dim3(256), 0, stream, a);
+    if (a.b.max_rows * a.G > a.few) hipLaunchKernelGGL((paged_row_kernel<F8, Q>), dim3(a.H, a.b.M), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+
+}  // namespace
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream)
 {
-    const dim3 grid(a.H, a.b.M);
-    if (a.k_scale) {
-        if (a.half) hipLaunchKernelGGL((paged_row_kernel<true, _Float16>), grid, dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((paged_row_kernel<true, float>), grid, dim3(256), 0, stream, a);
-    } else {
-        if (a.half) hipLaunchKernelGGL((paged_row_kernel<false, _Float16>), grid, dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((paged_row_kernel<false, float>), grid, dim3(256), 0, stream, a);
-    }
-    return hipGetLastError();
+    if (a.k_scale) return a.half ? launch<true, _Float16>(a, stream) : launch<true, float>(a, stream);
+    return a.half ? launch<false, _Float16>(a, stream) : launch<false, float>(a, stream);
 }
 
 }  // namespace ql
