@@ -111,6 +111,82 @@ struct DecodeTile {
     static __device__ __forceinline__ int col(int t, int g) { return F8 ? 64 * (t >> 1) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g; }
 };
 
+// q's fragments of the lane's pair; returns what scores are multiplied by
+template <typename C, typename Q>
+__device__ __forceinline__ float load_q(const Q* q, int g, int D, float scale, f16x8 (&qf)[C::kSteps][C::kParts])
+{
+    if constexpr (C::kHalf) {
+#pragma unroll
+        for (int t = 0; t < C::kSteps; t++) {
+            const int d = C::col(t, g);
+            qf[t][0] = d < D ? __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(q + d))) : f16x8{};
+        }
+        return scale;
+    } else {
+        f32x4 x[C::kSteps][2];
+        float mx = 0.f;
+#pragma unroll
+        for (int t = 0; t < C::kSteps; t++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int d = C::col(t, g) + 4 * k;
+                x[t][k] = d < D ? ld_global(reinterpret_cast<const f32x4*>(q + d)) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[t][k][e]));
+            }
+        mx = pair_max<32>(pair_max<16>(mx));
+        // the row's power of two: its largest value to [2^14, 2^15)
+        const float s = mx > 0.f && mx <= kMaxFinite ? ldexpf(1.f, min(100, 14 - ilogbf(mx))) : 1.f;
+#pragma unroll
+        for (int t = 0; t < C::kSteps; t++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float y = x[t][e >> 2][e & 3] * s;
+                const _Float16 hi = (_Float16)y;
+                qf[t][0][e] = hi;
+                qf[t][1][e] = (_Float16)((y - (float)hi) * 2048.f);
+            }
+        return fmaxf(scale / s, 1.17549435e-38f);
+    }
+}
+
+// Sums are kept in units of a power of two vref near the blocks' own: rv, the block's scales in it, at most one and, for the block's largest, no
+// less than 2^-6. Returns what the sums so far are multiplied by. Groups from lim on have no token, and scales that may hold anything.
+__device__ __forceinline__ float v_reference(const float (&vs)[4], int lim, float& vref, float (&rv)[4])
+{
+    float top = 0.f, al = 1.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (16 * i < lim) top = fmaxf(top, vs[i]);
+    if (top > vref || top < vref * (1.f / 64.f)) {
+        if (top > 0.f) {
+            al = vref / top;
+            vref = top;
+        }
+    }
+    const float inv = vref > 0.f ? 1.f / vref : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) rv[i] = 16 * i < lim ? vs[i] * inv : 0.f;
+    return al;
+}
+
+// which of word j of part h of V's fragment are of tokens before lim: four tokens of group j (e4m3), or two of group 2 h + j / 2
+template <bool F8>
+__device__ __forceinline__ uint32_t v_there(int lim, int h, int j, int g)
+{
+    constexpr int kIn = F8 ? 4 : 2;
+    const int n = min(max(lim - (F8 ? 16 * j + 4 * g : 32 * h + 16 * (j >> 1) + 4 * g + 2 * (j & 1)), 0), kIn);
+    return n == kIn ? ~0u : (1u << (n * (32 / kIn))) - 1;
+}
+
+// 16 bytes a lane to LDS, a wave's in a row from `to`
+__device__ __forceinline__ void load_to_lds(const void* from, void* to)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+#endif
+}
+
 template <bool F8, typename Q, int DP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_kernel(const PagedAttnArgs a)
 {
@@ -159,42 +235,7 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
         const int all = p.q.len - p.q.n;                    // every row of the sequence sees the tokens up to it
 
         f16x8 qf[C::kSteps][C::kParts];
-        float f = a.scale;
-        {
-            const Q* q = static_cast<const Q*>(a.q) + q_row;
-            if constexpr (C::kHalf) {
-#pragma unroll
-                for (int t = 0; t < C::kSteps; t++) {
-                    const int d = C::col(t, g);
-                    qf[t][0] = d < D ? __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(q + d))) : f16x8{};
-                }
-            } else {
-                f32x4 x[C::kSteps][2];
-                float mx = 0.f;
-#pragma unroll
-                for (int t = 0; t < C::kSteps; t++)
-#pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        const int d = C::col(t, g) + 4 * k;
-                        x[t][k] = d < D ? ld_global(reinterpret_cast<const f32x4*>(q + d)) : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(x[t][k][e]));
-                    }
-                mx = pair_max<32>(pair_max<16>(mx));
-                // the row's power of two: its largest value to [2^14, 2^15)
-                const float s = mx > 0.f && mx <= kMaxFinite ? ldexpf(1.f, min(100, 14 - ilogbf(mx))) : 1.f;
-                f = fmaxf(a.scale / s, 1.17549435e-38f);
-#pragma unroll
-                for (int t = 0; t < C::kSteps; t++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float y = x[t][e >> 2][e & 3] * s;
-                        const _Float16 hi = (_Float16)y;
-                        qf[t][0][e] = hi;
-                        qf[t][C::kParts - 1][e] = (_Float16)((y - (float)hi) * 2048.f);
-                    }
-            }
-        }
+        const float f = load_q<C>(static_cast<const Q*>(a.q) + q_row, g, D, a.scale, qf);
         f32x4 acc[C::kCT];
         float mr = -INFINITY, l = 0.f;
 #pragma unroll
@@ -204,7 +245,7 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
         const int first = p.b0 + wave, mine = first < p.b1 ? (p.b1 - first + WAVES - 1) / WAVES : 0;
         int pages = 0;
         u32x4 kraw[4][C::kUnits], vraw[C::kVB][C::kCT];
-        float ks[4], vs[4];
+        float ks[4], vs[4], vref = 0.f;
         struct At {
             size_t head;
             int in_page, t0, lim;                           // lim: tokens of the block that a row may see
@@ -248,19 +289,10 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
         for (int k = 0; k < mine; k++) {
             const At x = now;
             load_v(x);
-            float fk[4], rv[4], vtop = 1.f;
-            if constexpr (F8) {
-                // groups without a token the sequence has may hold anything
-                vtop = 0.f;
+            float fk[4], vb[4];
+            if constexpr (F8)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    fk[i] = f * ks[i];
-                    if (16 * i < x.lim) vtop = fmaxf(vtop, vs[i]);
-                }
-                const float inv = vtop > 0.f ? 1.f / vtop : 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) rv[i] = 16 * i < x.lim ? vs[i] * inv : 0.f;
-            }
+                for (int i = 0; i < 4; i++) fk[i] = f * ks[i], vb[i] = vs[i];
             f32x4 s[4];
 #pragma unroll
             for (int kt = 0; kt < 4; kt++) {
@@ -305,6 +337,13 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
 #pragma unroll
                 for (int c = 0; c < C::kCT; c++) acc[c] *= al;
             }
+            float rv[4];
+            if constexpr (F8) {
+                const float al = v_reference(vb, x.lim, vref, rv);
+                if (al != 1.f)
+#pragma unroll
+                    for (int c = 0; c < C::kCT; c++) acc[c] *= al;
+            }
             const float ref = mr == -INFINITY ? 0.f : mr;
             f16x8 pf[2][C::kParts];
 #pragma unroll
@@ -323,9 +362,7 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
                 for (int h = 0; h < C::kVB; h++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        // word j: four tokens of group j (e4m3), or two of group 2 h + j / 2
-                        const int there = x.lim - (F8 ? 16 * j + 4 * g : 32 * h + 16 * (j >> 1) + 4 * g + 2 * (j & 1)), n = min(max(there, 0), F8 ? 4 : 2);
-                        const uint32_t keep = n == (F8 ? 4 : 2) ? ~0u : (1u << (n * (F8 ? 8 : 16))) - 1;
+                        const uint32_t keep = v_there<F8>(x.lim, h, j, g);
 #pragma unroll
                         for (int c = 0; c < C::kCT; c++) vraw[h][c][j] &= keep;
                     }
@@ -344,7 +381,7 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
                     for (int part = C::kParts - 1; part >= 0; part--) o = mfma_16x16x32_f16(v, pf[h][part], o);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[c][i] = F8 ? fmaf(o[i], vtop, acc[c][i]) : acc[c][i] + o[i];
+                for (int i = 0; i < 4; i++) acc[c][i] += o[i];
             }
         }
         float odd = l * 0.f;                                // NaN if a sum is not finite
@@ -356,7 +393,7 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
         if (redo) paged_again<F8, Q, C::kCT>(a, p, kvh, q_row, last, first, WAVES, mr, l, acc);
 
         // the waves' states
-        const float unit = redo ? 1.f : 1.f / kPScale;
+        const float unit = redo ? 1.f : F8 ? vref / kPScale : 1.f / kPScale;
         l = pair_sum<32>(pair_sum<16>(l));
         __syncthreads();                                    // the last piece's are read
         if (g == 0) {
@@ -473,70 +510,226 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttnArgs a)
     paged_out(static_cast<Q*>(a.out) + ((size_t)(q.row0 + m) * a.H + kvh * a.G + (r - m * a.G)) * D + 4 * tid, f32x4{o.x * inv, o.y * inv, o.z * inv, o.w * inv});
 }
 
-template <bool F8, typename Q>
-__global__ __launch_bounds__(256) void paged_row_kernel(const PagedAttnArgs a)
+// Sequences of many rows: a workgroup has 64 NT (row, head) pairs of one kv head, 16 NT a wave, and goes through their tokens, 64 at a time, which all its waves
+// read from LDS; the next 64 are on their way there meanwhile, as they lie in memory. Scores, softmax and products as above.
+template <bool F8, typename Q, int DP, int NT>
+struct PromptTile {
+    using C = DecodeTile<F8, Q, DP>;
+    static constexpr int kWaves = 4, kRows = 16 * NT * kWaves;
+    static constexpr int kBytes = kBlock * DP * (F8 ? 1 : 2);    // of K or V of a block
+};
+
+template <bool F8, typename Q, int DP, int NT>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(const PagedAttnArgs a)
 {
+    using C = DecodeTile<F8, Q, DP>;
+    using T = PromptTile<F8, Q, DP, NT>;
     typedef PagedLayout<F8 ? 1 : 2> Lay;
-    __shared__ float q[256], p[4][64], st[2][4], part[4][256];
-    const int h = blockIdx.x, m = blockIdx.y, kvh = h / a.G, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, D = a.D;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][T::kBytes];
+    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4, D = a.D;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const PagedBatch& b = a.b;
-    int s;
-    PagedSeq seq;
-    if (!paged_row(b, m, s, seq) || few(a, seq)) return;
-    const int last = seq.len - seq.n + m - seq.row0;
-    const size_t row = ((size_t)m * a.H + h) * D;
-    if (tid < D) q[tid] = (float)static_cast<const Q*>(a.q)[row + tid];
-    __syncthreads();
-    float mx = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int t0 = 64 * wave; t0 <= last; t0 += 256) {
-        const int t = t0 + lane, page = paged_page(b, s, t0), in_page = t0 & ((1 << b.log_page) - 1);
-        if (page < 0) continue;
-        const size_t head = (size_t)page * a.KV + kvh, base = (head << b.log_page) * D, sc0 = (head << (b.log_page - 4)) + (in_page >> 4);
-        float sc = -INFINITY;
-        if (t <= last) {
-            sc = 0.f;
-            for (int d = 0; d < D; d++) sc = fmaf(q[d], value_at<F8>(a.k, base + Lay::k_at(D, in_page + lane, d / Lay::kUnit) + d % Lay::kUnit), sc);
-            sc *= a.scale * (F8 ? a.k_scale[sc0 + lane / 16] : 1.f);
-        }
-        float bm = sc;
+    const int kvh = blockIdx.x % a.KV, tiles = gridDim.x / a.KV;
+    Piece p;
+    int tile;
+    // the last tiles first: they see most
+    auto count = [&](const PagedSeq& q) { return few(a, q) ? 0 : (q.n * a.G + T::kRows - 1) / T::kRows; };
+    if (!paged_unit(b, tiles - 1 - (int)(blockIdx.x / a.KV), count, p.s, tile, p.q)) return;
+    const int R = p.q.n * a.G, all = p.q.len - p.q.n;       // every row sees the tokens up to `all`
+    p.r0 = T::kRows * tile;
+    p.nb = (all + (min(p.r0 + T::kRows, R) - 1) / a.G) / kBlock + 1;
+    p.b0 = 0;
+    p.b1 = p.nb;
+    const int low = all + p.r0 / a.G;                       // every row of the tile sees the tokens up to it
+
+    size_t q_row[NT];
+    int last[NT];
+    f16x8 qf[NT][C::kSteps][C::kParts];
+    float f[NT];
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor(bm, o));
-        const float mn = fmaxf(mx, bm), ref = mn == -INFINITY ? 0.f : mn, al = ex2(mx - ref);
-        mx = mn;
-        const float e = t <= last ? ex2(sc - ref) : 0.f;
-        float sum = e;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-        l = l * al + sum;
-        p[wave][lane] = e * (F8 ? a.v_scale[sc0 + lane / 16] : 1.f);
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int d = lane + 64 * i;
-            acc[i] *= al;
-            if (d < D)
-                for (int k = 0; k < 64 && t0 + k <= last; k++)
-                    acc[i] = fmaf(p[wave][k], value_at<F8>(a.v, base + Lay::v_at(D, in_page + k / 4 * 4, d) + k % 4), acc[i]);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+    for (int nt = 0; nt < NT; nt++) {
+        const int r = min(p.r0 + 16 * (NT * wave + nt) + i16, R - 1), row = r / a.G;
+        q_row[nt] = ((size_t)(p.q.row0 + row) * a.H + kvh * a.G + (r - row * a.G)) * D;
+        last[nt] = all + row;
+        f[nt] = load_q<C>(static_cast<const Q*>(a.q) + q_row[nt], g, D, a.scale, qf[nt]);
     }
-    if (lane == 0) st[0][wave] = mx, st[1][wave] = l;
+    f32x4 acc[C::kCT][NT];
+    float mr[NT], l[NT];
 #pragma unroll
-    for (int i = 0; i < 4; i++) part[wave][lane + 64 * i] = acc[i];
-    __syncthreads();
-    if (tid >= D) return;
-    float top = st[0][0], total = 0.f, o = 0.f;
-    for (int w = 1; w < 4; w++) top = fmaxf(top, st[0][w]);
-    for (int w = 0; w < 4; w++) {
-        const float f = st[0][w] == -INFINITY ? (st[1][w] != st[1][w] ? st[1][w] : 0.f) : ex2(st[0][w] - top);
-        if (f == 0.f) continue;
-        total += f * st[1][w];
-        o += f * part[w][tid];
+    for (int nt = 0; nt < NT; nt++) {
+        mr[nt] = -INFINITY;
+        l[nt] = 0.f;
+#pragma unroll
+        for (int c = 0; c < C::kCT; c++) acc[c][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    o = total == 0.f ? 0.f : o / total;
-    static_cast<Q*>(a.out)[row + tid] = (Q)o;
+    int pages = 0;
+    float ks[4], vs[4], vref = 0.f;
+    const int chunks = D * (F8 ? 1 : 2) / 16;               // of 1 KB, of K or V of a block
+    auto page_of = [&](int k) {
+        if ((k & 63) == 0) pages = k + lane < p.b1 ? paged_page(b, p.s, (k + lane) * kBlock) : -1;
+        return __builtin_amdgcn_readlane(pages, k & 63);
+    };
+    auto fetch = [&](int k, int page, int buf) {
+        const int in_page = (k * kBlock) & ((1 << b.log_page) - 1);
+        const size_t head = (size_t)max(page, 0) * a.KV + kvh, at = ((head << b.log_page) + in_page) * D * (F8 ? 1 : 2);
+        for (int c = wave; c < 2 * chunks; c += T::kWaves) {
+            const bool v = c >= chunks;
+            const int cc = v ? c - chunks : c;
+            load_to_lds(static_cast<const char*>(v ? a.v : a.k) + at + cc * 1024 + lane * 16, &lds[buf][v][cc * 1024]);
+        }
+        if constexpr (F8) {
+            const float* ss = a.k_scale + (head << (b.log_page - 4)) + (in_page >> 4);
+            const float* sv = a.v_scale + (head << (b.log_page - 4)) + (in_page >> 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) ks[i] = ld_global(ss + i), vs[i] = ld_global(sv + i);
+        }
+    };
+    int page = page_of(0);
+    fetch(0, page, 0);
+    for (int k = 0; k < p.b1; k++) {
+        const int buf = k & 1, t0 = k * kBlock, lim = page < 0 ? 0 : min(kBlock, p.q.len - t0);
+        // this block has arrived, and every wave is done with the one that the next takes the place of
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        float kss[4], vss[4];
+        if constexpr (F8)
+#pragma unroll
+            for (int i = 0; i < 4; i++) kss[i] = ks[i], vss[i] = vs[i];
+        if (k + 1 < p.b1) {
+            page = page_of(k + 1);
+            fetch(k + 1, page, buf ^ 1);
+        }
+        const u32x4* const kl = reinterpret_cast<const u32x4*>(lds[buf][0]) + lane;
+        const u32x4* const vl = reinterpret_cast<const u32x4*>(lds[buf][1]) + lane;
+        f32x4 s[4][NT];
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++) {
+            f32x4 hi[NT], lo[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) hi[nt] = lo[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < C::kUnits; c++) {
+                const u32x4 w = (4 * c + g) * Lay::kUnit < D ? kl[kt * (D / Lay::kUnit) * 16 + c * 64] : u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < (F8 ? 2 : 1); j++) {
+                    const f16x8 y = F8 ? f8_to_f16(w[2 * j], w[2 * j + 1]) : __builtin_bit_cast(f16x8, w);
+                    const int t = F8 ? 2 * c + j : c;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        if constexpr (!C::kHalf) lo[nt] = mfma_16x16x32_f16(y, qf[nt][t][1], lo[nt]);
+                        hi[nt] = mfma_16x16x32_f16(y, qf[nt][t][0], hi[nt]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[kt][nt][i] = (C::kHalf ? hi[nt][i] : fmaf(lo[nt][i], 1.f / 2048.f, hi[nt][i])) * (F8 ? f[nt] * kss[kt] : f[nt]);
+        }
+        if (lim < kBlock || t0 + kBlock - 1 > low)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const int see = min(lim, last[nt] - t0 + 1) - 4 * g;
+#pragma unroll
+                for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (16 * kt + i >= see) s[kt][nt][i] = -INFINITY;
+            }
+        float bm[NT];
+        bool up = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            bm[nt] = s[0][nt][0];
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) bm[nt] = fmaxf(bm[nt], s[kt][nt][i]);
+            bm[nt] = pair_max<32>(pair_max<16>(bm[nt]));
+            up = up || bm[nt] > mr[nt] + kRaise;
+        }
+        if (__any(up))
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const float mn = fmaxf(mr[nt], bm[nt]), al = ex2(mr[nt] - (mn == -INFINITY ? 0.f : mn));
+                mr[nt] = mn;
+                l[nt] *= al;
+#pragma unroll
+                for (int c = 0; c < C::kCT; c++) acc[c][nt] *= al;
+            }
+        float rv[4];
+        if constexpr (F8) {
+            const float al = v_reference(vss, lim, vref, rv);
+            if (al != 1.f)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < C::kCT; c++) acc[c][nt] *= al;
+        }
+        f16x8 pf[2][NT][C::kParts];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const float ref = mr[nt] == -INFINITY ? 0.f : mr[nt];
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float e = ex2(s[kt][nt][i] - ref);
+                    l[nt] += e;
+                    const float y = e * (F8 ? kPScale * rv[kt] : kPScale);
+                    const _Float16 hi = (_Float16)y;
+                    pf[kt >> 1][nt][0][4 * (kt & 1) + i] = hi;
+                    if constexpr (!C::kHalf) pf[kt >> 1][nt][1][4 * (kt & 1) + i] = (_Float16)(y - (float)hi);
+                }
+        }
+#pragma unroll
+        for (int c = 0; c < C::kCT; c++) {
+            if (16 * c >= D) continue;
+            u32x4 w[C::kVB];
+#pragma unroll
+            for (int h = 0; h < C::kVB; h++) w[h] = vl[h * 4 * D + c * 64];
+            if (lim < kBlock)                               // what no row sees may hold anything: zero
+#pragma unroll
+                for (int h = 0; h < C::kVB; h++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[h][j] &= v_there<F8>(lim, h, j, g);
+            f32x4 o[NT];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) o[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const f16x8 v = F8 ? f8_to_f16(w[0][2 * h], w[0][2 * h + 1]) : __builtin_bit_cast(f16x8, w[F8 ? 0 : h]);
+#pragma unroll
+                for (int part = C::kParts - 1; part >= 0; part--)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) o[nt] = mfma_16x16x32_f16(v, pf[h][nt][part], o[nt]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) acc[c][nt] += o[nt];
+        }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        float odd = l[nt] * 0.f;                            // NaN if a sum is not finite
+        f32x4 mine[C::kCT];
+#pragma unroll
+        for (int c = 0; c < C::kCT; c++) {
+            mine[c] = acc[c][nt];
+#pragma unroll
+            for (int i = 0; i < 4; i++) odd = fmaf(mine[c][i], 0.f, odd);
+        }
+        float unit = F8 ? vref / kPScale : 1.f / kPScale;
+        if (__any(odd != 0.f)) {
+            paged_again<F8, Q, C::kCT>(a, p, kvh, q_row[nt], last[nt], p.b0, 1, mr[nt], l[nt], mine);
+            unit = 1.f;
+        }
+        const float total = pair_sum<32>(pair_sum<16>(l[nt])), inv = total == 0.f ? 0.f : unit / total;
+        if (p.r0 + 16 * (NT * wave + nt) + i16 >= R) continue;
+#pragma unroll
+        for (int c = 0; c < C::kCT; c++)
+            if (16 * c < D) paged_out(static_cast<Q*>(a.out) + q_row[nt] + 16 * c + 4 * g, f32x4{mine[c][0] * inv, mine[c][1] * inv, mine[c][2] * inv, mine[c][3] * inv});
+    }
 }
 
 }  // namespace
@@ -561,7 +754,13 @@ hipError_t launch(const PagedAttnArgs& a, hipStream_t stream)
     else if (a.D <= 128) hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 128, 4>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 256, 4>), grid, dim3(256), 0, stream, a);
     if (!a.whole && a.ranges > 1) hipLaunchKernelGGL((paged_merge_kernel<Q, 4>), dim3(kPairs, a.units, a.KV), dim3(256), 0, stream, a);
-    if (a.b.max_rows * a.G > a.few) hipLaunchKernelGGL((paged_row_kernel<F8, Q>), dim3(a.H, a.b.M), dim3(256), 0, stream, a);
+    if (a.b.max_rows * a.G > a.few) {
+        const int rows = a.D <= 128 ? 128 : 64, tiles = (int)std::min<long long>(((long long)a.b.M * a.G + rows - 1) / rows + a.b.S, (long long)a.b.M * a.G / a.few + 1 + (long long)a.b.M * a.G / rows);
+        const dim3 grid(tiles * a.KV);
+        if (a.D <= 64) hipLaunchKernelGGL((paged_prompt_kernel<F8, Q, 64, 2>), grid, dim3(256), 0, stream, a);
+        else if (a.D <= 128) hipLaunchKernelGGL((paged_prompt_kernel<F8, Q, 128, 2>), grid, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL((paged_prompt_kernel<F8, Q, 256, 1>), grid, dim3(256), 0, stream, a);
+    }
     return hipGetLastError();
 }
 
