@@ -59,7 +59,8 @@ class Call:
                 x, a, b = (v.astype(np.float64) for v in (self.x[i][m], self.a[i][k], self.b[i][k]))
                 s = float(self.scale[i][k]) if self.scales else 1.0
                 want[m] += s * (x @ a.T) @ b.T
-                # fp32 sums of K and of r products, each off by as many u of the products' sizes at most, and the scale's product
+                # fp32 sums of K and of r products, each off by as many u of the products' sizes at most, and the scale's product; many rows:
+                # x's and t's two parts carry 2^-22 of the largest of their 32 columns, or of the row's ranks
                 tol[m] = s * ((K + 4) * U * (np.abs(x) @ np.abs(a).T) + (r + 4) * U * np.abs(x @ a.T)) @ np.abs(b).T
             tol += 2 * U * np.abs(want)
             with np.errstate(invalid="ignore"):
@@ -81,6 +82,7 @@ CASES = [  # M, targets, how the ids lie
     (300, [(520, 260, 40, 7)], "mixed"),
     (1000, [(896, 128, 16, 6)], "runs"),
     (130, [(2056, 12, 96, 3)], "one"),
+    (20000, [(16, 8, 128, 3)] * 8, "runs"),                                      # more rows than the workspace has room for at once
 ]
 
 
@@ -122,9 +124,10 @@ def test_ids_that_are_none(ql, ctx):
     call.box.release()
 
 
-def test_rows_apart(ql, ctx):
+@pytest.mark.parametrize("M", [40, 600])
+def test_rows_apart(ql, ctx, M):
     """A row that is not finite, its adapter's too, stays with itself: every other row has the bits that it has without."""
-    M, ids = 40, np.arange(40) % 3
+    ids = np.arange(M) % 3
     call = Call(ql, ctx, M, [(256, 64, 16, 3)], False, ids)
     call.run()
     plain = call.check()[0]
@@ -142,7 +145,7 @@ def test_rows_apart(ql, ctx):
     call.box.release()
 
 
-@pytest.mark.parametrize("M", [3, 100])
+@pytest.mark.parametrize("M", [3, 100, 600])
 def test_sizes_of_x(ql, ctx, M):
     """fp32 rows of any size keep fp32's accuracy."""
     call = Call(ql, ctx, M, [(256, 64, 16, 3)], False, np.arange(M) % 3)
@@ -158,7 +161,7 @@ def test_sizes_of_x(ql, ctx, M):
 
 
 def test_graph_streams_and_other_calls(ql, ctx):
-    calls = [Call(ql, ctx, M, [(896, 896, 16, 6), (896, 128, 16, 6)], False, ids_of("mixed", M, 6), same=True, seed=M) for M in (5, 90)]
+    calls = [Call(ql, ctx, M, [(896, 896, 16, 6), (896, 128, 16, 6)], False, ids_of("mixed", M, 6), same=True, seed=M) for M in (5, 90, 700)]
     ctx.graph_begin()
     for c in calls:
         c.run(sync=False)

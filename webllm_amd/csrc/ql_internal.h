@@ -414,7 +414,12 @@ struct LoraArgs {
     const int32_t* ids;        // [M]
     float* ws;
     int count, M, half;        // half: x is fp16
+    // plan_lora fills these: 0, a workgroup a row; or how many rows are done in tiles at once, and where t [rows, rank] of each projection lies
+    // in ws, in values
+    int rows;
+    uint64_t t_off[kMaxBatch];
 };
+constexpr int kLoraRowMax = 128;   // most rows that have a workgroup each
 uint64_t plan_lora(LoraArgs* a, size_t ws_bytes);
 hipError_t launch_lora(const LoraArgs& a, hipStream_t stream);
 

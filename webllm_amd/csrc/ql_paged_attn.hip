@@ -725,10 +725,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
             unit = 1.f;
         }
         const float total = pair_sum<32>(pair_sum<16>(l[nt])), inv = total == 0.f ? 0.f : unit / total;
-        if (p.r0 + 16 * (NT * wave + nt) + i16 >= R) continue;
+        const bool there = p.r0 + 16 * (NT * wave + nt) + i16 < R;
 #pragma unroll
         for (int c = 0; c < C::kCT; c++)
-            if (16 * c < D) paged_out(static_cast<Q*>(a.out) + q_row[nt] + 16 * c + 4 * g, f32x4{mine[c][0] * inv, mine[c][1] * inv, mine[c][2] * inv, mine[c][3] * inv});
+            if (there && 16 * c < D) paged_out(static_cast<Q*>(a.out) + q_row[nt] + 16 * c + 4 * g, f32x4{mine[c][0] * inv, mine[c][1] * inv, mine[c][2] * inv, mine[c][3] * inv});
     }
 }
 
