@@ -396,7 +396,7 @@ struct PagedAttnArgs {
     float scale;               // fp32(log2(e) / sqrt(D))
     // plan_paged_attention fills these: most (row, head) pairs of a sequence of few rows, most tiles of 16 of them that such sequences have,
     // whether each tile is one workgroup's, or all their blocks are dealt to `ranges` workgroups a kv head
-    int few, units, whole, ranges;
+    int few, units, whole, ranges, merge_pairs;
 };
 uint64_t plan_paged_attention(PagedAttnArgs* a, size_t ws_bytes);   // the workspace it needs
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);

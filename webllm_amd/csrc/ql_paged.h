@@ -18,52 +18,68 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedBatch& b, int s)
     return {r0, ok ? r1 - r0 : 0, len};
 }
 
-// Unit number j of the units that the sequences have, count(sequence) of each, in order: its sequence s and its number in it. Every
-// lane of a wave takes part and gets the same; false beyond the last one.
-template <typename F>
-__device__ __forceinline__ bool paged_unit(const PagedBatch& b, long long j, F count, int& s, int& local, PagedSeq& q)
+// inclusive sums over a wave: rows of 16 by shifts, then the rows before
+__device__ __forceinline__ int wave_upto(int v)
 {
-    const int lane = threadIdx.x & 63;
-    long long before = 0;
-    for (int s0 = 0; s0 < b.S; s0 += 64) {
-        PagedSeq me = {0, 0, 0};
-        if (s0 + lane < b.S) me = paged_seq(b, s0 + lane);
-        const int c = me.n ? count(me) : 0;
-        int upto = c;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int t = __shfl_up(upto, o);
-            if (lane >= o) upto += t;
-        }
-        const uint64_t past = __ballot(before + upto > j);
-        if (past) {
-            const int at = __builtin_ctzll(past);
-            s = s0 + at;
-            local = (int)(j - before) - (__shfl(upto, at) - __shfl(c, at));
-            q = {__shfl(me.row0, at), __shfl(me.n, at), __shfl(me.len, at)};
-            return true;
-        }
-        before += __shfl(upto, 63);
-    }
-    return false;
+    v += (int)__builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // row_shr 1, 2, 4, 8: nothing comes in at a row's start
+    v += (int)__builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += (int)__builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += (int)__builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += (int)__builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // the last of a row to the next, rows 1 and 3
+    v += (int)__builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // that of the first half to the second
+    return v;
 }
 
-// The units of all sequences, or of those before the first `upto`
+// The units that the sequences have, count(sequence) of each, in order. Every lane of a wave takes part and gets the same; a lane knows a sequence
+// of the 64 that were looked at last, so that tables of up to 64 are read once.
 template <typename F>
-__device__ __forceinline__ long long paged_total(const PagedBatch& b, F count, int upto = kPagedMaxSeqs)
-{
-    const int lane = threadIdx.x & 63, S = min(b.S, upto);
-    long long total = 0;
-    for (int s0 = 0; s0 < S; s0 += 64) {
-        PagedSeq me = {0, 0, 0};
-        if (s0 + lane < S) me = paged_seq(b, s0 + lane);
-        int c = me.n ? count(me) : 0;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o);
-        total += c;
+struct PagedUnits {
+    const PagedBatch& b;
+    F count;
+    PagedSeq me;
+    int c, upto, s0 = 0;
+    long long before = 0;
+
+    __device__ __forceinline__ PagedUnits(const PagedBatch& b, F count) : b(b), count(count) { load(); }
+    __device__ __forceinline__ void load()
+    {
+        const int s = s0 + (threadIdx.x & 63);
+        me = {0, 0, 0};
+        if (s < b.S) me = paged_seq(b, s);
+        c = me.n ? count(me) : 0;
+        upto = wave_upto(c);
     }
-    return total;
-}
+    __device__ __forceinline__ int here() const { return __builtin_amdgcn_readlane(upto, 63); }
+    __device__ __forceinline__ bool next()
+    {
+        if (s0 + 64 >= b.S) return false;
+        before += here();
+        s0 += 64;
+        load();
+        return true;
+    }
+    __device__ __forceinline__ long long total()
+    {
+        while (next()) {}
+        return before + here();
+    }
+    // unit number j: its sequence s and its number in it; false beyond the last one
+    __device__ __forceinline__ bool find(long long j, int& s, int& local, PagedSeq& q)
+    {
+        if (j < before) {
+            s0 = 0;
+            before = 0;
+            load();
+        }
+        while (j >= before + here())
+            if (!next()) return false;
+        const int at = __builtin_ctzll(__ballot(before + upto > j));
+        s = s0 + at;
+        local = (int)(j - before) - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(c, at));
+        q = {__builtin_amdgcn_readlane(me.row0, at), __builtin_amdgcn_readlane(me.n, at), __builtin_amdgcn_readlane(me.len, at)};
+        return true;
+    }
+};
 
 // The sequence of a row, for a whole wave; false: padding.
 __device__ __forceinline__ bool paged_row(const PagedBatch& b, int row, int& s, PagedSeq& q)

@@ -151,7 +151,7 @@ __global__ __launch_bounds__(16 * LN) void paged_append_kernel(const PagedAppend
     int s, g;
     PagedSeq q;
     auto count = [](const PagedSeq& q) { return (q.len - 1) / 16 - (q.len - q.n) / 16 + 1; };
-    if (!paged_unit(b, job, count, s, g, q)) return;
+    if (!PagedUnits(b, count).find(job, s, g, q)) return;
     const int t0 = ((q.len - q.n) / 16 + g) * 16;       // the group's first token
     const int start = max(q.len - q.n - t0, 0), end = min(q.len - t0, 16);   // of it the pass brings start .. end - 1
     const int page = paged_page(b, s, t0);

@@ -25,7 +25,7 @@ namespace ql {
 
 namespace {
 
-constexpr int kBlock = 64;               // tokens of a block; pages are whole blocks
+constexpr int kBlock = 64;               // tokens of a block of a prompt's kernel; pages are whole blocks
 constexpr int kPairs = 16;
 constexpr float kRaise = 7.f;            // log2 that scores may rise above the running reference before it is raised
 constexpr float kPScale = 256.f;         // parts of P: 2^8 P, at most 2^15
@@ -56,10 +56,14 @@ struct Piece {
 
 __device__ __forceinline__ bool few(const PagedAttnArgs& a, const PagedSeq& q) { return q.n * a.G <= a.few; }
 __device__ __forceinline__ int tiles_of(const PagedAttnArgs& a, const PagedSeq& q) { return (q.n * a.G + kPairs - 1) / kPairs; }
-__device__ __forceinline__ int blocks_of(const PagedSeq& q) { return (q.len + kBlock - 1) / kBlock; }
+template <int BLOCK>
+__device__ __forceinline__ int blocks_of(const PagedSeq& q) { return (q.len + BLOCK - 1) / BLOCK; }
+// the blocks of a range of the `ranges` that `total` are dealt in, a multiple of the workgroup's waves
+template <int WAVES>
+__device__ __forceinline__ long long per_range(const PagedAttnArgs& a, long long total) { return ((total + a.ranges - 1) / a.ranges + WAVES - 1) / WAVES * WAVES; }
 
 // A wave's blocks on the VALU, into the sums' own layout: lane (i, g) has pair i, columns 16 ct + 4 g + r. The four lanes of a pair share a dot product.
-template <bool F8, typename Q, int CT>
+template <bool F8, typename Q, int CT, int BLOCK>
 __device__ __forceinline__ void paged_again(const PagedAttnArgs& a, const Piece& p, int kvh, size_t q_row, int last, int first, int step, float& mr, float& l, f32x4 (&acc)[CT])
 {
     typedef PagedLayout<F8 ? 1 : 2> Lay;
@@ -71,11 +75,11 @@ __device__ __forceinline__ void paged_again(const PagedAttnArgs& a, const Piece&
     for (int c = 0; c < CT; c++) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
     for (int b = first; b < p.b1; b += step) {
-        const int t0 = b * kBlock, page = paged_page(a.b, p.s, t0), in_page = t0 & ((1 << a.b.log_page) - 1);
+        const int t0 = b * BLOCK, page = paged_page(a.b, p.s, t0), in_page = t0 & ((1 << a.b.log_page) - 1);
         if (page < 0) continue;
         const size_t head = (size_t)page * a.KV + kvh, base = (head << a.b.log_page) * D, sc0 = (head << (a.b.log_page - 4)) + (in_page >> 4);
 #pragma unroll 1
-        for (int i = 0; i < kBlock && t0 + i < p.q.len; i++) {
+        for (int i = 0; i < BLOCK && t0 + i < p.q.len; i++) {
             const bool seen = t0 + i <= last;
             float sc = 0.f;
 #pragma unroll 1
@@ -192,6 +196,7 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
 {
     using C = DecodeTile<F8, Q, DP>;
     typedef PagedLayout<F8 ? 1 : 2> Lay;
+    constexpr int kKT = F8 ? 4 : 2, kTokens = 16 * kKT;    // tiles of 16 tokens, tokens of a block: V's that lie together
     __shared__ __attribute__((aligned(16))) float merge[WAVES * kPairs * C::kMerge];
     __shared__ float stat[2][WAVES][kPairs], row_inv[kPairs];
     __shared__ int row_at[kPairs];
@@ -201,22 +206,19 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
     const int kvh = blockIdx.x % a.KV, w = blockIdx.x / a.KV;
 
     // this workgroup's range [at, end) of all sequences' blocks, or of their tiles where each is done whole (a.whole)
-    auto count = [&](const PagedSeq& q) { return few(a, q) ? tiles_of(a, q) * (a.whole ? 1 : blocks_of(q)) : 0; };
-    long long at, end;
-    if (a.whole) {
-        at = w;
-        end = w + 1;
-    } else {
-        const long long total = paged_total(b, count);
-        const long long per = (max((total + a.ranges - 1) / a.ranges, 1ll) + WAVES - 1) / WAVES * WAVES;
+    auto count = [&](const PagedSeq& q) { return few(a, q) ? tiles_of(a, q) * (a.whole ? 1 : blocks_of<kTokens>(q)) : 0; };
+    PagedUnits units(b, count);
+    long long at = w, end = w + 1;
+    if (!a.whole) {
+        const long long total = units.total(), per = per_range<WAVES>(a, total);
         at = w * per;
         end = min(at + per, total);
     }
     while (at < end) {
         Piece p;
         int local;
-        if (!paged_unit(b, at, count, p.s, local, p.q)) return;
-        p.nb = blocks_of(p.q);
+        if (!units.find(at, p.s, local, p.q)) return;
+        p.nb = blocks_of<kTokens>(p.q);
         if (a.whole) {
             p.r0 = kPairs * local;
             p.b0 = 0;
@@ -244,26 +246,26 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
         // The wave's blocks first, first + WAVES, ...; lane j knows the page of number (base + j) of them
         const int first = p.b0 + wave, mine = first < p.b1 ? (p.b1 - first + WAVES - 1) / WAVES : 0;
         int pages = 0;
-        u32x4 kraw[4][C::kUnits], vraw[C::kVB][C::kCT];
+        u32x4 kraw[kKT][C::kUnits], vraw[C::kCT];
         float ks[4], vs[4], vref = 0.f;
         struct At {
             size_t head;
             int in_page, t0, lim;                           // lim: tokens of the block that a row may see
         };
         auto block = [&](int k) {
-            if ((k & 63) == 0) pages = k + lane < mine ? paged_page(b, p.s, (first + (k + lane) * WAVES) * kBlock) : -1;
+            if ((k & 63) == 0) pages = k + lane < mine ? paged_page(b, p.s, (first + (k + lane) * WAVES) * kTokens) : -1;
             const int page = __builtin_amdgcn_readlane(pages, k & 63);
             At x;
-            x.t0 = (first + k * WAVES) * kBlock;
+            x.t0 = (first + k * WAVES) * kTokens;
             x.in_page = x.t0 & ((1 << b.log_page) - 1);
-            x.lim = page < 0 ? 0 : min(kBlock, p.q.len - x.t0);
+            x.lim = page < 0 ? 0 : min(kTokens, p.q.len - x.t0);
             x.head = (size_t)max(page, 0) * a.KV + kvh;
             return x;
         };
         auto load_k = [&](const At& x) {
             const u32x4* k = reinterpret_cast<const u32x4*>(static_cast<const char*>(a.k) + ((x.head << b.log_page) + x.in_page) * D * (F8 ? 1 : 2));
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++)
+            for (int kt = 0; kt < kKT; kt++)
 #pragma unroll
                 for (int c = 0; c < C::kUnits; c++) {
                     const int unit = 4 * c + g;             // D / kUnit units of 16 tokens
@@ -279,10 +281,8 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
         auto load_v = [&](const At& x) {
             const u32x4* v = reinterpret_cast<const u32x4*>(static_cast<const char*>(a.v) + ((x.head << b.log_page) + x.in_page) * D * (F8 ? 1 : 2));
 #pragma unroll
-            for (int h = 0; h < C::kVB; h++)
-#pragma unroll
-                for (int c = 0; c < C::kCT; c++)
-                    if (16 * c < D) vraw[h][c] = ld_global(v + h * 4 * D + c * 64 + lane);
+            for (int c = 0; c < C::kCT; c++)
+                if (16 * c < D) vraw[c] = ld_global(v + c * 64 + lane);
         };
         At now = block(0);
         if (mine > 0) load_k(now);
@@ -293,9 +293,9 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
             if constexpr (F8)
 #pragma unroll
                 for (int i = 0; i < 4; i++) fk[i] = f * ks[i], vb[i] = vs[i];
-            f32x4 s[4];
+            f32x4 s[kKT];
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++) {
+            for (int kt = 0; kt < kKT; kt++) {
                 f32x4 hi = {0.f, 0.f, 0.f, 0.f}, lo = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int t = 0; t < C::kSteps; t++) {
@@ -316,17 +316,17 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
                 now = block(k + 1);
                 load_k(now);
             }
-            if (x.lim < kBlock || x.t0 + kBlock - 1 > all) {
+            if (x.lim < kTokens || x.t0 + kTokens - 1 > all) {
                 const int see = min(x.lim, last - x.t0 + 1);
 #pragma unroll
-                for (int kt = 0; kt < 4; kt++)
+                for (int kt = 0; kt < kKT; kt++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
                         if (16 * kt + 4 * g + i >= see) s[kt][i] = -INFINITY;
             }
             float bm = s[0][0];
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++)
+            for (int kt = 0; kt < kKT; kt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) bm = fmaxf(bm, s[kt][i]);
             bm = pair_max<32>(pair_max<16>(bm));
@@ -345,9 +345,9 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
                     for (int c = 0; c < C::kCT; c++) acc[c] *= al;
             }
             const float ref = mr == -INFINITY ? 0.f : mr;
-            f16x8 pf[2][C::kParts];
+            f16x8 pf[kKT / 2][C::kParts];
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++)
+            for (int kt = 0; kt < kKT; kt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float e = ex2(s[kt][i] - ref);
@@ -357,26 +357,23 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
                     pf[kt >> 1][0][4 * (kt & 1) + i] = hi;
                     if constexpr (!C::kHalf) pf[kt >> 1][1][4 * (kt & 1) + i] = (_Float16)(y - (float)hi);
                 }
-            if (x.lim < kBlock) {                           // what no row sees may hold anything: zero
+            if (x.lim < kTokens)                            // what no row sees may hold anything: zero
 #pragma unroll
-                for (int h = 0; h < C::kVB; h++)
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t keep = v_there<F8>(x.lim, 0, j, g);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t keep = v_there<F8>(x.lim, h, j, g);
-#pragma unroll
-                        for (int c = 0; c < C::kCT; c++) vraw[h][c][j] &= keep;
-                    }
-            }
+                    for (int c = 0; c < C::kCT; c++) vraw[c][j] &= keep;
+                }
             // a block's sums start from zero and are added to the others by the VALU: the matrix unit carries no long sum
 #pragma unroll
             for (int c = 0; c < C::kCT; c++) {
                 if (16 * c >= D) continue;
                 f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int h = 0; h < kKT / 2; h++) {
                     f16x8 v;
-                    if constexpr (F8) v = f8_to_f16(vraw[0][c][2 * h], vraw[0][c][2 * h + 1]);
-                    else v = __builtin_bit_cast(f16x8, vraw[h][c]);
+                    if constexpr (F8) v = f8_to_f16(vraw[c][2 * h], vraw[c][2 * h + 1]);
+                    else v = __builtin_bit_cast(f16x8, vraw[c]);
 #pragma unroll
                     for (int part = C::kParts - 1; part >= 0; part--) o = mfma_16x16x32_f16(v, pf[h][part], o);
                 }
@@ -390,7 +387,7 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
 #pragma unroll
             for (int i = 0; i < 4; i++) odd = fmaf(acc[c][i], 0.f, odd);
         const bool redo = __any(odd != 0.f);
-        if (redo) paged_again<F8, Q, C::kCT>(a, p, kvh, q_row, last, first, WAVES, mr, l, acc);
+        if (redo) paged_again<F8, Q, C::kCT, kTokens>(a, p, kvh, q_row, last, first, WAVES, mr, l, acc);
 
         // the waves' states
         const float unit = redo ? 1.f : F8 ? vref / kPScale : 1.f / kPScale;
@@ -446,68 +443,80 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
     }
 }
 
-// The parts of the pairs whose blocks more than one workgroup had: out = sum_i acc_i 2^(m_i - m) / sum_i l_i 2^(m_i - m). A workgroup a pair;
-// the parts lie with the workgroups of the kv head in a row, the first part in its workgroup's second place, the others in their first.
-template <typename Q, int WAVES>
+// The parts of the pairs whose blocks more than one workgroup had: out = sum_i acc_i 2^(m_i - m) / sum_i l_i 2^(m_i - m). A workgroup has `pairs` of a tile's
+// pairs; the parts lie with the workgroups of the kv head in a row, the first part in its workgroup's second place, the others in their first. A wave
+// makes a pair's weights, then thread (slot, pair, four columns) adds parts slot, slot + slots, ... in order, and the slots are added in order.
+constexpr int kMergeWeights = 4096;
+template <typename Q, int WAVES, int BLOCK>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttnArgs a)
 {
-    __shared__ float wgt[256];
-    __shared__ float red[4][2];
+    __shared__ float wgt[kMergeWeights];
     __shared__ f32x4 sums[256];
     const PagedBatch& b = a.b;
-    const int pair = blockIdx.x, kvh = blockIdx.z, tid = threadIdx.x, lane = tid & 63, D = a.D;
-    auto tiles = [&](const PagedSeq& q) { return few(a, q) ? tiles_of(a, q) : 0; };
-    auto count = [&](const PagedSeq& q) { return few(a, q) ? tiles_of(a, q) * blocks_of(q) : 0; };
-    int s, tile;
-    PagedSeq q;
-    if (!paged_unit(b, blockIdx.y, tiles, s, tile, q)) return;
-    const int r = kPairs * tile + pair;
-    if (r >= q.n * a.G) return;
-    const long long total = paged_total(b, count), before = paged_total(b, count, s) + (long long)tile * blocks_of(q);
-    const long long per = (max((total + a.ranges - 1) / a.ranges, 1ll) + WAVES - 1) / WAVES * WAVES;
-    const int w0 = (int)(before / per), w1 = (int)((before + blocks_of(q) - 1) / per), n = w1 - w0 + 1;
-    if (n == 1) return;
-    // part i of pair: state at .., sums at ..
+    const int pair0 = blockIdx.x * a.merge_pairs, kvh = blockIdx.z, tid = threadIdx.x, lane = tid & 63, D = a.D, unit = blockIdx.y;
+    // the tile, and how many blocks lie before it and in all
+    long long total = 0, before = 0;
+    int tiles = 0, s = -1, tile = 0;
+    PagedSeq q = {0, 0, 0};
+    for (int s0 = 0; s0 < b.S; s0 += 64) {
+        PagedSeq me = {0, 0, 0};
+        if (s0 + lane < b.S) me = paged_seq(b, s0 + lane);
+        const int ct = me.n && few(a, me) ? tiles_of(a, me) : 0, cb = ct ? ct * blocks_of<BLOCK>(me) : 0;
+        const int ut = wave_upto(ct), ub = wave_upto(cb);
+        if (s < 0 && unit < tiles + __builtin_amdgcn_readlane(ut, 63)) {
+            const int at = __builtin_ctzll(__ballot(tiles + ut > unit));
+            s = s0 + at;
+            q = {__builtin_amdgcn_readlane(me.row0, at), __builtin_amdgcn_readlane(me.n, at), __builtin_amdgcn_readlane(me.len, at)};
+            tile = unit - tiles - (__builtin_amdgcn_readlane(ut, at) - __builtin_amdgcn_readlane(ct, at));
+            before = total + __builtin_amdgcn_readlane(ub, at) - __builtin_amdgcn_readlane(cb, at) + (long long)tile * blocks_of<BLOCK>(q);
+        }
+        tiles += __builtin_amdgcn_readlane(ut, 63);
+        total += __builtin_amdgcn_readlane(ub, 63);
+    }
+    if (s < 0) return;
+    const int r0 = kPairs * tile + pair0, pairs = min(min(a.merge_pairs, kPairs - pair0), q.n * a.G - r0);
+    const long long per = per_range<WAVES>(a, total);
+    const int w0 = (int)(before / per), w1 = (int)((before + blocks_of<BLOCK>(q) - 1) / per), n = w1 - w0 + 1;
+    if (n == 1 || pairs <= 0) return;
     const size_t stride = (size_t)kPairs * (D + 2);
     auto part = [&](int i) { return a.ws + ((size_t)((w0 + i) * a.KV + kvh) * 2 + (i == 0)) * stride; };
-    const int nc = D / 4, slot = tid / nc, c = tid - slot * nc, slots = 256 / nc;
-    float top = -INFINITY;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    // 256 parts at a time, each with the reference of all so far
-    for (int i0 = 0; i0 < n; i0 += 256) {
-        const int here = min(256, n - i0);
-        const f32x2 st = tid < here ? ld_global(reinterpret_cast<const f32x2*>(part(i0 + tid) + kPairs * D) + pair) : f32x2{-INFINITY, 0.f};
-        float mx = wave_max(st.x, lane);
-        __syncthreads();
-        if (lane == 0) red[tid >> 6][0] = mx;
-        __syncthreads();
-        mx = fmaxf(fmaxf(red[0][0], red[1][0]), fmaxf(red[2][0], red[3][0]));
-        const float now = fmaxf(top, mx), ref = now == -INFINITY ? 0.f : now, al = top == -INFINITY ? (l != l ? 1.f : 0.f) : ex2(top - ref);
-        const float mi = st.x, li = st.y, e = mi == -INFINITY ? (li != li ? 1.f : 0.f) : ex2(mi - ref);
-        wgt[tid] = e;
-        const float sum = wave_sum(e == 0.f ? 0.f : li * e, lane);
-        if (lane == 0) red[tid >> 6][1] = sum;
-        __syncthreads();
-        l = (al == 0.f ? 0.f : l * al) + ((red[0][1] + red[1][1]) + (red[2][1] + red[3][1]));
-        o *= al;
-        if (slot < slots)
-            for (int i = slot; i < here; i += slots) {
-                const float wi = wgt[i];
-                if (wi == 0.f) continue;
-                const f32x4 x = ld_global(reinterpret_cast<const f32x4*>(part(i0 + i) + pair * D) + c);
-#pragma unroll
-                for (int k = 0; k < 4; k++) o[k] = fmaf(wi, x[k], o[k]);
-            }
-        top = now;
+    for (int p = tid >> 6; p < pairs; p += 4) {
+        float mx = -INFINITY, l = 0.f;
+        for (int i = lane; i < n; i += 64) mx = fmaxf(mx, ld_global(part(i) + kPairs * D + 2 * (pair0 + p)));
+        mx = wave_max(mx, lane);
+        for (int i = lane; i < n; i += 64) {
+            const f32x2 st = ld_global(reinterpret_cast<const f32x2*>(part(i) + kPairs * D) + pair0 + p);
+            const float mi = st.x, li = st.y, e = mi == -INFINITY ? (li != li ? 1.f : 0.f) : ex2(mi - mx);   // NaN: no score is a number
+            wgt[p * n + i] = e;
+            l += e == 0.f ? 0.f : li * e;
+        }
+        l = wave_sum(l, lane);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        for (int i = lane; i < n; i += 64) wgt[p * n + i] *= inv;
     }
-    sums[tid] = o;
     __syncthreads();
-    if (tid >= nc) return;
-    for (int i = 1; i < slots; i++) o += sums[tid + i * nc];
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int m = r / a.G;
-    paged_out(static_cast<Q*>(a.out) + ((size_t)(q.row0 + m) * a.H + kvh * a.G + (r - m * a.G)) * D + 4 * tid, f32x4{o.x * inv, o.y * inv, o.z * inv, o.w * inv});
+    const int nc = D / 4, items = pairs * nc, slots = max(1, 256 / items), slot = tid / items;
+    for (int it = tid - slot * items; it < items; it += 256) {        // more than one round only where a slot is the whole workgroup
+        const int p = it / nc, c = it - p * nc;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+        if (slot < slots)
+#pragma unroll 4
+            for (int i = slot; i < n; i += slots) {
+                const float wi = wgt[p * n + i];
+                const f32x4 x = ld_global(reinterpret_cast<const f32x4*>(part(i) + (pair0 + p) * D) + c);
+#pragma unroll
+                for (int k = 0; k < 4; k++) o[k] = wi == 0.f ? o[k] : fmaf(wi, x[k], o[k]);
+            }
+        if (slots > 1) {
+            sums[tid] = o;
+            __syncthreads();
+        }
+        if (slot > 0) break;
+        if (slots > 1)
+            for (int i = 1; i < slots; i++) o += sums[it + i * items];
+        const int rr = r0 + p, m = rr / a.G;
+        paged_out(static_cast<Q*>(a.out) + ((size_t)(q.row0 + m) * a.H + kvh * a.G + (rr - m * a.G)) * D + 4 * c, o);
+    }
 }
 
 // Sequences of many rows: a workgroup has 64 NT (row, head) pairs of one kv head, 16 NT a wave, and goes through their tokens, 64 at a time, which all its waves
@@ -534,7 +543,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
     int tile;
     // the last tiles first: they see most
     auto count = [&](const PagedSeq& q) { return few(a, q) ? 0 : (q.n * a.G + T::kRows - 1) / T::kRows; };
-    if (!paged_unit(b, tiles - 1 - (int)(blockIdx.x / a.KV), count, p.s, tile, p.q)) return;
+    if (!PagedUnits(b, count).find(tiles - 1 - (int)(blockIdx.x / a.KV), p.s, tile, p.q)) return;
     const int R = p.q.n * a.G, all = p.q.len - p.q.n;       // every row sees the tokens up to `all`
     p.r0 = T::kRows * tile;
     p.nb = (all + (min(p.r0 + T::kRows, R) - 1) / a.G) / kBlock + 1;
@@ -721,7 +730,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
         }
         float unit = F8 ? vref / kPScale : 1.f / kPScale;
         if (__any(odd != 0.f)) {
-            paged_again<F8, Q, C::kCT>(a, p, kvh, q_row[nt], last[nt], p.b0, 1, mr[nt], l[nt], mine);
+            paged_again<F8, Q, C::kCT, kBlock>(a, p, kvh, q_row[nt], last[nt], p.b0, 1, mr[nt], l[nt], mine);
             unit = 1.f;
         }
         const float total = pair_sum<32>(pair_sum<16>(l[nt])), inv = total == 0.f ? 0.f : unit / total;
@@ -741,6 +750,9 @@ uint64_t plan_paged_attention(PagedAttnArgs* a, size_t)
     a->units = most;
     a->whole = a->b.max_len <= 1024;
     a->ranges = std::max(1, 512 / a->KV);
+    // the merge's workgroups: some hundreds, their weights in LDS
+    a->merge_pairs = 1;
+    while (a->merge_pairs < kPairs && (long long)a->units * a->KV * (kPairs / a->merge_pairs) > 512 && 2 * a->merge_pairs * a->ranges <= kMergeWeights) a->merge_pairs *= 2;
     return a->whole || a->ranges == 1 ? 0 : (uint64_t)a->ranges * a->KV * 2 * kPairs * (a->D + 2) * sizeof(float);
 }
 
@@ -753,7 +765,7 @@ hipError_t launch(const PagedAttnArgs& a, hipStream_t stream)
     if (a.D <= 64) hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 64, 4>), grid, dim3(256), 0, stream, a);
     else if (a.D <= 128) hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 128, 4>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 256, 4>), grid, dim3(256), 0, stream, a);
-    if (!a.whole && a.ranges > 1) hipLaunchKernelGGL((paged_merge_kernel<Q, 4>), dim3(kPairs, a.units, a.KV), dim3(256), 0, stream, a);
+    if (!a.whole && a.ranges > 1) hipLaunchKernelGGL((paged_merge_kernel<Q, 4, F8 ? 64 : 32>), dim3(kPairs / a.merge_pairs, a.units, a.KV), dim3(256), 0, stream, a);
     if (a.b.max_rows * a.G > a.few) {
         const int rows = a.D <= 128 ? 128 : 64, tiles = (int)std::min<long long>(((long long)a.b.M * a.G + rows - 1) / rows + a.b.S, (long long)a.b.M * a.G / a.few + 1 + (long long)a.b.M * a.G / rows);
         const dim3 grid(tiles * a.KV);
