@@ -394,9 +394,11 @@ struct PagedAttnArgs {
     PagedBatch b;
     int H, KV, G, D, half;
     float scale;               // fp32(log2(e) / sqrt(D))
-    // plan_paged_attention fills these: most (row, head) pairs of a sequence of few rows, most tiles of 16 of them that such sequences have,
-    // whether each tile is one workgroup's, or all their blocks are dealt to `ranges` workgroups a kv head
-    int few, units, whole, ranges, merge_pairs;
+    // plan_paged_attention fills these. Few: most (row, head) pairs of a sequence of few rows; units: most tiles of 16 of them that such sequences
+    // have; whole: each of these tiles is one workgroup's, or all their blocks are dealt to `ranges` workgroups a kv head and joined by a merge of
+    // merge_pairs pairs a workgroup. Workgroups of both kinds, tiles of many rows that may be done in parts, and where their parts lie in ws, in floats
+    int few, units, whole, ranges, merge, merge_pairs, decode, prompt, join;
+    size_t prompt_ws;
 };
 uint64_t plan_paged_attention(PagedAttnArgs* a, size_t ws_bytes);   // the workspace it needs
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);

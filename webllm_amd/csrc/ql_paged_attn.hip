@@ -1,7 +1,7 @@
 // Attention of a batch's rows over their sequences' pages (ql_paged_attention):
 //   out[m, h] = sum_t p_t V[t] / sum_t p_t,  p_t = exp(q[m, h] . K[t] / sqrt(D) - max)   over the tokens t up to the row's own.
 //
-// paged_decode_kernel: sequences of few rows. A workgroup has 16 (row, head) pairs of one kv head and a range of blocks of 64 tokens; its
+// paged_decode: sequences of few rows. A workgroup has 16 (row, head) pairs of one kv head and a range of blocks of 64 tokens; its
 // four waves take the blocks in turn, K and V from memory to the registers of one wave. The cache lies as the matrix instructions take it: a load
 // is 16 bytes a lane and 1 KB in a row. Scores are computed transposed, S^T = K Q^T (lane = pair, registers = tokens), and what a lane then has of P is the
 // B fragment of O^T = V^T P^T, with nothing crossing lanes: tile kt of S is the block's tokens 16 kt + 4 g + r (g: lane / 16, r: register), and the
@@ -27,11 +27,25 @@ namespace {
 
 constexpr int kBlock = 64;               // tokens of a block of a prompt's kernel; pages are whole blocks
 constexpr int kPairs = 16;
+constexpr int kDecodeWaves = 4;
+constexpr int kPromptParts = 512;         // workgroups up to which the tiles of many rows are done in parts of their tokens
+constexpr int kPromptMost = 8;            // parts of a tile at most
 constexpr float kRaise = 7.f;            // log2 that scores may rise above the running reference before it is raised
-constexpr float kPScale = 256.f;         // parts of P: 2^8 P, at most 2^15
+constexpr float kPLog = 8.f, kPScale = 256.f;   // parts of P: 2^8 P, at most 2^15
 constexpr float kMaxFinite = 3.4028235e38f;
 
 __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The larger of two, NaN if one is: one instruction (fmaxf first makes numbers of what may be signalling). A NaN score leaves the reference as it is and
+// makes its row's sums NaN by its own weight.
+__device__ __forceinline__ float maxi(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+template <int O>
+__device__ __forceinline__ float pair_maxi(float v)
+{
+    const u32pair p = lane_pair<O>(__builtin_bit_cast(uint32_t, v));
+    const uint32_t x = p.x, y = p.y;
+    return maxi(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y));
+}
 
 template <bool F8>
 __device__ __forceinline__ float value_at(const void* p, size_t i)
@@ -111,6 +125,7 @@ struct DecodeTile {
     static constexpr int kCT = DP / 16;                          // tiles of 16 columns
     static constexpr int kVB = F8 ? 1 : 2;                       // parts of a block whose tokens of V lie together
     static constexpr int kMerge = DP + 4;                        // floats of a row of the merge buffer
+    static constexpr int kMergeBytes = kDecodeWaves * kPairs * (kMerge + 2) * 4 + kPairs * 8;
     // the column of element e of step t of a K or Q fragment, lane group g
     static __device__ __forceinline__ int col(int t, int g) { return F8 ? 64 * (t >> 1) + 16 * g + 8 * (t & 1) : 32 * t + 8 * g; }
 };
@@ -191,19 +206,20 @@ __device__ __forceinline__ void load_to_lds(const void* from, void* to)
 #endif
 }
 
-template <bool F8, typename Q, int DP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_kernel(const PagedAttnArgs a)
+template <bool F8, typename Q, int DP, int WAVES, bool FULL>
+__device__ __forceinline__ void paged_decode(const PagedAttnArgs& a, float* merge, int wg)
 {
     using C = DecodeTile<F8, Q, DP>;
     typedef PagedLayout<F8 ? 1 : 2> Lay;
     constexpr int kKT = F8 ? 4 : 2, kTokens = 16 * kKT;    // tiles of 16 tokens, tokens of a block: V's that lie together
-    __shared__ __attribute__((aligned(16))) float merge[WAVES * kPairs * C::kMerge];
-    __shared__ float stat[2][WAVES][kPairs], row_inv[kPairs];
-    __shared__ int row_at[kPairs];
-    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4, D = a.D;
+    // all of LDS is one variable of the kernel's: with several, the compiler takes the reads of LDS in paged_prompt to meet the loads on their way there
+    auto& stat = *reinterpret_cast<float(*)[2][WAVES][kPairs]>(merge + WAVES * kPairs * C::kMerge);
+    float* const row_inv = merge + WAVES * kPairs * (C::kMerge + 2);
+    int* const row_at = reinterpret_cast<int*>(row_inv + kPairs);
+    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4, D = FULL ? DP : a.D;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const PagedBatch& b = a.b;
-    const int kvh = blockIdx.x % a.KV, w = blockIdx.x / a.KV;
+    const int kvh = wg % a.KV, w = wg / a.KV;
 
     // this workgroup's range [at, end) of all sequences' blocks, or of their tiles where each is done whole (a.whole)
     auto count = [&](const PagedSeq& q) { return few(a, q) ? tiles_of(a, q) * (a.whole ? 1 : blocks_of<kTokens>(q)) : 0; };
@@ -328,8 +344,8 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
 #pragma unroll
             for (int kt = 0; kt < kKT; kt++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) bm = fmaxf(bm, s[kt][i]);
-            bm = pair_max<32>(pair_max<16>(bm));
+                for (int i = 0; i < 4; i++) bm = maxi(bm, s[kt][i]);
+            bm = pair_maxi<32>(pair_maxi<16>(bm));
             if (__any(bm > mr + kRaise)) {
                 const float mn = fmaxf(mr, bm), al = ex2(mr - (mn == -INFINITY ? 0.f : mn));
                 mr = mn;
@@ -410,7 +426,7 @@ __global__ __launch_bounds__(64 * WAVES, DP > 128 ? 1 : 2) void paged_decode_ker
             *reinterpret_cast<f32x4*>(merge + (wave * kPairs + i16) * C::kMerge + 16 * c + 4 * g) = v;
         }
         const bool cut = p.b0 > 0 || p.b1 < p.nb;
-        float* const part = a.ws + ((size_t)blockIdx.x * 2 + (p.b0 == 0)) * (kPairs * (D + 2));
+        float* const part = a.ws + ((size_t)wg * 2 + (p.b0 == 0)) * (kPairs * (D + 2));
         if (tid < kPairs) {
             float top = stat[0][0][tid], total = 0.f;
 #pragma unroll
@@ -521,34 +537,89 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttnArgs a)
 
 // Sequences of many rows: a workgroup has 64 NT (row, head) pairs of one kv head, 16 NT a wave, and goes through their tokens, 64 at a time, which all its waves
 // read from LDS; the next 64 are on their way there meanwhile, as they lie in memory. Scores, softmax and products as above.
+// Their tiles come the longest first where a wave's lanes hold all sequences, and in parts of their tokens where there are few of them; paged_join_kernel joins
+// the parts.
+struct PromptTiles {
+    const PagedAttnArgs& a;
+    const int rows;                                         // pairs of a tile
+    struct Count {
+        const PagedAttnArgs& a;
+        int rows;
+        __device__ __forceinline__ int operator()(const PagedSeq& q) const { return few(a, q) ? 0 : (q.n * a.G + rows - 1) / rows; }
+    };
+    PagedUnits<Count> units;
+    long long total;
+    int most;                                               // parts of a tile at most
+
+    __device__ __forceinline__ PromptTiles(const PagedAttnArgs& a, int rows) : a(a), rows(rows), units(a.b, Count{a, rows})
+    {
+        total = units.total();
+        most = total > 0 ? (int)max(1ll, min(kPromptParts / (total * a.KV), (long long)kPromptMost)) : 1;
+    }
+    // tile number j as a piece, whole; in how many parts it is done
+    __device__ __forceinline__ bool find(long long j, Piece& p, int& parts)
+    {
+        if (j >= total) return false;
+        int tile;
+        if (a.b.S > 64) {
+            if (!units.find(total - 1 - j, p.s, tile, p.q)) return false;
+        } else {
+            const PagedSeq me = units.me;
+            const int mine = units.c, all = me.len - me.n;
+            // the lane's sequence's tiles of less than x blocks: those whose last row's token lies before block x - 1
+            auto below = [&](int x) {
+                const int y = (x - 1) * kBlock - all;
+                return y <= 0 ? 0 : y >= me.n ? mine : min(mine, y * a.G / rows);
+            };
+            auto from = [&](int x) { return (int)total - __builtin_amdgcn_readlane(wave_upto(below(x)), 63); };   // all tiles of x blocks or more
+            int lo = 1, hi = (a.b.max_len + kBlock - 1) / kBlock + 1;
+            while (hi - lo > 1) {
+                const int x = (lo + hi) >> 1;
+                if (from(x) > j) lo = x;
+                else hi = x;
+            }
+            const int first = below(lo), c = below(lo + 1) - first, upto = wave_upto(c), k = (int)j - from(lo + 1), at = __builtin_ctzll(__ballot(upto > k));
+            p.s = at;
+            p.q = {__builtin_amdgcn_readlane(me.row0, at), __builtin_amdgcn_readlane(me.n, at), __builtin_amdgcn_readlane(me.len, at)};
+            tile = __builtin_amdgcn_readlane(first, at) + k - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(c, at));
+        }
+        p.r0 = rows * tile;
+        p.nb = (p.q.len - p.q.n + (min(p.r0 + rows, p.q.n * a.G) - 1) / a.G) / kBlock + 1;
+        p.b0 = 0;
+        p.b1 = p.nb;
+        parts = max(1, min(most, p.nb / 4));
+        return true;
+    }
+};
+
 template <bool F8, typename Q, int DP, int NT>
 struct PromptTile {
     using C = DecodeTile<F8, Q, DP>;
     static constexpr int kWaves = 4, kRows = 16 * NT * kWaves;
     static constexpr int kBytes = kBlock * DP * (F8 ? 1 : 2);    // of K or V of a block
+    static constexpr int kLds = 4 * kBytes > C::kMergeBytes ? 2 * kBytes : C::kMergeBytes / 2;   // half of what a workgroup of either kind has
 };
 
-template <bool F8, typename Q, int DP, int NT>
-__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(const PagedAttnArgs a)
+template <bool F8, typename Q, int DP, int NT, bool FULL>
+__device__ __forceinline__ void paged_prompt(const PagedAttnArgs& a, char (&lds)[2][PromptTile<F8, Q, DP, NT>::kLds], int wg)
 {
     using C = DecodeTile<F8, Q, DP>;
     using T = PromptTile<F8, Q, DP, NT>;
     typedef PagedLayout<F8 ? 1 : 2> Lay;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][T::kBytes];
-    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4, D = a.D;
+    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4, D = FULL ? DP : a.D;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const PagedBatch& b = a.b;
-    const int kvh = blockIdx.x % a.KV, tiles = gridDim.x / a.KV;
+    const int kvh = wg % a.KV;
     Piece p;
-    int tile;
-    // the last tiles first: they see most
-    auto count = [&](const PagedSeq& q) { return few(a, q) ? 0 : (q.n * a.G + T::kRows - 1) / T::kRows; };
-    if (!PagedUnits(b, count).find(tiles - 1 - (int)(blockIdx.x / a.KV), p.s, tile, p.q)) return;
+    int parts;
+    {
+        PromptTiles tiles(a, T::kRows);
+        const int number = wg / a.KV, part = number % tiles.most;
+        if (!tiles.find(number / tiles.most, p, parts) || part >= parts) return;
+        p.b0 = (int)((long long)p.nb * part / parts);
+        p.b1 = (int)((long long)p.nb * (part + 1) / parts);
+    }
     const int R = p.q.n * a.G, all = p.q.len - p.q.n;       // every row sees the tokens up to `all`
-    p.r0 = T::kRows * tile;
-    p.nb = (all + (min(p.r0 + T::kRows, R) - 1) / a.G) / kBlock + 1;
-    p.b0 = 0;
-    p.b1 = p.nb;
     const int low = all + p.r0 / a.G;                       // every row of the tile sees the tokens up to it
 
     size_t q_row[NT];
@@ -562,12 +633,15 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
         last[nt] = all + row;
         f[nt] = load_q<C>(static_cast<const Q*>(a.q) + q_row[nt], g, D, a.scale, qf[nt]);
     }
-    f32x4 acc[C::kCT][NT];
+    const _Float16 one = (_Float16)1.f;
+    const f16x8 ones = {one, one, one, one, one, one, one, one};
+    f32x4 acc[C::kCT][NT], ls[NT];                          // ls, l: the sums of P, of fp16 rows by the matrix unit, in every register
     float mr[NT], l[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
         mr[nt] = -INFINITY;
         l[nt] = 0.f;
+        ls[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < C::kCT; c++) acc[c][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
@@ -575,16 +649,25 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
     float ks[4], vs[4], vref = 0.f;
     const int chunks = D * (F8 ? 1 : 2) / 16;               // of 1 KB, of K or V of a block
     auto page_of = [&](int k) {
-        if ((k & 63) == 0) pages = k + lane < p.b1 ? paged_page(b, p.s, (k + lane) * kBlock) : -1;
-        return __builtin_amdgcn_readlane(pages, k & 63);
+        const int r = (k - p.b0) & 63;
+        if (r == 0) pages = k + lane < p.b1 ? paged_page(b, p.s, (k + lane) * kBlock) : -1;
+        return __builtin_amdgcn_readlane(pages, r);
     };
-    auto fetch = [&](int k, int page, int buf) {
+    auto fetch = [&](int k, int page) {
+        char* const to = lds[k & 1];
         const int in_page = (k * kBlock) & ((1 << b.log_page) - 1);
         const size_t head = (size_t)max(page, 0) * a.KV + kvh, at = ((head << b.log_page) + in_page) * D * (F8 ? 1 : 2);
-        for (int c = wave; c < 2 * chunks; c += T::kWaves) {
-            const bool v = c >= chunks;
-            const int cc = v ? c - chunks : c;
-            load_to_lds(static_cast<const char*>(v ? a.v : a.k) + at + cc * 1024 + lane * 16, &lds[buf][v][cc * 1024]);
+        // an address that the wave shares, the lane's own part of it, and an LDS address per KB
+        const uint32_t mine = 16 * lane;
+        const char* const kp = static_cast<const char*>(a.k) + at;
+        const char* const vp = static_cast<const char*>(a.v) + at;
+#pragma unroll
+        for (int c = 0; c < (DP * (F8 ? 1 : 2) / 16 + T::kWaves - 1) / T::kWaves; c++) {
+            const int u = wave + T::kWaves * c;
+            if ((FULL && DP * (F8 ? 1 : 2) / 16 % T::kWaves == 0) || u < chunks) {
+                load_to_lds(kp + u * 1024 + mine, to + u * 1024);
+                load_to_lds(vp + u * 1024 + mine, to + T::kBytes + u * 1024);
+            }
         }
         if constexpr (F8) {
             const float* ss = a.k_scale + (head << (b.log_page - 4)) + (in_page >> 4);
@@ -593,24 +676,35 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
             for (int i = 0; i < 4; i++) ks[i] = ld_global(ss + i), vs[i] = ld_global(sv + i);
         }
     };
-    int page = page_of(0);
-    fetch(0, page, 0);
-    for (int k = 0; k < p.b1; k++) {
-        const int buf = k & 1, t0 = k * kBlock, lim = page < 0 ? 0 : min(kBlock, p.q.len - t0);
+    int page = page_of(p.b0);
+    fetch(p.b0, page);
+    for (int k = p.b0; k < p.b1; k++) {
+        char* const from = lds[k & 1];
+        const int t0 = k * kBlock, lim = page < 0 ? 0 : min(kBlock, p.q.len - t0);
         // this block has arrived, and every wave is done with the one that the next takes the place of
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x70);                   // vmcnt(0) lgkmcnt(0), in a form that the compiler counts
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        if (lim < kBlock) {                                 // V that no row sees may hold anything: zero
+            for (int u = tid; u < 4 * chunks * 16; u += 64 * T::kWaves) {
+                u32x4* w = reinterpret_cast<u32x4*>(from + T::kBytes) + u;
+                const int h = F8 ? 0 : u / (4 * D);
+#pragma unroll
+                for (int j = 0; j < 4; j++) (*w)[j] &= v_there<F8>(lim, h, j, u >> 4 & 3);
+            }
+            __syncthreads();
+        }
         float kss[4], vss[4];
         if constexpr (F8)
 #pragma unroll
-            for (int i = 0; i < 4; i++) kss[i] = ks[i], vss[i] = vs[i];
+            for (int i = 0; i < 4; i++) kss[i] = 16 * i < lim ? ks[i] : 1.f, vss[i] = vs[i];   // groups without a token may hold anything
         if (k + 1 < p.b1) {
             page = page_of(k + 1);
-            fetch(k + 1, page, buf ^ 1);
+            fetch(k + 1, page);
         }
-        const u32x4* const kl = reinterpret_cast<const u32x4*>(lds[buf][0]) + lane;
-        const u32x4* const vl = reinterpret_cast<const u32x4*>(lds[buf][1]) + lane;
+        const u32x4* const kl = reinterpret_cast<const u32x4*>(from) + lane;
+        const u32x4* const vl = reinterpret_cast<const u32x4*>(from + T::kBytes) + lane;
         f32x4 s[4][NT];
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
@@ -634,9 +728,9 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) s[kt][nt][i] = (C::kHalf ? hi[nt][i] : fmaf(lo[nt][i], 1.f / 2048.f, hi[nt][i])) * (F8 ? f[nt] * kss[kt] : f[nt]);
+                for (int i = 0; i < 4; i++) s[kt][nt][i] = C::kHalf ? hi[nt][i] : fmaf(lo[nt][i], 1.f / 2048.f, hi[nt][i]);
         }
-        if (lim < kBlock || t0 + kBlock - 1 > low)
+        if (lim < kBlock || t0 + kBlock - 1 > low)          // some row sees not all
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 const int see = min(lim, last[nt] - t0 + 1) - 4 * g;
@@ -650,12 +744,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
         bool up = false;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            bm[nt] = s[0][nt][0];
+            float mk[4];
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) bm[nt] = fmaxf(bm[nt], s[kt][nt][i]);
-            bm[nt] = pair_max<32>(pair_max<16>(bm[nt]));
+            for (int kt = 0; kt < 4; kt++) mk[kt] = maxi(maxi(s[kt][nt][0], s[kt][nt][1]), maxi(s[kt][nt][2], s[kt][nt][3])) * (F8 ? kss[kt] : 1.f);
+            bm[nt] = pair_maxi<32>(pair_maxi<16>(maxi(maxi(mk[0], mk[1]), maxi(mk[2], mk[3])))) * f[nt];
             up = up || bm[nt] > mr[nt] + kRaise;
         }
         if (__any(up))
@@ -664,6 +756,7 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
                 const float mn = fmaxf(mr[nt], bm[nt]), al = ex2(mr[nt] - (mn == -INFINITY ? 0.f : mn));
                 mr[nt] = mn;
                 l[nt] *= al;
+                ls[nt] *= al;
 #pragma unroll
                 for (int c = 0; c < C::kCT; c++) acc[c][nt] *= al;
             }
@@ -679,18 +772,39 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
         f16x8 pf[2][NT][C::kParts];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const float ref = mr[nt] == -INFINITY ? 0.f : mr[nt];
+            const float ref = (mr[nt] == -INFINITY ? 0.f : mr[nt]) - kPLog;
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++)
+            for (int kt = 0; kt < 4; kt++) {
+                const float fk = F8 ? f[nt] * kss[kt] : f[nt];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float e = ex2(s[kt][nt][i] - ref);
-                    l[nt] += e;
-                    const float y = e * (F8 ? kPScale * rv[kt] : kPScale);
-                    const _Float16 hi = (_Float16)y;
-                    pf[kt >> 1][nt][0][4 * (kt & 1) + i] = hi;
-                    if constexpr (!C::kHalf) pf[kt >> 1][nt][1][4 * (kt & 1) + i] = (_Float16)(y - (float)hi);
+                    const float e = ex2(fmaf(s[kt][nt][i], fk, -ref));
+                    if constexpr (C::kHalf) {
+                        pf[kt >> 1][nt][0][4 * (kt & 1) + i] = (_Float16)e;
+                    } else {
+                        l[nt] += e;
+                        const float y = F8 ? e * rv[kt] : e;
+                        const _Float16 hi = (_Float16)y;
+                        pf[kt >> 1][nt][0][4 * (kt & 1) + i] = hi;
+                        pf[kt >> 1][nt][1][4 * (kt & 1) + i] = (_Float16)(y - (float)hi);
+                    }
                 }
+            }
+        }
+        if constexpr (C::kHalf) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) ls[nt] = mfma_16x16x32_f16(ones, pf[h][nt][0], ls[nt]);   // of P as it is rounded
+            if constexpr (F8) {
+                if (rv[0] != 1.f || rv[1] != 1.f || rv[2] != 1.f || rv[3] != 1.f)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) pf[kt >> 1][nt][0][4 * (kt & 1) + i] *= (_Float16)rv[kt];
+            }
         }
 #pragma unroll
         for (int c = 0; c < C::kCT; c++) {
@@ -698,14 +812,10 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
             u32x4 w[C::kVB];
 #pragma unroll
             for (int h = 0; h < C::kVB; h++) w[h] = vl[h * 4 * D + c * 64];
-            if (lim < kBlock)                               // what no row sees may hold anything: zero
-#pragma unroll
-                for (int h = 0; h < C::kVB; h++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) w[h][j] &= v_there<F8>(lim, h, j, g);
+            // fp32 rows: a block's sums start from zero and are added to the others by the VALU: the matrix unit carries no long sum
             f32x4 o[NT];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) o[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int nt = 0; nt < NT; nt++) o[nt] = C::kHalf ? acc[c][nt] : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const f16x8 v = F8 ? f8_to_f16(w[0][2 * h], w[0][2 * h + 1]) : __builtin_bit_cast(f16x8, w[F8 ? 0 : h]);
@@ -715,12 +825,12 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
                     for (int nt = 0; nt < NT; nt++) o[nt] = mfma_16x16x32_f16(v, pf[h][nt][part], o[nt]);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) acc[c][nt] += o[nt];
+            for (int nt = 0; nt < NT; nt++) acc[c][nt] = C::kHalf ? o[nt] : acc[c][nt] + o[nt];
         }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-        float odd = l[nt] * 0.f;                            // NaN if a sum is not finite
+        float odd = (C::kHalf ? ls[nt][0] : l[nt]) * 0.f;   // NaN if a sum is not finite
         f32x4 mine[C::kCT];
 #pragma unroll
         for (int c = 0; c < C::kCT; c++) {
@@ -728,60 +838,155 @@ __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_prompt_kernel(con
 #pragma unroll
             for (int i = 0; i < 4; i++) odd = fmaf(mine[c][i], 0.f, odd);
         }
-        float unit = F8 ? vref / kPScale : 1.f / kPScale;
+        float unit = (F8 ? vref : 1.f) / kPScale, total = (C::kHalf ? ls[nt][0] : pair_sum<32>(pair_sum<16>(l[nt]))) * (1.f / kPScale);
         if (__any(odd != 0.f)) {
             paged_again<F8, Q, C::kCT, kBlock>(a, p, kvh, q_row[nt], last[nt], p.b0, 1, mr[nt], l[nt], mine);
             unit = 1.f;
+            total = pair_sum<32>(pair_sum<16>(l[nt]));
         }
-        const float total = pair_sum<32>(pair_sum<16>(l[nt])), inv = total == 0.f ? 0.f : unit / total;
-        const bool there = p.r0 + 16 * (NT * wave + nt) + i16 < R;
+        const int pair = 16 * (NT * wave + nt) + i16;
+        if (parts > 1) {                                    // a part's sums and state
+            float* const ws = a.ws + a.prompt_ws + (size_t)wg * (T::kRows * (D + 2));
 #pragma unroll
-        for (int c = 0; c < C::kCT; c++)
-            if (there && 16 * c < D) paged_out(static_cast<Q*>(a.out) + q_row[nt] + 16 * c + 4 * g, f32x4{mine[c][0] * inv, mine[c][1] * inv, mine[c][2] * inv, mine[c][3] * inv});
+            for (int c = 0; c < C::kCT; c++)
+                if (16 * c < D) st_global(reinterpret_cast<f32x4*>(ws + pair * D + 16 * c + 4 * g), f32x4{mine[c][0] * unit, mine[c][1] * unit, mine[c][2] * unit, mine[c][3] * unit});
+            if (g == 0) st_global(reinterpret_cast<f32x2*>(ws + T::kRows * D) + pair, f32x2{mr[nt], total});
+        } else {
+            const float inv = total == 0.f ? 0.f : unit / total;
+            const bool there = p.r0 + pair < R;
+#pragma unroll
+            for (int c = 0; c < C::kCT; c++)
+                if (there && 16 * c < D) paged_out(static_cast<Q*>(a.out) + q_row[nt] + 16 * c + 4 * g, f32x4{mine[c][0] * inv, mine[c][1] * inv, mine[c][2] * inv, mine[c][3] * inv});
+        }
     }
+}
+
+// The parts of a tile of many rows, as paged_merge_kernel: a workgroup has a quarter of a tile's pairs.
+template <typename Q, int ROWS>
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a)
+{
+    constexpr int kHere = ROWS / 4;
+    __shared__ float wgt[kHere][kPromptMost];
+    const int kvh = blockIdx.y, tid = threadIdx.x, D = a.D, pair0 = kHere * blockIdx.z;
+    Piece p;
+    int parts;
+    PromptTiles tiles(a, ROWS);
+    if (tiles.most == 1 || !tiles.find(blockIdx.x, p, parts) || parts == 1) return;
+    const int R = p.q.n * a.G, pairs = min(kHere, R - p.r0 - pair0);
+    if (pairs <= 0) return;
+    auto part = [&](int i) { return a.ws + a.prompt_ws + (size_t)(((int)blockIdx.x * tiles.most + i) * a.KV + kvh) * (ROWS * (D + 2)); };
+    if (tid < pairs) {
+        f32x2 st[kPromptMost];
+        float mx = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < kPromptMost; i++) {
+            st[i] = i < parts ? ld_global(reinterpret_cast<const f32x2*>(part(i) + ROWS * D) + pair0 + tid) : f32x2{-INFINITY, 0.f};
+            mx = fmaxf(mx, st[i].x);
+        }
+#pragma unroll
+        for (int i = 0; i < kPromptMost; i++) {
+            const float mi = st[i].x, li = st[i].y, e = mi == -INFINITY ? (li != li ? 1.f : 0.f) : ex2(mi - mx);   // NaN: no score is a number
+            l += e == 0.f ? 0.f : li * e;
+            st[i].x = e;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < kPromptMost; i++) wgt[tid][i] = st[i].x * inv;
+    }
+    __syncthreads();
+    const int nc = D / 4;
+    for (int u = tid; u < pairs * nc; u += 256) {
+        const int pair = u / nc, c = u - pair * nc;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int i = 0; i < parts; i++) {
+            const float w = wgt[pair][i];
+            const f32x4 x = ld_global(reinterpret_cast<const f32x4*>(part(i) + (pair0 + pair) * D) + c);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = w == 0.f ? o[e] : fmaf(w, x[e], o[e]);
+        }
+        const int r = p.r0 + pair0 + pair, m = r / a.G;
+        paged_out(static_cast<Q*>(a.out) + ((size_t)(p.q.row0 + m) * a.H + kvh * a.G + (r - m * a.G)) * D + 4 * c, o);
+    }
+}
+
+// One launch for both: the first a.decode workgroups have the sequences of few rows, whose reads of memory go on beside the others' products
+template <bool F8, typename Q, int DP, int NT, bool FULL>
+__global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_attention_kernel(const PagedAttnArgs a)
+{
+    using T = PromptTile<F8, Q, DP, NT>;
+    __shared__ __attribute__((aligned(16))) char lds[2][T::kLds];
+    if ((int)blockIdx.x < a.decode) paged_decode<F8, Q, DP, kDecodeWaves, FULL>(a, reinterpret_cast<float*>(lds[0]), blockIdx.x);
+    else paged_prompt<F8, Q, DP, NT, FULL>(a, lds, blockIdx.x - a.decode);
+}
+template <bool F8, typename Q, int DP, bool FULL>
+__global__ __launch_bounds__(64 * kDecodeWaves, DP > 128 ? 1 : 2) void paged_decode_kernel(const PagedAttnArgs a)
+{
+    __shared__ __attribute__((aligned(16))) char lds[DecodeTile<F8, Q, DP>::kMergeBytes];
+    paged_decode<F8, Q, DP, kDecodeWaves, FULL>(a, reinterpret_cast<float*>(lds), blockIdx.x);
 }
 
 }  // namespace
 
-uint64_t plan_paged_attention(PagedAttnArgs* a, size_t)
+uint64_t plan_paged_attention(PagedAttnArgs* a, size_t ws_bytes)
 {
+    const long long pairs = (long long)a->b.M * a->G;
     a->few = 4 * kPairs;
-    const int most = std::min<long long>(4ll * a->b.S, a->b.S + (long long)a->b.M * a->G / kPairs);
-    a->units = most;
+    a->units = (int)std::min<long long>(4ll * a->b.S, a->b.S + pairs / kPairs);
     a->whole = a->b.max_len <= 1024;
     a->ranges = std::max(1, 512 / a->KV);
     // the merge's workgroups: some hundreds, their weights in LDS
     a->merge_pairs = 1;
     while (a->merge_pairs < kPairs && (long long)a->units * a->KV * (kPairs / a->merge_pairs) > 512 && 2 * a->merge_pairs * a->ranges <= kMergeWeights) a->merge_pairs *= 2;
-    return a->whole || a->ranges == 1 ? 0 : (uint64_t)a->ranges * a->KV * 2 * kPairs * (a->D + 2) * sizeof(float);
+    a->merge = !a->whole && a->ranges > 1;
+    a->decode = (a->whole ? a->units : a->ranges) * a->KV;
+    a->prompt_ws = a->merge ? (size_t)a->ranges * a->KV * 2 * kPairs * (a->D + 2) : 0;
+    a->prompt = a->join = 0;
+    uint64_t bytes = a->prompt_ws * sizeof(float);
+    if ((long long)a->b.max_rows * a->G > a->few) {
+        const int rows = a->D > 128 ? 64 : 128;
+        // tiles of whole rows, and one more of each sequence of so many rows that it is none of the few
+        const long long tiles = pairs / rows + std::min<long long>(a->b.S, pairs / a->few) + 1;
+        a->prompt = (int)std::max<long long>(tiles * a->KV, kPromptParts);
+        // tiles are done in parts where they have eight blocks and there are so few that two parts of each are no more than kPromptParts
+        if (a->b.max_len > 7 * kBlock && kPromptParts / a->KV >= 2) {
+            a->join = (int)std::min<long long>(tiles, kPromptParts / a->KV / 2);
+            bytes += (uint64_t)kPromptParts * rows * (a->D + 2) * sizeof(float);
+        }
+    }
+    return bytes <= ws_bytes ? bytes : ~0ull;
 }
 
 namespace {
 
-template <bool F8, typename Q>
+template <bool F8, typename Q, int DP, bool FULL>
 hipError_t launch(const PagedAttnArgs& a, hipStream_t stream)
 {
-    const dim3 grid((a.whole ? a.units : a.ranges) * a.KV);
-    if (a.D <= 64) hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 64, 4>), grid, dim3(256), 0, stream, a);
-    else if (a.D <= 128) hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 128, 4>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((paged_decode_kernel<F8, Q, 256, 4>), grid, dim3(256), 0, stream, a);
-    if (!a.whole && a.ranges > 1) hipLaunchKernelGGL((paged_merge_kernel<Q, 4, F8 ? 64 : 32>), dim3(kPairs / a.merge_pairs, a.units, a.KV), dim3(256), 0, stream, a);
-    if (a.b.max_rows * a.G > a.few) {
-        const int rows = a.D <= 128 ? 128 : 64, tiles = (int)std::min<long long>(((long long)a.b.M * a.G + rows - 1) / rows + a.b.S, (long long)a.b.M * a.G / a.few + 1 + (long long)a.b.M * a.G / rows);
-        const dim3 grid(tiles * a.KV);
-        if (a.D <= 64) hipLaunchKernelGGL((paged_prompt_kernel<F8, Q, 64, 2>), grid, dim3(256), 0, stream, a);
-        else if (a.D <= 128) hipLaunchKernelGGL((paged_prompt_kernel<F8, Q, 128, 2>), grid, dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL((paged_prompt_kernel<F8, Q, 256, 1>), grid, dim3(256), 0, stream, a);
-    }
+    constexpr int kNT = DP > 128 ? 1 : 2;
+    if (a.prompt) hipLaunchKernelGGL((paged_attention_kernel<F8, Q, DP, kNT, FULL>), dim3(a.decode + a.prompt), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((paged_decode_kernel<F8, Q, DP, FULL>), dim3(a.decode), dim3(256), 0, stream, a);
+    if (a.merge) hipLaunchKernelGGL((paged_merge_kernel<Q, kDecodeWaves, F8 ? 64 : 32>), dim3(kPairs / a.merge_pairs, a.units, a.KV), dim3(256), 0, stream, a);
+    if (a.join) hipLaunchKernelGGL((paged_join_kernel<Q, 64 * kNT>), dim3(a.join, a.KV, 4), dim3(256), 0, stream, a);
     return hipGetLastError();
+}
+
+template <bool F8, typename Q>
+hipError_t launch_d(const PagedAttnArgs& a, hipStream_t stream)
+{
+    if (a.D == 64) return launch<F8, Q, 64, true>(a, stream);
+    if (a.D == 128) return launch<F8, Q, 128, true>(a, stream);
+    if (a.D == 256) return launch<F8, Q, 256, true>(a, stream);
+    if (a.D < 64) return launch<F8, Q, 64, false>(a, stream);
+    if (a.D < 128) return launch<F8, Q, 128, false>(a, stream);
+    return launch<F8, Q, 256, false>(a, stream);
 }
 
 }  // namespace
 
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream)
 {
-    if (a.k_scale) return a.half ? launch<true, _Float16>(a, stream) : launch<true, float>(a, stream);
-    return a.half ? launch<false, _Float16>(a, stream) : launch<false, float>(a, stream);
+    if (a.k_scale) return a.half ? launch_d<true, _Float16>(a, stream) : launch_d<true, float>(a, stream);
+    return a.half ? launch_d<false, _Float16>(a, stream) : launch_d<false, float>(a, stream);
 }
 
 }  // namespace ql
