@@ -5,7 +5,7 @@
 // workgroups of one row's column ranges each make t for themselves: A comes from L2, and a second launch would cost more.
 //
 // Many rows, two launches: lora_down_kernel makes t of 16 rows, eight waves a part of K each, on the matrix cores, T^T = A x^T
-// (lane = row, registers = ranks), for all projections that read one x; lora_up_kernel has 64 rows and a range of columns, y^T = B t^T. Rows of
+// (lane = row, registers = ranks), for all projections that read one x; lora_up_kernel has 16 rows and 64 columns a wave, y^T = B t^T. Rows of
 // several adapters in one tile: it is gone through once for each adapter, and a row takes its own. fp32 x enters as two fp16 parts (22 bits) under the
 // exponent of the row's 32 columns at a time; t likewise under the row's.
 #include <algorithm>
@@ -91,21 +91,47 @@ __global__ __launch_bounds__(64 * kRowWaves) void lora_row_kernel(const LoraArgs
 // ---- many rows
 
 constexpr int kDownWaves = 8, kDownTiles = 12;   // waves of a workgroup; tiles of 16 ranks that it makes at once
-constexpr int kUpRows = 64, kUpCols = 256;
+constexpr int kUpRows = 32, kUpCols = 256;      // rows of a pass are a multiple; columns of a workgroup
+constexpr int kTwoTiles = 1024;                // rows from which a wave has two tiles of 16 for what it reads of A and B
 
-// the ranks of all projections that read one x, in tiles of 16: tile u is of projection p[u], its first rank r[u]
+// The ranks of all projections that read one x, in tiles of 16
 struct LoraDown {
-    LoraArgs a;
+    struct Tile {
+        const uint16_t* a;         // row of the tile's first rank, of adapter 0
+        const float* scale;
+        float* t;                  // its first rank's column of t [rows, rank]
+        long long step;            // values from an adapter to the next
+        int ranks, rank, n;        // ranks of the tile, of the projection; adapters
+    } tile[kDownTiles];
     const void* x;
-    int K, tiles;
-    short p[kDownTiles], r[kDownTiles];
+    const int32_t* ids;
+    int K, M, tiles, most;         // most: adapters of the projection that has most
 };
 
-// the other rows' adapters of a tile come later: those of `left` that are the first one's
-__device__ __forceinline__ uint64_t next_adapter(int id, uint64_t left, int& which)
+// The adapters of RT tiles of 16 rows, one after the other: bit 16 t + i of `left` is row i of tile t, whose adapter lane i knows in id[t]
+template <int RT>
+__device__ __forceinline__ uint32_t rows_with(const int (&id)[RT], int which)
 {
-    which = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
-    return left & __ballot(id == which);
+    uint32_t m = 0;
+#pragma unroll
+    for (int t = 0; t < RT; t++) m |= (uint32_t)(__ballot(id[t] == which) & 0xFFFF) << (16 * t);
+    return m;
+}
+template <int RT>
+__device__ __forceinline__ uint32_t rows_below(const int (&id)[RT], int n)
+{
+    uint32_t m = 0;
+#pragma unroll
+    for (int t = 0; t < RT; t++) m |= (uint32_t)(__ballot((uint32_t)id[t] < (uint32_t)n) & 0xFFFF) << (16 * t);
+    return m;
+}
+template <int RT>
+__device__ __forceinline__ int first_adapter(const int (&id)[RT], uint32_t left)
+{
+    const int r = __builtin_ctz(left);
+    int which = __builtin_amdgcn_readlane(id[0], r & 15);
+    if (RT > 1 && r >= 16) which = __builtin_amdgcn_readlane(id[RT - 1], r & 15);
+    return which;
 }
 
 // x's two parts: hi + 2^-11 lo of x * s
@@ -121,139 +147,195 @@ __device__ __forceinline__ void split_f16(const float (&x)[8], float s, f16x8& h
 // the power of two that brings mx to [2^14, 2^15)
 __device__ __forceinline__ float scale_of(float mx) { return mx > 0.f && mx <= kMaxFinite ? ldexpf(1.f, min(100, 14 - ilogbf(mx))) : 1.f; }
 
-template <bool HALF>
+// 64 of K at a time: lane group g has 16 of them, a line of each rank's row of A in all, in two products
+template <bool HALF, int TILES, int RT>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDown d)
 {
-    __shared__ f32x4 part[kDownWaves][kDownTiles][64];
-    const int m0 = 16 * blockIdx.x, tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
+    __shared__ f32x4 part[kDownWaves][TILES][64];
+    const int m0 = 16 * RT * blockIdx.x, tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int m = min(m0 + i16, d.a.M - 1), id = m0 + i16 < d.a.M ? ld_global(d.a.ids + m) : -1;
-    int most = 0;
-    for (int u = 0; u < d.tiles; u++) most = max(most, d.a.p[d.p[u]].n);
-    uint64_t left = __ballot((uint32_t)id < (uint32_t)most) & 0xFFFF;
-    const int steps = (d.K + 31) / 32, per = (steps + kDownWaves - 1) / kDownWaves, s0 = wave * per, s1 = min(steps, s0 + per);
+    int id[RT];
+    const char* x[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int m = min(m0 + 16 * t + i16, d.M - 1);
+        id[t] = m0 + 16 * t + i16 < d.M ? ld_global(d.ids + m) : -1;
+        x[t] = static_cast<const char*>(d.x) + (size_t)m * d.K * (HALF ? 2 : 4);
+    }
+    uint32_t left = rows_below(id, d.most);
+    const int steps = (d.K + 63) / 64, per = (steps + kDownWaves - 1) / kDownWaves, s0 = wave * per, s1 = min(steps, s0 + per);
     while (left) {
-        int which;
-        const uint64_t mine = next_adapter(id, left, which);
+        const int which = first_adapter(id, left);
+        const uint32_t mine = left & rows_with(id, which);
         left &= ~mine;
-        f32x4 acc[kDownTiles];
+        const uint16_t* w[TILES];
 #pragma unroll
-        for (int u = 0; u < kDownTiles; u++) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < TILES; u++) {                   // a rank that is not there: the first one's, not stored
+            const LoraDown::Tile& t = d.tile[min(u, d.tiles - 1)];
+            w[u] = t.a + (which < t.n ? which : 0) * t.step + (size_t)(i16 < t.ranks ? i16 : 0) * d.K;
+        }
+        f32x4 acc[TILES][RT];
+#pragma unroll
+        for (int u = 0; u < TILES; u++)
+#pragma unroll
+            for (int t = 0; t < RT; t++) acc[u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int st = s0; st < s1; st++) {
-            const int k = 32 * st + 8 * g;
-            const bool in = k < d.K;
-            f16x8 hi, lo;
-            float up = 1.f;
-            if constexpr (HALF) {
-                hi = in ? __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(d.x) + (size_t)m * d.K + k))) : f16x8{};
-            } else {
-                float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (in) load8(d.x, 0, (size_t)m * d.K + k, x);
-                float mx = 0.f;
+            const int k = 64 * st + 16 * g;
+            const bool in[2] = {k < d.K, k + 8 < d.K};      // K is a multiple of eight
+            u32x4 raw[TILES][2];
 #pragma unroll
-                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[e]));
-                mx = pair_max<32>(pair_max<16>(mx));
-                const float s = scale_of(mx);
-                up = 1.f / s;
-                split_f16(x, s, hi, lo);
+            for (int u = 0; u < TILES; u++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) raw[u][h] = ld_global(reinterpret_cast<const u32x4*>(w[u] + (in[h] ? k + 8 * h : 0)));
+            f16x8 hi[RT][2], lo[RT][2];
+            float up[RT];
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                if constexpr (HALF) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        hi[t][h] = __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(x[t] + 2 * (in[h] ? k + 8 * h : 0))));
+                        if (!in[h]) hi[t][h] = f16x8{};
+                    }
+                } else {
+                    float v[2][8], mx = 0.f;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        load8(x[t], 0, in[h] ? k + 8 * h : 0, v[h]);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            v[h][e] = in[h] ? v[h][e] : 0.f;
+                            mx = fmaxf(mx, fabsf(v[h][e]));
+                        }
+                    }
+                    mx = pair_max<32>(pair_max<16>(mx));
+                    const float s = scale_of(mx);
+                    up[t] = 1.f / s;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) split_f16(v[h], s, hi[t][h], lo[t][h]);
+                }
             }
 #pragma unroll
-            for (int u = 0; u < kDownTiles; u++) {
-                if (u >= d.tiles) continue;
-                const LoraArgs::One& p = d.a.p[d.p[u]];
-                const int r = d.r[u] + i16;
-                const bool there = in && r < p.rank && which < p.n;
-                const f16x8 w = there ? __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(p.a + ((size_t)which * p.rank + r) * p.K + k))) : f16x8{};
-                if constexpr (HALF) {
-                    acc[u] = mfma_16x16x32_f16(w, hi, acc[u]);
-                } else {
-                    f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
-                    ol = mfma_16x16x32_f16(w, lo, ol);
-                    o = mfma_16x16x32_f16(w, hi, o);
+            for (int u = 0; u < TILES; u++) {
+                f16x8 wu[2];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[u][e] = fmaf(fmaf(ol[e], 1.f / 2048.f, o[e]), up, acc[u][e]);
+                for (int h = 0; h < 2; h++) wu[h] = in[h] ? __builtin_bit_cast(f16x8, raw[u][h]) : f16x8{};   // zeros on both sides: 0 * NaN
+#pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    if constexpr (HALF) {
+#pragma unroll
+                        for (int h = 0; h < 2; h++) acc[u][t] = mfma_16x16x32_f16(wu[h], hi[t][h], acc[u][t]);
+                    } else {
+                        f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            ol = mfma_16x16x32_f16(wu[h], lo[t][h], ol);
+                            o = mfma_16x16x32_f16(wu[h], hi[t][h], o);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[u][t][e] = fmaf(fmaf(ol[e], 1.f / 2048.f, o[e]), up[t], acc[u][t][e]);
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int u = 0; u < kDownTiles; u++)
-            if (u < d.tiles) part[wave][u][lane] = acc[u];
-        __syncthreads();
-        for (int u = wave; u < d.tiles; u += kDownWaves) {
-            const LoraArgs::One& p = d.a.p[d.p[u]];
-            f32x4 v = part[0][u][lane];
+        for (int t = 0; t < RT; t++) {
 #pragma unroll
-            for (int k = 1; k < kDownWaves; k++) v += part[k][u][lane];
-            if (!(mine >> i16 & 1) || which >= p.n || d.r[u] + 4 * g >= p.rank) continue;
-            const float s = p.scale ? ld_global(p.scale + which) : 1.f;
-            float* t = d.a.ws + d.a.t_off[d.p[u]] + (size_t)m * p.rank + d.r[u] + 4 * g;
-            st_global(reinterpret_cast<f32x4*>(t), f32x4{v[0] * s, v[1] * s, v[2] * s, v[3] * s});
+            for (int u = 0; u < TILES; u++) part[wave][u][lane] = acc[u][t];
+            __syncthreads();
+            for (int u = wave; u < d.tiles; u += kDownWaves) {
+                const LoraDown::Tile& tl = d.tile[u];
+                f32x4 v = part[0][u][lane];
+#pragma unroll
+                for (int k = 1; k < kDownWaves; k++) v += part[k][u][lane];
+                if ((mine >> (16 * t + i16) & 1) && which < tl.n && 4 * g < tl.ranks) {
+                    const float s = tl.scale ? ld_global(tl.scale + which) : 1.f;
+                    st_global(reinterpret_cast<f32x4*>(tl.t + (size_t)(m0 + 16 * t + i16) * tl.rank + 4 * g), f32x4{v[0] * s, v[1] * s, v[2] * s, v[3] * s});
+                }
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 
-template <int STEPS>
-__global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a, const int proj)
+// A workgroup has 16 RT rows and 256 columns of a projection, a wave 64; the projections' columns lie one behind the other in blockIdx.x
+template <int STEPS, int RT>
+__global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
 {
-    const LoraArgs::One& p = a.p[proj];
     const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int m0 = kUpRows * blockIdx.y, n0 = kUpCols * blockIdx.x + 64 * wave;
-    const float* t = a.ws + a.t_off[proj];
-#pragma unroll 1
-    for (int mt = 0; mt < kUpRows / 16; mt++) {
-        const int m = m0 + 16 * mt + i16;
-        if (m0 + 16 * mt >= a.M) break;
-        const bool row = m < a.M;
-        const int id = row ? ld_global(a.ids + m) : -1;
-        const bool has = (uint32_t)id < (uint32_t)p.n;
-        if (!__any(has) && p.base == p.y) continue;
-        f32x4 y[4];
+    int proj = 0, xb = blockIdx.x;
+    while (xb >= (a.p[proj].N + kUpCols - 1) / kUpCols) xb -= (a.p[proj++].N + kUpCols - 1) / kUpCols;
+    const LoraArgs::One& p = a.p[proj];
+    const int m0 = 16 * RT * blockIdx.y, n0 = kUpCols * xb + 64 * wave;
+    const float* t_in = a.ws + a.t_off[proj];
+    const bool apart = p.base != p.y;
+    int id[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) id[t] = m0 + 16 * t + i16 < a.M ? ld_global(a.ids + m0 + 16 * t + i16) : -1;
+    uint32_t left = rows_below(id, p.n);
+    const uint32_t all = left;
+    if ((!left && !apart) || n0 >= p.N) return;
+    f32x4 y[RT][4];
+    f16x8 hi[RT][STEPS], lo[RT][STEPS];
+    float up[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int m = m0 + 16 * t + i16;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int n = n0 + 16 * j + 4 * g;
-            y[j] = row && n < p.N ? ld_global(reinterpret_cast<const f32x4*>(p.base + (size_t)m * p.N + n)) : f32x4{0.f, 0.f, 0.f, 0.f};
+            y[t][j] = m < a.M && n < p.N ? ld_global(reinterpret_cast<const f32x4*>(p.base + (size_t)m * p.N + n)) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        f16x8 hi[STEPS], lo[STEPS];
-        float mx = 0.f, x[STEPS][8];
+        float mx = 0.f, v[STEPS][8];
 #pragma unroll
         for (int st = 0; st < STEPS; st++) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[st][e] = 0.f;
-            if (has && 32 * st + 8 * g < p.rank) load8(t, 0, (size_t)m * p.rank + 32 * st + 8 * g, x[st]);
+            for (int e = 0; e < 8; e++) v[st][e] = 0.f;
+            if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank) load8(t_in, 0, (size_t)m * p.rank + 32 * st + 8 * g, v[st]);
 #pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[st][e]));
+            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[st][e]));
         }
         mx = pair_max<32>(pair_max<16>(mx));
-        const float s = scale_of(mx), up = 1.f / s;
+        const float s = scale_of(mx);
+        up[t] = 1.f / s;
 #pragma unroll
-        for (int st = 0; st < STEPS; st++) split_f16(x[st], s, hi[st], lo[st]);
-        uint64_t left = __ballot(has) & 0xFFFF;
-        while (left) {
-            int which;
-            const uint64_t mine = next_adapter(id, left, which);
-            left &= ~mine;
+        for (int st = 0; st < STEPS; st++) split_f16(v[st], s, hi[t][st], lo[t][st]);
+    }
+    while (left) {
+        const int which = first_adapter(id, left);
+        const uint32_t mine = left & rows_with(id, which);
+        left &= ~mine;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int n = n0 + 16 * j + i16;
+        for (int j = 0; j < 4; j++) {
+            const int n = n0 + 16 * j + i16;
+            f16x8 w[STEPS];
+#pragma unroll
+            for (int st = 0; st < STEPS; st++) {
+                const int r = 32 * st + 8 * g;
+                w[st] = n < p.N && r < p.rank ? __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(p.b + ((size_t)which * p.N + n) * p.rank + r))) : f16x8{};
+            }
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
                 f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int st = 0; st < STEPS; st++) {
-                    const int r = 32 * st + 8 * g;
-                    const f16x8 w = n < p.N && r < p.rank ? __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(p.b + ((size_t)which * p.N + n) * p.rank + r))) : f16x8{};
-                    ol = mfma_16x16x32_f16(w, lo[st], ol);
-                    o = mfma_16x16x32_f16(w, hi[st], o);
+                    ol = mfma_16x16x32_f16(w[st], lo[t][st], ol);
+                    o = mfma_16x16x32_f16(w[st], hi[t][st], o);
                 }
-                if (mine >> i16 & 1)
+                const bool take = mine >> (16 * t + i16) & 1;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) y[j][e] = fmaf(fmaf(ol[e], 1.f / 2048.f, o[e]), up, y[j][e]);
+                for (int e = 0; e < 4; e++) y[t][j][e] = take ? fmaf(fmaf(ol[e], 1.f / 2048.f, o[e]), up[t], y[t][j][e]) : y[t][j][e];
             }
         }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int m = m0 + 16 * t + i16;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int n = n0 + 16 * j + 4 * g;
-            if (row && n < p.N && (has || p.base != p.y)) st_global(reinterpret_cast<f32x4*>(p.y + (size_t)m * p.N + n), y[j]);
+            if (m < a.M && n < p.N && ((all >> (16 * t + i16) & 1) || apart)) st_global(reinterpret_cast<f32x4*>(p.y + (size_t)m * p.N + n), y[t][j]);
         }
     }
 }
@@ -277,39 +359,61 @@ uint64_t plan_lora(LoraArgs* a, size_t ws_bytes)
 
 namespace {
 
+template <bool HALF, int RT>
+void launch_down(const LoraDown& d, hipStream_t stream)
+{
+    const dim3 grid((d.M + 16 * RT - 1) / (16 * RT)), block(64 * kDownWaves);
+    if (d.tiles <= 1) hipLaunchKernelGGL((lora_down_kernel<HALF, 1, RT>), grid, block, 0, stream, d);
+    else if (d.tiles <= 2) hipLaunchKernelGGL((lora_down_kernel<HALF, 2, RT>), grid, block, 0, stream, d);
+    else if (d.tiles <= 4) hipLaunchKernelGGL((lora_down_kernel<HALF, 4, RT>), grid, block, 0, stream, d);
+    else if (d.tiles <= 8) hipLaunchKernelGGL((lora_down_kernel<HALF, 8, RT>), grid, block, 0, stream, d);
+    else hipLaunchKernelGGL((lora_down_kernel<HALF, kDownTiles, RT>), grid, block, 0, stream, d);
+}
+
+template <int RT>
+void launch_up(const LoraArgs& a, hipStream_t stream)
+{
+    int cols = 0, rank = 0;
+    for (int i = 0; i < a.count; i++) {
+        cols += (a.p[i].N + kUpCols - 1) / kUpCols;
+        rank = std::max(rank, a.p[i].rank);
+    }
+    const dim3 grid(cols, (a.M + 16 * RT - 1) / (16 * RT));
+    if (rank <= 32) hipLaunchKernelGGL((lora_up_kernel<1, RT>), grid, dim3(256), 0, stream, a);
+    else if (rank <= 64) hipLaunchKernelGGL((lora_up_kernel<2, RT>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((lora_up_kernel<4, RT>), grid, dim3(256), 0, stream, a);
+}
+
 hipError_t launch_tiled(const LoraArgs& a, hipStream_t stream)
 {
-    const dim3 tiles((a.M + 15) / 16);
     bool done[kMaxBatch] = {};
     for (int i = 0; i < a.count; i++) {
         if (done[i]) continue;
         LoraDown d;
-        d.a = a;
         d.x = a.p[i].x;
+        d.ids = a.ids;
         d.K = a.p[i].K;
-        d.tiles = 0;
+        d.M = a.M;
+        d.tiles = d.most = 0;
         auto flush = [&] {
-            if (a.half) hipLaunchKernelGGL(lora_down_kernel<true>, tiles, dim3(64 * kDownWaves), 0, stream, d);
-            else hipLaunchKernelGGL(lora_down_kernel<false>, tiles, dim3(64 * kDownWaves), 0, stream, d);
-            d.tiles = 0;
+            if (a.M >= kTwoTiles) a.half ? launch_down<true, 2>(d, stream) : launch_down<false, 2>(d, stream);
+            else a.half ? launch_down<true, 1>(d, stream) : launch_down<false, 1>(d, stream);
+            d.tiles = d.most = 0;
         };
         for (int k = i; k < a.count; k++) {
-            if (done[k] || a.p[k].x != d.x || a.p[k].K != d.K) continue;
+            const LoraArgs::One& p = a.p[k];
+            if (done[k] || p.x != d.x || p.K != d.K) continue;
             done[k] = true;
-            for (int r = 0; r < a.p[k].rank; r += 16) {
+            for (int r = 0; r < p.rank; r += 16) {
                 if (d.tiles == kDownTiles) flush();
-                d.p[d.tiles] = (short)k;
-                d.r[d.tiles++] = (short)r;
+                d.tile[d.tiles++] = {p.a + (size_t)r * p.K, p.scale, a.ws + a.t_off[k] + r, (long long)p.rank * p.K, std::min(16, p.rank - r), p.rank, p.n};
+                d.most = std::max(d.most, p.n);
             }
         }
         if (d.tiles) flush();
     }
-    for (int i = 0; i < a.count; i++) {
-        const dim3 grid((a.p[i].N + kUpCols - 1) / kUpCols, (a.M + kUpRows - 1) / kUpRows);
-        if (a.p[i].rank <= 32) hipLaunchKernelGGL(lora_up_kernel<1>, grid, dim3(256), 0, stream, a, i);
-        else if (a.p[i].rank <= 64) hipLaunchKernelGGL(lora_up_kernel<2>, grid, dim3(256), 0, stream, a, i);
-        else hipLaunchKernelGGL(lora_up_kernel<4>, grid, dim3(256), 0, stream, a, i);
-    }
+    if (a.M >= kTwoTiles) launch_up<2>(a, stream);
+    else launch_up<1>(a, stream);
     return hipGetLastError();
 }
 
