@@ -416,7 +416,7 @@ typedef struct ql_lora_desc {
  * 0..n_adapter - 1 (-1: a row without an adapter). ids is int32 [M] in `act`; x [M, K] in x_dtype (fp32 or fp16), base and y fp32 [M, N] at
  * x_offs[i], base_offs[i], y_offs[i] in `act`. y_offs[i] may be base_offs[i] (a row without an adapter is not touched);
  * any other overlap of what is written with what is read fails with QL_E_INVALID. Sums in fp32, fp16 products exact; many rows take fp32 x, and x . A^T, as
- * two fp16 parts of about 22 bits each under the exponent of 32 columns, or of the row's ranks.
+ * two fp16 parts of about 22 bits each under the exponent of 64 columns, or of the row's ranks.
  * M = 1..65535. Offsets 16-byte aligned (ids, scales: 4). Uses the context's 64 MiB workspace. */
 int ql_lora_add(ql_ctx* ctx, int32_t count, const ql_lora_desc* descs, const ql_arena* weights, ql_arena* act, uint64_t ids_off,
                 const uint64_t* x_offs, int32_t x_dtype, int32_t M, const uint64_t* base_offs, const uint64_t* y_offs);

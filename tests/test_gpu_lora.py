@@ -60,7 +60,7 @@ class Call:
                 s = float(self.scale[i][k]) if self.scales else 1.0
                 want[m] += s * (x @ a.T) @ b.T
                 # fp32 sums of K and of r products, each off by as many u of the products' sizes at most, and the scale's product; many rows:
-                # x's and t's two parts carry 2^-22 of the largest of their 32 columns, or of the row's ranks
+                # x's and t's two parts carry 2^-22 of the largest of their 64 columns, or of the row's ranks
                 tol[m] = s * ((K + 4) * U * (np.abs(x) @ np.abs(a).T) + (r + 4) * U * np.abs(x @ a.T)) @ np.abs(b).T
             tol += 2 * U * np.abs(want)
             with np.errstate(invalid="ignore"):
@@ -82,6 +82,8 @@ CASES = [  # M, targets, how the ids lie
     (300, [(520, 260, 40, 7)], "mixed"),
     (1000, [(896, 128, 16, 6)], "runs"),
     (130, [(2056, 12, 96, 3)], "one"),
+    (1500, [(904, 300, 64, 9), (904, 20, 24, 9)], "mixed"),
+    (1030, [(72, 516, 8, 2)], "runs"),
     (20000, [(16, 8, 128, 3)] * 8, "runs"),                                      # more rows than the workspace has room for at once
 ]
 

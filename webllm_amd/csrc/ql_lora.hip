@@ -4,10 +4,10 @@
 // four ranks, so that x is read once for them, and a part of K, the parts' sums meet in LDS; then a thread has a column of y, and B's row of it. The
 // workgroups of one row's column ranges each make t for themselves: A comes from L2, and a second launch would cost more.
 //
-// Many rows, two launches: lora_down_kernel makes t of 16 rows, eight waves a part of K each, on the matrix cores, T^T = A x^T
-// (lane = row, registers = ranks), for all projections that read one x; lora_up_kernel has 16 rows and 64 columns a wave, y^T = B t^T. Rows of
+// Many rows, two launches: lora_down_kernel makes t of 16 rows, four waves a part of K each, on the matrix cores, T^T = A x^T
+// (lane = row, registers = ranks), for all projections that read one x; lora_up_kernel has 16 or 32 rows and 64 columns a wave, Y = T B^T. Rows of
 // several adapters in one tile: it is gone through once for each adapter, and a row takes its own. fp32 x enters as two fp16 parts (22 bits) under the
-// exponent of the row's 32 columns at a time; t likewise under the row's.
+// exponent of the row's 64 columns at a time; t likewise under the row's.
 #include <algorithm>
 
 #include "ql_device.h"
@@ -90,9 +90,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void lora_row_kernel(const LoraArgs
 
 // ---- many rows
 
-constexpr int kDownWaves = 8, kDownTiles = 12;   // waves of a workgroup; tiles of 16 ranks that it makes at once
-constexpr int kUpRows = 32, kUpCols = 256;      // rows of a pass are a multiple; columns of a workgroup
-constexpr int kTwoTiles = 1024;                // rows from which a wave has two tiles of 16 for what it reads of A and B
+constexpr int kDownWaves = 4, kDownGroup = 4;      // waves of a workgroup; most tiles of 16 ranks that it makes
+constexpr int kDownTiles = 24;                     // of a launch
+constexpr int kUpRows = 32, kUpCols = 256;         // rows of a pass are a multiple; columns of a workgroup
+constexpr int kTwoTiles = 1024;                    // rows from which an adapter's B in LDS serves two tiles of 16 rows (4096 rows of rank 64: one 47 us, two 45, four 59)
 
 // The ranks of all projections that read one x, in tiles of 16
 struct LoraDown {
@@ -110,28 +111,44 @@ struct LoraDown {
 
 // The adapters of RT tiles of 16 rows, one after the other: bit 16 t + i of `left` is row i of tile t, whose adapter lane i knows in id[t]
 template <int RT>
-__device__ __forceinline__ uint32_t rows_with(const int (&id)[RT], int which)
+__device__ __forceinline__ uint64_t rows_with(const int (&id)[RT], int which)
 {
-    uint32_t m = 0;
+    uint64_t m = 0;
 #pragma unroll
-    for (int t = 0; t < RT; t++) m |= (uint32_t)(__ballot(id[t] == which) & 0xFFFF) << (16 * t);
+    for (int t = 0; t < RT; t++) m |= (__ballot(id[t] == which) & 0xFFFF) << (16 * t);
     return m;
 }
 template <int RT>
-__device__ __forceinline__ uint32_t rows_below(const int (&id)[RT], int n)
+__device__ __forceinline__ uint64_t rows_below(const int (&id)[RT], int n)
 {
-    uint32_t m = 0;
+    uint64_t m = 0;
 #pragma unroll
-    for (int t = 0; t < RT; t++) m |= (uint32_t)(__ballot((uint32_t)id[t] < (uint32_t)n) & 0xFFFF) << (16 * t);
+    for (int t = 0; t < RT; t++) m |= (__ballot((uint32_t)id[t] < (uint32_t)n) & 0xFFFF) << (16 * t);
     return m;
 }
 template <int RT>
-__device__ __forceinline__ int first_adapter(const int (&id)[RT], uint32_t left)
+__device__ __forceinline__ int first_adapter(const int (&id)[RT], uint64_t left)
 {
-    const int r = __builtin_ctz(left);
-    int which = __builtin_amdgcn_readlane(id[0], r & 15);
-    if (RT > 1 && r >= 16) which = __builtin_amdgcn_readlane(id[RT - 1], r & 15);
+    const int r = __builtin_ctzll(left);
+    int which = 0;
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+        if (r >> 4 == t) which = __builtin_amdgcn_readlane(id[t], r & 15);
     return which;
+}
+// 16 bytes a lane to LDS, a wave's in a row from `to`
+__device__ __forceinline__ void load_to_lds(const void* from, void* to)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+#endif
+}
+// what a wave has asked for of memory and LDS is there
+__device__ __forceinline__ void wave_arrived()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x70);                       // vmcnt(0) lgkmcnt(0), in a form that the compiler counts
+    asm volatile("" ::: "memory");
 }
 
 // x's two parts: hi + 2^-11 lo of x * s
@@ -147,155 +164,173 @@ __device__ __forceinline__ void split_f16(const float (&x)[8], float s, f16x8& h
 // the power of two that brings mx to [2^14, 2^15)
 __device__ __forceinline__ float scale_of(float mx) { return mx > 0.f && mx <= kMaxFinite ? ldexpf(1.f, min(100, 14 - ilogbf(mx))) : 1.f; }
 
-// 64 of K at a time: lane group g has 16 of them, a line of each rank's row of A in all, in two products
-template <bool HALF, int TILES, int RT>
+// A wave has a quarter of K, 64 columns at a time. Fragments are 16 rows' 16 bytes, which as loads would be a line a lane (60 lines a load, 45 us a pass of 4096
+// rows of rank 64 for 8): rows come whole into a part of LDS that is the wave's own, 128 bytes of eight rows a load, and are turned there; the next
+// 64 columns are on their way meanwhile. The 16-byte pieces of row r lie in the order c ^ (r % 8), so that a fragment's reads meet no bank twice.
+template <bool HALF, int TILES>
+struct DownLds {
+    static constexpr int kXRow = HALF ? 128 : 256;          // bytes of a row of x, of 64 columns
+    static constexpr int kStep = TILES * 2048 + 16 * kXRow; // of a wave's step
+    static constexpr int kBytes = 2 * kDownWaves * kStep > kDownWaves * TILES * 1024 ? 2 * kDownWaves * kStep : kDownWaves * TILES * 1024;
+};
+
+template <bool HALF, int TILES>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDown d)
 {
-    __shared__ f32x4 part[kDownWaves][TILES][64];
-    const int m0 = 16 * RT * blockIdx.x, tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
+    using L = DownLds<HALF, TILES>;
+    __shared__ __attribute__((aligned(16))) char lds[2][L::kBytes / 2];
+    const int m0 = 16 * blockIdx.x, u0 = TILES * blockIdx.y, tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id[RT];
-    const char* x[RT];
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int m = min(m0 + 16 * t + i16, d.M - 1);
-        id[t] = m0 + 16 * t + i16 < d.M ? ld_global(d.ids + m) : -1;
-        x[t] = static_cast<const char*>(d.x) + (size_t)m * d.K * (HALF ? 2 : 4);
-    }
-    uint32_t left = rows_below(id, d.most);
+    int id[1] = {m0 + i16 < d.M ? ld_global(d.ids + m0 + i16) : -1};
+    uint64_t left = rows_below(id, d.most);
     const int steps = (d.K + 63) / 64, per = (steps + kDownWaves - 1) / kDownWaves, s0 = wave * per, s1 = min(steps, s0 + per);
+    // of the loads, a lane's row and piece
+    const int ar = lane >> 3, ac = (lane & 7) ^ ar, xr = HALF ? ar : lane >> 4, xp = HALF ? 8 : 4;
     while (left) {
         const int which = first_adapter(id, left);
-        const uint32_t mine = left & rows_with(id, which);
+        const uint64_t mine = left & rows_with(id, which);
         left &= ~mine;
-        const uint16_t* w[TILES];
+        const uint16_t* w[TILES][2];
 #pragma unroll
-        for (int u = 0; u < TILES; u++) {                   // a rank that is not there: the first one's, not stored
-            const LoraDown::Tile& t = d.tile[min(u, d.tiles - 1)];
-            w[u] = t.a + (which < t.n ? which : 0) * t.step + (size_t)(i16 < t.ranks ? i16 : 0) * d.K;
+        for (int u = 0; u < TILES; u++) {                   // a rank or tile that is not there: another one, not stored
+            const LoraDown::Tile& t = d.tile[min(u0 + u, d.tiles - 1)];
+#pragma unroll
+            for (int h = 0; h < 2; h++) w[u][h] = t.a + (which < t.n ? which : 0) * t.step + (size_t)min(8 * h + ar, t.ranks - 1) * d.K;
         }
-        f32x4 acc[TILES][RT];
-#pragma unroll
-        for (int u = 0; u < TILES; u++)
-#pragma unroll
-            for (int t = 0; t < RT; t++) acc[u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int st = s0; st < s1; st++) {
-            const int k = 64 * st + 16 * g;
-            const bool in[2] = {k < d.K, k + 8 < d.K};      // K is a multiple of eight
-            u32x4 raw[TILES][2];
+        auto fetch = [&](int st, int buf) {
+            char* const to = lds[buf] + wave * L::kStep;
+            const int ka = 64 * st + 8 * ac, k = ka < d.K ? ka : 0;          // beyond K: what is there, not used
 #pragma unroll
             for (int u = 0; u < TILES; u++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) raw[u][h] = ld_global(reinterpret_cast<const u32x4*>(w[u] + (in[h] ? k + 8 * h : 0)));
-            f16x8 hi[RT][2], lo[RT][2];
-            float up[RT];
+                for (int h = 0; h < 2; h++) load_to_lds(w[u][h] + k, to + u * 2048 + h * 1024);
 #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                if constexpr (HALF) {
+            for (int j = 0; j < 16 / xp; j++) {
+                const int r = j * xp + xr, m = min(m0 + r, d.M - 1);
+                const int c = HALF ? ac : (lane & 15) ^ r, kx = 64 * st + (HALF ? 8 : 4) * c, kk = kx < d.K ? kx : 0;
+                load_to_lds(static_cast<const char*>(d.x) + ((size_t)m * d.K + kk) * (HALF ? 2 : 4), to + TILES * 2048 + j * 1024);
+            }
+        };
+        f32x4 acc[TILES];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        hi[t][h] = __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(x[t] + 2 * (in[h] ? k + 8 * h : 0))));
-                        if (!in[h]) hi[t][h] = f16x8{};
+        for (int u = 0; u < TILES; u++) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (s0 < s1) fetch(s0, s0 & 1);
+        for (int st = s0; st < s1; st++) {
+            wave_arrived();
+            if (st + 1 < s1) fetch(st + 1, (st + 1) & 1);
+            const char* const from = lds[st & 1] + wave * L::kStep;
+            const int k = 64 * st + 16 * g;
+            const bool in[2] = {k < d.K, k + 8 < d.K};      // K is a multiple of eight
+            f16x8 hi[2], lo[2];
+            float up = 1.f;
+            const char* const x = from + TILES * 2048 + i16 * L::kXRow;
+            if constexpr (HALF) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) hi[h] = in[h] ? *reinterpret_cast<const f16x8*>(x + ((2 * g + h) ^ (i16 & 7)) * 16) : f16x8{};
+            } else {
+                float v[2][8], mx = 0.f;
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const f32x4 y = *reinterpret_cast<const f32x4*>(x + ((4 * g + q) ^ i16) * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        v[q >> 1][4 * (q & 1) + e] = in[q >> 1] ? y[e] : 0.f;
+                        mx = fmaxf(mx, fabsf(v[q >> 1][4 * (q & 1) + e]));
                     }
-                } else {
-                    float v[2][8], mx = 0.f;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        load8(x[t], 0, in[h] ? k + 8 * h : 0, v[h]);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            v[h][e] = in[h] ? v[h][e] : 0.f;
-                            mx = fmaxf(mx, fabsf(v[h][e]));
-                        }
-                    }
-                    mx = pair_max<32>(pair_max<16>(mx));
-                    const float s = scale_of(mx);
-                    up[t] = 1.f / s;
-#pragma unroll
-                    for (int h = 0; h < 2; h++) split_f16(v[h], s, hi[t][h], lo[t][h]);
                 }
+                mx = pair_max<32>(pair_max<16>(mx));
+                const float s = scale_of(mx);
+                up = 1.f / s;
+#pragma unroll
+                for (int h = 0; h < 2; h++) split_f16(v[h], s, hi[h], lo[h]);
             }
 #pragma unroll
             for (int u = 0; u < TILES; u++) {
-                f16x8 wu[2];
+                const char* const a = from + u * 2048 + i16 * 128;
+                f16x8 wu[2];                                // beyond K zeros on both sides: 0 * NaN
 #pragma unroll
-                for (int h = 0; h < 2; h++) wu[h] = in[h] ? __builtin_bit_cast(f16x8, raw[u][h]) : f16x8{};   // zeros on both sides: 0 * NaN
+                for (int h = 0; h < 2; h++) wu[h] = in[h] ? *reinterpret_cast<const f16x8*>(a + ((2 * g + h) ^ (i16 & 7)) * 16) : f16x8{};
+                if constexpr (HALF) {
 #pragma unroll
-                for (int t = 0; t < RT; t++) {
-                    if constexpr (HALF) {
+                    for (int h = 0; h < 2; h++) acc[u] = mfma_16x16x32_f16(wu[h], hi[h], acc[u]);
+                } else {
+                    f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int h = 0; h < 2; h++) acc[u][t] = mfma_16x16x32_f16(wu[h], hi[t][h], acc[u][t]);
-                    } else {
-                        f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            ol = mfma_16x16x32_f16(wu[h], lo[t][h], ol);
-                            o = mfma_16x16x32_f16(wu[h], hi[t][h], o);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) acc[u][t][e] = fmaf(fmaf(ol[e], 1.f / 2048.f, o[e]), up[t], acc[u][t][e]);
+                    for (int h = 0; h < 2; h++) {
+                        ol = mfma_16x16x32_f16(wu[h], lo[h], ol);
+                        o = mfma_16x16x32_f16(wu[h], hi[h], o);
                     }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[u][e] = fmaf(fmaf(ol[e], 1.f / 2048.f, o[e]), up, acc[u][e]);
                 }
             }
         }
+        // the waves' parts, where their steps lay
+        f32x4* const part = reinterpret_cast<f32x4*>(lds);
+        __syncthreads();
 #pragma unroll
-        for (int t = 0; t < RT; t++) {
+        for (int u = 0; u < TILES; u++) part[(wave * TILES + u) * 64 + lane] = acc[u];
+        __syncthreads();
+        for (int u = wave; u < min(TILES, d.tiles - u0); u += kDownWaves) {
+            const LoraDown::Tile& t = d.tile[u0 + u];
+            f32x4 v = part[u * 64 + lane];
 #pragma unroll
-            for (int u = 0; u < TILES; u++) part[wave][u][lane] = acc[u][t];
-            __syncthreads();
-            for (int u = wave; u < d.tiles; u += kDownWaves) {
-                const LoraDown::Tile& tl = d.tile[u];
-                f32x4 v = part[0][u][lane];
-#pragma unroll
-                for (int k = 1; k < kDownWaves; k++) v += part[k][u][lane];
-                if ((mine >> (16 * t + i16) & 1) && which < tl.n && 4 * g < tl.ranks) {
-                    const float s = tl.scale ? ld_global(tl.scale + which) : 1.f;
-                    st_global(reinterpret_cast<f32x4*>(tl.t + (size_t)(m0 + 16 * t + i16) * tl.rank + 4 * g), f32x4{v[0] * s, v[1] * s, v[2] * s, v[3] * s});
-                }
+            for (int k = 1; k < kDownWaves; k++) v += part[(k * TILES + u) * 64 + lane];
+            if ((mine >> i16 & 1) && which < t.n && 4 * g < t.ranks) {
+                const float s = t.scale ? ld_global(t.scale + which) : 1.f;
+                st_global(reinterpret_cast<f32x4*>(t.t + (size_t)(m0 + i16) * t.rank + 4 * g), f32x4{v[0] * s, v[1] * s, v[2] * s, v[3] * s});
             }
-            __syncthreads();
         }
+        __syncthreads();
     }
 }
 
-// A workgroup has 16 RT rows and 256 columns of a projection, a wave 64; the projections' columns lie one behind the other in blockIdx.x
+// Y = T B^T: lane = column, registers = rows 4 g + r, so that 16 lanes of y are a row's 64 bytes. A workgroup has 16 RT rows and 256 columns of a
+// projection, a wave 64 of them; the projections' columns lie one behind the other in blockIdx.x. An adapter's B of the 256 columns is one
+// stretch of memory: it goes to LDS as it lies, but for the order of a row's pieces, c ^ (n % their number) where that is a power of two.
 template <int STEPS, int RT>
 __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
 {
+    __shared__ __attribute__((aligned(16))) char lds[kUpCols * STEPS * 64];
     const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int proj = 0, xb = blockIdx.x;
     while (xb >= (a.p[proj].N + kUpCols - 1) / kUpCols) xb -= (a.p[proj++].N + kUpCols - 1) / kUpCols;
     const LoraArgs::One& p = a.p[proj];
-    const int m0 = 16 * RT * blockIdx.y, n0 = kUpCols * xb + 64 * wave;
+    const int m0 = 16 * RT * blockIdx.y, n0 = kUpCols * xb, cols = min(kUpCols, p.N - n0), pieces = p.rank / 8;
+    const int turn = pieces & (pieces - 1) ? 0 : min(pieces, 8) - 1;
     const float* t_in = a.ws + a.t_off[proj];
     const bool apart = p.base != p.y;
     int id[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) id[t] = m0 + 16 * t + i16 < a.M ? ld_global(a.ids + m0 + 16 * t + i16) : -1;
-    uint32_t left = rows_below(id, p.n);
-    const uint32_t all = left;
-    if ((!left && !apart) || n0 >= p.N) return;
-    f32x4 y[RT][4];
+    uint64_t left = rows_below(id, p.n);
+    const uint64_t all = left;
+    if (!left && !apart) return;
+    float y[RT][4][4];
     f16x8 hi[RT][STEPS], lo[RT][STEPS];
     float up[RT];
 #pragma unroll
     for (int t = 0; t < RT; t++) {
         const int m = m0 + 16 * t + i16;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int n = n0 + 16 * j + 4 * g;
-            y[t][j] = m < a.M && n < p.N ? ld_global(reinterpret_cast<const f32x4*>(p.base + (size_t)m * p.N + n)) : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
         float mx = 0.f, v[STEPS][8];
 #pragma unroll
         for (int st = 0; st < STEPS; st++) {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[st][e] = 0.f;
             if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank) load8(t_in, 0, (size_t)m * p.rank + 32 * st + 8 * g, v[st]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int mr = m0 + 16 * t + 4 * g + r, n = 64 * wave + 16 * j + i16;
+                y[t][j][r] = mr < a.M && n < cols ? ld_global(p.base + (size_t)mr * p.N + n0 + n) : 0.f;
+            }
+#pragma unroll
+        for (int st = 0; st < STEPS; st++)
 #pragma unroll
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[st][e]));
-        }
         mx = pair_max<32>(pair_max<16>(mx));
         const float s = scale_of(mx);
         up[t] = 1.f / s;
@@ -304,40 +339,52 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
     }
     while (left) {
         const int which = first_adapter(id, left);
-        const uint32_t mine = left & rows_with(id, which);
+        const uint64_t mine = left & rows_with(id, which);
         left &= ~mine;
+        const char* const B = reinterpret_cast<const char*>(p.b + ((size_t)which * p.N + n0) * p.rank);
+        const int all_pieces = cols * pieces;
+        for (int u = tid; u < (all_pieces + 63) / 64 * 64; u += 256) {
+            const int at = min(u, all_pieces - 1), n = at / pieces, c = at - n * pieces;
+            load_to_lds(B + (n * pieces + (c ^ (n & turn))) * 16, lds + (u - lane) * 16);
+        }
+        wave_arrived();
+        __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int n = n0 + 16 * j + i16;
+            const int n = 64 * wave + 16 * j + i16;
             f16x8 w[STEPS];
 #pragma unroll
             for (int st = 0; st < STEPS; st++) {
-                const int r = 32 * st + 8 * g;
-                w[st] = n < p.N && r < p.rank ? __builtin_bit_cast(f16x8, ld_global(reinterpret_cast<const u32x4*>(p.b + ((size_t)which * p.N + n) * p.rank + r))) : f16x8{};
+                const int c = 4 * st + g;
+                w[st] = n < cols && c < pieces ? *reinterpret_cast<const f16x8*>(lds + (n * pieces + (c ^ (n & turn))) * 16) : f16x8{};
             }
 #pragma unroll
             for (int t = 0; t < RT; t++) {
                 f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int st = 0; st < STEPS; st++) {
-                    ol = mfma_16x16x32_f16(w[st], lo[t][st], ol);
-                    o = mfma_16x16x32_f16(w[st], hi[t][st], o);
+                    ol = mfma_16x16x32_f16(lo[t][st], w[st], ol);
+                    o = mfma_16x16x32_f16(hi[t][st], w[st], o);
                 }
-                const bool take = mine >> (16 * t + i16) & 1;
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[t][j][e] = take ? fmaf(fmaf(ol[e], 1.f / 2048.f, o[e]), up[t], y[t][j][e]) : y[t][j][e];
+                for (int r = 0; r < 4; r++) {
+                    const float ur = __shfl(up[t], 4 * g + r);
+                    const bool take = mine >> (16 * t + 4 * g + r) & 1;
+                    y[t][j][r] = take ? fmaf(fmaf(ol[r], 1.f / 2048.f, o[r]), ur, y[t][j][r]) : y[t][j][r];
+                }
             }
         }
+        __syncthreads();
     }
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int m = m0 + 16 * t + i16;
+    for (int t = 0; t < RT; t++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int n = n0 + 16 * j + 4 * g;
-            if (m < a.M && n < p.N && ((all >> (16 * t + i16) & 1) || apart)) st_global(reinterpret_cast<f32x4*>(p.y + (size_t)m * p.N + n), y[t][j]);
-        }
-    }
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int mr = m0 + 16 * t + 4 * g + r, n = 64 * wave + 16 * j + i16;
+                if (mr < a.M && n < cols && ((all >> (16 * t + 4 * g + r) & 1) || apart)) st_global(p.y + (size_t)mr * p.N + n0 + n, y[t][j][r]);
+            }
 }
 
 }  // namespace
@@ -359,15 +406,14 @@ uint64_t plan_lora(LoraArgs* a, size_t ws_bytes)
 
 namespace {
 
-template <bool HALF, int RT>
+template <bool HALF>
 void launch_down(const LoraDown& d, hipStream_t stream)
 {
-    const dim3 grid((d.M + 16 * RT - 1) / (16 * RT)), block(64 * kDownWaves);
-    if (d.tiles <= 1) hipLaunchKernelGGL((lora_down_kernel<HALF, 1, RT>), grid, block, 0, stream, d);
-    else if (d.tiles <= 2) hipLaunchKernelGGL((lora_down_kernel<HALF, 2, RT>), grid, block, 0, stream, d);
-    else if (d.tiles <= 4) hipLaunchKernelGGL((lora_down_kernel<HALF, 4, RT>), grid, block, 0, stream, d);
-    else if (d.tiles <= 8) hipLaunchKernelGGL((lora_down_kernel<HALF, 8, RT>), grid, block, 0, stream, d);
-    else hipLaunchKernelGGL((lora_down_kernel<HALF, kDownTiles, RT>), grid, block, 0, stream, d);
+    const dim3 block(64 * kDownWaves);
+    const int rows = (d.M + 15) / 16;
+    if (d.tiles == 1) hipLaunchKernelGGL((lora_down_kernel<HALF, 1>), dim3(rows, 1), block, 0, stream, d);
+    else if (d.tiles <= 3 || d.tiles == 5) hipLaunchKernelGGL((lora_down_kernel<HALF, 3>), dim3(rows, (d.tiles + 2) / 3), block, 0, stream, d);
+    else hipLaunchKernelGGL((lora_down_kernel<HALF, kDownGroup>), dim3(rows, (d.tiles + kDownGroup - 1) / kDownGroup), block, 0, stream, d);
 }
 
 template <int RT>
@@ -396,8 +442,8 @@ hipError_t launch_tiled(const LoraArgs& a, hipStream_t stream)
         d.M = a.M;
         d.tiles = d.most = 0;
         auto flush = [&] {
-            if (a.M >= kTwoTiles) a.half ? launch_down<true, 2>(d, stream) : launch_down<false, 2>(d, stream);
-            else a.half ? launch_down<true, 1>(d, stream) : launch_down<false, 1>(d, stream);
+            if (a.half) launch_down<true>(d, stream);
+            else launch_down<false>(d, stream);
             d.tiles = d.most = 0;
         };
         for (int k = i; k < a.count; k++) {
