@@ -416,12 +416,14 @@ struct LoraArgs {
     const int32_t* ids;        // [M]
     float* ws;
     int count, M, half;        // half: x is fp16
-    // plan_lora fills these: 0, a workgroup a row; or how many rows are done in tiles at once, and where t [rows, rank] of each projection lies
-    // in ws, in values
-    int rows;
+    // plan_lora fills these: 0, a workgroup a row; or how many rows are done in tiles at once, and of each projection the parts that K is done in, and
+    // where t [parts, rows, rank] lies in ws, in values
+    int rows, parts[kMaxBatch];
     uint64_t t_off[kMaxBatch];
 };
-constexpr int kLoraRowMax = 128;   // most rows that have a workgroup each
+// A workgroup a row up to so many rows, or rows times the largest rank: 100 rows, 5 adapters in runs, rows against tiles in us: q/k/v of 3584 columns rank 16
+// 9, 14, rank 64 27, 22; 18944 columns from 3584 twice, rank 16 20, 22, rank 64 104, 37. Rows of many adapters mixed, which few rows are, cost tiles a pass each.
+constexpr int kLoraRowMax = 64, kLoraRowRanks = 2048;
 uint64_t plan_lora(LoraArgs* a, size_t ws_bytes);
 hipError_t launch_lora(const LoraArgs& a, hipStream_t stream);
 

@@ -73,6 +73,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void lora_row_kernel(const LoraArgs
         }
         __syncthreads();
     }
+    // (lanes that share a column, so that a load is a stretch of memory: no faster at rank 64, and 100 rows of rank 16 to 18944 columns 32 us for 20)
 #pragma unroll 2
     for (int n = n0 + tid; n < n1; n += 64 * kRowWaves) {
         const uint16_t* B = p.b + ((size_t)id * p.N + n) * p.rank;
@@ -103,10 +104,11 @@ struct LoraDown {
         float* t;                  // its first rank's column of t [rows, rank]
         long long step;            // values from an adapter to the next
         int ranks, rank, n;        // ranks of the tile, of the projection; adapters
+        size_t part;               // values from a part of K's t to the next
     } tile[kDownTiles];
     const void* x;
     const int32_t* ids;
-    int K, M, tiles, most;         // most: adapters of the projection that has most
+    int K, M, tiles, most, parts;  // most: adapters of the projection that has most; parts of K, of workgroups each
 };
 
 // The adapters of RT tiles of 16 rows, one after the other: bit 16 t + i of `left` is row i of tile t, whose adapter lane i knows in id[t]
@@ -183,7 +185,8 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDo
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id[1] = {m0 + i16 < d.M ? ld_global(d.ids + m0 + i16) : -1};
     uint64_t left = rows_below(id, d.most);
-    const int steps = (d.K + 63) / 64, per = (steps + kDownWaves - 1) / kDownWaves, s0 = wave * per, s1 = min(steps, s0 + per);
+    const int steps = (d.K + 63) / 64, per = (steps + d.parts * kDownWaves - 1) / (d.parts * kDownWaves);
+    const int s0 = (blockIdx.z * kDownWaves + wave) * per, s1 = min(steps, s0 + per);
     // of the loads, a lane's row and piece
     const int ar = lane >> 3, ac = (lane & 7) ^ ar, xr = HALF ? ar : lane >> 4, xp = HALF ? 8 : 4;
     while (left) {
@@ -278,7 +281,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDo
             for (int k = 1; k < kDownWaves; k++) v += part[(k * TILES + u) * 64 + lane];
             if ((mine >> i16 & 1) && which < t.n && 4 * g < t.ranks) {
                 const float s = t.scale ? ld_global(t.scale + which) : 1.f;
-                st_global(reinterpret_cast<f32x4*>(t.t + (size_t)(m0 + i16) * t.rank + 4 * g), f32x4{v[0] * s, v[1] * s, v[2] * s, v[3] * s});
+                st_global(reinterpret_cast<f32x4*>(t.t + blockIdx.z * t.part + (size_t)(m0 + i16) * t.rank + 4 * g), f32x4{v[0] * s, v[1] * s, v[2] * s, v[3] * s});
             }
         }
         __syncthreads();
@@ -318,7 +321,13 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
         for (int st = 0; st < STEPS; st++) {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[st][e] = 0.f;
-            if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank) load8(t_in, 0, (size_t)m * p.rank + 32 * st + 8 * g, v[st]);
+            if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank)
+                for (int k = 0; k < a.parts[proj]; k++) {   // of K, in order
+                    float w[8];
+                    load8(t_in, 0, ((size_t)k * a.M + m) * p.rank + 32 * st + 8 * g, w);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[st][e] += w[e];
+                }
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -392,16 +401,26 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
 uint64_t plan_lora(LoraArgs* a, size_t ws_bytes)
 {
     a->rows = 0;
-    if (a->M <= kLoraRowMax) return 0;
-    int64_t ranks = 0;
-    for (int i = 0; i < a->count; i++) ranks += a->p[i].rank;
+    int rank = 0;
+    for (int i = 0; i < a->count; i++) rank = std::max(rank, a->p[i].rank);
+    if (a->M <= kLoraRowMax || (long long)a->M * rank <= kLoraRowRanks) return 0;
+    // K in parts where the tiles of 16 rows and up to four of 16 ranks that read one x are few: two steps of 64 a wave at least
+    int64_t values = 0;                                     // of t, a row
+    for (int i = 0; i < a->count; i++) {
+        int tiles = 0;
+        for (int k = 0; k < a->count; k++)
+            if (a->p[k].x == a->p[i].x && a->p[k].K == a->p[i].K) tiles += (a->p[k].rank + 15) / 16;
+        const int groups = (a->M + 15) / 16 * ((tiles + kDownGroup - 1) / kDownGroup);
+        a->parts[i] = std::max(1, std::min({512 / groups, 16, a->p[i].K / (64 * 2 * kDownWaves)}));
+        values += a->p[i].rank * a->parts[i];
+    }
     // as many rows at once as have room
-    a->rows = (int)std::min<int64_t>(a->M, (int64_t)(ws_bytes / sizeof(float)) / ranks / kUpRows * kUpRows);
+    a->rows = (int)std::min<int64_t>(a->M, (int64_t)(ws_bytes / sizeof(float)) / values / kUpRows * kUpRows);
     for (int64_t i = 0, at = 0; i < a->count; i++) {
         a->t_off[i] = at;
-        at += (int64_t)a->rows * a->p[i].rank;
+        at += (int64_t)a->rows * a->p[i].rank * a->parts[i];
     }
-    return ranks * a->rows * sizeof(float);
+    return values * a->rows * sizeof(float);
 }
 
 namespace {
@@ -411,9 +430,9 @@ void launch_down(const LoraDown& d, hipStream_t stream)
 {
     const dim3 block(64 * kDownWaves);
     const int rows = (d.M + 15) / 16;
-    if (d.tiles == 1) hipLaunchKernelGGL((lora_down_kernel<HALF, 1>), dim3(rows, 1), block, 0, stream, d);
-    else if (d.tiles <= 3 || d.tiles == 5) hipLaunchKernelGGL((lora_down_kernel<HALF, 3>), dim3(rows, (d.tiles + 2) / 3), block, 0, stream, d);
-    else hipLaunchKernelGGL((lora_down_kernel<HALF, kDownGroup>), dim3(rows, (d.tiles + kDownGroup - 1) / kDownGroup), block, 0, stream, d);
+    if (d.tiles == 1) hipLaunchKernelGGL((lora_down_kernel<HALF, 1>), dim3(rows, 1, d.parts), block, 0, stream, d);
+    else if (d.tiles <= 3 || d.tiles == 5) hipLaunchKernelGGL((lora_down_kernel<HALF, 3>), dim3(rows, (d.tiles + 2) / 3, d.parts), block, 0, stream, d);
+    else hipLaunchKernelGGL((lora_down_kernel<HALF, kDownGroup>), dim3(rows, (d.tiles + kDownGroup - 1) / kDownGroup, d.parts), block, 0, stream, d);
 }
 
 template <int RT>
@@ -440,6 +459,7 @@ hipError_t launch_tiled(const LoraArgs& a, hipStream_t stream)
         d.ids = a.ids;
         d.K = a.p[i].K;
         d.M = a.M;
+        d.parts = a.parts[i];
         d.tiles = d.most = 0;
         auto flush = [&] {
             if (a.half) launch_down<true>(d, stream);
@@ -452,7 +472,7 @@ hipError_t launch_tiled(const LoraArgs& a, hipStream_t stream)
             done[k] = true;
             for (int r = 0; r < p.rank; r += 16) {
                 if (d.tiles == kDownTiles) flush();
-                d.tile[d.tiles++] = {p.a + (size_t)r * p.K, p.scale, a.ws + a.t_off[k] + r, (long long)p.rank * p.K, std::min(16, p.rank - r), p.rank, p.n};
+                d.tile[d.tiles++] = {p.a + (size_t)r * p.K, p.scale, a.ws + a.t_off[k] + r, (long long)p.rank * p.K, std::min(16, p.rank - r), p.rank, p.n, (size_t)a.M * p.rank};
                 d.most = std::max(d.most, p.n);
             }
         }
