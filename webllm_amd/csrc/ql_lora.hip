@@ -321,13 +321,7 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
         for (int st = 0; st < STEPS; st++) {
 #pragma unroll
             for (int e = 0; e < 8; e++) v[st][e] = 0.f;
-            if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank)
-                for (int k = 0; k < a.parts[proj]; k++) {   // of K, in order
-                    float w[8];
-                    load8(t_in, 0, ((size_t)k * a.M + m) * p.rank + 32 * st + 8 * g, w);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) v[st][e] += w[e];
-                }
+            if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank) load8(t_in, 0, (size_t)m * p.rank + 32 * st + 8 * g, v[st]);
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -336,6 +330,16 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
                 const int mr = m0 + 16 * t + 4 * g + r, n = 64 * wave + 16 * j + i16;
                 y[t][j][r] = mr < a.M && n < cols ? ld_global(p.base + (size_t)mr * p.N + n0 + n) : 0.f;
             }
+        if (a.parts[proj] > 1)                              // the other parts of K, in order
+#pragma unroll
+            for (int st = 0; st < STEPS; st++)
+                if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank)
+                    for (int k = 1; k < a.parts[proj]; k++) {
+                        float w[8];
+                        load8(t_in, 0, ((size_t)k * a.M + m) * p.rank + 32 * st + 8 * g, w);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) v[st][e] += w[e];
+                    }
 #pragma unroll
         for (int st = 0; st < STEPS; st++)
 #pragma unroll
@@ -346,6 +350,11 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
 #pragma unroll
         for (int st = 0; st < STEPS; st++) split_f16(v[st], s, hi[t][st], lo[t][st]);
     }
+    float up_of[RT][4];                                     // of the rows that the lane's results are of
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) up_of[t][r] = __shfl(up[t], 4 * g + r);
     while (left) {
         const int which = first_adapter(id, left);
         const uint64_t mine = left & rows_with(id, which);
@@ -377,9 +386,8 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float ur = __shfl(up[t], 4 * g + r);
                     const bool take = mine >> (16 * t + 4 * g + r) & 1;
-                    y[t][j][r] = take ? fmaf(fmaf(ol[r], 1.f / 2048.f, o[r]), ur, y[t][j][r]) : y[t][j][r];
+                    y[t][j][r] = take ? fmaf(fmaf(ol[r], 1.f / 2048.f, o[r]), up_of[t][r], y[t][j][r]) : y[t][j][r];
                 }
             }
         }
