@@ -370,6 +370,198 @@ class KvCache:
 
 
 @dataclass
+class Batch:
+    """A pass's rows of several sequences (PagedKvCache.batch): M rows of the tensors, `rows` of them the sequences', the rest padding."""
+    desc: ql.BatchDesc
+    M: int
+    rows: int
+    tables: tuple                # row_start, kv_len and pages in the activation arena
+
+
+class PagedKvCache:
+    """K and V of many sequences in pages that they take as they grow, in one device arena, for passes over many requests at once:
+    append and attend run per layer over a Batch. dtype "f16", or "f8": e4m3 values with a power of two for every 16 tokens of a
+    head, half the memory and its reads. Sequences are numbers (new_sequence); what they hold is counted on the host.
+
+    batch() takes the pages that a pass needs and counts its tokens, so it is called once, before the pass's layers. Its tables are
+    read on the device when a pass runs."""
+
+    def __init__(self, ctx: ql.Context, config: QwenConfig, pages: int, page_size: int = 64, dtype: str = "f16"):
+        if dtype not in ("f16", "f8"):
+            raise ValueError(f"paged kv cache: dtype {dtype}")
+        if pages < 1 or page_size not in (64, 128, 256):
+            raise ValueError("paged kv cache: at least one page, of 64, 128 or 256 tokens")
+        self.ctx, self.config, self.dtype, self.page_size, self.pages = ctx, config, dtype, page_size, pages
+        self.D, self.row_len = qwen_head_dim(config), qwen_kv_dim(config)
+        self.page_bytes = page_size * self.row_len * (1 if dtype == "f8" else 2)
+        self.scale_bytes = config.n_kv_head * (page_size // 16) * 4 if dtype == "f8" else 0     # of a page
+        layout = ql.ArenaLayout()
+        self.regions = [layout.take(pages * self.page_bytes) for _ in range(2 * config.n_layer)]
+        self.scales = [layout.take(pages * self.scale_bytes) for _ in range(2 * config.n_layer)] if self.scale_bytes else []
+        self.arena = ctx.arena(layout.used)
+        self._free = list(range(pages - 1, -1, -1))
+        self._users = [0] * pages                    # sequences that hold a page
+        self._lists: dict[int, list[int]] = {}
+        self._lengths: dict[int, int] = {}
+        self._next = 0
+
+    def new_sequence(self) -> int:
+        s, self._next = self._next, self._next + 1
+        self._lists[s], self._lengths[s] = [], 0
+        return s
+
+    def length(self, sequence: int) -> int:
+        return self._lengths[sequence]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _take(self) -> int:
+        p = self._free.pop()
+        self._users[p] = 1
+        return p
+
+    def free(self, sequence: int):
+        """A finished sequence's pages go back, but for those that others hold."""
+        for p in self._lists.pop(sequence):
+            self._drop(p)
+        del self._lengths[sequence]
+
+    def _drop(self, page: int):
+        self._users[page] -= 1
+        if self._users[page] == 0:
+            self._free.append(page)
+
+    def cut(self, sequence: int, tokens: int):
+        """The sequence's first tokens are kept (a rejected draft, an edited prompt)."""
+        if not 0 <= tokens <= self._lengths[sequence]:
+            raise ValueError(f"cut: sequence {sequence} has {self._lengths[sequence]} tokens")
+        pages = self._lists[sequence]
+        while len(pages) > -(-tokens // self.page_size):
+            self._drop(pages.pop())
+        self._lengths[sequence] = tokens
+
+    def fork(self, sequence: int) -> int:
+        """A sequence that continues another one: its whole pages are shared, the last one, where it is not full, is copied."""
+        pages, tokens = self._lists[sequence], self._lengths[sequence]
+        whole = tokens // self.page_size
+        if whole < len(pages) and not self._free:
+            raise ValueError("fork: no page left")
+        s = self.new_sequence()
+        for p in pages[:whole]:
+            self._users[p] += 1
+        self._lists[s], self._lengths[s] = pages[:whole], tokens
+        if whole < len(pages):
+            self._lists[s].append(self._copy(pages[whole]))
+        return s
+
+    def _copy(self, page: int) -> int:
+        new = self._take()
+        for offs, size in ((self.regions, self.page_bytes), (self.scales, self.scale_bytes)):
+            for i in range(0, len(offs), 256):
+                some = ql.offsets(offs[i:i + 256])
+                self.ctx.kv_move(self.arena, some, self.pages, self.arena, some, self.pages, size, new, page, 1)
+        return new
+
+    def batch(self, pool: "ActivationArena", sequences, M: int | None = None) -> Batch:
+        """Rows of a pass: (sequence, rows) in the order of the rows, each sequence once. Takes the pages that their tokens need and counts the
+        tokens; M: rows of the pass's tensors (those behind the sequences' are padding)."""
+        order, rows = [s for s, _ in sequences], [n for _, n in sequences]
+        if not order or len(set(order)) != len(order) or min(rows) < 0:
+            raise ValueError("batch: at least one sequence, each once, with no negative rows")
+        total = sum(rows)
+        M = max(total, 1) if M is None else M
+        if M < total:
+            raise ValueError(f"batch: {total} rows for tensors of {M}")
+        lengths = [self._lengths[s] + n for s, n in sequences]
+        lists = [self._lists[s] for s in order]
+        # a page that the pass appends to is the sequence's alone: one that others hold as well (cut in the middle of a shared one) is copied first
+        shared = [i for i, (s, n) in enumerate(sequences) if n and self._lengths[s] % self.page_size and self._users[lists[i][self._lengths[s] // self.page_size]] > 1]
+        need = sum(max(0, -(-L // self.page_size) - len(p)) for L, p in zip(lengths, lists)) + len(shared)
+        if need > len(self._free):
+            raise ValueError(f"batch: {need} pages for {len(self._free)} that are left")
+        for i in shared:
+            at = self._lengths[order[i]] // self.page_size
+            if self._users[lists[i][at]] > 1:                              # not since another of the pass left it
+                new = self._copy(lists[i][at])
+                self._drop(lists[i][at])
+                lists[i][at] = new
+        for s, L, pages in zip(order, lengths, lists):
+            while len(pages) < -(-L // self.page_size):
+                pages.append(self._take())
+            self._lengths[s] = L
+        most = max(1, max(len(p) for p in lists))
+        row_start, kv_len, pages = pool.alloc((len(order) + 1,), "i32"), pool.alloc((len(order),), "i32"), pool.alloc((len(order), most), "i32")
+        row_start.write(np.cumsum([0] + rows).astype(np.int32))
+        kv_len.write(np.array(lengths, np.int32))
+        pages.write(np.array([p + [-1] * (most - len(p)) for p in lists], np.int32))
+        desc = ql.make_batch(row_start.offset, kv_len.offset, pages.offset, len(order), most, max_rows=max(1, max(rows)), max_len=max(1, max(lengths)))
+        return Batch(desc, M, total, (row_start, kv_len, pages))
+
+    def desc(self, layer: int) -> ql.PagedDesc:
+        if not 0 <= layer < self.config.n_layer:
+            raise ValueError(f"layer {layer} out of range")
+        k, v = 2 * layer, 2 * layer + 1
+        more = dict(k_scale_off=self.scales[k], v_scale_off=self.scales[v]) if self.scales else {}
+        return ql.make_paged(self.regions[k], self.regions[v], self.pages, self.page_size, self.config.n_kv_head, self.D,
+                             cache_dtype=ql.DTYPE_F8 if self.scales else ql.DTYPE_F16, **more)
+
+    def append(self, layer: int, model: "QuantLinearModel", q: Tensor, k: Tensor, v: Tensor, batch: Batch, q_out: Tensor, rope: str = "rope",
+               q_norm: str | None = None, k_norm: str | None = None, eps: float = 1e-6):
+        """q and k turned by their rows' positions, normed per head first where norm weights are named; q to q_out (f32, where q itself may
+        be given, or f16), k and v to their places in the sequences' pages. Rows of padding stay as they were."""
+        c, M = self.config, batch.M
+        if q.length < M * c.n_head * self.D or q_out.length < M * c.n_head * self.D:
+            raise ValueError("append: q/q_out smaller than [M, n_head * D]")
+        if k.length < M * self.row_len or v.length < M * self.row_len:
+            raise ValueError("append: k/v smaller than [M, n_kv_head * D]")
+        if any(t.dtype != "f32" for t in (q, k, v)) or q_out.dtype not in ("f32", "f16"):
+            raise ValueError("append: q, k and v must be f32, q_out f32 or f16")
+        if any(t.arena is not q.arena for t in (k, v, q_out) + batch.tables):
+            raise ValueError("append: tensors must live in one activation arena")
+        table = model.f32.get(rope)
+        if table is None or len(table.shape) != 2:
+            raise ValueError(f"missing rope table: {rope}")
+        norms = [None if n is None else model.f32.get(n) for n in (q_norm, k_norm)]
+        for name, w in zip((q_norm, k_norm), norms):
+            if name is not None and (w is None or w.length != self.D):
+                raise ValueError(f"missing f32 weight of {self.D} values: {name}")
+        paged = self.desc(layer)
+        desc = ql.make_rope(table.offset, table.shape[0], c.n_head, c.n_kv_head, self.D, rot_dim=table.shape[1],
+                            q_norm_off=None if norms[0] is None else norms[0].offset, k_norm_off=None if norms[1] is None else norms[1].offset,
+                            norm_eps=eps, cache_dtype=paged.cache_dtype)
+        self.ctx.paged_append(desc, model.weights, q.arena, q.offset, k.offset, v.offset, batch.desc, M, q_out.offset,
+                              ql.DTYPE_F16 if q_out.dtype == "f16" else ql.DTYPE_F32, self.arena, paged)
+
+    def attend(self, layer: int, q: Tensor, out: Tensor, batch: Batch):
+        """out [M, n_head * D] = causal GQA attention of the batch's rows over their sequences; q and out both f32 or both f16."""
+        c, M = self.config, batch.M
+        if q.length < M * c.n_head * self.D or out.length < M * c.n_head * self.D:
+            raise ValueError("attend: q/out smaller than [M, n_head * D]")
+        if q.dtype not in ("f32", "f16") or out.dtype != q.dtype:
+            raise ValueError("attend: q and out must both be f32 or both f16")
+        if any(t.arena is not q.arena for t in (out,) + batch.tables):
+            raise ValueError("attend: q, out and the batch must live in one activation arena")
+        self.ctx.paged_attention(q.arena, q.offset, ql.DTYPE_F16 if q.dtype == "f16" else ql.DTYPE_F32, self.arena, self.desc(layer), batch.desc,
+                                 M, c.n_head, out.offset)
+
+    def release(self):
+        self.arena.release()
+
+
+@dataclass
+class _Lora:
+    a: int
+    b: int
+    scale: int
+    K: int
+    N: int
+    rank: int
+    n: int
+
+
+@dataclass
 class _Linear:
     desc: ql.GptqDesc
     K: int
@@ -388,6 +580,7 @@ class QuantLinearModel:
         self.linears: dict[str, _Linear] = {}
         self.f32: dict[str, Tensor] = {}
         self.f16: dict[str, Tensor] = {}
+        self.loras: dict[str, _Lora] = {}
         self.scratch = ctx.arena(scratch_capacity)
 
     @property
@@ -429,6 +622,45 @@ class QuantLinearModel:
             raise ValueError(f"weight already exists: {name}")
         off = self._place(bits)
         self.f16[name] = Tensor(self.weights, off, int(np.prod(shape)), tuple(shape), "f16")
+
+    def upload_lora(self, weight: str, a, b, scale=None):
+        """Low-rank adapters of a linear, all of them: a fp16 [n, rank, K], b fp16 [n, N, rank], scale f32 [n] (each one's alpha / rank; None: 1).
+        Adapters of lower ranks have zeros behind their own."""
+        if weight in self.loras:
+            raise ValueError(f"adapters already exist: {weight}")
+        lin = self.linear(weight)
+        a, b = np.ascontiguousarray(a, dtype=np.float16), np.ascontiguousarray(b, dtype=np.float16)
+        if a.ndim != 3 or b.shape != (a.shape[0], lin.N, a.shape[1]) or a.shape[2] != lin.K:
+            raise ValueError(f"lora: {weight} is [{lin.N},{lin.K}], adapters {list(a.shape)} and {list(b.shape)}")
+        n, rank, _ = a.shape
+        scale = np.ones(n, np.float32) if scale is None else np.ascontiguousarray(scale, dtype=np.float32).reshape(-1)
+        if scale.size != n:
+            raise ValueError(f"lora: {scale.size} scales for {n} adapters")
+        if rank < 8 or rank > 128 or rank % 8 or lin.K % 8 or lin.N % 4:
+            raise ValueError("lora: rank must be 8..128, a multiple of 8, K a multiple of 8, N of 4")
+        self.loras[weight] = _Lora(self._place(a), self._place(b), self._place(scale), lin.K, lin.N, rank, n)
+
+    def lora_add(self, A: Tensor, weights: list, ids: Tensor, Cs: list, M: int):
+        """Each C [M, N] += scale * (A . a^T) . b^T of its linear's adapters, by each row's id (i32 [M]; -1: none): after gemm or gemm_batch on the same
+        A (f32 or f16), up to 8 linears (q/k/v, gate/up) in one call."""
+        loras = []
+        for w in weights:
+            if w not in self.loras:
+                raise ValueError(f"missing adapters: {w}")
+            loras.append(self.loras[w])
+        if len(Cs) != len(loras):
+            raise ValueError(f"lora_add: {len(Cs)} outputs for {len(loras)} linears")
+        if ids.dtype != "i32" or ids.length < M:
+            raise ValueError("lora_add: ids must be an i32 tensor of at least M")
+        if A.dtype not in ("f32", "f16") or any(c.dtype != "f32" for c in Cs):
+            raise ValueError("lora_add: A must be f32 or f16, C f32")
+        if any(t.arena is not A.arena for t in Cs + [ids]):
+            raise ValueError("lora_add: tensors must live in one activation arena")
+        if any(A.length < M * x.K or c.length < M * x.N for x, c in zip(loras, Cs)):
+            raise ValueError("lora_add: tensor too small for [M,K] / [M,N]")
+        offs = [c.offset for c in Cs]
+        self.ctx.lora_add([ql.make_lora(x.a, x.b, x.K, x.N, x.rank, x.n, scale_off=x.scale) for x in loras], self.weights, A.arena, ids.offset,
+                          [A.offset] * len(Cs), ql.DTYPE_F16 if A.dtype == "f16" else ql.DTYPE_F32, M, offs, offs)
 
     def release(self):
         """Frees the weight arena (the reference's QwenGpt.destroy of its weight buffers)."""
