@@ -25,6 +25,9 @@ CASES = [  # seqs, page, H, KV, D
     ([(1, 90), (17, 33)], 64, 64, 2, 16),
     ([(400, 400), (300, 1000)], 64, 16, 16, 128),
     ([(1, 70), (90, 170)], 64, 12, 2, 192),
+    ([(1, 30)] * 50 + [(50, 700), (33, 33), (0, 4)] * 7, 64, 8, 2, 64),         # more sequences than a wave has lanes, of both kinds
+    ([(40, 2000)], 128, 9, 3, 64),                                               # parts of a tile's tokens, kv heads that do not divide 512
+    ([(1, 1100), (20, 1200)], 64, 96, 1, 32),                                    # a row of more pairs than the few have
 ]
 
 

@@ -3086,7 +3086,8 @@ int ql_paged_attention(ql_ctx* ctx, ql_arena* act, uint64_t q_off, int32_t q_dty
     a.D = paged->D;
     a.half = qb == 2;
     a.scale = (float)(1.4426950408889634 / std::sqrt((double)paged->D));
-    const uint64_t bytes = ql::plan_paged_attention(&a, ql::kAttnTileWsBytes);
+    const uint64_t bytes = ql::plan_paged_attention(&a);
+    if (bytes > ql::kAttnTileWsBytes) return fail(QL_E_INVALID, "attention shape does not fit the workspace");
     std::lock_guard<std::mutex> guard(ctx->ws_lock);
     void* ws;
     QL_HIP(workspace(ctx, ctx->tile_ws, bytes, &ws));

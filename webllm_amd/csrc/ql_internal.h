@@ -400,7 +400,7 @@ struct PagedAttnArgs {
     int few, units, whole, ranges, merge, merge_pairs, decode, prompt, join;
     size_t prompt_ws;
 };
-uint64_t plan_paged_attention(PagedAttnArgs* a, size_t ws_bytes);   // the workspace it needs
+uint64_t plan_paged_attention(PagedAttnArgs* a);   // the workspace it needs, less than kAttnTileWsBytes
 hipError_t launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
 
 constexpr int kLoraMaxRank = 128;
