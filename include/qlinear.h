@@ -355,7 +355,8 @@ int ql_kv_move(ql_ctx* ctx, ql_arena* dst, const uint64_t* dst_offs, int32_t dst
  * rows is token kv_len[s] - 1, the first kv_len[s] - n, and a row's position is its token. Token t lies in page pages[s][t / page_size].
  * The tables are int32 in `act` and read on the device, so a captured graph serves every pass of its sizes. What they may not say is
  * skipped, not followed: a sequence with row_start descending or outside 0..M, with more than max_rows rows, or with kv_len outside n..max_len has no
- * rows at all; a token whose page is outside 0..n_page - 1 is not stored, and no row sees it. Rows behind the last sequence are padding.
+ * rows at all; a token whose page is outside 0..n_page - 1 is not stored, and no row sees it. Rows that two sequences claim have either's result, or none. Rows behind
+ * the last sequence are padding.
  * Rows of q_out and out that belong to no sequence stay as they were. No two sequences may append to one page; they may share pages that they
  * only read. */
 typedef struct ql_batch_desc {
@@ -364,8 +365,8 @@ typedef struct ql_batch_desc {
     uint64_t pages_off;     /* int32 [n_seq, max_pages] */
     int32_t n_seq;          /* 1..4096 */
     int32_t max_pages;      /* pages of a sequence's list */
-    int32_t max_rows;       /* most rows that a sequence has in this pass, and the most tokens that one has: at most max_pages * page_size. */
-    int32_t max_len;        /* and 2^26. They choose the launches; bounds near what the tables hold serve best */
+    int32_t max_rows;       /* no sequence has more rows in this pass, */
+    int32_t max_len;        /* none more tokens: at most max_pages * page_size, and 2^26. Both choose the launches; bounds near what the tables hold serve best */
 } ql_batch_desc;
 /* A layer's paged cache, regions of n_page pages in a cache arena, offsets 16-byte aligned. A page holds page_size tokens of all kv heads, each
  * head's behind the other. D is a multiple of 16, u = 16 bytes of values: 8 (fp16) or 16 (e4m3).
@@ -392,7 +393,7 @@ typedef struct ql_paged_desc {
  * where it grows, the group's earlier tokens are rounded anew under it (exact but for values below 2^-6 of the new scale). Each value is rounded
  * once to e4m3; an infinity or NaN is stored as NaN and does not enter the scale.
  * q_out may be q itself (fp32, same offset, dense rows); any other overlap of what is written with what is read, tables included, fails with
- * QL_E_INVALID. M = 1..65535 rows of the buffers, M * (n_head + 2 n_kv_head) <= 2^26. Offsets 16-byte aligned (tables: 4). */
+ * QL_E_INVALID. M = 1..65535 rows of the buffers, M * (n_head + 2 n_kv_head) <= 2^23. Offsets 16-byte aligned (tables: 4). */
 int ql_paged_append(ql_ctx* ctx, const ql_rope_desc* rope, const ql_arena* weights, ql_arena* act, uint64_t q_off, uint64_t k_off,
                     uint64_t v_off, const ql_batch_desc* batch, int32_t M, uint64_t q_out_off, int32_t q_dtype, ql_arena* cache,
                     const ql_paged_desc* paged);
@@ -400,7 +401,8 @@ int ql_paged_append(ql_ctx* ctx, const ql_rope_desc* rope, const ql_arena* weigh
  * sequence, which the cache holds (ql_paged_append has run). q and out are [M, n_head, D] in `act`, both of q_dtype: fp32 (q as two fp16
  * parts of about 22 bits under its row's exponent, probabilities likewise), or fp16 (probabilities rounded once to fp16, as the result is). Sums and softmax in
  * fp32. A row that sees nothing, or no score above -inf, is zero. What a row does not see adds nothing to it, infinities and NaN included;
- * a value of q that is not finite makes its head's row NaN. Offsets 16-byte aligned. Uses the context's 64 MiB workspace. */
+ * a value of q that is not finite gives its head's row what the formula gives: NaN, or zero where every score is -inf. M * n_head <= 2^23,
+ * n_seq * n_kv_head <= 2^22. Offsets 16-byte aligned. Uses the context's 64 MiB workspace. */
 int ql_paged_attention(ql_ctx* ctx, ql_arena* act, uint64_t q_off, int32_t q_dtype, const ql_arena* cache, const ql_paged_desc* paged,
                        const ql_batch_desc* batch, int32_t M, int32_t n_head, uint64_t out_off);
 /* Low-rank adapters of one projection, all n_adapter of them, in `weights`. */
@@ -416,7 +418,8 @@ typedef struct ql_lora_desc {
  * 0..n_adapter - 1 (-1: a row without an adapter). ids is int32 [M] in `act`; x [M, K] in x_dtype (fp32 or fp16), base and y fp32 [M, N] at
  * x_offs[i], base_offs[i], y_offs[i] in `act`. y_offs[i] may be base_offs[i] (a row without an adapter is not touched);
  * any other overlap of what is written with what is read fails with QL_E_INVALID. Sums in fp32, fp16 products exact; many rows take fp32 x, and x . A^T, as
- * two fp16 parts of about 22 bits each under the exponent of 64 columns, or of the row's ranks.
+ * two fp16 parts of about 22 bits each under the exponent of 64 columns, or of the row's ranks. A value of x that is not finite makes its own row's y infinite or
+ * NaN, no other's.
  * M = 1..65535. Offsets 16-byte aligned (ids, scales: 4). Uses the context's 64 MiB workspace. */
 int ql_lora_add(ql_ctx* ctx, int32_t count, const ql_lora_desc* descs, const ql_arena* weights, ql_arena* act, uint64_t ids_off,
                 const uint64_t* x_offs, int32_t x_dtype, int32_t M, const uint64_t* base_offs, const uint64_t* y_offs);

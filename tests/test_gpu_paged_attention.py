@@ -281,6 +281,50 @@ def test_graph_streams_and_other_calls(ql, ctx):
     other.destroy()
 
 
+@pytest.mark.parametrize("f8", [False, True])
+def test_pages_beyond_32_bits(ql, ctx, f8):
+    """Keys and values appended to and read from the first and last pages of regions of more than 4 GiB, as from pages of a small cache."""
+    KV, D, page, H = 4, 128, 256, 8
+    size = KV * page * D * (1 if f8 else 2)
+    seqs, far = [(300, 300), (1, 70), (40, 600)], (9 << 29) // size
+    batch = Batch(seqs, page, spare=0)
+    small = batch.n_page
+    g = np.random.default_rng(3)
+    box = Box(ql, ctx)
+    box.put("q", g.standard_normal((batch.M, H, D)).astype(np.float32))
+    for n in "kv":
+        box.put(n, g.standard_normal((batch.M, KV, D)).astype(np.float32))
+    box.put("qr", np.zeros((batch.M, H, D), np.float32))
+    box.put("out", np.zeros((batch.M, H, D), np.float32))
+    box.put("table", np.zeros((batch.max_len, D), np.float32))
+    batch.put(box)
+    box.place()
+    ctx.rope_table(box.arena, box.off("table"), batch.max_len, D, 1e4)
+    rope = ql.make_rope(box.off("table"), batch.max_len, H, KV, D, cache_dtype=ql.DTYPE_F8 if f8 else ql.DTYPE_F16)
+    got = []
+    for n_page in (small, far):
+        lay = ql.ArenaLayout()
+        at = [lay.take(n_page * size), lay.take(n_page * size)] + [lay.take(n_page * KV * page // 16 * 4) for _ in range(2 * f8)]
+        cache = ctx.arena(lay.used)
+        where = lambda p: np.where(p < small // 2, p, p + n_page - small)  # noqa: E731
+        box.arena.write(box.off("pages"), np.where(batch.pages < 0, -1, where(batch.pages)).astype(np.int32))
+        for region, bytes_ in zip(at, [size, size, size // D // 4, size // D // 4]):      # zeros, so that what is not appended reads the same
+            for p in where(np.arange(small)):
+                cache.write(int(region + p * bytes_), np.zeros(bytes_, np.uint8))
+        paged = ql.make_paged(at[0], at[1], n_page, page, KV, D, cache_dtype=ql.DTYPE_F8 if f8 else ql.DTYPE_F16,
+                              **(dict(k_scale_off=at[2], v_scale_off=at[3]) if f8 else {}))
+        desc = batch.desc(ql, box)
+        ctx.paged_append(rope, box.arena, box.arena, box.off("q"), box.off("k"), box.off("v"), desc, batch.M, box.off("qr"), ql.DTYPE_F32, cache, paged)
+        ctx.paged_attention(box.arena, box.off("qr"), ql.DTYPE_F32, cache, paged, desc, batch.M, H, box.off("out"))
+        ctx.sync()
+        got.append((box.get("out"), [cache.read(int(at[1] + p * size), (size,), np.uint8) for p in where(np.arange(small))]))
+        cache.release()
+    (a, pa), (b, pb) = got
+    assert a.any() and np.array_equal(a.view(np.uint32), b.view(np.uint32))
+    assert all(np.array_equal(x, y) for x, y in zip(pa, pb)) and any(x.any() for x in pa)
+    box.release()
+
+
 def test_refusals(ql, ctx):
     batch = Batch([(3, 60), (1, 9)], 64)
     call = Call(ql, ctx, batch, 4, 2, 64, True, False)
@@ -299,7 +343,8 @@ def test_refusals(ql, ctx):
         assert e.value.name == name, e.value
 
     for kw in (dict(M=0), dict(M=65536), dict(dt=2), dict(H=0), dict(H=5), dict(H=4098), dict(paged={"cache_dtype": 0}), dict(paged={"page_size": 32}),
-               dict(paged={"n_page": -1}), dict(paged={"D": 8}), dict(desc={"n_seq": 0}), dict(desc={"max_len": (1 << 26) + 1, "max_pages": 1 << 30})):
+               dict(paged={"n_page": -1}), dict(paged={"D": 8}), dict(desc={"n_seq": 0}), dict(desc={"max_len": (1 << 26) + 1, "max_pages": 1 << 30}),
+               dict(M=65535, H=256)):
         refused("QL_E_INVALID", **kw)
     for kw in (dict(q=size), dict(out=size - 16), dict(desc={"max_len": 65}), dict(paged={"n_page": 1 << 30}), dict(paged={"v_scale_off": size}),
                dict(desc={"max_pages": 1 << 28, "max_len": 64})):

@@ -2986,7 +2986,7 @@ int ql_paged_append(ql_ctx* ctx, const ql_rope_desc* d, const ql_arena* weights,
     if (d->n_head < 1 || d->n_head > 4096) return fail(QL_E_INVALID, "n_head must be 1..4096");
     if (d->n_kv_head != paged->n_kv_head || d->D != paged->D || d->cache_dtype != paged->cache_dtype)
         return fail(QL_E_INVALID, "n_kv_head, D or cache_dtype differ between the rotation and the cache");
-    if ((int64_t)M * (d->n_head + 2 * d->n_kv_head) > ql::kRopeMaxHeads) return fail(QL_E_INVALID, "M x (n_head + 2 n_kv_head) above %d", ql::kRopeMaxHeads);
+    if ((int64_t)M * (d->n_head + 2 * d->n_kv_head) > ql::kPagedMaxHeads) return fail(QL_E_INVALID, "M x (n_head + 2 n_kv_head) above %d", ql::kPagedMaxHeads);
     if (d->rot_dim < 8 || d->rot_dim > d->D || d->rot_dim % 8) return fail(QL_E_INVALID, "rot_dim must be 8..D, a multiple of 8 (got %d)", d->rot_dim);
     if ((d->interleaved & ~1) || d->reserved) return fail(QL_E_INVALID, "interleaved must be 0 or 1, reserved 0");
     if (d->max_pos < batch->max_len) return fail(QL_E_RANGE, "max_len %d exceeds the rope table's %d positions", batch->max_len, d->max_pos);
@@ -3064,6 +3064,8 @@ int ql_paged_attention(ql_ctx* ctx, ql_arena* act, uint64_t q_off, int32_t q_dty
     int rc = paged_regions(paged, cache, &cb, reads);
     if (rc || (rc = batch_tables(batch, paged, act, M, &a.b, reads + 4))) return rc;
     if (n_head < 1 || n_head > 4096 || n_head % paged->n_kv_head) return fail(QL_E_INVALID, "n_head (%d) must be 1..4096, a multiple of n_kv_head (%d)", n_head, paged->n_kv_head);
+    if ((int64_t)M * n_head > ql::kPagedMaxHeads || (int64_t)batch->n_seq * paged->n_kv_head > ql::kPagedMaxSeqHeads)
+        return fail(QL_E_INVALID, "M x n_head above %d, or n_seq x n_kv_head above %d", ql::kPagedMaxHeads, ql::kPagedMaxSeqHeads);
     if (!dtype_bytes(q_dtype, &qb)) return fail(QL_E_INVALID, "bad q_dtype %d", q_dtype);
     if ((rc = check_devices(ctx, act, cache, nullptr))) return rc;
     const uint64_t qo = (uint64_t)M * n_head * paged->D * qb;

@@ -370,6 +370,7 @@ hipError_t launch_kv_move(MoveArgs& a, hipStream_t stream);
 
 constexpr int kPagedMaxSeqs = 4096;
 constexpr int kPagedMaxLen = 1 << 26;            // blocks of 64 sequences at a time are counted in 32 bits
+constexpr int kPagedMaxHeads = 1 << 23, kPagedMaxSeqHeads = 1 << 22;   // rows' heads, sequences' kv heads: a grid has less than 2^32 threads, 256 for each at most
 // a batch's tables on the device and their bounds
 struct PagedBatch {
     const int32_t *row_start, *kv_len, *pages;   // [S + 1], [S], [S, max_pages]
