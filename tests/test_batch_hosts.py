@@ -80,6 +80,25 @@ def test_batches_that_are_none():
             gptq.PagedKvCache(ctx, CFG, **{"pages": 4, **kw})
 
 
+def test_pages_that_two_append_to():
+    """Two sequences cut within a page that both hold: one copy, if nobody else holds it; a batch whose tables find no room takes nothing."""
+    ctx, kv, pool = cache_of(3)
+    a = kv.new_sequence()
+    kv.batch(pool, [(a, 64)])
+    b = kv.fork(a)
+    kv.cut(a, 10), kv.cut(b, 10)
+    kv.batch(pool, [(kv.new_sequence(), 64)])
+    assert kv.free_pages == 1
+    with pytest.raises(ValueError, match="exhausted"):
+        kv.batch(gptq.ActivationArena(ctx, 256), [(a, 1), (b, 1)])
+    assert kv.free_pages == 1 and kv.length(a) == 10 and kv._lists[a] == kv._lists[b] and not ctx.log
+    kv.batch(pool, [(a, 1), (b, 1)])
+    assert kv.free_pages == 0 and kv._lists[a] != kv._lists[b] and len(ctx.log) == 2 and kv.length(b) == 11
+    c = kv.fork(kv.new_sequence())
+    with pytest.raises(ValueError, match="1 pages"):
+        kv.batch(pool, [(c, 1)])
+
+
 def test_fork_shares_whole_pages():
     ctx, kv, pool = cache_of(6)
     a = kv.new_sequence()

@@ -476,23 +476,25 @@ class PagedKvCache:
             raise ValueError(f"batch: {total} rows for tensors of {M}")
         lengths = [self._lengths[s] + n for s, n in sequences]
         lists = [self._lists[s] for s in order]
-        # a page that the pass appends to is the sequence's alone: one that others hold as well (cut in the middle of a shared one) is copied first
-        shared = [i for i, (s, n) in enumerate(sequences) if n and self._lengths[s] % self.page_size and self._users[lists[i][self._lengths[s] // self.page_size]] > 1]
-        need = sum(max(0, -(-L // self.page_size) - len(p)) for L, p in zip(lengths, lists)) + len(shared)
+        # a page that the pass appends to is the sequence's alone: one that others hold as well (cut in the middle of a shared one) is copied first,
+        # by all who append to it, or by all but the last where nobody else holds it
+        at = [self._lengths[s] // self.page_size if n and self._lengths[s] % self.page_size else -1 for s, n in sequences]
+        writers = [p[i] for p, i in zip(lists, at) if i >= 0]
+        copies = sum(writers.count(p) - (self._users[p] == writers.count(p)) for p in set(writers))
+        need = sum(max(0, -(-L // self.page_size) - len(p)) for L, p in zip(lengths, lists)) + copies
         if need > len(self._free):
             raise ValueError(f"batch: {need} pages for {len(self._free)} that are left")
-        for i in shared:
-            at = self._lengths[order[i]] // self.page_size
-            if self._users[lists[i][at]] > 1:                              # not since another of the pass left it
-                new = self._copy(lists[i][at])
-                self._drop(lists[i][at])
-                lists[i][at] = new
-        for s, L, pages in zip(order, lengths, lists):
-            while len(pages) < -(-L // self.page_size):
-                pages.append(self._take())
-            self._lengths[s] = L
-        most = max(1, max(len(p) for p in lists))
+        most = max(1, max(max(len(p), -(-L // self.page_size)) for L, p in zip(lengths, lists)))
         row_start, kv_len, pages = pool.alloc((len(order) + 1,), "i32"), pool.alloc((len(order),), "i32"), pool.alloc((len(order), most), "i32")
+        for i, own in zip(at, lists):
+            if i >= 0 and self._users[own[i]] > 1:
+                new = self._copy(own[i])
+                self._drop(own[i])
+                own[i] = new
+        for s, L, own in zip(order, lengths, lists):
+            while len(own) < -(-L // self.page_size):
+                own.append(self._take())
+            self._lengths[s] = L
         row_start.write(np.cumsum([0] + rows).astype(np.int32))
         kv_len.write(np.array(lengths, np.int32))
         pages.write(np.array([p + [-1] * (most - len(p)) for p in lists], np.int32))
