@@ -118,6 +118,10 @@ export class QuantLinearModel {
     tokenLogprobs(logits: Tensor, M: number, V: number, o: {
         tokens?: Tensor | null; logprobs?: Tensor | null; entropy?: Tensor | null; topIds?: Tensor | null; topLogprobs?: Tensor | null;
     }): void;
+    /** low-rank adapters of a linear: a fp16 bits [n, rank, K], b fp16 bits [n, N, rank], scale [n] (left out: 1) */
+    uploadLora(weight: string, a: Uint16Array, b: Uint16Array, n: number, rank: number, scale?: ArrayLike<number> | null): void;
+    /** each C += scale * (A . a^T) . b^T by each row's id (i32 [M]; -1: none), up to 8 linears (ql_lora_add) */
+    loraAdd(A: Tensor, weights: string[], ids: Tensor, Cs: Tensor[], M: number): void;
     unpackF16(name: string, out: Tensor): void;
     /** fp16 [N,K] copies of many weights in a few launches (ql_unpack_f16_batch). */
     unpackAllF16(names: string[], outs: Tensor[]): void;
@@ -144,6 +148,35 @@ export class KvCache {
     accept(pastLen: number, path: Tensor, n: number): void;
     /** the first rows of every layer into another cache (ql_kv_move); one of another context: waits for its stream and for the copy */
     fork(to: KvCache, rows: number): void;
+    release(): void;
+}
+
+/** QL_DTYPE_F8: e4m3 values under powers of two (paged caches) */
+export const QL_DTYPE_F8: 2;
+/** A pass's rows of several sequences (PagedKvCache.batch): M rows of the tensors, `rows` of them the sequences'. */
+export interface Batch {
+    desc: { rowStartOff: number; kvLenOff: number; pagesOff: number; nSeq: number; maxPages: number; maxRows: number; maxLen: number };
+    M: number; rows: number; tables: Tensor[];
+}
+/** K and V of many sequences in pages of 64, 128 or 256 tokens, fp16 or e4m3 under powers of two; sequences are numbers. */
+export class PagedKvCache {
+    constructor(ctx: Context, config: QwenConfig, pages: number, pageSize?: 64 | 128 | 256, dtype?: 'f16' | 'f8');
+    readonly D: number;
+    readonly rowLen: number;
+    readonly freePages: number;
+    newSequence(): number;
+    length(sequence: number): number;
+    free(sequence: number): void;
+    cut(sequence: number, tokens: number): void;
+    /** a sequence that continues another one: whole pages shared, the last one copied (ql_kv_move) */
+    fork(sequence: number): number;
+    /** takes the pages of a pass's rows and counts its tokens: once a pass, before its layers */
+    batch(pool: ActivationArena, sequences: [number, number][], M?: number): Batch;
+    /** norms (where named), rotation by the rows' positions, k and v to their pages (ql_paged_append) */
+    append(layer: number, model: QuantLinearModel, q: Tensor, k: Tensor, v: Tensor, batch: Batch, qOut: Tensor,
+           options?: { rope?: string; qNorm?: string; kNorm?: string; eps?: number }): void;
+    /** causal GQA attention of the batch's rows over their sequences (ql_paged_attention); q and out both f32 or both f16 */
+    attend(layer: number, q: Tensor, out: Tensor, batch: Batch): void;
     release(): void;
 }
 

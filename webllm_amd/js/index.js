@@ -28,9 +28,11 @@ if (!fs.existsSync(ADDON_PATH)) {
     throw new Error(`qlinear: addon not built at ${ADDON_PATH} (run __graft_entry__.build())`);
 }
 const addon = require(ADDON_PATH);
+const batchAddon = require(path.join(__dirname, '..', 'lib', 'qlinear_batch_napi.node'));   // passes over many requests, on the same handles
 
 const QL_DTYPE_F32 = 0;
 const QL_DTYPE_F16 = 1;
+const QL_DTYPE_F8 = 2;
 
 // ------------------------------------------------------------------ config (qwen-config.ts)
 
@@ -361,6 +363,7 @@ class QuantLinearModel {
         this.linears = new Map();
         this.f32Weights = new Map();
         this.f16Weights = new Map();
+        this.loras = new Map();
     }
     get weightBytes() { return this.layout.used; }
     _place(typed) {
@@ -514,6 +517,37 @@ class QuantLinearModel {
         addon.linearBatch(this.ctx.handle, descs, this.weights.handle, A.arena.handle,
             descs.map(() => A.offset), A.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32, M,
             Cs.map((c) => c.offset), scratch);
+    }
+    /**
+     * Low-rank adapters of a linear, all of them: a fp16 bits [n, rank, K], b fp16 bits [n, N, rank] (Uint16Array), scale [n] (each one's
+     * alpha / rank; left out: 1). Adapters of lower ranks have zeros behind their own.
+     */
+    uploadLora(weight, a, b, n, rank, scale) {
+        if (this.loras.has(weight)) throw new Error(`adapters already exist: ${weight}`);
+        const { K, N } = this.linear(weight);
+        if (!(n >= 1) || rank < 8 || rank > 128 || rank % 8 || K % 8 || N % 4) throw new Error('lora: rank must be 8..128, a multiple of 8, K a multiple of 8, N of 4');
+        if (!(a instanceof Uint16Array) || !(b instanceof Uint16Array) || a.length !== n * rank * K || b.length !== n * rank * N || (scale && scale.length !== n))
+            throw new Error(`lora: ${weight} is [${N},${K}], ${n} adapters of rank ${rank} do not fit`);
+        const s = scale ? Float32Array.from(scale) : new Float32Array(n).fill(1);
+        this.loras.set(weight, { aOff: this._place(a), bOff: this._place(b), scaleOff: this._place(s), K, N, rank, nAdapter: n });
+    }
+    /**
+     * Each C [M, N] += scale * (A . a^T) . b^T of its linear's adapters, by each row's id (i32 [M]; -1: none): after gemm or gemmBatch on the
+     * same A (f32 or f16), up to 8 linears (q/k/v, gate/up) in one call.
+     */
+    loraAdd(A, weights, ids, Cs, M) {
+        const loras = weights.map((w) => {
+            if (!this.loras.has(w)) throw new Error(`missing adapters: ${w}`);
+            return this.loras.get(w);
+        });
+        if (Cs.length !== loras.length) throw new Error(`loraAdd: ${Cs.length} outputs for ${loras.length} linears`);
+        if (ids.dtype !== 'i32' || ids.length < M) throw new Error('loraAdd: ids must be an i32 tensor of at least M');
+        if ((A.dtype !== 'f32' && A.dtype !== 'f16') || Cs.some((c) => c.dtype !== 'f32')) throw new Error('loraAdd: A must be f32 or f16, C f32');
+        if (ids.arena !== A.arena || Cs.some((c) => c.arena !== A.arena)) throw new Error('loraAdd: tensors must share one arena');
+        if (loras.some((l, i) => A.length < M * l.K || Cs[i].length < M * l.N)) throw new Error('loraAdd: tensor too small for [M,K] / [M,N]');
+        const offs = Cs.map((c) => c.offset);
+        batchAddon.loraAdd(this.ctx.handle, loras, this.weights.handle, A.arena.handle, ids.offset, Cs.map(() => A.offset),
+            A.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32, M, offs, offs);
     }
     /** fp16 [N,K] copy, bit-identical to the reference's uploaded f16 weight buffer. */
     unpackF16(name, out) {
@@ -799,11 +833,180 @@ class KvCache {
     release() { this.arena.release(); }
 }
 
+/**
+ * K and V of many sequences in pages that they take as they grow, in one device arena, for passes over many requests at once: append and
+ * attend run per layer over a batch. dtype 'f16', or 'f8': e4m3 values with a power of two for every 16 tokens of a head. Sequences are
+ * numbers (newSequence); what they hold is counted on the host. batch() takes the pages that a pass needs and counts its tokens, so it is
+ * called once, before the pass's layers; its tables are read on the device when a pass runs.
+ */
+class PagedKvCache {
+    constructor(ctx, config, pages, pageSize, dtype) {
+        this.dtype = dtype || 'f16';
+        this.pageSize = pageSize || 64;
+        if (this.dtype !== 'f16' && this.dtype !== 'f8') throw new Error(`paged kv cache: dtype ${dtype}`);
+        if (!(pages >= 1) || ![64, 128, 256].includes(this.pageSize)) throw new Error('paged kv cache: at least one page, of 64, 128 or 256 tokens');
+        this.ctx = ctx;
+        this.config = config;
+        this.pages = pages;
+        this.D = qwenHeadDim(config);
+        this.rowLen = qwenKvDim(config);
+        const f8 = this.dtype === 'f8';
+        this.pageBytes = this.pageSize * this.rowLen * (f8 ? 1 : 2);
+        this.scaleBytes = f8 ? config.nKvHead * (this.pageSize / 16) * 4 : 0;      // of a page
+        const layout = new ArenaLayout();
+        this.regions = Array.from({ length: 2 * config.nLayer }, () => layout.take(pages * this.pageBytes));
+        this.scales = f8 ? Array.from({ length: 2 * config.nLayer }, () => layout.take(pages * this.scaleBytes)) : [];
+        this.arena = ctx.arena(layout.used);
+        this._free = Array.from({ length: pages }, (_, i) => pages - 1 - i);
+        this._users = new Array(pages).fill(0);           // sequences that hold a page
+        this._lists = new Map();
+        this._lengths = new Map();
+        this._next = 0;
+    }
+    get freePages() { return this._free.length; }
+    newSequence() {
+        const s = this._next++;
+        this._lists.set(s, []);
+        this._lengths.set(s, 0);
+        return s;
+    }
+    length(sequence) { return this._lengths.get(this._known(sequence)); }
+    _known(sequence) {
+        if (!this._lists.has(sequence)) throw new Error(`no such sequence: ${sequence}`);
+        return sequence;
+    }
+    _take() {
+        const p = this._free.pop();
+        this._users[p] = 1;
+        return p;
+    }
+    _drop(page) { if (--this._users[page] === 0) this._free.push(page); }
+    _copy(page) {
+        const to = this._take();
+        for (const [offs, size] of [[this.regions, this.pageBytes], [this.scales, this.scaleBytes]]) {
+            for (let i = 0; i < offs.length; i += 256) {
+                const some = offs.slice(i, i + 256);
+                addon.kvMove(this.ctx.handle, this.arena.handle, some, this.pages, this.arena.handle, some, this.pages, size, to, page, 1, null, null);
+            }
+        }
+        return to;
+    }
+    /** A finished sequence's pages go back, but for those that others hold. */
+    free(sequence) {
+        for (const p of this._lists.get(this._known(sequence))) this._drop(p);
+        this._lists.delete(sequence);
+        this._lengths.delete(sequence);
+    }
+    /** The sequence's first tokens are kept (a rejected draft, an edited prompt). */
+    cut(sequence, tokens) {
+        if (!(tokens >= 0 && tokens <= this.length(sequence)) || !Number.isInteger(tokens)) throw new Error(`cut: sequence ${sequence} has ${this.length(sequence)} tokens`);
+        const pages = this._lists.get(sequence);
+        while (pages.length > Math.ceil(tokens / this.pageSize)) this._drop(pages.pop());
+        this._lengths.set(sequence, tokens);
+    }
+    /** A sequence that continues another one: its whole pages are shared, the last one, where it is not full, is copied. */
+    fork(sequence) {
+        const tokens = this.length(sequence), pages = this._lists.get(sequence), whole = Math.floor(tokens / this.pageSize);
+        if (whole < pages.length && !this._free.length) throw new Error('fork: no page left');
+        const s = this.newSequence(), own = pages.slice(0, whole);
+        for (const p of own) this._users[p]++;
+        this._lists.set(s, own);
+        this._lengths.set(s, tokens);
+        if (whole < pages.length) own.push(this._copy(pages[whole]));
+        return s;
+    }
+    /**
+     * Rows of a pass: [sequence, rows] in the order of the rows, each sequence once. Takes the pages that their tokens need and counts the tokens;
+     * M: rows of the pass's tensors (those behind the sequences' are padding).
+     */
+    batch(pool, sequences, M) {
+        const order = sequences.map(([s]) => this._known(s)), rows = sequences.map(([, n]) => n);
+        if (!order.length || new Set(order).size !== order.length || rows.some((n) => !Number.isInteger(n) || n < 0))
+            throw new Error('batch: at least one sequence, each once, with no negative rows');
+        const total = rows.reduce((a, b) => a + b, 0), m = M === undefined ? Math.max(total, 1) : M, P = this.pageSize;
+        if (m < total) throw new Error(`batch: ${total} rows for tensors of ${m}`);
+        const lists = order.map((s) => this._lists.get(s)), lengths = order.map((s, i) => this._lengths.get(s) + rows[i]);
+        // a page that the pass appends to is the sequence's alone: one that others hold as well (cut in the middle of a shared one) is copied first,
+        // by all who append to it, or by all but the last where nobody else holds it
+        const at = order.map((s, i) => (rows[i] && this._lengths.get(s) % P ? Math.floor(this._lengths.get(s) / P) : -1));
+        const writers = new Map();
+        at.forEach((k, i) => { if (k >= 0) writers.set(lists[i][k], (writers.get(lists[i][k]) || 0) + 1); });
+        let need = 0;
+        for (const [p, n] of writers) need += n - (this._users[p] === n ? 1 : 0);
+        lengths.forEach((L, i) => { need += Math.max(0, Math.ceil(L / P) - lists[i].length); });
+        if (need > this._free.length) throw new Error(`batch: ${need} pages for ${this._free.length} that are left`);
+        const most = Math.max(1, ...lengths.map((L, i) => Math.max(lists[i].length, Math.ceil(L / P))));
+        const rowStart = pool.alloc([order.length + 1], 'i32'), kvLen = pool.alloc([order.length], 'i32'), pages = pool.alloc([order.length, most], 'i32');
+        at.forEach((k, i) => {
+            if (k < 0 || this._users[lists[i][k]] === 1) return;
+            const to = this._copy(lists[i][k]);
+            this._drop(lists[i][k]);
+            lists[i][k] = to;
+        });
+        const table = new Int32Array(order.length * most).fill(-1), starts = new Int32Array(order.length + 1);
+        order.forEach((s, i) => {
+            while (lists[i].length < Math.ceil(lengths[i] / P)) lists[i].push(this._take());
+            this._lengths.set(s, lengths[i]);
+            table.set(lists[i], i * most);
+            starts[i + 1] = starts[i] + rows[i];
+        });
+        rowStart.write(starts);
+        kvLen.write(Int32Array.from(lengths));
+        pages.write(table);
+        const desc = {
+            rowStartOff: rowStart.offset, kvLenOff: kvLen.offset, pagesOff: pages.offset, nSeq: order.length, maxPages: most,
+            maxRows: Math.max(1, ...rows), maxLen: Math.max(1, ...lengths),
+        };
+        return { desc, M: m, rows: total, tables: [rowStart, kvLen, pages] };
+    }
+    desc(layer) {
+        if (!(layer >= 0 && layer < this.config.nLayer)) throw new Error(`layer ${layer} out of range`);
+        const k = 2 * layer, v = k + 1, f8 = this.dtype === 'f8';
+        return {
+            kOff: this.regions[k], vOff: this.regions[v], kScaleOff: f8 ? this.scales[k] : null, vScaleOff: f8 ? this.scales[v] : null, nPage: this.pages,
+            pageSize: this.pageSize, nKvHead: this.config.nKvHead, D: this.D, cacheDtype: f8 ? QL_DTYPE_F8 : QL_DTYPE_F16,
+        };
+    }
+    /**
+     * q and k turned by their rows' positions, normed per head first where weights are named; q to qOut (f32, where q itself may be given, or f16),
+     * k and v to their places in the sequences' pages. Rows of padding stay as they were.
+     */
+    append(layer, model, q, k, v, batch, qOut, options) {
+        const o = options || {}, c = this.config, M = batch.M;
+        if ([k, v, qOut, ...batch.tables].some((t) => t.arena !== q.arena)) throw new Error('append: tensors must share one arena');
+        if (q.length < M * c.nHead * this.D || qOut.length < M * c.nHead * this.D || k.length < M * this.rowLen || v.length < M * this.rowLen ||
+            [q, k, v].some((t) => t.dtype !== 'f32') || (qOut.dtype !== 'f32' && qOut.dtype !== 'f16'))
+            throw new Error('append: a tensor is too small or of another type');
+        const weight = (name, length) => {
+            const w = model.f32Weights.get(name);
+            if (!w || (length ? w.length !== length : w.shape.length !== 2)) throw new Error(`missing f32 weight: ${name}`);
+            return w;
+        };
+        const table = weight(o.rope || 'rope'), paged = this.desc(layer);
+        batchAddon.pagedAppend(this.ctx.handle, {
+            tableOff: table.offset, maxPos: table.shape[0], nHead: c.nHead, nKvHead: c.nKvHead, D: this.D, rotDim: table.shape[1], interleaved: 0,
+            qNormOff: o.qNorm ? weight(o.qNorm, this.D).offset : null, kNormOff: o.kNorm ? weight(o.kNorm, this.D).offset : null,
+            normEps: o.eps === undefined ? 1e-6 : o.eps, qStride: 0, kStride: 0, vStride: 0, cacheDtype: paged.cacheDtype,
+        }, model.weights.handle, q.arena.handle, q.offset, k.offset, v.offset, batch.desc, M, qOut.offset,
+        qOut.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32, this.arena.handle, paged);
+    }
+    /** out [M, nHead * D] = causal GQA attention of the batch's rows over their sequences; q and out both f32 or both f16. */
+    attend(layer, q, out, batch) {
+        const c = this.config, M = batch.M;
+        if ([out, ...batch.tables].some((t) => t.arena !== q.arena)) throw new Error('attend: q, out and the batch must share one arena');
+        if ((q.dtype !== 'f32' && q.dtype !== 'f16') || out.dtype !== q.dtype || q.length < M * c.nHead * this.D || out.length < M * c.nHead * this.D)
+            throw new Error('attend: a tensor is too small or of another type');
+        batchAddon.pagedAttention(this.ctx.handle, q.arena.handle, q.offset, q.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32, this.arena.handle,
+            this.desc(layer), batch.desc, M, c.nHead, out.offset);
+    }
+    release() { this.arena.release(); }
+}
+
 module.exports = {
     addon, ADDON_PATH, QL_DTYPE_F32, QL_DTYPE_F16, QWEN25_05B, qwenHeadDim, qwenKvDim, Seq,
     dtypeByteSize, parseSafetensorsHeader, parseSafetensors, tensorCount, requireTensor,
     expectTensor, f16BitsToF32, readTensorBytes, readTensorF32, ArenaLayout, Arena, Context,
     makeDesc, dequantizeGptqInt4, Tensor, ActivationArena, QuantLinearModel,
     qwenLinearShapes, loadQwenWeights, KvCache, QWEN_LOCAL_DIR, urlToPath, readF16Rows, checkGIdx,
-    countStoredZeros, treeMasks,
+    countStoredZeros, treeMasks, batchAddon, QL_DTYPE_F8, PagedKvCache,
 };
