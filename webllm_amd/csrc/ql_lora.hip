@@ -288,9 +288,9 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDo
     }
 }
 
-// Y = T B^T: lane = column, registers = rows 4 g + r, so that 16 lanes of y are a row's 64 bytes. A workgroup has 16 RT rows and 256 columns of a
-// projection, a wave 64 of them; the projections' columns lie one behind the other in blockIdx.x. An adapter's B of the 256 columns is one
-// stretch of memory: it goes to LDS as it lies, but for the order of a row's pieces, c ^ (n % their number) where that is a power of two.
+// Y = T B^T: lane = column, registers = rows 4 g + r. A workgroup has 16 RT rows and 256 columns of a projection, a wave 64 of them in four tiles, tile j's column i
+// being 4 i + j: a lane's four results of a row are 16 bytes, a row's 256 in a row; the projections' columns lie one behind the other in blockIdx.x. An adapter's B of the 256 columns is one
+// stretch of memory: it goes to LDS as it lies, but for the order of a row's pieces, c ^ (n / 4 % their number) where that is a power of two.
 template <int STEPS, int RT>
 __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
 {
@@ -310,7 +310,8 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
     uint64_t left = rows_below(id, p.n);
     const uint64_t all = left;
     if (!left && !apart) return;
-    float y[RT][4][4];
+    f32x4 y[RT][4];                                         // rows 4 g + r, the lane's four columns
+    const int nl = 64 * wave + 4 * i16;
     f16x8 hi[RT][STEPS], lo[RT][STEPS];
     float up[RT];
 #pragma unroll
@@ -324,12 +325,10 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
             if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank) load8(t_in, 0, (size_t)m * p.rank + 32 * st + 8 * g, v[st]);
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int mr = m0 + 16 * t + 4 * g + r, n = 64 * wave + 16 * j + i16;
-                y[t][j][r] = mr < a.M && n < cols ? ld_global(p.base + (size_t)mr * p.N + n0 + n) : 0.f;
-            }
+        for (int r = 0; r < 4; r++) {
+            const int mr = m0 + 16 * t + 4 * g + r;
+            y[t][r] = mr < a.M && nl < cols ? ld_global(reinterpret_cast<const f32x4*>(p.base + (size_t)mr * p.N + n0 + nl)) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
         if (a.parts[proj] > 1)                              // the other parts of K, in order
 #pragma unroll
             for (int st = 0; st < STEPS; st++)
@@ -363,18 +362,18 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
         const int all_pieces = cols * pieces;
         for (int u = tid; u < (all_pieces + 63) / 64 * 64; u += 256) {
             const int at = min(u, all_pieces - 1), n = at / pieces, c = at - n * pieces;
-            load_to_lds(B + (n * pieces + (c ^ (n & turn))) * 16, lds + (u - lane) * 16);
+            load_to_lds(B + (n * pieces + (c ^ (n >> 2 & turn))) * 16, lds + (u - lane) * 16);
         }
         wave_arrived();
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const int n = 64 * wave + 16 * j + i16;
+            const int n = nl + j;
             f16x8 w[STEPS];
 #pragma unroll
             for (int st = 0; st < STEPS; st++) {
                 const int c = 4 * st + g;
-                w[st] = n < cols && c < pieces ? *reinterpret_cast<const f16x8*>(lds + (n * pieces + (c ^ (n & turn))) * 16) : f16x8{};
+                w[st] = n < cols && c < pieces ? *reinterpret_cast<const f16x8*>(lds + (n * pieces + (c ^ (n >> 2 & turn))) * 16) : f16x8{};
             }
 #pragma unroll
             for (int t = 0; t < RT; t++) {
@@ -387,7 +386,7 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const bool take = mine >> (16 * t + 4 * g + r) & 1;
-                    y[t][j][r] = take ? fmaf(fmaf(ol[r], 1.f / 2048.f, o[r]), up_of[t][r], y[t][j][r]) : y[t][j][r];
+                    y[t][r][j] = take ? fmaf(fmaf(ol[r], 1.f / 2048.f, o[r]), up_of[t][r], y[t][r][j]) : y[t][r][j];
                 }
             }
         }
@@ -396,12 +395,10 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
 #pragma unroll
     for (int t = 0; t < RT; t++)
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int mr = m0 + 16 * t + 4 * g + r, n = 64 * wave + 16 * j + i16;
-                if (mr < a.M && n < cols && ((all >> (16 * t + 4 * g + r) & 1) || apart)) st_global(p.y + (size_t)mr * p.N + n0 + n, y[t][j][r]);
-            }
+        for (int r = 0; r < 4; r++) {
+            const int mr = m0 + 16 * t + 4 * g + r;
+            if (mr < a.M && nl < cols && ((all >> (16 * t + 4 * g + r) & 1) || apart)) st_global(reinterpret_cast<f32x4*>(p.y + (size_t)mr * p.N + n0 + nl), y[t][r]);
+        }
 }
 
 }  // namespace
