@@ -94,7 +94,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void lora_row_kernel(const LoraArgs
 constexpr int kDownWaves = 4, kDownGroup = 4;      // waves of a workgroup; most tiles of 16 ranks that it makes
 constexpr int kDownTiles = 24;                     // of a launch
 constexpr int kUpRows = 32, kUpCols = 256;         // rows of a pass are a multiple; columns of a workgroup
-constexpr int kTwoTiles = 1024;                    // rows from which an adapter's B in LDS serves two tiles of 16 rows (4096 rows of rank 64: one 47 us, two 45, four 59)
+constexpr int kTwoTiles = 1024;                    // rows from which what is in LDS of an adapter serves two tiles of 16 rows (its B, 4096 rows of rank 64: one 47 us, two 45, four 59)
 
 // The ranks of all projections that read one x, in tiles of 16
 struct LoraDown {
@@ -166,24 +166,56 @@ __device__ __forceinline__ void split_f16(const float (&x)[8], float s, f16x8& h
 // the power of two that brings mx to [2^14, 2^15)
 __device__ __forceinline__ float scale_of(float mx) { return mx > 0.f && mx <= kMaxFinite ? ldexpf(1.f, min(100, 14 - ilogbf(mx))) : 1.f; }
 
+// Of a step of 64 columns: a lane's 16 columns of row i16 of x from `x`, as parts under `1 / up`. Columns that are not there are zeros.
+template <bool HALF>
+__device__ __forceinline__ void x_parts(const char* x, int i16, int g, const bool (&in)[2], f16x8 (&hi)[2], f16x8 (&lo)[2], float& up)
+{
+    up = 1.f;
+    if constexpr (HALF) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) hi[h] = in[h] ? *reinterpret_cast<const f16x8*>(x + ((2 * g + h) ^ (i16 & 7)) * 16) : f16x8{};
+    } else {
+        float v[2][8], mx = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const f32x4 y = *reinterpret_cast<const f32x4*>(x + ((4 * g + q) ^ i16) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v[q >> 1][4 * (q & 1) + e] = in[q >> 1] ? y[e] : 0.f;
+                mx = fmaxf(mx, fabsf(v[q >> 1][4 * (q & 1) + e]));
+            }
+        }
+        mx = pair_max<32>(pair_max<16>(mx));
+        const float s = scale_of(mx);
+        up = 1.f / s;
+#pragma unroll
+        for (int h = 0; h < 2; h++) split_f16(v[h], s, hi[h], lo[h]);
+    }
+}
 // A wave has a quarter of K, 64 columns at a time. Fragments are 16 rows' 16 bytes, which as loads would be a line a lane (60 lines a load, 45 us a pass of 4096
 // rows of rank 64 for 8): rows come whole into a part of LDS that is the wave's own, 128 bytes of eight rows a load, and are turned there; the next
 // 64 columns are on their way meanwhile. The 16-byte pieces of row r lie in the order c ^ (r % 8), so that a fragment's reads meet no bank twice.
-template <bool HALF, int TILES>
+template <bool HALF, int TILES, int RT>
 struct DownLds {
-    static constexpr int kXRow = HALF ? 128 : 256;          // bytes of a row of x, of 64 columns
-    static constexpr int kStep = TILES * 2048 + 16 * kXRow; // of a wave's step
-    static constexpr int kBytes = 2 * kDownWaves * kStep > kDownWaves * TILES * 1024 ? 2 * kDownWaves * kStep : kDownWaves * TILES * 1024;
+    static constexpr int kXRow = HALF ? 128 : 256;               // bytes of a row of x, of 64 columns
+    static constexpr int kStep = TILES * 2048 + RT * 16 * kXRow; // of a wave's step
+    static constexpr int kEnd = kDownWaves * RT * TILES * 1024;  // of the waves' sums
+    static constexpr int kBytes = 2 * kDownWaves * kStep > kEnd ? 2 * kDownWaves * kStep : kEnd;
 };
 
-template <bool HALF, int TILES>
+template <bool HALF, int TILES, int RT>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDown d)
 {
-    using L = DownLds<HALF, TILES>;
+    using L = DownLds<HALF, TILES, RT>;
     __shared__ __attribute__((aligned(16))) char lds[2][L::kBytes / 2];
-    const int m0 = 16 * blockIdx.x, u0 = TILES * blockIdx.y, tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
+    // the groups of ranks of the same rows on one XCD, one after the other: x comes from its L2 for all but the first
+    const int groups = (d.tiles + TILES - 1) / TILES, turn = blockIdx.x / (8 * groups), in_turn = blockIdx.x - turn * 8 * groups;
+    const int m0 = 16 * RT * (8 * turn + in_turn % 8), u0 = TILES * (in_turn / 8), tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
+    if (m0 >= d.M) return;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id[1] = {m0 + i16 < d.M ? ld_global(d.ids + m0 + i16) : -1};
+    int id[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) id[t] = m0 + 16 * t + i16 < d.M ? ld_global(d.ids + m0 + 16 * t + i16) : -1;
     uint64_t left = rows_below(id, d.most);
     const int steps = (d.K + 63) / 64, per = (steps + d.parts * kDownWaves - 1) / (d.parts * kDownWaves);
     const int s0 = (blockIdx.z * kDownWaves + wave) * per, s1 = min(steps, s0 + per);
@@ -208,15 +240,17 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDo
 #pragma unroll
                 for (int h = 0; h < 2; h++) load_to_lds(w[u][h] + k, to + u * 2048 + h * 1024);
 #pragma unroll
-            for (int j = 0; j < 16 / xp; j++) {
+            for (int j = 0; j < RT * 16 / xp; j++) {
                 const int r = j * xp + xr, m = min(m0 + r, d.M - 1);
-                const int c = HALF ? ac : (lane & 15) ^ r, kx = 64 * st + (HALF ? 8 : 4) * c, kk = kx < d.K ? kx : 0;
+                const int c = HALF ? ac : (lane & 15) ^ (r & 15), kx = 64 * st + (HALF ? 8 : 4) * c, kk = kx < d.K ? kx : 0;
                 load_to_lds(static_cast<const char*>(d.x) + ((size_t)m * d.K + kk) * (HALF ? 2 : 4), to + TILES * 2048 + j * 1024);
             }
         };
-        f32x4 acc[TILES];
+        f32x4 acc[TILES][RT];
 #pragma unroll
-        for (int u = 0; u < TILES; u++) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < TILES; u++)
+#pragma unroll
+            for (int t = 0; t < RT; t++) acc[u][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (s0 < s1) fetch(s0, s0 & 1);
         for (int st = s0; st < s1; st++) {
             wave_arrived();
@@ -224,47 +258,30 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDo
             const char* const from = lds[st & 1] + wave * L::kStep;
             const int k = 64 * st + 16 * g;
             const bool in[2] = {k < d.K, k + 8 < d.K};      // K is a multiple of eight
-            f16x8 hi[2], lo[2];
-            float up = 1.f;
-            const char* const x = from + TILES * 2048 + i16 * L::kXRow;
-            if constexpr (HALF) {
+            f16x8 hi[RT][2], lo[RT][2];
+            float up[RT];
 #pragma unroll
-                for (int h = 0; h < 2; h++) hi[h] = in[h] ? *reinterpret_cast<const f16x8*>(x + ((2 * g + h) ^ (i16 & 7)) * 16) : f16x8{};
-            } else {
-                float v[2][8], mx = 0.f;
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const f32x4 y = *reinterpret_cast<const f32x4*>(x + ((4 * g + q) ^ i16) * 16);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        v[q >> 1][4 * (q & 1) + e] = in[q >> 1] ? y[e] : 0.f;
-                        mx = fmaxf(mx, fabsf(v[q >> 1][4 * (q & 1) + e]));
-                    }
-                }
-                mx = pair_max<32>(pair_max<16>(mx));
-                const float s = scale_of(mx);
-                up = 1.f / s;
-#pragma unroll
-                for (int h = 0; h < 2; h++) split_f16(v[h], s, hi[h], lo[h]);
-            }
+            for (int t = 0; t < RT; t++) x_parts<HALF>(from + TILES * 2048 + (16 * t + i16) * L::kXRow, i16, g, in, hi[t], lo[t], up[t]);
 #pragma unroll
             for (int u = 0; u < TILES; u++) {
-                const char* const a = from + u * 2048 + i16 * 128;
-                f16x8 wu[2];                                // beyond K zeros on both sides: 0 * NaN
+                f16x8 w[2];                                 // beyond K zeros on both sides: 0 * NaN
 #pragma unroll
-                for (int h = 0; h < 2; h++) wu[h] = in[h] ? *reinterpret_cast<const f16x8*>(a + ((2 * g + h) ^ (i16 & 7)) * 16) : f16x8{};
-                if constexpr (HALF) {
+                for (int h = 0; h < 2; h++) w[h] = in[h] ? *reinterpret_cast<const f16x8*>(from + u * 2048 + i16 * 128 + ((2 * g + h) ^ (i16 & 7)) * 16) : f16x8{};
 #pragma unroll
-                    for (int h = 0; h < 2; h++) acc[u] = mfma_16x16x32_f16(wu[h], hi[h], acc[u]);
-                } else {
-                    f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < RT; t++) {
+                    if constexpr (HALF) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        ol = mfma_16x16x32_f16(wu[h], lo[h], ol);
-                        o = mfma_16x16x32_f16(wu[h], hi[h], o);
+                        for (int h = 0; h < 2; h++) acc[u][t] = mfma_16x16x32_f16(w[h], hi[t][h], acc[u][t]);
+                    } else {
+                        f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            ol = mfma_16x16x32_f16(w[h], lo[t][h], ol);
+                            o = mfma_16x16x32_f16(w[h], hi[t][h], o);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[u][t][e] = fmaf(fmaf(ol[e], 1.f / 2048.f, o[e]), up[t], acc[u][t][e]);
                     }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[u][e] = fmaf(fmaf(ol[e], 1.f / 2048.f, o[e]), up, acc[u][e]);
                 }
             }
         }
@@ -272,16 +289,19 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDo
         f32x4* const part = reinterpret_cast<f32x4*>(lds);
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < TILES; u++) part[(wave * TILES + u) * 64 + lane] = acc[u];
-        __syncthreads();
-        for (int u = wave; u < min(TILES, d.tiles - u0); u += kDownWaves) {
-            const LoraDown::Tile& t = d.tile[u0 + u];
-            f32x4 v = part[u * 64 + lane];
+        for (int u = 0; u < TILES; u++)
 #pragma unroll
-            for (int k = 1; k < kDownWaves; k++) v += part[(k * TILES + u) * 64 + lane];
-            if ((mine >> i16 & 1) && which < t.n && 4 * g < t.ranks) {
+            for (int t = 0; t < RT; t++) part[((wave * TILES + u) * RT + t) * 64 + lane] = acc[u][t];
+        __syncthreads();
+        for (int v = wave; v < min(TILES, d.tiles - u0) * RT; v += kDownWaves) {
+            const int u = v / RT, row = 16 * (v - u * RT) + i16;
+            const LoraDown::Tile& t = d.tile[u0 + u];
+            f32x4 sum = part[v * 64 + lane];
+#pragma unroll
+            for (int k = 1; k < kDownWaves; k++) sum += part[(k * TILES * RT + v) * 64 + lane];
+            if ((mine >> row & 1) && which < t.n && 4 * g < t.ranks) {
                 const float s = t.scale ? ld_global(t.scale + which) : 1.f;
-                st_global(reinterpret_cast<f32x4*>(t.t + blockIdx.z * t.part + (size_t)(m0 + i16) * t.rank + 4 * g), f32x4{v[0] * s, v[1] * s, v[2] * s, v[3] * s});
+                st_global(reinterpret_cast<f32x4*>(t.t + blockIdx.z * t.part + (size_t)(m0 + row) * t.rank + 4 * g), f32x4{sum[0] * s, sum[1] * s, sum[2] * s, sum[3] * s});
             }
         }
         __syncthreads();
@@ -433,11 +453,15 @@ namespace {
 template <bool HALF>
 void launch_down(const LoraDown& d, hipStream_t stream)
 {
-    const dim3 block(64 * kDownWaves);
-    const int rows = (d.M + 15) / 16;
-    if (d.tiles == 1) hipLaunchKernelGGL((lora_down_kernel<HALF, 1>), dim3(rows, 1, d.parts), block, 0, stream, d);
-    else if (d.tiles <= 3 || d.tiles == 5) hipLaunchKernelGGL((lora_down_kernel<HALF, 3>), dim3(rows, (d.tiles + 2) / 3, d.parts), block, 0, stream, d);
-    else hipLaunchKernelGGL((lora_down_kernel<HALF, kDownGroup>), dim3(rows, (d.tiles + kDownGroup - 1) / kDownGroup, d.parts), block, 0, stream, d);
+    auto go = [&](auto kernel, int tiles, int rt) {
+        const int rows = (d.M + 16 * rt - 1) / (16 * rt);
+        hipLaunchKernelGGL(kernel, dim3((rows + 7) / 8 * 8 * ((d.tiles + tiles - 1) / tiles), 1, d.parts), dim3(64 * kDownWaves), 0, stream, d);
+    };
+    // 32 rows where they still fill the device (q/k/v of rank 64, fp16, both launches, 16 and 32 rows: 4096 rows 72.5, 67.5 us, 1024 30.1, 29.0; fp32 89.9, 102.6)
+    if (HALF && d.M >= kTwoTiles && d.tiles > 1) go(lora_down_kernel<HALF, 3, HALF ? 2 : 1>, 3, HALF ? 2 : 1);
+    else if (d.tiles == 1) go(lora_down_kernel<HALF, 1, 1>, 1, 1);
+    else if (d.tiles <= 3 || d.tiles == 5) go(lora_down_kernel<HALF, 3, 1>, 3, 1);
+    else go(lora_down_kernel<HALF, kDownGroup, 1>, kDownGroup, 1);
 }
 
 template <int RT>
