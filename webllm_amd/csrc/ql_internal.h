@@ -397,7 +397,8 @@ struct PagedAttnArgs {
     float scale;               // fp32(log2(e) / sqrt(D))
     // plan_paged_attention fills these. Few: most (row, head) pairs of a sequence of few rows; units: most tiles of 16 of them that such sequences
     // have; whole: each of these tiles is one workgroup's, or all their blocks are dealt to `ranges` workgroups a kv head and joined by a merge of
-    // merge_pairs pairs a workgroup. Workgroups of both kinds, tiles of many rows that may be done in parts, and where their parts lie in ws, in floats
+    // merge_pairs pairs a workgroup. Workgroups of the merge and of what joins the parts of tiles of many rows, of both kinds of sequences, and where those tiles'
+    // parts lie in ws, in floats
     int few, units, whole, ranges, merge, merge_pairs, decode, prompt, join;
     size_t prompt_ws;
 };

@@ -8,7 +8,7 @@
 // tokens of V that a lane reads together are 16 b + 4 g + r. Softmax in fp32 with a running reference, raised by leaps only; the waves' states are
 // merged through LDS.
 // Sequences differ in length, so the blocks of all of them, one behind the other, are dealt to the workgroups in equal ranges; a workgroup goes through
-// the sequences that its range meets. Where a sequence's range is cut, paged_merge_kernel joins the parts. Every workgroup finds its range from
+// the sequences that its range meets. Where a sequence's range is cut, paged_merge joins the parts. Every workgroup finds its range from
 // the tables by itself: lengths stay on the device.
 //
 // Numbers: K and V enter as they are (e4m3 is exact in fp16), K's scales multiply scores, V's the probabilities, relative to the block's largest, which multiplies
@@ -464,12 +464,11 @@ __device__ __forceinline__ void paged_decode(const PagedAttnArgs& a, float* merg
 // makes a pair's weights, then thread (slot, pair, four columns) adds parts slot, slot + slots, ... in order, and the slots are added in order.
 constexpr int kMergeWeights = 4096;
 template <typename Q, int WAVES, int BLOCK>
-__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttnArgs a)
+__device__ __forceinline__ void paged_merge(const PagedAttnArgs& a, float (&wgt)[kMergeWeights], f32x4 (&sums)[256], int wg)
 {
-    __shared__ float wgt[kMergeWeights];
-    __shared__ f32x4 sums[256];
     const PagedBatch& b = a.b;
-    const int pair0 = blockIdx.x * a.merge_pairs, kvh = blockIdx.z, tid = threadIdx.x, lane = tid & 63, D = a.D, unit = blockIdx.y;
+    const int per_tile = kPairs / a.merge_pairs, kvh = wg % a.KV, rest = wg / a.KV, unit = rest / per_tile, pair0 = (rest - unit * per_tile) * a.merge_pairs;
+    const int tid = threadIdx.x, lane = tid & 63, D = a.D;
     // the tile, and how many blocks lie before it and in all
     long long total = 0, before = 0;
     int tiles = 0, s = -1, tile = 0;
@@ -537,7 +536,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedAttnArgs a)
 
 // Sequences of many rows: a workgroup has 64 NT (row, head) pairs of one kv head, 16 NT a wave, and goes through their tokens, 64 at a time, which all its waves
 // read from LDS; the next 64 are on their way there meanwhile, as they lie in memory. Scores, softmax and products as above.
-// Their tiles come the longest first where a wave's lanes hold all sequences, and in parts of their tokens where there are few of them; paged_join_kernel joins
+// Their tiles come the longest first where a wave's lanes hold all sequences, and in parts of their tokens where there are few of them; paged_join joins
 // the parts.
 struct PromptTiles {
     const PagedAttnArgs& a;
@@ -861,20 +860,20 @@ __device__ __forceinline__ void paged_prompt(const PagedAttnArgs& a, char (&lds)
     }
 }
 
-// The parts of a tile of many rows, as paged_merge_kernel: a workgroup has a quarter of a tile's pairs.
+// The parts of a tile of many rows likewise: a workgroup has a quarter of a tile's pairs.
 template <typename Q, int ROWS>
-__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a)
+__device__ __forceinline__ void paged_join(const PagedAttnArgs& a, float (&all)[kMergeWeights], int wg)
 {
     constexpr int kHere = ROWS / 4;
-    __shared__ float wgt[kHere][kPromptMost];
-    const int kvh = blockIdx.y, tid = threadIdx.x, D = a.D, pair0 = kHere * blockIdx.z;
+    auto& wgt = reinterpret_cast<float(&)[kHere][kPromptMost]>(all);
+    const int kvh = wg % a.KV, rest = wg / a.KV, tile = rest / 4, tid = threadIdx.x, D = a.D, pair0 = kHere * (rest & 3);
     Piece p;
     int parts;
     PromptTiles tiles(a, ROWS);
-    if (tiles.most == 1 || !tiles.find(blockIdx.x, p, parts) || parts == 1) return;
+    if (tiles.most == 1 || !tiles.find(tile, p, parts) || parts == 1) return;
     const int R = p.q.n * a.G, pairs = min(kHere, R - p.r0 - pair0);
     if (pairs <= 0) return;
-    auto part = [&](int i) { return a.ws + a.prompt_ws + (size_t)(((int)blockIdx.x * tiles.most + i) * a.KV + kvh) * (ROWS * (D + 2)); };
+    auto part = [&](int i) { return a.ws + a.prompt_ws + (size_t)((tile * tiles.most + i) * a.KV + kvh) * (ROWS * (D + 2)); };
     if (tid < pairs) {
         f32x2 st[kPromptMost];
         float mx = -INFINITY, l = 0.f;
@@ -910,6 +909,16 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnArgs a)
     }
 }
 
+// Both kinds of parts in one launch
+template <typename Q, int WAVES, int BLOCK, int ROWS>
+__global__ __launch_bounds__(256) void paged_parts_kernel(const PagedAttnArgs a)
+{
+    __shared__ float wgt[kMergeWeights];
+    __shared__ f32x4 sums[256];
+    if ((int)blockIdx.x < a.merge) paged_merge<Q, WAVES, BLOCK>(a, wgt, sums, blockIdx.x);
+    else paged_join<Q, ROWS>(a, wgt, blockIdx.x - a.merge);
+}
+
 // One launch for both: the first a.decode workgroups have the sequences of few rows, whose reads of memory go on beside the others' products
 template <bool F8, typename Q, int DP, int NT, bool FULL>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_attention_kernel(const PagedAttnArgs a)
@@ -939,9 +948,10 @@ uint64_t plan_paged_attention(PagedAttnArgs* a)
     // the merge's workgroups: some hundreds, their weights in LDS
     a->merge_pairs = 1;
     while (a->merge_pairs < kPairs && (long long)a->units * a->KV * (kPairs / a->merge_pairs) > 512 && 2 * a->merge_pairs * a->ranges <= kMergeWeights) a->merge_pairs *= 2;
-    a->merge = !a->whole && a->ranges > 1;
+    const bool merge = !a->whole && a->ranges > 1;
+    a->merge = merge ? a->units * a->KV * (kPairs / a->merge_pairs) : 0;
     a->decode = (a->whole ? a->units : a->ranges) * a->KV;
-    a->prompt_ws = a->merge ? (size_t)a->ranges * a->KV * 2 * kPairs * (a->D + 2) : 0;
+    a->prompt_ws = merge ? (size_t)a->ranges * a->KV * 2 * kPairs * (a->D + 2) : 0;
     a->prompt = a->join = 0;
     uint64_t bytes = a->prompt_ws * sizeof(float);
     if ((long long)a->b.max_rows * a->G > a->few) {
@@ -951,7 +961,7 @@ uint64_t plan_paged_attention(PagedAttnArgs* a)
         a->prompt = (int)std::max<long long>(tiles * a->KV, kPromptParts);
         // tiles are done in parts where they have eight blocks and there are so few that two parts of each are no more than kPromptParts
         if (a->b.max_len > 7 * kBlock && kPromptParts / a->KV >= 2) {
-            a->join = (int)std::min<long long>(tiles, kPromptParts / a->KV / 2);
+            a->join = (int)std::min<long long>(tiles, kPromptParts / a->KV / 2) * a->KV * 4;
             bytes += (uint64_t)kPromptParts * rows * (a->D + 2) * sizeof(float);
         }
     }
@@ -966,8 +976,7 @@ hipError_t launch(const PagedAttnArgs& a, hipStream_t stream)
     constexpr int kNT = DP > 128 ? 1 : 2;
     if (a.prompt) hipLaunchKernelGGL((paged_attention_kernel<F8, Q, DP, kNT, FULL>), dim3(a.decode + a.prompt), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((paged_decode_kernel<F8, Q, DP, FULL>), dim3(a.decode), dim3(256), 0, stream, a);
-    if (a.merge) hipLaunchKernelGGL((paged_merge_kernel<Q, kDecodeWaves, F8 ? 64 : 32>), dim3(kPairs / a.merge_pairs, a.units, a.KV), dim3(256), 0, stream, a);
-    if (a.join) hipLaunchKernelGGL((paged_join_kernel<Q, 64 * kNT>), dim3(a.join, a.KV, 4), dim3(256), 0, stream, a);
+    if (a.merge + a.join) hipLaunchKernelGGL((paged_parts_kernel<Q, kDecodeWaves, F8 ? 64 : 32, 64 * kNT>), dim3(a.merge + a.join), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
