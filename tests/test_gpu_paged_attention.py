@@ -28,6 +28,11 @@ CASES = [  # seqs, page, H, KV, D
     ([(1, 30)] * 50 + [(50, 700), (33, 33), (0, 4)] * 7, 64, 8, 2, 64),         # more sequences than a wave has lanes, of both kinds
     ([(40, 2000)], 128, 9, 3, 64),                                               # parts of a tile's tokens, kv heads that do not divide 512
     ([(1, 1100), (20, 1200)], 64, 96, 1, 32),                                    # a row of more pairs than the few have
+    ([(500, 500), (1, 9), (300, 900)], 64, 64, 4, 64),                           # many rows: tiles of 128 pairs, and below of each kind of D
+    ([(600, 600), (200, 700), (1, 1)], 128, 64, 8, 128),
+    ([(790, 800)], 64, 64, 8, 96),
+    ([(790, 790)], 64, 64, 2, 32),
+    ([(1, 1500 + 9 * i) for i in range(40)] + [(30, 2000)], 64, 16, 4, 64),      # whole tiles of many sequences beside one of many rows
 ]
 
 
@@ -241,6 +246,20 @@ def test_bounds_that_are_far(ql, ctx):
         call.run()
         call.check()
         call.box.release()
+
+
+@pytest.mark.parametrize("D", [64, 128, 48, 112])
+@pytest.mark.parametrize("q16", [False, True])
+@pytest.mark.parametrize("f8", [False, True])
+def test_tiles_in_parts(ql, ctx, f8, q16, D):
+    """Bounds so far that tiles have 128 pairs, and so few of them that each is done in parts of its tokens."""
+    batch = Batch([(1, 30), (70, 2100), (20, 800), (0, 7)], 256, seed=1, pad=1)
+    batch.pages = np.pad(batch.pages, ((0, 0), (0, 2000 - batch.max_pages)), constant_values=-1)
+    batch.max_pages = 2000
+    call = Call(ql, ctx, batch, 14, 2, D, f8, q16, max_len=2000 * 256)
+    call.run()
+    call.check()
+    call.box.release()
 
 
 def test_many_sequences(ql, ctx):

@@ -397,9 +397,9 @@ struct PagedAttnArgs {
     float scale;               // fp32(log2(e) / sqrt(D))
     // plan_paged_attention fills these. Few: most (row, head) pairs of a sequence of few rows; units: most tiles of 16 of them that such sequences
     // have; whole: each of these tiles is one workgroup's, or all their blocks are dealt to `ranges` workgroups a kv head and joined by a merge of
-    // merge_pairs pairs a workgroup. Workgroups of the merge and of what joins the parts of tiles of many rows, of both kinds of sequences, and where those tiles'
-    // parts lie in ws, in floats
-    int few, units, whole, ranges, merge, merge_pairs, decode, prompt, join;
+    // merge_pairs pairs a workgroup. Workgroups of the merge, of both kinds of sequences, pairs of a tile of many rows (64 or 128), workgroups that join such tiles' parts,
+    // their pairs, and where the parts lie in ws, in floats
+    int few, units, whole, ranges, merge, merge_pairs, decode, prompt, rows, join, join_pairs;
     size_t prompt_ws;
 };
 uint64_t plan_paged_attention(PagedAttnArgs* a);   // the workspace it needs, less than kAttnTileWsBytes

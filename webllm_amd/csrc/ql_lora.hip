@@ -4,10 +4,16 @@
 // four ranks, so that x is read once for them, and a part of K, the parts' sums meet in LDS; then a thread has a column of y, and B's row of it. The
 // workgroups of one row's column ranges each make t for themselves: A comes from L2, and a second launch would cost more.
 //
-// Many rows, two launches: lora_down_kernel makes t of 16 rows, four waves a part of K each, on the matrix cores, T^T = A x^T
+// Four rows of 3 adapters of rank 8 beside q/k/v of 896 columns 4.6 us, 64 rows of 24 of rank 16 beside those of 3584 8.4 us (15 MB): a launch, a chain of two
+// products and their loads from L2, where rows of one adapter read it each for themselves.
+//
+// Many rows, two launches: lora_down_kernel makes t of 16 or 32 rows, four waves a part of K each, on the matrix cores, T^T = A x^T
 // (lane = row, registers = ranks), for all projections that read one x; lora_up_kernel has 16 or 32 rows and 64 columns a wave, Y = T B^T. Rows of
 // several adapters in one tile: it is gone through once for each adapter, and a row takes its own. fp32 x enters as two fp16 parts (22 bits) under the
 // exponent of the row's 64 columns at a time; t likewise under the row's.
+// 4096 rows, 4 adapters of rank 64 beside q/k/v of 3584 columns, fp16 x, 188 MB: 67 us. The second launch, 38 us, is at 4.0 TB/s of base and y; the first, 30, at
+// 10 TB/s of A and x from L2, which its tiles read again (a tile of 64 rows whose waves share A in LDS needs K in parts for as many workgroups, and the parts' sums
+// cost the second launch 20 us; rank groups of the same rows on one XCD brought 5).
 #include <algorithm>
 
 #include "ql_device.h"
@@ -192,8 +198,7 @@ __device__ __forceinline__ void x_parts(const char* x, int i16, int g, const boo
         for (int h = 0; h < 2; h++) split_f16(v[h], s, hi[h], lo[h]);
     }
 }
-// A wave has a quarter of K, 64 columns at a time. Fragments are 16 rows' 16 bytes, which as loads would be a line a lane (60 lines a load, 45 us a pass of 4096
-// rows of rank 64 for 8): rows come whole into a part of LDS that is the wave's own, 128 bytes of eight rows a load, and are turned there; the next
+// A wave has a quarter of K, 64 columns at a time. Fragments are 16 rows' 16 bytes, which as loads would be a line a lane (about 60 lines a load): rows come whole into a part of LDS that is the wave's own, 128 bytes of eight rows a load, and are turned there; the next
 // 64 columns are on their way meanwhile. The 16-byte pieces of row r lie in the order c ^ (r % 8), so that a fragment's reads meet no bank twice.
 template <bool HALF, int TILES, int RT>
 struct DownLds {

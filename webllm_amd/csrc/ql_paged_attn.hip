@@ -1,20 +1,30 @@
 // Attention of a batch's rows over their sequences' pages (ql_paged_attention):
 //   out[m, h] = sum_t p_t V[t] / sum_t p_t,  p_t = exp(q[m, h] . K[t] / sqrt(D) - max)   over the tokens t up to the row's own.
 //
-// paged_decode: sequences of few rows. A workgroup has 16 (row, head) pairs of one kv head and a range of blocks of 64 tokens; its
-// four waves take the blocks in turn, K and V from memory to the registers of one wave. The cache lies as the matrix instructions take it: a load
-// is 16 bytes a lane and 1 KB in a row. Scores are computed transposed, S^T = K Q^T (lane = pair, registers = tokens), and what a lane then has of P is the
-// B fragment of O^T = V^T P^T, with nothing crossing lanes: tile kt of S is the block's tokens 16 kt + 4 g + r (g: lane / 16, r: register), and the
-// tokens of V that a lane reads together are 16 b + 4 g + r. Softmax in fp32 with a running reference, raised by leaps only; the waves' states are
-// merged through LDS.
-// Sequences differ in length, so the blocks of all of them, one behind the other, are dealt to the workgroups in equal ranges; a workgroup goes through
-// the sequences that its range meets. Where a sequence's range is cut, paged_merge joins the parts. Every workgroup finds its range from
-// the tables by itself: lengths stay on the device.
+// Sequences of up to 64 (row, head) pairs a kv head (`few`), paged_decode: a workgroup has 16 pairs and a range of blocks (32 tokens of an fp16 cache, 64 of an e4m3
+// one: the tokens of V that lie together); its four waves take the blocks in turn, K and V from memory to one wave's registers. The cache lies as the matrix
+// instructions take it: a load is 16 bytes a lane and 1 KB in a row. Scores are computed transposed, S^T = K Q^T (lane = pair, registers = tokens), and what a lane
+// then has of P is the B fragment of O^T = V^T P^T, with nothing crossing lanes: tile kt of S is the block's tokens 16 kt + 4 g + r (g: lane / 16, r: register), and
+// the tokens of V that a lane reads together are 16 b + 4 g + r. Softmax in fp32 with a running reference, raised by leaps only; the waves' states meet in LDS.
+// Sequences differ in length, so the blocks of all of them, one behind the other, are dealt to the workgroups in equal ranges (two workgroups a CU); a workgroup goes
+// through the sequences that its range meets, and paged_merge joins the parts of those that are cut. Every workgroup finds its range from the tables by itself:
+// lengths stay on the device. Up to max_len 1024 each tile of 16 pairs is one workgroup's, and there is no second launch.
+// Bound by memory: 64 requests of up to 8000 tokens, e4m3, 28 / 4 heads of 128, 299 MB, 68 us, 4.4 TB/s (57 in the kernel at best, the rest the merge's launch);
+// one of 60000 tokens, fp16, 123 MB, 33 us, 26 of them the first launch (4.7 TB/s) and 7 the merge. 1.02 of the bytes cross the memory's bus. Four requests of 300
+// tokens, 14 / 2 heads of 64: 5.5 us, a launch and its chain of loads. Blocks of 64 tokens of fp16 took 38 us for the one request's 33 (twice the registers).
 //
-// Numbers: K and V enter as they are (e4m3 is exact in fp16), K's scales multiply scores, V's the probabilities, relative to the block's largest, which multiplies
-// the block's sum. fp32 rows: q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P: about 22 bits. fp16 rows: q as it
-// is, 2^8 P rounded once. A product of an infinity's parts is a NaN, and 0 * V is one where V is not finite: a wave whose sums end that way does its blocks
-// again on the VALU from q, K and V themselves, skipping what a pair does not see (paged_again).
+// Sequences of more rows, paged_prompt: 128 pairs of a kv head a workgroup (64 of D over 128), 32 a wave, which read the tokens, 64 at a time, from LDS; the next 64
+// come there from memory meanwhile, past the registers. Tiles are dealt the longest first, and in parts of their tokens where they are few; paged_join joins those.
+// 9000 tokens of five prompts, fp16, 28 / 4 heads of 128: 171 us, 139 GFLOP, 810 TFLOP/s, where an 8192^3 product of the library reaches 1185. The matrix unit is busy
+// 37 % of the cycles (at 1.9 GHz), the VALU (an exponential, a product and a conversion for each score) 40 %: two waves a SIMD overlap them in part. Slower or no faster:
+// 64 pairs a wave (its sums in the accumulators' registers are moved for every product), 32 tokens a step, scores one step ahead of the products, an order of
+// instructions given to the compiler. e4m3 is made fp16 by every wave for itself: 24 requests of 4000 tokens beside 700 rows of two prompts of 4200, 76 us, 28 GFLOP.
+//
+// Numbers: K and V enter as they are (e4m3 is exact in fp16), K's scales multiply scores, V's the probabilities, relative to a running reference of a power of two. fp32
+// rows: q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P: about 22 bits. fp16 rows: q as it is, 2^8 P rounded once, which costs a
+// result up to half a step of its own type (2.5e-4 relative over the prompts, 2.1e-4 for fp32 arithmetic rounded once). A product of an infinity's parts is a NaN, and
+// 0 * V is one where V is not finite: a wave whose sums end that way does its blocks again on the VALU from q, K and V themselves, skipping what a pair does not see
+// (paged_again).
 #include <algorithm>
 #include <type_traits>
 
@@ -29,7 +39,7 @@ constexpr int kBlock = 64;               // tokens of a block of a prompt's kern
 constexpr int kPairs = 16;
 constexpr int kDecodeWaves = 4;
 constexpr int kPromptParts = 512;         // workgroups up to which the tiles of many rows are done in parts of their tokens
-constexpr int kPromptMost = 8;            // parts of a tile at most
+constexpr int kPromptMost = 32;           // parts of a tile at most
 constexpr float kRaise = 7.f;            // log2 that scores may rise above the running reference before it is raised
 constexpr float kPLog = 8.f, kPScale = 256.f;   // parts of P: 2^8 P, at most 2^15
 constexpr float kMaxFinite = 3.4028235e38f;
@@ -860,18 +870,18 @@ __device__ __forceinline__ void paged_prompt(const PagedAttnArgs& a, char (&lds)
     }
 }
 
-// The parts of a tile of many rows likewise: a workgroup has a quarter of a tile's pairs.
+// The parts of a tile of many rows likewise: a workgroup has a.join_pairs of a tile's pairs.
 template <typename Q, int ROWS>
 __device__ __forceinline__ void paged_join(const PagedAttnArgs& a, float (&all)[kMergeWeights], int wg)
 {
-    constexpr int kHere = ROWS / 4;
-    auto& wgt = reinterpret_cast<float(&)[kHere][kPromptMost]>(all);
-    const int kvh = wg % a.KV, rest = wg / a.KV, tile = rest / 4, tid = threadIdx.x, D = a.D, pair0 = kHere * (rest & 3);
+    auto& wgt = reinterpret_cast<float(&)[32][kPromptMost]>(all);
+    const int per_tile = ROWS / a.join_pairs;
+    const int kvh = wg % a.KV, rest = wg / a.KV, tile = rest / per_tile, tid = threadIdx.x, D = a.D, pair0 = a.join_pairs * (rest % per_tile);
     Piece p;
     int parts;
     PromptTiles tiles(a, ROWS);
     if (tiles.most == 1 || !tiles.find(tile, p, parts) || parts == 1) return;
-    const int R = p.q.n * a.G, pairs = min(kHere, R - p.r0 - pair0);
+    const int R = p.q.n * a.G, pairs = min(a.join_pairs, R - p.r0 - pair0);
     if (pairs <= 0) return;
     auto part = [&](int i) { return a.ws + a.prompt_ws + (size_t)((tile * tiles.most + i) * a.KV + kvh) * (ROWS * (D + 2)); };
     if (tid < pairs) {
@@ -897,7 +907,7 @@ __device__ __forceinline__ void paged_join(const PagedAttnArgs& a, float (&all)[
     for (int u = tid; u < pairs * nc; u += 256) {
         const int pair = u / nc, c = u - pair * nc;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < parts; i++) {
             const float w = wgt[pair][i];
             const f32x4 x = ld_global(reinterpret_cast<const f32x4*>(part(i) + (pair0 + pair) * D) + c);
@@ -941,9 +951,13 @@ __global__ __launch_bounds__(64 * kDecodeWaves, DP > 128 ? 1 : 2) void paged_dec
 uint64_t plan_paged_attention(PagedAttnArgs* a)
 {
     const long long pairs = (long long)a->b.M * a->G;
+    // Tiles of 16 pairs read the tokens each for themselves, tiles of 64 or 128 once but through LDS. Few as 4 tiles or fewer, against all as many, in us (28 / 4 heads of
+    // 128, fp32 rows): 16 sequences of 8 rows (56 pairs) after 2000 tokens 31, 43, e4m3 26, 42; of 16 rows (112 pairs) 80, 39 and 50, 41
     a->few = 4 * kPairs;
     a->units = (int)std::min<long long>(4ll * a->b.S, a->b.S + pairs / kPairs);
-    a->whole = a->b.max_len <= 1024;
+    // Whole tiles of sequences that are short, or not very long and many, against ranges and their second launch, which lengths far apart need: one row after 500 tokens
+    // 8.2, 10.5, after 1000 11.3, 10.6; 64 after 2048 43, 49, e4m3 25, 32, of 100 to 2048 20, 35; one after 2000 17.6, 11; one of 2048 and 63 of 200 18, 15 to 20
+    a->whole = a->b.max_len <= 1024 || (a->b.max_len <= 2048 && (long long)a->b.S * a->KV >= 128);
     a->ranges = std::max(1, 512 / a->KV);
     // the merge's workgroups: some hundreds, their weights in LDS
     a->merge_pairs = 1;
@@ -952,16 +966,22 @@ uint64_t plan_paged_attention(PagedAttnArgs* a)
     a->merge = merge ? a->units * a->KV * (kPairs / a->merge_pairs) : 0;
     a->decode = (a->whole ? a->units : a->ranges) * a->KV;
     a->prompt_ws = merge ? (size_t)a->ranges * a->KV * 2 * kPairs * (a->D + 2) : 0;
-    a->prompt = a->join = 0;
+    a->prompt = a->join = a->join_pairs = 0;
+    // Tiles of 64 pairs (registers allow no more over D = 128) where those of 128 would leave much of the device without work: few of them, and few tokens to part. 128 and 64
+    // pairs, fp32 rows (fp16 rows), in us: 64 rows 14, 8.4 (10, 6.8); 1000 of one prompt 55, 40 (40, 30); 1500 78, 56 (53, 41); 300 after 8000 97, 101 (64, 72);
+    // 8 x 300 41, 42 (29, 32); 4 x 128 after 4000 90, 87 (59, 61, e4m3 66, 77)
+    const long long full = pairs * a->KV / 128, tokens = a->b.max_len - std::min(a->b.max_rows, a->b.max_len) / 2;
+    a->rows = a->D > 128 || (full <= 384 && full * tokens <= (a->half ? 4 : 7) << 16) ? 64 : 128;
     uint64_t bytes = a->prompt_ws * sizeof(float);
     if ((long long)a->b.max_rows * a->G > a->few) {
-        const int rows = a->D > 128 ? 64 : 128;
+        const int rows = a->rows;
         // tiles of whole rows, and one more of each sequence of so many rows that it is none of the few
         const long long tiles = pairs / rows + std::min<long long>(a->b.S, pairs / a->few) + 1;
         a->prompt = (int)std::max<long long>(tiles * a->KV, kPromptParts);
         // tiles are done in parts where they have eight blocks and there are so few that two parts of each are no more than kPromptParts
         if (a->b.max_len > 7 * kBlock && kPromptParts / a->KV >= 2) {
-            a->join = (int)std::min<long long>(tiles, kPromptParts / a->KV / 2) * a->KV * 4;
+            a->join_pairs = tiles * a->KV > 64 ? 32 : 8;      // few tiles have many parts: more workgroups for them
+            a->join = (int)std::min<long long>(tiles, kPromptParts / a->KV / 2) * a->KV * (rows / a->join_pairs);
             bytes += (uint64_t)kPromptParts * rows * (a->D + 2) * sizeof(float);
         }
     }
@@ -970,25 +990,30 @@ uint64_t plan_paged_attention(PagedAttnArgs* a)
 
 namespace {
 
-template <bool F8, typename Q, int DP, bool FULL>
+template <bool F8, typename Q, int DP, int NT, bool FULL>
 hipError_t launch(const PagedAttnArgs& a, hipStream_t stream)
 {
-    constexpr int kNT = DP > 128 ? 1 : 2;
-    if (a.prompt) hipLaunchKernelGGL((paged_attention_kernel<F8, Q, DP, kNT, FULL>), dim3(a.decode + a.prompt), dim3(256), 0, stream, a);
+    if (a.prompt) hipLaunchKernelGGL((paged_attention_kernel<F8, Q, DP, NT, FULL>), dim3(a.decode + a.prompt), dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((paged_decode_kernel<F8, Q, DP, FULL>), dim3(a.decode), dim3(256), 0, stream, a);
-    if (a.merge + a.join) hipLaunchKernelGGL((paged_parts_kernel<Q, kDecodeWaves, F8 ? 64 : 32, 64 * kNT>), dim3(a.merge + a.join), dim3(256), 0, stream, a);
+    if (a.merge + a.join) hipLaunchKernelGGL((paged_parts_kernel<Q, kDecodeWaves, F8 ? 64 : 32, 64 * NT>), dim3(a.merge + a.join), dim3(256), 0, stream, a);
     return hipGetLastError();
+}
+
+template <bool F8, typename Q, int NT>
+hipError_t launch_nt(const PagedAttnArgs& a, hipStream_t stream)
+{
+    if (a.D == 64) return launch<F8, Q, 64, NT, true>(a, stream);
+    if (a.D == 128) return launch<F8, Q, 128, NT, true>(a, stream);
+    if (a.D < 64) return launch<F8, Q, 64, NT, false>(a, stream);
+    return launch<F8, Q, 128, NT, false>(a, stream);
 }
 
 template <bool F8, typename Q>
 hipError_t launch_d(const PagedAttnArgs& a, hipStream_t stream)
 {
-    if (a.D == 64) return launch<F8, Q, 64, true>(a, stream);
-    if (a.D == 128) return launch<F8, Q, 128, true>(a, stream);
-    if (a.D == 256) return launch<F8, Q, 256, true>(a, stream);
-    if (a.D < 64) return launch<F8, Q, 64, false>(a, stream);
-    if (a.D < 128) return launch<F8, Q, 128, false>(a, stream);
-    return launch<F8, Q, 256, false>(a, stream);
+    if (a.D == 256) return launch<F8, Q, 256, 1, true>(a, stream);
+    if (a.D > 128) return launch<F8, Q, 256, 1, false>(a, stream);
+    return a.rows == 64 ? launch_nt<F8, Q, 1>(a, stream) : launch_nt<F8, Q, 2>(a, stream);
 }
 
 }  // namespace
