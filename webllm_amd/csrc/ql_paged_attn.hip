@@ -9,16 +9,17 @@
 // Sequences differ in length, so the blocks of all of them, one behind the other, are dealt to the workgroups in equal ranges (two workgroups a CU); a workgroup goes
 // through the sequences that its range meets, and paged_merge joins the parts of those that are cut. Every workgroup finds its range from the tables by itself:
 // lengths stay on the device. Up to max_len 1024 each tile of 16 pairs is one workgroup's, and there is no second launch.
-// Bound by memory: 64 requests of up to 8000 tokens, e4m3, 28 / 4 heads of 128, 299 MB, 68 us, 4.4 TB/s (57 in the kernel at best, the rest the merge's launch);
+// Bound by memory: 64 requests of up to 8000 tokens, e4m3, 28 / 4 heads of 128, 299 MB, 68 us, 4.4 TB/s (61 to 63 in the first launch's trace, 6 the merge's);
 // one of 60000 tokens, fp16, 123 MB, 33 us, 26 of them the first launch (4.7 TB/s) and 7 the merge. 1.02 of the bytes cross the memory's bus. Four requests of 300
 // tokens, 14 / 2 heads of 64: 5.5 us, a launch and its chain of loads. Blocks of 64 tokens of fp16 took 38 us for the one request's 33 (twice the registers).
 //
-// Sequences of more rows, paged_prompt: 128 pairs of a kv head a workgroup (64 of D over 128), 32 a wave, which read the tokens, 64 at a time, from LDS; the next 64
+// Sequences of more rows, paged_prompt: 64 or 128 pairs of a kv head a workgroup, 16 or 32 a wave, which read the tokens, 64 at a time, from LDS; the next 64
 // come there from memory meanwhile, past the registers. Tiles are dealt the longest first, and in parts of their tokens where they are few; paged_join joins those.
-// 9000 tokens of five prompts, fp16, 28 / 4 heads of 128: 171 us, 139 GFLOP, 810 TFLOP/s, where an 8192^3 product of the library reaches 1185. The matrix unit is busy
+// 9000 tokens of five prompts, fp16, 28 / 4 heads of 128: 166 to 174 us, 139 GFLOP, 800 to 840 TFLOP/s, where an 8192^3 product of the library reaches 1185. The matrix unit is busy
 // 37 % of the cycles (at 1.9 GHz), the VALU (an exponential, a product and a conversion for each score) 40 %: two waves a SIMD overlap them in part. Slower or no faster:
 // 64 pairs a wave (its sums in the accumulators' registers are moved for every product), 32 tokens a step, scores one step ahead of the products, an order of
-// instructions given to the compiler. e4m3 is made fp16 by every wave for itself: 24 requests of 4000 tokens beside 700 rows of two prompts of 4200, 76 us, 28 GFLOP.
+// instructions given to the compiler. e4m3 is made fp16 by every wave for itself: 24 requests of up to 4000 tokens beside 700 rows of two prompts
+// of up to 4200, 77 us, 28 GFLOP; 71 the first launch.
 //
 // Numbers: K and V enter as they are (e4m3 is exact in fp16), K's scales multiply scores, V's the probabilities, relative to a running reference of a power of two. fp32
 // rows: q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P: about 22 bits. fp16 rows: q as it is, 2^8 P rounded once, which costs a
