@@ -8,10 +8,10 @@
 // products and their loads from L2, where rows of one adapter read it each for themselves.
 //
 // Many rows, two launches: lora_down_kernel makes t of 16 or 32 rows, four waves a part of K each, on the matrix cores, T^T = A x^T
-// (lane = row, registers = ranks), for all projections that read one x; lora_up_kernel has 16 or 32 rows and 64 columns a wave, Y = T B^T. Rows of
+// (lane = row, registers = ranks), for all projections that read one x; lora_up_kernel has 16 rows and 64 columns a wave, Y = T B^T. Rows of
 // several adapters in one tile: it is gone through once for each adapter, and a row takes its own. fp32 x enters as two fp16 parts (22 bits) under the
 // exponent of the row's 64 columns at a time; t likewise under the row's.
-// 4096 rows, 4 adapters of rank 64 beside q/k/v of 3584 columns, fp16 x, 188 MB: 67 us. The second launch, 38 us, is at 4.0 TB/s of base and y; the first, 30, at
+// 4096 rows, 4 adapters of rank 64 beside q/k/v of 3584 columns, fp16 x, 188 MB: 66 us. The second launch, 37 us, is at 4.1 TB/s of base and y; the first, 30, at
 // 10 TB/s of A and x from L2, which its tiles read again (a tile of 64 rows whose waves share A in LDS needs K in parts for as many workgroups, and the parts' sums
 // cost the second launch 20 us; rank groups of the same rows on one XCD brought 5).
 #include <algorithm>
@@ -99,8 +99,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void lora_row_kernel(const LoraArgs
 
 constexpr int kDownWaves = 4, kDownGroup = 4;      // waves of a workgroup; most tiles of 16 ranks that it makes
 constexpr int kDownTiles = 24;                     // of a launch
-constexpr int kUpRows = 32, kUpCols = 256;         // rows of a pass are a multiple; columns of a workgroup
-constexpr int kTwoTiles = 1024;                    // rows from which what is in LDS of an adapter serves two tiles of 16 rows (its B, 4096 rows of rank 64: one 47 us, two 45, four 59)
+constexpr int kUpRows = 32, kUpCols = 256;         // rows of a pass are a multiple of the first launch's; columns of a workgroup of the second
+constexpr int kTwoTiles = 1024;                    // rows from which the first launch's A serves two tiles of 16 rows
 
 // The ranks of all projections that read one x, in tiles of 16
 struct LoraDown {
@@ -214,9 +214,12 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDo
 {
     using L = DownLds<HALF, TILES, RT>;
     __shared__ __attribute__((aligned(16))) char lds[2][L::kBytes / 2];
-    // the groups of ranks of the same rows on one XCD, one after the other: x comes from its L2 for all but the first
-    const int groups = (d.tiles + TILES - 1) / TILES, turn = blockIdx.x / (8 * groups), in_turn = blockIdx.x - turn * 8 * groups;
-    const int m0 = 16 * RT * (8 * turn + in_turn % 8), u0 = TILES * (in_turn / 8), tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
+    // The groups of ranks of the same rows come one after the other on one XCD, so that x comes from its L2 for all but the first. Of fewer rows an XCD has a range, and few
+    // adapters then; of more it has every eighth tile, since ranges meet on memory's channels (4 adapters of rank 64 in runs, q/k/v, fp16 and fp32 x, ranges against tiles in
+    // turn, us: 512 rows 22, 25; 1024 26, 28 and 40, 41; 1500 33, 34 and 52, 46; 4096 68, 67 and 101, 90)
+    const int groups = (d.tiles + TILES - 1) / TILES, per_xcd = gridDim.x / (8 * groups), xcd = blockIdx.x % 8, in_xcd = blockIdx.x / 8, at = in_xcd / groups;
+    const int m0 = 16 * RT * (d.M > kTwoTiles ? 8 * at + xcd : per_xcd * xcd + at), u0 = TILES * (in_xcd - at * groups);
+    const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
     if (m0 >= d.M) return;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int id[RT];
@@ -314,12 +317,12 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_kernel(const LoraDo
     }
 }
 
-// Y = T B^T: lane = column, registers = rows 4 g + r. A workgroup has 16 RT rows and 256 columns of a projection, a wave 64 of them in four tiles, tile j's column i
-// being 4 i + j: a lane's four results of a row are 16 bytes, a row's 256 in a row (columns 16 j + i, 64 bytes: 45 us for 38). The projections' columns lie one behind
+// Y = T B^T: lane = column, registers = rows 4 g + r. A workgroup has 16 rows and 256 columns of a projection, a wave 64 of them in four tiles, tile j's column i
+// being 4 i + j: a lane's four results of a row are 16 bytes, a row's 256 in a row (columns 16 j + i, 64 bytes: 45 us for 38; 32 rows a workgroup, of which the registers leave half as many: 38 for 37, 64: 59). The projections' columns lie one behind
 // the other in blockIdx.x. An adapter's B of the 256 columns is one stretch of memory: it goes to LDS as it lies, but for the order of a row's pieces,
 // c ^ (n / 4 % their number) where that is a power of two.
-template <int STEPS, int RT>
-__global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
+template <int STEPS>
+__global__ __launch_bounds__(256, 2) void lora_up_kernel(const LoraArgs a)
 {
     __shared__ __attribute__((aligned(16))) char lds[kUpCols * STEPS * 64];
     const int tid = threadIdx.x, lane = tid & 63, i16 = lane & 15, g = lane >> 4;
@@ -327,105 +330,83 @@ __global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs a)
     int proj = 0, xb = blockIdx.x;
     while (xb >= (a.p[proj].N + kUpCols - 1) / kUpCols) xb -= (a.p[proj++].N + kUpCols - 1) / kUpCols;
     const LoraArgs::One& p = a.p[proj];
-    const int m0 = 16 * RT * blockIdx.y, n0 = kUpCols * xb, cols = min(kUpCols, p.N - n0), pieces = p.rank / 8;
+    const int m0 = 16 * blockIdx.y, n0 = kUpCols * xb, cols = min(kUpCols, p.N - n0), pieces = p.rank / 8, nl = 64 * wave + 4 * i16;
     const int turn = pieces & (pieces - 1) ? 0 : min(pieces, 8) - 1;
-    const float* t_in = a.ws + a.t_off[proj];
     const bool apart = p.base != p.y;
-    int id[RT];
-#pragma unroll
-    for (int t = 0; t < RT; t++) id[t] = m0 + 16 * t + i16 < a.M ? ld_global(a.ids + m0 + 16 * t + i16) : -1;
+    const int id[1] = {m0 + i16 < a.M ? ld_global(a.ids + m0 + i16) : -1};
     uint64_t left = rows_below(id, p.n);
-    const uint64_t all = left;
+    const uint32_t all = (uint32_t)left;
     if (!left && !apart) return;
-    f32x4 y[RT][4];                                         // rows 4 g + r, the lane's four columns
-    const int nl = 64 * wave + 4 * i16;
-    f16x8 hi[RT][STEPS], lo[RT][STEPS];
-    float up[RT];
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int m = m0 + 16 * t + i16;
-        float mx = 0.f, v[STEPS][8];
-#pragma unroll
-        for (int st = 0; st < STEPS; st++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[st][e] = 0.f;
-            if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank) load8(t_in, 0, (size_t)m * p.rank + 32 * st + 8 * g, v[st]);
-        }
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int mr = m0 + 16 * t + 4 * g + r;
-            y[t][r] = mr < a.M && nl < cols ? ld_global(reinterpret_cast<const f32x4*>(p.base + (size_t)mr * p.N + n0 + nl)) : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-        if (a.parts[proj] > 1)                              // the other parts of K, in order
-#pragma unroll
-            for (int st = 0; st < STEPS; st++)
-                if ((all >> (16 * t + i16) & 1) && 32 * st + 8 * g < p.rank)
-                    for (int k = 1; k < a.parts[proj]; k++) {
-                        float w[8];
-                        load8(t_in, 0, ((size_t)k * a.M + m) * p.rank + 32 * st + 8 * g, w);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) v[st][e] += w[e];
-                    }
-#pragma unroll
-        for (int st = 0; st < STEPS; st++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[st][e]));
-        mx = pair_max<32>(pair_max<16>(mx));
-        const float s = scale_of(mx);
-        up[t] = 1.f / s;
-#pragma unroll
-        for (int st = 0; st < STEPS; st++) split_f16(v[st], s, hi[t][st], lo[t][st]);
-    }
-    float up_of[RT][4];                                     // of the rows that the lane's results are of
-#pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) up_of[t][r] = __shfl(up[t], 4 * g + r);
-    while (left) {
-        const int which = first_adapter(id, left);
-        const uint64_t mine = left & rows_with(id, which);
-        left &= ~mine;
+    auto fetch = [&](int which) {
         const char* const B = reinterpret_cast<const char*>(p.b + ((size_t)which * p.N + n0) * p.rank);
         const int all_pieces = cols * pieces;
         for (int u = tid; u < (all_pieces + 63) / 64 * 64; u += 256) {
             const int at = min(u, all_pieces - 1), n = at / pieces, c = at - n * pieces;
             load_to_lds(B + (n * pieces + (c ^ (n >> 2 & turn))) * 16, lds + (u - lane) * 16);
         }
+    };
+    int which = 0;
+    if (left) fetch(which = first_adapter(id, left));
+    f32x4 y[4];                                             // rows 4 g + r, the lane's four columns
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int m = m0 + 4 * g + r;
+        y[r] = m < a.M && nl < cols ? ld_global(reinterpret_cast<const f32x4*>(p.base + (size_t)m * p.N + n0 + nl)) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float mx = 0.f, v[STEPS][8];
+    const float* const t = a.ws + a.t_off[proj];
+#pragma unroll
+    for (int st = 0; st < STEPS; st++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[st][e] = 0.f;
+        if ((all >> i16 & 1) && 32 * st + 8 * g < p.rank) {
+            const size_t at = (size_t)(m0 + i16) * p.rank + 32 * st + 8 * g;
+            load8(t, 0, at, v[st]);
+            for (int k = 1; k < a.parts[proj]; k++) {       // the other parts of K, in order
+                float w[8];
+                load8(t, 0, (size_t)k * a.M * p.rank + at, w);
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[st][e] += w[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[st][e]));
+    }
+    mx = pair_max<32>(pair_max<16>(mx));
+    const float s = scale_of(mx), up = 1.f / s;
+    f16x8 hi[STEPS], lo[STEPS];
+#pragma unroll
+    for (int st = 0; st < STEPS; st++) split_f16(v[st], s, hi[st], lo[st]);
+    float up_of[4];                                         // of the rows that the lane's results are of
+#pragma unroll
+    for (int r = 0; r < 4; r++) up_of[r] = __shfl(up, 4 * g + r);
+    while (left) {
+        const uint64_t mine = left & rows_with(id, which);
+        left &= ~mine;
         wave_arrived();
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const int n = nl + j;
-            f16x8 w[STEPS];
+            f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int st = 0; st < STEPS; st++) {
                 const int c = 4 * st + g;
-                w[st] = n < cols && c < pieces ? *reinterpret_cast<const f16x8*>(lds + (n * pieces + (c ^ (n >> 2 & turn))) * 16) : f16x8{};
+                const f16x8 w = n < cols && c < pieces ? *reinterpret_cast<const f16x8*>(lds + (n * pieces + (c ^ (n >> 2 & turn))) * 16) : f16x8{};
+                ol = mfma_16x16x32_f16(lo[st], w, ol);
+                o = mfma_16x16x32_f16(hi[st], w, o);
             }
 #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                f32x4 o = {0.f, 0.f, 0.f, 0.f}, ol = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int st = 0; st < STEPS; st++) {
-                    ol = mfma_16x16x32_f16(lo[t][st], w[st], ol);
-                    o = mfma_16x16x32_f16(hi[t][st], w[st], o);
-                }
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const bool take = mine >> (16 * t + 4 * g + r) & 1;
-                    y[t][r][j] = take ? fmaf(fmaf(ol[r], 1.f / 2048.f, o[r]), up_of[t][r], y[t][r][j]) : y[t][r][j];
-                }
-            }
+            for (int r = 0; r < 4; r++) y[r][j] = mine >> (4 * g + r) & 1 ? fmaf(fmaf(ol[r], 1.f / 2048.f, o[r]), up_of[r], y[r][j]) : y[r][j];
         }
         __syncthreads();
+        if (left) fetch(which = first_adapter(id, left));
     }
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int mr = m0 + 16 * t + 4 * g + r;
-            if (mr < a.M && nl < cols && ((all >> (16 * t + 4 * g + r) & 1) || apart)) st_global(reinterpret_cast<f32x4*>(p.y + (size_t)mr * p.N + n0 + nl), y[t][r]);
-        }
+    for (int r = 0; r < 4; r++) {
+        const int m = m0 + 4 * g + r;
+        if (m < a.M && nl < cols && ((all >> (4 * g + r) & 1) || apart)) st_global(reinterpret_cast<f32x4*>(p.y + (size_t)m * p.N + n0 + nl), y[r]);
+    }
 }
 
 }  // namespace
@@ -471,7 +452,6 @@ void launch_down(const LoraDown& d, hipStream_t stream)
     else go(lora_down_kernel<HALF, kDownGroup, 1>, kDownGroup, 1);
 }
 
-template <int RT>
 void launch_up(const LoraArgs& a, hipStream_t stream)
 {
     int cols = 0, rank = 0;
@@ -479,10 +459,10 @@ void launch_up(const LoraArgs& a, hipStream_t stream)
         cols += (a.p[i].N + kUpCols - 1) / kUpCols;
         rank = std::max(rank, a.p[i].rank);
     }
-    const dim3 grid(cols, (a.M + 16 * RT - 1) / (16 * RT));
-    if (rank <= 32) hipLaunchKernelGGL((lora_up_kernel<1, RT>), grid, dim3(256), 0, stream, a);
-    else if (rank <= 64) hipLaunchKernelGGL((lora_up_kernel<2, RT>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((lora_up_kernel<4, RT>), grid, dim3(256), 0, stream, a);
+    const dim3 grid(cols, (a.M + 15) / 16);
+    if (rank <= 32) hipLaunchKernelGGL(lora_up_kernel<1>, grid, dim3(256), 0, stream, a);
+    else if (rank <= 64) hipLaunchKernelGGL(lora_up_kernel<2>, grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(lora_up_kernel<4>, grid, dim3(256), 0, stream, a);
 }
 
 hipError_t launch_tiled(const LoraArgs& a, hipStream_t stream)
@@ -514,8 +494,7 @@ hipError_t launch_tiled(const LoraArgs& a, hipStream_t stream)
         }
         if (d.tiles) flush();
     }
-    if (a.M >= kTwoTiles) launch_up<2>(a, stream);
-    else launch_up<1>(a, stream);
+    launch_up(a, stream);
     return hipGetLastError();
 }
 
