@@ -84,6 +84,9 @@ CASES = [  # M, targets, how the ids lie
     (130, [(2056, 12, 96, 3)], "one"),
     (1500, [(904, 300, 64, 9), (904, 20, 24, 9)], "mixed"),
     (1030, [(72, 516, 8, 2)], "runs"),
+    (1100, [(200, 60, 72, 3), (200, 20, 24, 3)], "mixed"),                       # tiles of 32 rows, groups of ranks that end inside
+    (2000, [(64, 36, 128, 5)] * 4, "runs"),                                      # more tiles of ranks than a launch has
+    (1024, [(264, 256, 48, 3), (264, 260, 16, 3)], "runs"),
     (20000, [(16, 8, 128, 3)] * 8, "runs"),                                      # more rows than the workspace has room for at once
 ]
 
@@ -144,6 +147,27 @@ def test_rows_apart(ql, ctx, M):
     rest = ~np.isin(np.arange(M), (7, 20, 21)) & (ids != 2)
     assert np.array_equal(got[rest].view(np.uint32), plain[rest].view(np.uint32))
     assert np.isnan(got[7]).all() and not np.isfinite(got[20]).any() and np.isnan(got[ids == 2]).all()
+    call.box.release()
+
+
+def test_rows_apart_in_tiles_of_32(ql, ctx):
+    ids = np.arange(1300) % 3
+    call = Call(ql, ctx, 1300, [(256, 64, 48, 3)], True, ids)
+    call.run()
+    plain = call.check()[0]
+    x = call.x[0].copy()
+    x[7, 3], x[1220, 9], x[1299, 255] = np.nan, np.inf, np.nan
+    call.box.arena.write(call.xo[0], x)
+    b = call.b[0].copy()
+    b[1, 3, 5] = np.nan
+    call.box.arena.write(call.box.off("b0"), b)
+    call.run()
+    got = call.box.get("y0")
+    rest = ~np.isin(np.arange(1300), (7, 1220, 1299))
+    other = np.arange(64) != 3
+    assert np.array_equal(got[rest][:, other].view(np.uint32), plain[rest][:, other].view(np.uint32))
+    assert np.isnan(got[7]).all() and np.isnan(got[1299]).all() and not np.isfinite(got[1220]).any()
+    assert np.array_equal(np.isnan(got[rest][:, 3]), ids[rest] == 1)
     call.box.release()
 
 

@@ -25,7 +25,6 @@ namespace {
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kMaxFinite = 3.4028235e38f;
-constexpr float kF8Max = 448.f;
 constexpr int kLeast = -120;
 
 // the least power of two p >= 2^kLeast with top <= 448 p
