@@ -21,11 +21,12 @@
 // instructions given to the compiler. e4m3 is made fp16 by every wave for itself: 24 requests of up to 4000 tokens beside 700 rows of two prompts
 // of up to 4200, 77 us, 28 GFLOP; 71 the first launch.
 //
-// Numbers: K and V enter as they are (e4m3 is exact in fp16), K's scales multiply scores, V's the probabilities, relative to a running reference of a power of two. fp32
-// rows: q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P: about 22 bits. fp16 rows: q as it is, 2^8 P rounded once, which costs a
-// result up to half a step of its own type (2.5e-4 relative over the prompts, 2.1e-4 for fp32 arithmetic rounded once). A product of an infinity's parts is a NaN, and
-// 0 * V is one where V is not finite: a wave whose sums end that way does its blocks again on the VALU from q, K and V themselves, skipping what a pair does not see
-// (paged_again).
+// Numbers: K and V enter as they are (e4m3 is exact in fp16); K's scales multiply scores, V's its values as they become fp16, in units of a running power of two, which is
+// exact where scales lie up to 2^15 apart in a block (v_reference). A probability keeps its own range that way: it would leave fp16's under the scale of a group far
+// below another one, also in rows that do not see the other. fp32 rows: q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P: about 22 bits, down
+// to 2^-33 of the row's largest. fp16 rows: q as it is, 2^8 P rounded once, which costs a result up to half a step of its own type (2.5e-4 relative over the prompts,
+// 2.1e-4 for fp32 arithmetic rounded once). A product of an infinity's parts is a NaN, and 0 * V is one where V is not finite: a wave whose sums end that way, or
+// whose scales lie further apart than its units reach, does its blocks again on the VALU from q, K and V themselves, skipping what a pair does not see (paged_again).
 #include <algorithm>
 #include <type_traits>
 
@@ -65,11 +66,11 @@ __device__ __forceinline__ float value_at(const void* p, size_t i)
     return (float)ld_global(static_cast<const _Float16*>(p) + i);
 }
 
-// eight e4m3 values, exactly
-__device__ __forceinline__ f16x8 f8_to_f16(uint32_t lo, uint32_t hi)
+// eight e4m3 values, exactly, four and four times a power of two 2^-15 .. 2^7 or zero
+__device__ __forceinline__ f16x8 f8_to_f16(uint32_t lo, uint32_t hi, float s = 1.f, float t = 1.f)
 {
-    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.f, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, 1.f, true);
-    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.f, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, 1.f, true);
+    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, s, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)lo, s, true);
+    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, t, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)hi, t, true);
     return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
@@ -180,24 +181,50 @@ __device__ __forceinline__ float load_q(const Q* q, int g, int D, float scale, f
     }
 }
 
-// Sums are kept in units of a power of two vref near the blocks' own: rv, the block's scales in it, at most one and, for the block's largest, no
-// less than 2^-6. Returns what the sums so far are multiplied by. Groups from lim on have no token, and scales that may hold anything.
-__device__ __forceinline__ float v_reference(const float (&vs)[4], int lim, float& vref, float (&rv)[4])
+// Sums are kept in units of a power of two, ref, that follows the blocks' scales of V: 2^-6 of a largest one. far: scales lie where the unit's products and sums do not
+// reach, and the wave's blocks are done again.
+struct ValueUnit {
+    float ref = 0.f, low = INFINITY;                        // low: the smallest unit so far
+    bool far = false;
+};
+// rv: a block's scales in units of u.ref, which V is multiplied by as it becomes fp16: at most 2^6, and exact from 2^-15 on, 2^-15 of the block's largest at least. Probabilities
+// stay as they are, so that a row has its accuracy from the tokens that it sees. Groups whose scale is smaller still are `late`, rv zero: zeros (under 2^-120), or far. Scales of
+// 2^-100 and less, and of a block more than 2^-32 below the unit's, move no unit. Returns what the sums so far are multiplied by. Groups from lim on have no token, and
+// scales that may hold anything.
+__device__ __forceinline__ float v_reference(const float (&vs)[4], int lim, ValueUnit& u, float (&rv)[4], uint32_t& late)
 {
     float top = 0.f, al = 1.f;
 #pragma unroll
     for (int i = 0; i < 4; i++)
         if (16 * i < lim) top = fmaxf(top, vs[i]);
-    if (top > vref || top < vref * (1.f / 64.f)) {
-        if (top > 0.f) {
-            al = vref / top;
-            vref = top;
+    if (top > 0x1p-100f && (top > u.ref * 0x1p6f || (top < u.ref && top > u.ref * 0x1p-26f))) {
+        const float ref = top * 0x1p-6f;
+        al = u.ref / ref;
+        u.ref = ref;
+        u.low = fminf(u.low, ref);
+        u.far |= u.low < ref * 0x1p-100f;
+    }
+    const float inv = u.ref > 0.f ? 1.f / u.ref : 0.f;
+    late = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        rv[i] = 16 * i < lim ? vs[i] * inv : 0.f;
+        if (rv[i] < 0x1p-15f) {
+            rv[i] = 0.f;
+            if (16 * i < lim) late |= 1u << i;
         }
     }
-    const float inv = vref > 0.f ? 1.f / vref : 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) rv[i] = 16 * i < lim ? vs[i] * inv : 0.f;
+    late = __builtin_amdgcn_readfirstlane(late);
     return al;
+}
+// whether any value of the late groups is not zero, group i being word i of v
+__device__ __forceinline__ uint32_t v_late(u32x4 v, uint32_t late)
+{
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (late >> i & 1) any |= v[i] & 0x7F7F7F7F;
+    return any;
 }
 
 // which of word j of part h of V's fragment are of tokens before lim: four tokens of group j (e4m3), or two of group 2 h + j / 2
@@ -274,7 +301,8 @@ __device__ __forceinline__ void paged_decode(const PagedAttnArgs& a, float* merg
         const int first = p.b0 + wave, mine = first < p.b1 ? (p.b1 - first + WAVES - 1) / WAVES : 0;
         int pages = 0;
         u32x4 kraw[kKT][C::kUnits], vraw[C::kCT];
-        float ks[4], vs[4], vref = 0.f;
+        float ks[4], vs[4];
+        ValueUnit vu;
         struct At {
             size_t head;
             int in_page, t0, lim;                           // lim: tokens of the block that a row may see
@@ -365,8 +393,9 @@ __device__ __forceinline__ void paged_decode(const PagedAttnArgs& a, float* merg
                 for (int c = 0; c < C::kCT; c++) acc[c] *= al;
             }
             float rv[4];
+            uint32_t late = 0;
             if constexpr (F8) {
-                const float al = v_reference(vb, x.lim, vref, rv);
+                const float al = v_reference(vb, x.lim, vu, rv, late);
                 if (al != 1.f)
 #pragma unroll
                     for (int c = 0; c < C::kCT; c++) acc[c] *= al;
@@ -379,7 +408,7 @@ __device__ __forceinline__ void paged_decode(const PagedAttnArgs& a, float* merg
                 for (int i = 0; i < 4; i++) {
                     const float e = ex2(s[kt][i] - ref);
                     l += e;
-                    const float y = e * (F8 ? kPScale * rv[kt] : kPScale);
+                    const float y = e * kPScale;
                     const _Float16 hi = (_Float16)y;
                     pf[kt >> 1][0][4 * (kt & 1) + i] = hi;
                     if constexpr (!C::kHalf) pf[kt >> 1][1][4 * (kt & 1) + i] = (_Float16)(y - (float)hi);
@@ -391,6 +420,13 @@ __device__ __forceinline__ void paged_decode(const PagedAttnArgs& a, float* merg
 #pragma unroll
                     for (int c = 0; c < C::kCT; c++) vraw[c][j] &= keep;
                 }
+            if (late) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int c = 0; c < C::kCT; c++)
+                    if (16 * c < D) any |= v_late(vraw[c], late);
+                vu.far |= __any(any != 0);
+            }
             // a block's sums start from zero and are added to the others by the VALU: the matrix unit carries no long sum
 #pragma unroll
             for (int c = 0; c < C::kCT; c++) {
@@ -399,7 +435,7 @@ __device__ __forceinline__ void paged_decode(const PagedAttnArgs& a, float* merg
 #pragma unroll
                 for (int h = 0; h < kKT / 2; h++) {
                     f16x8 v;
-                    if constexpr (F8) v = f8_to_f16(vraw[c][2 * h], vraw[c][2 * h + 1]);
+                    if constexpr (F8) v = f8_to_f16(vraw[c][2 * h], vraw[c][2 * h + 1], rv[2 * h], rv[2 * h + 1]);
                     else v = __builtin_bit_cast(f16x8, vraw[c]);
 #pragma unroll
                     for (int part = C::kParts - 1; part >= 0; part--) o = mfma_16x16x32_f16(v, pf[h][part], o);
@@ -413,11 +449,11 @@ __device__ __forceinline__ void paged_decode(const PagedAttnArgs& a, float* merg
         for (int c = 0; c < C::kCT; c++)
 #pragma unroll
             for (int i = 0; i < 4; i++) odd = fmaf(acc[c][i], 0.f, odd);
-        const bool redo = __any(odd != 0.f);
+        const bool redo = __any(odd != 0.f) || vu.far;
         if (redo) paged_again<F8, Q, C::kCT, kTokens>(a, p, kvh, q_row, last, first, WAVES, mr, l, acc);
 
         // the waves' states
-        const float unit = redo ? 1.f : F8 ? vref / kPScale : 1.f / kPScale;
+        const float unit = redo ? 1.f : F8 ? vu.ref / kPScale : 1.f / kPScale;
         l = pair_sum<32>(pair_sum<16>(l));
         __syncthreads();                                    // the last piece's are read
         if (g == 0) {
@@ -656,7 +692,8 @@ __device__ __forceinline__ void paged_prompt(const PagedAttnArgs& a, char (&lds)
         for (int c = 0; c < C::kCT; c++) acc[c][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     int pages = 0;
-    float ks[4], vs[4], vref = 0.f;
+    float ks[4], vs[4];
+    ValueUnit vu;
     const int chunks = D * (F8 ? 1 : 2) / 16;               // of 1 KB, of K or V of a block
     auto page_of = [&](int k) {
         const int r = (k - p.b0) & 63;
@@ -772,12 +809,20 @@ __device__ __forceinline__ void paged_prompt(const PagedAttnArgs& a, char (&lds)
             }
         float rv[4];
         if constexpr (F8) {
-            const float al = v_reference(vss, lim, vref, rv);
+            uint32_t late;
+            const float al = v_reference(vss, lim, vu, rv, late);
             if (al != 1.f)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int c = 0; c < C::kCT; c++) acc[c][nt] *= al;
+            if (late) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int c = 0; c < C::kCT; c++)
+                    if (16 * c < D) any |= v_late(vl[c * 64], late);
+                vu.far |= __any(any != 0);
+            }
         }
         f16x8 pf[2][NT][C::kParts];
 #pragma unroll
@@ -793,29 +838,18 @@ __device__ __forceinline__ void paged_prompt(const PagedAttnArgs& a, char (&lds)
                         pf[kt >> 1][nt][0][4 * (kt & 1) + i] = (_Float16)e;
                     } else {
                         l[nt] += e;
-                        const float y = F8 ? e * rv[kt] : e;
-                        const _Float16 hi = (_Float16)y;
+                        const _Float16 hi = (_Float16)e;
                         pf[kt >> 1][nt][0][4 * (kt & 1) + i] = hi;
-                        pf[kt >> 1][nt][1][4 * (kt & 1) + i] = (_Float16)(y - (float)hi);
+                        pf[kt >> 1][nt][1][4 * (kt & 1) + i] = (_Float16)(e - (float)hi);
                     }
                 }
             }
         }
-        if constexpr (C::kHalf) {
+        if constexpr (C::kHalf)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) ls[nt] = mfma_16x16x32_f16(ones, pf[h][nt][0], ls[nt]);   // of P as it is rounded
-            if constexpr (F8) {
-                if (rv[0] != 1.f || rv[1] != 1.f || rv[2] != 1.f || rv[3] != 1.f)
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int kt = 0; kt < 4; kt++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) pf[kt >> 1][nt][0][4 * (kt & 1) + i] *= (_Float16)rv[kt];
-            }
-        }
 #pragma unroll
         for (int c = 0; c < C::kCT; c++) {
             if (16 * c >= D) continue;
@@ -828,7 +862,7 @@ __device__ __forceinline__ void paged_prompt(const PagedAttnArgs& a, char (&lds)
             for (int nt = 0; nt < NT; nt++) o[nt] = C::kHalf ? acc[c][nt] : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const f16x8 v = F8 ? f8_to_f16(w[0][2 * h], w[0][2 * h + 1]) : __builtin_bit_cast(f16x8, w[F8 ? 0 : h]);
+                const f16x8 v = F8 ? f8_to_f16(w[0][2 * h], w[0][2 * h + 1], rv[2 * h], rv[2 * h + 1]) : __builtin_bit_cast(f16x8, w[F8 ? 0 : h]);
 #pragma unroll
                 for (int part = C::kParts - 1; part >= 0; part--)
 #pragma unroll
@@ -848,8 +882,8 @@ __device__ __forceinline__ void paged_prompt(const PagedAttnArgs& a, char (&lds)
 #pragma unroll
             for (int i = 0; i < 4; i++) odd = fmaf(mine[c][i], 0.f, odd);
         }
-        float unit = (F8 ? vref : 1.f) / kPScale, total = (C::kHalf ? ls[nt][0] : pair_sum<32>(pair_sum<16>(l[nt]))) * (1.f / kPScale);
-        if (__any(odd != 0.f)) {
+        float unit = (F8 ? vu.ref : 1.f) / kPScale, total = (C::kHalf ? ls[nt][0] : pair_sum<32>(pair_sum<16>(l[nt]))) * (1.f / kPScale);
+        if (__any(odd != 0.f) || vu.far) {
             paged_again<F8, Q, C::kCT, kBlock>(a, p, kvh, q_row[nt], last[nt], p.b0, 1, mr[nt], l[nt], mine);
             unit = 1.f;
             total = pair_sum<32>(pair_sum<16>(l[nt]));
