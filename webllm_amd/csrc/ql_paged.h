@@ -81,7 +81,8 @@ struct PagedUnits {
     }
 };
 
-// The sequence of a row, for a whole wave; false: padding.
+// The sequence of a row, for a whole wave; false: padding. Where the table ascends it is the first that ends behind the row; an entry that it may not have can miscount, so
+// a row that this one does not have is looked for in all (a row that no sequence ends behind is in none).
 __device__ __forceinline__ bool paged_row(const PagedBatch& b, int row, int& s, PagedSeq& q)
 {
     const int lane = threadIdx.x & 63;
@@ -89,7 +90,18 @@ __device__ __forceinline__ bool paged_row(const PagedBatch& b, int row, int& s, 
     for (int s0 = 0; s0 < b.S; s0 += 64) s += __popcll(__ballot(s0 + lane < b.S && ld_global(b.row_start + 1 + min(s0 + lane, b.S - 1)) <= row));
     if (s >= b.S) return false;
     q = paged_seq(b, s);
-    return row >= q.row0 && row < q.row0 + q.n;
+    if (__builtin_expect(!(row >= q.row0 && row < q.row0 + q.n), 0)) {
+        s = b.S;
+        for (int s0 = 0; s0 < b.S && s == b.S; s0 += 64) {
+            PagedSeq me = {0, 0, 0};
+            if (s0 + lane < b.S) me = paged_seq(b, s0 + lane);
+            const uint64_t has = __ballot(row >= me.row0 && row < me.row0 + me.n);
+            if (has) s = s0 + __builtin_ctzll(has);
+        }
+        if (s == b.S) return false;
+        q = paged_seq(b, s);
+    }
+    return true;
 }
 
 // The page of token t of sequence s, or -1
