@@ -393,6 +393,8 @@ class PagedKvCache:
             raise ValueError("paged kv cache: at least one page, of 64, 128 or 256 tokens")
         self.ctx, self.config, self.dtype, self.page_size, self.pages = ctx, config, dtype, page_size, pages
         self.D, self.row_len = qwen_head_dim(config), qwen_kv_dim(config)
+        if self.D < 16 or self.D > 256 or self.D % 16 or config.n_head > 4096 or config.n_head % config.n_kv_head:
+            raise ValueError("paged kv cache: head dim must be 16..256, a multiple of 16, n_head at most 4096, a multiple of n_kv_head")
         self.page_bytes = page_size * self.row_len * (1 if dtype == "f8" else 2)
         self.scale_bytes = config.n_kv_head * (page_size // 16) * 4 if dtype == "f8" else 0     # of a page
         layout = ql.ArenaLayout()
@@ -466,15 +468,21 @@ class PagedKvCache:
 
     def batch(self, pool: "ActivationArena", sequences, M: int | None = None) -> Batch:
         """Rows of a pass: (sequence, rows) in the order of the rows, each sequence once. Takes the pages that their tokens need and counts the
-        tokens; M: rows of the pass's tensors (those behind the sequences' are padding)."""
+        tokens; M: rows of the pass's tensors (those behind the sequences' are padding). A batch that is refused takes nothing. After a pass that fails later (a rope
+        table of fewer positions, for one) its sequences are cut back to their earlier lengths: the tokens counted are in no page."""
         order, rows = [s for s, _ in sequences], [n for _, n in sequences]
-        if not order or len(set(order)) != len(order) or min(rows) < 0:
-            raise ValueError("batch: at least one sequence, each once, with no negative rows")
+        if not order or len(set(order)) != len(order) or min(rows) < 0 or any(n != int(n) for n in rows):
+            raise ValueError("batch: at least one sequence, each once, with whole, no negative rows")
         total = sum(rows)
         M = max(total, 1) if M is None else M
         if M < total:
             raise ValueError(f"batch: {total} rows for tensors of {M}")
         lengths = [self._lengths[s] + n for s, n in sequences]
+        if M < 1 or M > ql.BATCH_ROWS or len(order) > ql.BATCH_SEQS or max(lengths) > ql.BATCH_TOKENS:
+            raise ValueError(f"batch: 1 to {ql.BATCH_ROWS} rows, at most {ql.BATCH_SEQS} sequences, {ql.BATCH_TOKENS} tokens of one (got {M}, {len(order)}, {max(lengths)})")
+        c = self.config
+        if M * (c.n_head + 2 * c.n_kv_head) > ql.BATCH_HEADS or len(order) * c.n_kv_head > ql.BATCH_SEQ_HEADS:
+            raise ValueError(f"batch: more than {ql.BATCH_HEADS} heads of rows or {ql.BATCH_SEQ_HEADS} kv heads of sequences")
         lists = [self._lists[s] for s in order]
         # a page that the pass appends to is the sequence's alone: one that others hold as well (cut in the middle of a shared one) is copied first,
         # by all who append to it, or by all but the last where nobody else holds it

@@ -33,6 +33,8 @@ const batchAddon = require(path.join(__dirname, '..', 'lib', 'qlinear_batch_napi
 const QL_DTYPE_F32 = 0;
 const QL_DTYPE_F16 = 1;
 const QL_DTYPE_F8 = 2;
+// most rows of a pass, sequences, tokens of one, rows times heads of q, k and v, sequences times kv heads (ql_batch_desc)
+const BATCH = Object.freeze({ rows: 65535, seqs: 4096, tokens: 2 ** 26, heads: 2 ** 23, seqHeads: 2 ** 22 });
 
 // ------------------------------------------------------------------ config (qwen-config.ts)
 
@@ -850,6 +852,8 @@ class PagedKvCache {
         this.pages = pages;
         this.D = qwenHeadDim(config);
         this.rowLen = qwenKvDim(config);
+        if (this.D < 16 || this.D > 256 || this.D % 16 || config.nHead > 4096 || config.nHead % config.nKvHead)
+            throw new Error('paged kv cache: head dim must be 16..256, a multiple of 16, nHead at most 4096, a multiple of nKvHead');
         const f8 = this.dtype === 'f8';
         this.pageBytes = this.pageSize * this.rowLen * (f8 ? 1 : 2);
         this.scaleBytes = f8 ? config.nKvHead * (this.pageSize / 16) * 4 : 0;      // of a page
@@ -917,7 +921,8 @@ class PagedKvCache {
     }
     /**
      * Rows of a pass: [sequence, rows] in the order of the rows, each sequence once. Takes the pages that their tokens need and counts the tokens;
-     * M: rows of the pass's tensors (those behind the sequences' are padding).
+     * M: rows of the pass's tensors (those behind the sequences' are padding). A batch that is refused takes nothing. After a pass that fails later (a
+     * rope table of fewer positions, for one) its sequences are cut back to their earlier lengths: the tokens counted are in no page.
      */
     batch(pool, sequences, M) {
         const order = sequences.map(([s]) => this._known(s)), rows = sequences.map(([, n]) => n);
@@ -926,6 +931,11 @@ class PagedKvCache {
         const total = rows.reduce((a, b) => a + b, 0), m = M === undefined ? Math.max(total, 1) : M, P = this.pageSize;
         if (m < total) throw new Error(`batch: ${total} rows for tensors of ${m}`);
         const lists = order.map((s) => this._lists.get(s)), lengths = order.map((s, i) => this._lengths.get(s) + rows[i]);
+        const longest = lengths.reduce((x, y) => Math.max(x, y)), { nHead, nKvHead } = this.config;
+        if (!(m >= 1 && m <= BATCH.rows) || !Number.isInteger(m) || order.length > BATCH.seqs || longest > BATCH.tokens)
+            throw new Error(`batch: 1 to ${BATCH.rows} rows, at most ${BATCH.seqs} sequences, ${BATCH.tokens} tokens of one (got ${m}, ${order.length}, ${longest})`);
+        if (m * (nHead + 2 * nKvHead) > BATCH.heads || order.length * nKvHead > BATCH.seqHeads)
+            throw new Error(`batch: more than ${BATCH.heads} heads of rows or ${BATCH.seqHeads} kv heads of sequences`);
         // a page that the pass appends to is the sequence's alone: one that others hold as well (cut in the middle of a shared one) is copied first,
         // by all who append to it, or by all but the last where nobody else holds it
         const at = order.map((s, i) => (rows[i] && this._lengths.get(s) % P ? Math.floor(this._lengths.get(s) / P) : -1));

@@ -25,6 +25,8 @@ NOALLOC_SCRATCH_BYTES = 8 << 20   # QL_NOALLOC_SCRATCH_BYTES
 DTYPE_F32 = 0
 DTYPE_F16 = 1
 DTYPE_F8 = 2                      # e4m3 under powers of two: paged caches
+# most rows of a pass, sequences, tokens of one, rows times heads of q, k and v, sequences times kv heads (ql_batch_desc)
+BATCH_ROWS, BATCH_SEQS, BATCH_TOKENS, BATCH_HEADS, BATCH_SEQ_HEADS = 65535, 4096, 1 << 26, 1 << 23, 1 << 22
 KIND_NAMES = {1: "gemv_mfma", 2: "gemv_simple", 3: "gemm_mfma", 4: "gemm_simple"}
 
 ERROR_NAMES = {
