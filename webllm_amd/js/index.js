@@ -18,7 +18,8 @@
  *   QWEN25_05B, qwenKvDim                        src/model/qwen-config.ts:1-54
  *
  * Errors are thrown as Error (the reference's `throw new Error(msg)`); library status codes carry
- * `err.code` = 'QL_E_*'. There is no CPU fallback: a missing addon throws at require time.
+ * `err.code` = 'QL_E_*'. There is no CPU fallback: a missing addon throws at require time,
+ * that of passes over many requests where it is needed first.
  */
 const fs = require('fs');
 const path = require('path');
@@ -28,7 +29,16 @@ if (!fs.existsSync(ADDON_PATH)) {
     throw new Error(`qlinear: addon not built at ${ADDON_PATH} (run __graft_entry__.build())`);
 }
 const addon = require(ADDON_PATH);
-const batchAddon = require(path.join(__dirname, '..', 'lib', 'qlinear_batch_napi.node'));   // passes over many requests, on the same handles
+// passes over many requests, on the same handles: loaded by the first that needs it
+let loadedBatchAddon = null;
+function batchAddon() {
+    if (!loadedBatchAddon) {
+        const at = path.join(path.dirname(ADDON_PATH), 'qlinear_batch_napi.node');
+        if (!fs.existsSync(at)) throw new Error(`qlinear: addon not built at ${at} (run __graft_entry__.build())`);
+        loadedBatchAddon = require(at);
+    }
+    return loadedBatchAddon;
+}
 
 const QL_DTYPE_F32 = 0;
 const QL_DTYPE_F16 = 1;
@@ -548,7 +558,7 @@ class QuantLinearModel {
         if (ids.arena !== A.arena || Cs.some((c) => c.arena !== A.arena)) throw new Error('loraAdd: tensors must share one arena');
         if (loras.some((l, i) => A.length < M * l.K || Cs[i].length < M * l.N)) throw new Error('loraAdd: tensor too small for [M,K] / [M,N]');
         const offs = Cs.map((c) => c.offset);
-        batchAddon.loraAdd(this.ctx.handle, loras, this.weights.handle, A.arena.handle, ids.offset, Cs.map(() => A.offset),
+        batchAddon().loraAdd(this.ctx.handle, loras, this.weights.handle, A.arena.handle, ids.offset, Cs.map(() => A.offset),
             A.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32, M, offs, offs);
     }
     /** fp16 [N,K] copy, bit-identical to the reference's uploaded f16 weight buffer. */
@@ -993,7 +1003,7 @@ class PagedKvCache {
             return w;
         };
         const table = weight(o.rope || 'rope'), paged = this.desc(layer);
-        batchAddon.pagedAppend(this.ctx.handle, {
+        batchAddon().pagedAppend(this.ctx.handle, {
             tableOff: table.offset, maxPos: table.shape[0], nHead: c.nHead, nKvHead: c.nKvHead, D: this.D, rotDim: table.shape[1], interleaved: 0,
             qNormOff: o.qNorm ? weight(o.qNorm, this.D).offset : null, kNormOff: o.kNorm ? weight(o.kNorm, this.D).offset : null,
             normEps: o.eps === undefined ? 1e-6 : o.eps, qStride: 0, kStride: 0, vStride: 0, cacheDtype: paged.cacheDtype,
@@ -1006,7 +1016,7 @@ class PagedKvCache {
         if ([out, ...batch.tables].some((t) => t.arena !== q.arena)) throw new Error('attend: q, out and the batch must share one arena');
         if ((q.dtype !== 'f32' && q.dtype !== 'f16') || out.dtype !== q.dtype || q.length < M * c.nHead * this.D || out.length < M * c.nHead * this.D)
             throw new Error('attend: a tensor is too small or of another type');
-        batchAddon.pagedAttention(this.ctx.handle, q.arena.handle, q.offset, q.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32, this.arena.handle,
+        batchAddon().pagedAttention(this.ctx.handle, q.arena.handle, q.offset, q.dtype === 'f16' ? QL_DTYPE_F16 : QL_DTYPE_F32, this.arena.handle,
             this.desc(layer), batch.desc, M, c.nHead, out.offset);
     }
     release() { this.arena.release(); }
@@ -1018,5 +1028,5 @@ module.exports = {
     expectTensor, f16BitsToF32, readTensorBytes, readTensorF32, ArenaLayout, Arena, Context,
     makeDesc, dequantizeGptqInt4, Tensor, ActivationArena, QuantLinearModel,
     qwenLinearShapes, loadQwenWeights, KvCache, QWEN_LOCAL_DIR, urlToPath, readF16Rows, checkGIdx,
-    countStoredZeros, treeMasks, batchAddon, QL_DTYPE_F8, PagedKvCache,
+    countStoredZeros, treeMasks, get batchAddon() { return batchAddon(); }, QL_DTYPE_F8, PagedKvCache,
 };
