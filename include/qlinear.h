@@ -400,8 +400,8 @@ int ql_paged_append(ql_ctx* ctx, const ql_rope_desc* rope, const ql_arena* weigh
 /* out[m, h, :] = softmax_t(q[m, h] . K[t, h / (n_head / n_kv_head)] / sqrt(D)) V[t, ...] over the tokens t <= the row's own of its
  * sequence, which the cache holds (ql_paged_append has run). q and out are [M, n_head, D] in `act`, both of q_dtype: fp32 (q as two fp16
  * parts of about 22 bits under its row's exponent, probabilities likewise, down to 2^-33 of the row's largest), or fp16 (probabilities rounded once to fp16, with
- * the same end, as the result is). Sums and softmax in fp32. e4m3 values of any scales have a row's accuracy; where those of V lie more than 2^15 apart in 64 tokens of a head
- * (zeros aside) their sequence takes a slower way. A row that sees nothing, or no score above -inf, is zero. What a row does not see adds nothing to it, infinities and NaN included;
+ * the same end, as the result is). Sums and softmax in fp32. e4m3 values of V count by their own scales, whatever others have; where these lie more than 2^15 apart in 64 tokens
+ * of a head (zeros aside) the tokens may be gone through a second, slower time. A row that sees nothing, or no score above -inf, is zero. What a row does not see adds nothing to it, infinities and NaN included;
  * a value of q that is not finite gives its head's row what the formula gives: NaN, or zero where every score is -inf. M * n_head <= 2^23,
  * n_seq * n_kv_head <= 2^22. Offsets 16-byte aligned. Uses the context's 64 MiB workspace. */
 int ql_paged_attention(ql_ctx* ctx, ql_arena* act, uint64_t q_off, int32_t q_dtype, const ql_arena* cache, const ql_paged_desc* paged,

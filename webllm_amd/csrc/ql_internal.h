@@ -423,8 +423,15 @@ struct LoraArgs {
     int rows, parts[kMaxBatch];
     uint64_t t_off[kMaxBatch];
 };
-// A workgroup a row up to so many rows, or rows times the largest rank: 100 rows, 5 adapters in runs, rows against tiles in us: q/k/v of 3584 columns rank 16
-// 9, 14, rank 64 27, 22; 18944 columns from 3584 twice, rank 16 20, 22, rank 64 104, 37. Rows of many adapters mixed, which few rows are, cost tiles a pass each.
+// A workgroup a row up to so many rows, or rows times the largest rank. Rows against tiles, us, fp32 x, 5 adapters in runs; 24 mixed, of which tiles make a pass each:
+//   q/k/v of 3584 columns         16 rows              64                   100                  256
+//     rank 16              6, 24;  6, 41       8, 17;  9, 48       9, 16; 10, 49      13, 16; 17, 51
+//     rank 64             16, 33; 16, 57      28, 25; 31, 66      36, 22; 42, 66     43, 26; 59, 108
+//   18944 columns from 3584, twice
+//     rank 16             10, 24; 10, 42      14, 20; 17, 52      18, 20; 23, 57     33, 28; 45, 81
+//     rank 64             33, 32; 33, 57      66, 31; 94, 85    107, 33; 145, 105  206, 56; 256, 181
+// The border lies where runs into q/k/v change sides. Runs into wide outputs of high ranks would do better in tiles from 32 rows on, rows of many adapters mixed by rows up to
+// some hundreds but for those outputs.
 constexpr int kLoraRowMax = 64, kLoraRowRanks = 2048;
 uint64_t plan_lora(LoraArgs* a, size_t ws_bytes);
 hipError_t launch_lora(const LoraArgs& a, hipStream_t stream);

@@ -11,8 +11,8 @@
 // of it. A group's values are put into LDS in the cache's type and go out in pieces of 16 bytes of K (columns of a token) or of
 // four tokens of V's column, or token by token where a group is not whole.
 //
-// Bound by memory where there is much: 4096 rows of 28 / 4 heads of 128 to e4m3 pages and fp16 q, 111 MB, 23.1 us, 4.8 TB/s (a copy: 5.2). A pass of single
-// tokens is one launch: 64 rows with norms 4.6 us (4.9 in the kernel's trace), four rows of 14 / 2 heads of 64 4.3. A group, and not a row, is a workgroup's, since its
+// Bound by memory where there is much: 4096 rows of 28 / 4 heads of 128 to e4m3 pages and fp16 q, 111 MB, 23.4 us, 4.7 TB/s (a copy: 5.2). A pass of single
+// tokens is one launch: 64 rows with norms 4.6 us (4.9 in the kernel's trace), four rows of 14 / 2 heads of 64 4.3 to 4.6. A group, and not a row, is a workgroup's, since its
 // tokens share a scale, and V's tokens their 16 bytes.
 #include <type_traits>
 

@@ -9,20 +9,21 @@
 // Sequences differ in length, so the blocks of all of them, one behind the other, are dealt to the workgroups in equal ranges (two workgroups a CU); a workgroup goes
 // through the sequences that its range meets, and paged_merge joins the parts of those that are cut. Every workgroup finds its range from the tables by itself:
 // lengths stay on the device. Up to max_len 1024 each tile of 16 pairs is one workgroup's, and there is no second launch.
-// Bound by memory: 64 requests of up to 8000 tokens, e4m3, 28 / 4 heads of 128, 299 MB, 68 us, 4.4 TB/s (61 to 63 in the first launch's trace, 6 the merge's);
+// Bound by memory: 64 requests of up to 8000 tokens, e4m3, 28 / 4 heads of 128, 299 MB, 69 us, 4.3 TB/s (61 to 63 in the first launch's trace, 6 the merge's);
 // one of 60000 tokens, fp16, 123 MB, 33 us, 26 of them the first launch (4.7 TB/s) and 7 the merge. 1.02 of the bytes cross the memory's bus. Four requests of 300
-// tokens, 14 / 2 heads of 64: 5.5 us, a launch and its chain of loads. Blocks of 64 tokens of fp16 took 38 us for the one request's 33 (twice the registers).
+// tokens, 14 / 2 heads of 64: 5.5 us, a launch and its chain of loads. Blocks of 64 tokens of fp16 take 41 us for the one request's 33 (registers go to memory).
 //
 // Sequences of more rows, paged_prompt: 64 or 128 pairs of a kv head a workgroup, 16 or 32 a wave, which read the tokens, 64 at a time, from LDS; the next 64
 // come there from memory meanwhile, past the registers. Tiles are dealt the longest first, and in parts of their tokens where they are few; paged_join joins those.
 // 9000 tokens of five prompts, fp16, 28 / 4 heads of 128: 166 to 174 us, 139 GFLOP, 800 to 840 TFLOP/s, where an 8192^3 product of the library reaches 1185. The matrix unit is busy
 // 37 % of the cycles (at 1.9 GHz), the VALU (an exponential, a product and a conversion for each score) 40 %: two waves a SIMD overlap them in part. Slower or no faster:
 // 64 pairs a wave (its sums in the accumulators' registers are moved for every product), 32 tokens a step, scores one step ahead of the products, an order of
-// instructions given to the compiler. e4m3 is made fp16 by every wave for itself: 24 requests of up to 4000 tokens beside 700 rows of two prompts
-// of up to 4200, 77 us, 28 GFLOP; 71 the first launch.
+// instructions given to the compiler. 24 requests of up to 4000 tokens beside 700 rows of two prompts of up to 4200, e4m3: 78 us, 28 GFLOP; 71 the first
+// launch, whose prompts' workgroups begin as the decoding ones end (512, all that the device holds at D = 128) and have 10 to 20 blocks each, where 13.4 would be equal
+// (every tile has as many parts as another); each wave makes e4m3 fp16 for itself.
 //
 // Numbers: K and V enter as they are (e4m3 is exact in fp16); K's scales multiply scores, V's its values as they become fp16, in units of a running power of two, which is
-// exact where scales lie up to 2^15 apart in a block (v_reference). A probability keeps its own range that way: it would leave fp16's under the scale of a group far
+// exact where scales lie up to 2^15 apart in a block, often 2^21 (v_reference). A probability keeps its own range that way: it would leave fp16's under the scale of a group far
 // below another one, also in rows that do not see the other. fp32 rows: q as hi + 2^-11 lo under its row's exponent, in two sums; P as hi + lo of 2^8 P: about 22 bits, down
 // to 2^-33 of the row's largest. fp16 rows: q as it is, 2^8 P rounded once, which costs a result up to half a step of its own type (2.5e-4 relative over the prompts,
 // 2.1e-4 for fp32 arithmetic rounded once). A product of an infinity's parts is a NaN, and 0 * V is one where V is not finite: a wave whose sums end that way, or
@@ -189,7 +190,8 @@ struct ValueUnit {
 };
 // rv: a block's scales in units of u.ref, which V is multiplied by as it becomes fp16: at most 2^6, and exact from 2^-15 on, 2^-15 of the block's largest at least. Probabilities
 // stay as they are, so that a row has its accuracy from the tokens that it sees. Groups whose scale is smaller still are `late`, rv zero: zeros (under 2^-120), or far. Scales of
-// 2^-100 and less, and of a block more than 2^-32 below the unit's, move no unit. Returns what the sums so far are multiplied by. Groups from lim on have no token, and
+// 2^-100 and less, and of a block more than 2^-32 below the unit's, move no unit. A wave that is far takes some hundred times as long (64 rows after 2000 tokens, 28 / 4
+// heads of 128, 27 us and 3.0 ms; with a quarter of the groups zeros 26). Returns what the sums so far are multiplied by. Groups from lim on have no token, and
 // scales that may hold anything.
 __device__ __forceinline__ float v_reference(const float (&vs)[4], int lim, ValueUnit& u, float (&rv)[4], uint32_t& late)
 {
@@ -964,7 +966,8 @@ __global__ __launch_bounds__(256) void paged_parts_kernel(const PagedAttnArgs a)
     else paged_join<Q, ROWS>(a, wgt, blockIdx.x - a.merge);
 }
 
-// One launch for both: the first a.decode workgroups have the sequences of few rows, whose reads of memory go on beside the others' products
+// One launch for both: the first a.decode workgroups have the sequences of few rows. Where these are as many as the device holds at once (two a CU at D = 128), the others begin
+// as they end; both kinds are at work together only where they are fewer.
 template <bool F8, typename Q, int DP, int NT, bool FULL>
 __global__ __launch_bounds__(256, DP > 128 ? 1 : 2) void paged_attention_kernel(const PagedAttnArgs a)
 {
