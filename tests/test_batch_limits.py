@@ -46,6 +46,22 @@ def test_rows():
     assert kv.batch(pool, [(a, np.int64(43690))]).M == 43690
 
 
+def test_numbers_that_are_not_whole():
+    kv, pool = cache(8)
+    a = kv.new_sequence()
+    kv.batch(pool, [(a, 9)])
+    for args in (([(a, 2.0)],), ([(a, 2.5)],), ([(a, float("nan"))],), ([(a, 2)], 4.0), ([(a, None)],)):
+        refuses(kv, pool, *args, match="whole")
+    for tokens in (1.5, 3.0, None):
+        with pytest.raises(ValueError, match="whole"):
+            kv.cut(a, tokens)
+    assert kv.length(a) == 9
+    b = kv.batch(pool, [(a, np.int32(3))], np.int64(4))
+    assert (type(b.M), type(kv.length(a)), kv.length(a), b.desc.max_rows) == (int, int, 12, 3)
+    kv.cut(a, np.int64(2))
+    assert (type(kv.length(a)), kv.length(a)) == (int, 2)
+
+
 def test_sequences():
     kv, pool = cache(5000)
     all_ = [(kv.new_sequence(), 1) for _ in range(4097)]

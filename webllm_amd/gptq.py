@@ -378,6 +378,12 @@ class Batch:
     tables: tuple                # row_start, kv_len and pages in the activation arena
 
 
+def _whole(what: str, *numbers) -> list[int]:
+    if not all(isinstance(n, (int, np.integer)) for n in numbers):
+        raise ValueError(f"{what} must be whole numbers (got {numbers})")
+    return [int(n) for n in numbers]
+
+
 class PagedKvCache:
     """K and V of many sequences in pages that they take as they grow, in one device arena, for passes over many requests at once:
     append and attend run per layer over a Batch. dtype "f16", or "f8": e4m3 values with a power of two for every 16 tokens of a
@@ -437,6 +443,7 @@ class PagedKvCache:
 
     def cut(self, sequence: int, tokens: int):
         """The sequence's first tokens are kept (a rejected draft, an edited prompt)."""
+        tokens, = _whole("cut: tokens", tokens)
         if not 0 <= tokens <= self._lengths[sequence]:
             raise ValueError(f"cut: sequence {sequence} has {self._lengths[sequence]} tokens")
         pages = self._lists[sequence]
@@ -470,11 +477,11 @@ class PagedKvCache:
         """Rows of a pass: (sequence, rows) in the order of the rows, each sequence once. Takes the pages that their tokens need and counts the
         tokens; M: rows of the pass's tensors (those behind the sequences' are padding). A batch that is refused takes nothing. After a pass that fails later (a rope
         table of fewer positions, for one) its sequences are cut back to their earlier lengths: the tokens counted are in no page."""
-        order, rows = [s for s, _ in sequences], [n for _, n in sequences]
-        if not order or len(set(order)) != len(order) or min(rows) < 0 or any(n != int(n) for n in rows):
-            raise ValueError("batch: at least one sequence, each once, with whole, no negative rows")
-        total = sum(rows)
-        M = max(total, 1) if M is None else M
+        order, rows = [s for s, _ in sequences], _whole("batch: rows", *(n for _, n in sequences))
+        if not order or len(set(order)) != len(order) or min(rows) < 0:
+            raise ValueError("batch: at least one sequence, each once, with no negative rows")
+        sequences, total = list(zip(order, rows)), sum(rows)
+        M, = _whole("batch: M", max(total, 1) if M is None else M)
         if M < total:
             raise ValueError(f"batch: {total} rows for tensors of {M}")
         lengths = [self._lengths[s] + n for s, n in sequences]
